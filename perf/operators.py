@@ -415,7 +415,7 @@ def _plain_fork(s):
     free = most[:n_pages] == 0
     order = free.sort(descending=True, stable=True)[1]  # the free pages, lowest first
     end = want.cumsum(0)
-    ok = fits & (end <= free.sum())
+    ok = fits & ((want == 0) | (end <= free.sum()))
     copy, got = copy & ok, torch.where(ok, want, 0)
     begin = end - want
     fresh = torch.where(ok & (grow > 0), (ln + grow + page - 1) // page, used)
