@@ -367,6 +367,114 @@ pai_status_t pai_b200_attn_decode_f16kv_noalloc(pai_b200_ctx_t *ctx, uint64_t h,
 pai_status_t pai_b200_argmax_f32(pai_b200_ctx_t *ctx, uint64_t rows, uint64_t n,
                                  const float *logits, int32_t *out);
 
+/* ---- several continuations of a prompt ------------------------------------------------
+ * Operators for decoding that follows more than one continuation: drafted
+ * trees that are verified in one pass, and beam search. No counterpart in
+ * the reference, whose decode is greedy over one sequence
+ * (models/model.c:450-507, models/sampler.c:89-99).
+ *
+ * A cache view says where the fp16 K/V rows of n_seq sequences lie. Row
+ * `pos` of sequence s, layer l, kv head i starts at element
+ *     l * layer_stride + page * page_stride + i * head_stride
+ *       + (pos % page_tokens) * head_dim
+ * of k and of v, with page = table[s * max_pages + pos / page_tokens]. A
+ * NULL table is a cache without pages, one run of page_tokens positions for
+ * each sequence: max_pages is 1 and the page is s (a session's cache:
+ * pai_b200_session_kv_view). A table entry outside [0, n_pages) is a hole:
+ * its positions are never read or written, and no query attends them.
+ * k and v are 16-byte aligned, the strides multiples of 8 elements,
+ * head_dim a multiple of 8 up to 256, n_seq at most 1024, and
+ * max_pages * page_tokens below 2^31. */
+typedef struct pai_b200_kv_view {
+  void *k, *v;          /* device, fp16 */
+  const int32_t *table; /* device [n_seq][max_pages], or NULL */
+  uint32_t n_layer, n_seq, kv_heads, head_dim;
+  uint32_t page_tokens, n_pages, max_pages;
+  uint64_t layer_stride, page_stride, head_stride; /* fp16 elements */
+} pai_b200_kv_view_t;
+
+/* Drafted nodes come as rows: sequence s owns the rows node_off[s] ..
+ * node_off[s + 1] - 1 of `rows` rows in all, in an order that puts every
+ * node behind its parent; node i of a sequence has its K/V at position
+ * lens[s] + i, behind the lens[s] committed positions. lens, node_off
+ * [n_seq + 1], depth, mask are device arrays. At most max_nodes (1 to 1024)
+ * nodes of a sequence and rows below `rows` are computed; other rows of the
+ * outputs are left as they were. A chain of one node is plain decoding, a
+ * chain of n with mask and depth NULL a causal chunk of n tokens. */
+
+/* Rotate q and k of every row at position lens[s] + depth[row] (depth NULL:
+ * lens[s] + i) as pai_ref_rope_f32 does (ref_ops.c:231-257, all head_dim / 2
+ * pairs), write q to q_out [rows][h][head_dim], and store k and v, rounded
+ * to fp16, in layer `layer` of the cache. qkv is [rows][h + 2 kv_heads]
+ * [head_dim] (the fused projection row), cos_t and sin_t [table_len]
+ * [head_dim / 2]. A node whose position is not below table_len gets NaN in
+ * q_out and is not stored. qkv, q_out, cos_t, sin_t 16-byte aligned. */
+pai_status_t pai_b200_rope_append_f16kv(pai_b200_ctx_t *ctx, const pai_b200_kv_view_t *kv, uint32_t layer, uint64_t h,
+                                        uint64_t rows, uint32_t max_nodes, const int32_t *lens,
+                                        const int32_t *node_off, const int32_t *depth, const float *qkv,
+                                        const float *cos_t, const float *sin_t, uint64_t table_len, float *q_out);
+/* GQA attention of every node over its sequence's committed positions and
+ * the nodes of its mask row: mask is [rows][ceil(max_nodes / 64)] words, bit
+ * j of word w for node 64 w + j (a node attends itself only if its bit is
+ * set); NULL lets node i attend nodes 0..i. Scores are scaled by
+ * 1/sqrtf(head_dim); q and out are [rows][h][head_dim] fp32, 16-byte
+ * aligned; head_dim 64 or 128, h a multiple of kv_heads. A node that attends
+ * nothing gets zeros. Non-finite K or V rows make the rows that attend them
+ * non-finite and no others. Results match fp32 arithmetic to about 1e-6
+ * relative: K and V enter the tensor cores as stored, q and the softmax
+ * weights as two fp16 parts each. The same call gives the same bits. */
+pai_status_t pai_b200_attn_tree_f16kv(pai_b200_ctx_t *ctx, const pai_b200_kv_view_t *kv, uint32_t layer, uint64_t h,
+                                      uint64_t rows, uint32_t max_nodes, const int32_t *lens,
+                                      const int32_t *node_off, const uint64_t *mask, const float *q, float *out);
+/* Keep the accepted nodes: in every layer, row lens[s] + path[s][i] moves to
+ * lens[s] + i for i < n_path[s] (path is [n_seq][max_path], max_path at most
+ * 1024), and lens_out[s] = lens[s] + the number of nodes kept. A path
+ * ascends strictly; it ends before an entry that does not, or whose row
+ * lies in a hole or behind the last page. lens_out may be lens. */
+pai_status_t pai_b200_kv_accept_f16(pai_b200_ctx_t *ctx, const pai_b200_kv_view_t *kv, uint32_t max_path,
+                                    const int32_t *lens, const int32_t *path, const int32_t *n_path,
+                                    int32_t *lens_out);
+/* Fork, reorder, end and extend sequences: sequence i becomes a copy of
+ * sequence parents[i] (an index outside [0, n_seq) ends it: length 0) with
+ * room to write grow[i] positions behind its lens_out[i] = lens[parents[i]]
+ * committed ones; granted[i] is grow[i], or 0 where there is no room.
+ * parents, grow NULL: i and 0. lens_out may be lens; the other outputs
+ * overlap no input.
+ * With a page table, table_out [n_seq][max_pages] is the new table (-1 behind
+ * each sequence's last page; kv->table stays as it is). Sequences share the
+ * pages of their common past. A partly filled last page that a sequence is
+ * about to extend stays its own if no other sequence uses as many rows of it
+ * (of several, the first that extends it keeps it); else its rows are copied
+ * to a new page, in all layers. New pages are those that no sequence's
+ * committed positions use after the fork, lowest first, given to the
+ * sequences in order; from the first that finds too few on, no sequence
+ * gets any. Pages are in use by being in a table: ending a sequence frees
+ * them, and pages behind the committed positions are free by themselves. A
+ * sequence whose partly filled last page is a hole, or whose
+ * positions would pass max_pages, gets no room.
+ * Without a table (n_seq at most 32), rows `first` .. lens - 1 of the parent
+ * are copied in all layers (rows below `first` are the same in all
+ * sequences, such as a shared prompt's); table_out is not used. */
+pai_status_t pai_b200_kv_fork_f16(pai_b200_ctx_t *ctx, const pai_b200_kv_view_t *kv, uint32_t first,
+                                  const int32_t *lens, const int32_t *parents, const int32_t *grow,
+                                  int32_t *table_out, int32_t *lens_out, int32_t *granted);
+/* The n_out best continuations of each of `prompts` groups of `beams`
+ * beams. Candidate (b, t): token t after beam b, with score
+ * scores[b] + logit - log sum exp of the beam's logits; a beam with done[b]
+ * != 0 (done NULL: none) has the one candidate `pad` with score scores[b].
+ * logits is [prompts * beams] rows of `vocab` with `stride` elements between
+ * rows, scores and done [prompts][beams]. Best first; equal scores go to
+ * the lowest beam, then the lowest token. out_parents holds rows (prompt *
+ * beams + b), so that it serves pai_b200_kv_fork_f16. Scores are computed in
+ * double and rounded once. A logit of NaN counts as -inf; where logits are
+ * +inf, they share the beam's probability; candidates of score -inf or NaN
+ * are never chosen: with fewer than n_out others the rest are score -inf,
+ * parent -1, token `pad`. beams and n_out at most 64. */
+pai_status_t pai_b200_beam_select_f32(pai_b200_ctx_t *ctx, uint64_t prompts, uint64_t beams, uint64_t vocab,
+                                      const float *logits, uint64_t stride, const float *scores,
+                                      const int32_t *done, int32_t pad, uint64_t n_out, float *out_scores,
+                                      int32_t *out_parents, int32_t *out_tokens);
+
 /* ---- registry ------------------------------------------------------------------- */
 
 /* Register this backend's op descriptors (caps PAI_OP_CAP_CUDA_B200,

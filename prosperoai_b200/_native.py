@@ -45,6 +45,23 @@ class GgufInfo(C.Structure):
                 ("weight_bytes", C.c_uint64), ("architecture", C.c_char * 64)]
 
 
+class KvView(C.Structure):
+    """pai_b200_kv_view_t: where the fp16 K/V rows of a cache's sequences lie."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p), ("n_layer", C.c_uint32),
+                ("n_seq", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("page_tokens", C.c_uint32), ("n_pages", C.c_uint32), ("max_pages", C.c_uint32),
+                ("layer_stride", C.c_uint64), ("page_stride", C.c_uint64), ("head_stride", C.c_uint64)]
+
+    @classmethod
+    def of(cls, k, v, n_layer: int, n_seq: int, kv_heads: int, head_dim: int, page_tokens: int, n_pages: int,
+           table=None, max_pages: int = 1) -> "KvView":
+        """View of planes laid out [layer][page][kv head][position of the page][head_dim];
+        k, v and table are device addresses (table None: one run of positions a sequence)."""
+        head = page_tokens * head_dim
+        return cls(k, v, table, n_layer, n_seq, kv_heads, head_dim, page_tokens, n_pages, max_pages,
+                   n_pages * kv_heads * head, kv_heads * head, head)
+
+
 class OpDescriptor(C.Structure):
     _fields_ = [("name", C.c_char_p), ("version", C.c_uint32), ("num_inputs", C.c_uint32),
                 ("num_outputs", C.c_uint32), ("in_dtype", C.c_int32), ("out_dtype", C.c_int32),
@@ -122,6 +139,11 @@ SIGNATURES = {
     "pai_b200_attn_decode_f16kv": (I32, [P, U64, U64, U64, U64, U64, P, P, P, P]),
     "pai_b200_attn_decode_f16kv_noalloc": (I32, [P, U64, U64, U64, U64, U64, P, P, P, P]),
     "pai_b200_argmax_f32": (I32, [P, U64, U64, P, P]),
+    "pai_b200_rope_append_f16kv": (I32, [P, P, U32, U64, U64, U32, P, P, P, P, P, P, U64, P]),
+    "pai_b200_attn_tree_f16kv": (I32, [P, P, U32, U64, U64, U32, P, P, P, P, P]),
+    "pai_b200_kv_accept_f16": (I32, [P, P, U32, P, P, P, P]),
+    "pai_b200_kv_fork_f16": (I32, [P, P, U32, P, P, P, P, P, P]),
+    "pai_b200_beam_select_f32": (I32, [P, U64, U64, U64, P, U64, P, P, I32, U64, P, P, P]),
     "pai_b200_register_ops": (I32, [P]),
     "pai_b200_op_count": (U32, []),
     "pai_b200_op": (C.POINTER(OpDescriptor), [U32]),

@@ -11,9 +11,9 @@ import os
 
 import numpy as np
 
-from ._native import (Q4_0, Q4_K, Q8_0, GgufInfo, ModelCfg, OpRegistry, PaiError, check, load)
+from ._native import (Q4_0, Q4_K, Q8_0, GgufInfo, KvView, ModelCfg, OpRegistry, PaiError, check, load)
 
-__all__ = ["Device", "Buffer", "PackedMatrix", "Model", "Session", "PaiError",
+__all__ = ["Device", "Buffer", "PackedMatrix", "Model", "Session", "KvView", "PaiError",
            "Q4_0", "Q8_0", "Q4_K", "block_bytes", "quantize", "rope_tables", "gguf_inspect",
            "pai_from_gguf", "pai_inspect"]
 
@@ -74,6 +74,11 @@ class Buffer:
             self.free()
         except Exception:
             pass
+
+
+def _at(x):
+    """Device address of a Buffer, or the address itself (None: NULL)."""
+    return x.ptr if isinstance(x, Buffer) else x
 
 
 class PackedMatrix:
@@ -192,6 +197,37 @@ class Device:
 
     def argmax(self, rows: int, n: int, logits: Buffer, out: Buffer):
         check(load().pai_b200_argmax_f32(self.ctx, rows, n, logits.ptr, out.ptr), "argmax")
+
+    # --- several continuations of a prompt (device arrays: Buffers or addresses) ------------
+    def rope_append(self, kv: KvView, layer: int, h: int, rows: int, max_nodes: int, lens, node_off, depth, qkv, cos_t,
+                    sin_t, table_len: int, q_out):
+        """Rotate the drafted rows' q and k, append their k and v to the cache, write q
+        (pai_b200_rope_append_f16kv)."""
+        check(load().pai_b200_rope_append_f16kv(self.ctx, C.byref(kv), layer, h, rows, max_nodes, _at(lens),
+                                                _at(node_off), _at(depth), _at(qkv), _at(cos_t), _at(sin_t),
+                                                table_len, _at(q_out)), "rope_append")
+
+    def attn_tree(self, kv: KvView, layer: int, h: int, rows: int, max_nodes: int, lens, node_off, mask, q, out):
+        """Attention of drafted nodes over the cache and their ancestors (pai_b200_attn_tree_f16kv)."""
+        check(load().pai_b200_attn_tree_f16kv(self.ctx, C.byref(kv), layer, h, rows, max_nodes, _at(lens),
+                                              _at(node_off), _at(mask), _at(q), _at(out)), "attn_tree")
+
+    def kv_accept(self, kv: KvView, max_path: int, lens, path, n_path, lens_out):
+        """Move the accepted nodes' rows behind the committed ones (pai_b200_kv_accept_f16)."""
+        check(load().pai_b200_kv_accept_f16(self.ctx, C.byref(kv), max_path, _at(lens), _at(path), _at(n_path),
+                                            _at(lens_out)), "kv_accept")
+
+    def kv_fork(self, kv: KvView, first: int, lens, parents, grow, table_out, lens_out, granted):
+        """Fork, reorder, end and extend the cache's sequences (pai_b200_kv_fork_f16)."""
+        check(load().pai_b200_kv_fork_f16(self.ctx, C.byref(kv), first, _at(lens), _at(parents), _at(grow),
+                                          _at(table_out), _at(lens_out), _at(granted)), "kv_fork")
+
+    def beam_select(self, prompts: int, beams: int, vocab: int, logits, stride: int, scores, done, pad: int, n_out: int,
+                    out_scores, out_parents, out_tokens):
+        """The n_out best continuations of each prompt's beams (pai_b200_beam_select_f32)."""
+        check(load().pai_b200_beam_select_f32(self.ctx, prompts, beams, vocab, _at(logits), stride, _at(scores),
+                                              _at(done), pad, n_out, _at(out_scores), _at(out_parents),
+                                              _at(out_tokens)), "beam_select")
 
     def register_ops(self, registry: OpRegistry):
         check(load().pai_b200_register_ops(C.byref(registry)), "register_ops")

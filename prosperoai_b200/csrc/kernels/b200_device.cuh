@@ -27,6 +27,26 @@ struct SmemOptIn {
   }
 };
 
+// The context's device is current while one of these lives; the caller's
+// own is put back.
+class CtxDeviceGuard {
+ public:
+  explicit CtxDeviceGuard(pai_b200_ctx_t *ctx) : want_(b200_ctx_device(ctx)) {
+    status_ = b200_cuda(cudaGetDevice(&prev_), "cudaGetDevice");
+    if (!status_ && prev_ != want_) status_ = b200_cuda(cudaSetDevice(want_), "cudaSetDevice");
+    set_ = !status_ && prev_ != want_;
+  }
+  ~CtxDeviceGuard() {
+    if (set_) cudaSetDevice(prev_);
+  }
+  pai_status_t status() const { return status_; }
+
+ private:
+  int want_, prev_ = 0;
+  bool set_ = false;
+  pai_status_t status_;
+};
+
 // ---- programmatic dependent launch ---------------------------------------------------------
 // pdl_wait blocks the calling thread until the previous kernel in the
 // stream has completed and its writes are visible (a no-op when the kernel

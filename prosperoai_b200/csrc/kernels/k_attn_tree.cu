@@ -1,0 +1,535 @@
+// Attention of drafted nodes over a cache view (pai_b200_attn_tree_f16kv).
+//
+// A sequence's query rows are its nodes times the G = h / kv_heads query heads
+// that share a kv head, in tiles of MR rows. Every row tile of every kv head
+// ("unit") goes over the same keys: the committed positions, then the nodes
+// themselves, in tiles of kTile positions, with one running softmax.
+//
+//   s_j = (q . k_j) / sqrt(hd) if row sees j, else -inf
+//   m = max s_j, l = sum e^(s_j - m), o = sum e^(s_j - m) v_j / l
+//
+// Work split: the (unit, tile) pairs of all sequences, in order, are cut into
+// gridDim.x even ranges, whatever the lengths are (they are known on the
+// device only). A CTA writes the units that lie in its range to `out`, and
+// (o, m, l) of a unit that it shares to scratch; the last CTA of such a unit
+// joins the parts in order, so that the result does not depend on which CTA
+// is last.
+//
+// Arithmetic: K and V are fp16 as stored. q, scaled by a power of two for
+// each row, and the softmax weights are split into an fp16 part and an fp16
+// remainder and multiplied twice, with fp32 sums: 22 bits of each, so that
+// the products are as exact as fp32 ones. The weights carry a factor 2^12
+// that keeps the remainders of small ones above fp16's smallest step.
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "../b200_internal.h"
+#include "b200_device.cuh"
+#include "kv_view.cuh"
+
+namespace {
+
+constexpr uint32_t kTile = 64, kThreads = 128, kMaxSeqs = 1024;
+constexpr int kStages = 3;
+constexpr float kPShift = 12.0f;
+
+struct TreeParams {
+  KvDev c;
+  uint32_t h, g, max_nodes, words, max_blocks;  // g: query heads of a kv head; max_blocks: row tiles of a sequence
+  uint64_t rows;
+  const int32_t *lens, *off;
+  const uint64_t *mask;
+  const float *q;
+  float *out;
+  float *part_o;   // scratch [2 gridDim.x][MR][hd]
+  float *part_ml;  // scratch [2 gridDim.x][MR][2]
+  uint32_t *cnt;   // counters [n_seq][kv head][row tile], left at zero
+  float scale;     // log2(e) / sqrt(hd)
+};
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const void *p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(smem_u32(p)));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const void *p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(smem_u32(p)));
+}
+// 16 bytes global -> shared; `ok` false writes zeros and reads nothing
+__device__ __forceinline__ void cp16(void *dst, const void *src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 16u : 0u)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// (x, y) -> packed fp16 parts and packed fp16 remainders
+__device__ __forceinline__ void split_f16(float x, float y, uint32_t &hi, uint32_t &lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+  hi = *reinterpret_cast<const uint32_t *>(&h);
+  lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+
+// Bits [at, at + 64) of a row of `words` 64-bit words; at may be negative.
+__device__ __forceinline__ uint64_t window(const uint64_t *m, uint32_t words, int32_t at) {
+  const int32_t w = at >> 6, sh = at & 63;
+  const uint64_t a = w >= 0 && w < (int32_t)words ? m[w] : 0;
+  const uint64_t b = w + 1 >= 0 && w + 1 < (int32_t)words ? m[w + 1] : 0;
+  return sh ? (a >> sh) | (b << (64 - sh)) : a;
+}
+// The lowest n bits (n below 0: none; above 63: all).
+__device__ __forceinline__ uint64_t low_bits(int64_t n) {
+  return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1;
+}
+
+// One sequence's share of the work.
+struct SeqWork {
+  uint32_t len, nodes, first, blocks, tiles;
+};
+template <uint32_t MR>
+__device__ __forceinline__ SeqWork seq_work(const TreeParams &p, uint32_t s) {
+  SeqWork w;
+  w.nodes = kv_nodes(p.off, s, p.rows, p.max_nodes, &w.first);
+  w.len = kv_len(p.c, p.lens, s);
+  w.blocks = (w.nodes * p.g + MR - 1) / MR;
+  w.tiles = (w.len + w.nodes + kTile - 1) / kTile;
+  return w;
+}
+
+// Shared memory of a stage: K then V rows, padded so that the eight rows of an ldmatrix lie in different banks.
+template <int HD>
+struct Stage {
+  __half k[kTile][HD + 8];
+  __half v[kTile][HD + 8];
+};
+
+// WM warps share a tile's rows (16 each), 4 / WM share its positions.
+template <int HD, int WM>
+__global__ void __launch_bounds__(kThreads, 2) k_attn_tree(TreeParams p) {
+  constexpr uint32_t MR = 16 * WM, WN = 4 / WM, NT = 8 / WN, CH = HD / 8;
+  extern __shared__ __align__(16) uint8_t smem[];
+  Stage<HD> *st = reinterpret_cast<Stage<HD> *>(smem);
+  __shared__ uint64_t upto[kMaxSeqs + 1];
+  __shared__ uint64_t valid[kStages];    // positions of a stage's tile that hold a row
+  __shared__ uint64_t odd;               // its nodes with a non-finite V row
+  __shared__ uint32_t ticket;
+  const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5, wm = warp % WM, wn = warp / WM;
+  const uint32_t gq = lane >> 2, tq = lane & 3;
+  const uint32_t n_seq = p.c.n_seq, hk = p.c.hk;
+  pdl_trigger();
+  pdl_wait();
+
+  // pairs before each sequence
+  for (uint32_t s = t; s < n_seq; s += kThreads) {
+    const SeqWork w = seq_work<MR>(p, s);
+    upto[s + 1] = (uint64_t)w.blocks * w.tiles * hk;
+  }
+  if (t == 0) upto[0] = 0;
+  __syncthreads();
+  if (warp == 0) {
+    uint64_t sum = 0;
+    for (uint32_t s0 = 0; s0 < n_seq; s0 += 32) {
+      const uint32_t s = s0 + lane;
+      uint64_t x = s < n_seq ? upto[s + 1] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= (uint32_t)o) x += y;
+      }
+      x += sum;
+      if (s < n_seq) upto[s + 1] = x;
+      sum = __shfl_sync(0xffffffffu, x, 31);
+    }
+  }
+  __syncthreads();
+  const uint64_t all = upto[n_seq], cta = blockIdx.x, grid = gridDim.x < all ? gridDim.x : all;
+  if (cta >= grid) return;  // every CTA of the cut has at least one pair
+  uint64_t at = cta * all / grid;
+  const uint64_t end = (cta + 1) * all / grid, begin = at;
+  uint32_t s = 0;
+  for (uint32_t lo = 0, hi = n_seq; at < end && lo < hi;) {  // the sequence of the first pair
+    const uint32_t mid = (lo + hi) / 2;
+    if (upto[mid + 1] <= at) lo = mid + 1; else hi = mid;
+    s = lo;
+  }
+
+  while (at < end) {
+    while (upto[s + 1] <= at) s++;
+    const SeqWork w = seq_work<MR>(p, s);
+    const uint64_t unit = (at - upto[s]) / w.tiles, unit0 = upto[s] + unit * w.tiles, unit1 = unit0 + w.tiles;
+    const uint32_t kvh = (uint32_t)(unit / w.blocks), block = (uint32_t)(unit % w.blocks);
+    const uint32_t tile0 = (uint32_t)(at - unit0), tile1 = (uint32_t)((end < unit1 ? end : unit1) - unit0);
+    const uint32_t total = w.len + w.nodes;
+    const __half *kp = p.c.k + (size_t)kvh * p.c.head_stride, *vp = p.c.v + (size_t)kvh * p.c.head_stride;
+
+    // this thread's two rows: node, query head, q fragments (part and remainder), factor of its scores
+    uint32_t node[2];
+    float factor[2];
+    bool live[2];
+    uint32_t qh[HD / 16][4], ql[HD / 16][4];
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      const uint32_t r = block * MR + wm * 16 + gq + 8 * x;
+      node[x] = r / p.g;
+      live[x] = node[x] < w.nodes;
+      const float *qr = p.q + ((size_t)(w.first + (live[x] ? node[x] : 0)) * p.h + kvh * p.g + r % p.g) * HD;
+      float top = 0.0f;
+#pragma unroll
+      for (int k = 0; k < HD / 16; k++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const float2 f = live[x] ? *reinterpret_cast<const float2 *>(qr + 16 * k + 8 * e + 2 * tq) : make_float2(0.f, 0.f);
+          qh[k][x + 2 * e] = __float_as_uint(f.x);
+          ql[k][x + 2 * e] = __float_as_uint(f.y);
+          top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^-e brings the row's largest element into [1, 2); a row of zeros, subnormals or infinities stays
+      const uint32_t ex = __float_as_uint(top) >> 23;
+      const bool turn = ex >= 1 && ex <= 252;
+      const float down = turn ? __uint_as_float((254 - ex) << 23) : 1.0f;
+      factor[x] = p.scale * (turn ? __uint_as_float(ex << 23) : 1.0f);
+#pragma unroll
+      for (int k = 0; k < HD / 16; k++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          uint32_t &a = qh[k][x + 2 * e], &b = ql[k][x + 2 * e];
+          split_f16(__uint_as_float(a) * down, __uint_as_float(b) * down, a, b);
+        }
+    }
+
+    float o[HD / 8][4];
+#pragma unroll
+    for (int n = 0; n < HD / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
+    auto load = [&](uint32_t tile, uint32_t slot) {
+      Stage<HD> &sg = st[slot];
+      uint32_t have = 0;  // rows of this thread's pass that exist
+#pragma unroll
+      for (uint32_t i = 0; i < kTile * CH / kThreads; i++) {
+        const uint32_t r = t / CH + i * (kThreads / CH), ch = t % CH, pos = tile * kTile + r;
+        const int64_t at_row = pos < total ? kv_row(p.c, s, pos) : -1;
+        const bool ok = at_row >= 0;
+        cp16(&sg.k[r][ch * 8], kp + (ok ? at_row : 0) + ch * 8, ok);
+        cp16(&sg.v[r][ch * 8], vp + (ok ? at_row : 0) + ch * 8, ok);
+        have |= (ok ? 1u : 0u) << i;
+      }
+      cp_commit();
+      if (t % CH == 0) {
+        uint64_t bits = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kTile * CH / kThreads; i++)
+          bits |= (uint64_t)((have >> i) & 1u) << (t / CH + i * (kThreads / CH));
+        atomicOr((unsigned long long *)&valid[slot], (unsigned long long)bits);
+      }
+    };
+
+    __syncthreads();  // the stages are free
+    if (t < kStages) valid[t] = 0;
+    __syncthreads();
+    for (uint32_t i = 0; i < kStages - 1; i++) {
+      if (tile0 + i < tile1) load(tile0 + i, i); else cp_commit();
+    }
+    for (uint32_t tile = tile0; tile < tile1; tile++) {
+      const uint32_t n = tile - tile0, slot = n % kStages;
+      cp_wait<kStages - 2>();
+      __syncthreads();  // this tile has landed, and the last one's stage is free
+      if (t == 0) valid[(n + kStages - 1) % kStages] = 0;
+      const bool drafted = (tile + 1) * kTile > w.len;  // the tile holds nodes
+      Stage<HD> &sg = st[slot];
+      if (drafted) {
+        // A non-finite V row may only reach the rows that see its node, and a weight of
+        // 0 does not keep it out of a product: such elements become 0 here and are
+        // added below where they are seen.
+        if (t == 0) odd = 0;
+        __syncthreads();
+        for (uint32_t e = t; e < kTile * CH; e += kThreads) {
+          uint4 &c4 = *reinterpret_cast<uint4 *>(&sg.v[e / CH][(e % CH) * 8]);
+          uint32_t *cw = reinterpret_cast<uint32_t *>(&c4);
+          bool bad = false;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            if ((cw[i] & 0x7C00u) == 0x7C00u) cw[i] &= 0xFFFF0000u, bad = true;
+            if ((cw[i] & 0x7C000000u) == 0x7C000000u) cw[i] &= 0xFFFFu, bad = true;
+          }
+          if (bad) atomicOr((unsigned long long *)&odd, 1ull << (e / CH));
+        }
+      }
+      __syncthreads();
+      if (tile + kStages - 1 < tile1) load(tile + kStages - 1, (n + kStages - 1) % kStages); else cp_commit();
+      const uint64_t rows_ok = valid[slot];
+      uint64_t sees[2] = {rows_ok, rows_ok};
+      if (drafted) {
+        const int32_t base = (int32_t)(tile * kTile - w.len);  // node of the tile's first position
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+          uint64_t b = low_bits(-(int64_t)base);
+          if (live[x])
+            b |= p.mask ? window(p.mask + (size_t)(w.first + node[x]) * p.words, p.words, base) & ~low_bits(-(int64_t)base)
+                        : low_bits((int64_t)node[x] + 1 - base);
+          sees[x] &= b;
+        }
+      }
+
+      // S = q K^T of this warp's NT x 8 positions
+      float sc[NT][4];
+#pragma unroll
+      for (uint32_t nt = 0; nt < NT; nt++) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < HD / 32; k++)
+#pragma unroll
+        for (uint32_t nt = 0; nt < NT; nt++) {
+          uint32_t b[4];
+          ldsm4(b, &sg.k[(wn * NT + nt) * 8 + (lane & 7)][32 * k + 8 * (lane >> 3)]);
+          mma_f16(sc[nt], qh[2 * k], b[0], b[1]);
+          mma_f16(sc[nt], ql[2 * k], b[0], b[1]);
+          mma_f16(sc[nt], qh[2 * k + 1], b[2], b[3]);
+          mma_f16(sc[nt], ql[2 * k + 1], b[2], b[3]);
+        }
+      // scores in powers of two, unseen ones -inf, running maximum of a row (its 4 threads share it)
+      float mt[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (uint32_t nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int x = e >> 1;
+          const uint32_t j = (wn * NT + nt) * 8 + 2 * tq + (e & 1);
+          sc[nt][e] = (sees[x] >> j) & 1 ? sc[nt][e] * factor[x] : -INFINITY;
+          mt[x] = fmaxf(mt[x], sc[nt][e]);
+        }
+      float corr[2], sub[2];
+#pragma unroll
+      for (int x = 0; x < 2; x++) {
+        mt[x] = fmaxf(mt[x], __shfl_xor_sync(0xffffffffu, mt[x], 1));
+        mt[x] = fmaxf(mt[x], __shfl_xor_sync(0xffffffffu, mt[x], 2));
+        const float mn = fmaxf(m[x], mt[x]);
+        corr[x] = m[x] == mn ? 1.0f : exp2f(m[x] - mn);
+        m[x] = mn;
+        sub[x] = mn == -INFINITY ? 0.0f : mn - kPShift;
+        l[x] *= corr[x];
+      }
+      if (__any_sync(0xffffffffu, corr[0] != 1.0f || corr[1] != 1.0f)) {
+#pragma unroll
+        for (int n2 = 0; n2 < HD / 8; n2++) {
+          o[n2][0] *= corr[0];
+          o[n2][1] *= corr[0];
+          o[n2][2] *= corr[1];
+          o[n2][3] *= corr[1];
+        }
+      }
+      // weights as A fragments; O += P V
+#pragma unroll
+      for (uint32_t ks = 0; ks < NT / 2; ks++) {
+        uint32_t ph[4], pl[4];
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+          float pv[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            pv[e] = exp2f(sc[2 * ks + y][e] - sub[e >> 1]);
+            l[e >> 1] += pv[e];
+          }
+          split_f16(pv[0], pv[1], ph[2 * y], pl[2 * y]);
+          split_f16(pv[2], pv[3], ph[2 * y + 1], pl[2 * y + 1]);
+        }
+#pragma unroll
+        for (int n2 = 0; n2 < HD / 16; n2++) {
+          uint32_t b[4];
+          ldsm4t(b, &sg.v[wn * (NT * 8) + 16 * ks + (lane & 15)][16 * n2 + 8 * (lane >> 4)]);
+          mma_f16(o[2 * n2], ph, b[0], b[1]);
+          mma_f16(o[2 * n2], pl, b[0], b[1]);
+          mma_f16(o[2 * n2 + 1], ph, b[2], b[3]);
+          mma_f16(o[2 * n2 + 1], pl, b[2], b[3]);
+        }
+      }
+      if (drafted && odd) {
+        // the non-finite elements of nodes in this warp's positions, for the rows that see them
+        for (uint64_t left = odd & (low_bits((wn + 1) * NT * 8) & ~low_bits(wn * NT * 8)); left; left &= left - 1) {
+          const uint32_t j = __ffsll((long long)left) - 1;
+          const int64_t at_row = kv_row(p.c, s, tile * kTile + j);
+#pragma unroll
+          for (int n2 = 0; n2 < HD / 8; n2++) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(vp + at_row + 8 * n2 + 2 * tq));
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+              if ((sees[x] >> j) & 1) {
+                if (!isfinite(f.x)) o[n2][2 * x] += f.x;
+                if (!isfinite(f.y)) o[n2][2 * x + 1] += f.y;
+              }
+          }
+        }
+      }
+    }
+    cp_wait<0>();
+    // row sums: each of a row's 4 threads holds a part
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+    }
+    __syncthreads();
+    // the warps that share rows join over their positions: o, m and l in shared memory (the stages are free)
+    float *so = reinterpret_cast<float *>(smem);            // [WN][MR][HD + 4]
+    float *sm = so + WN * MR * (HD + 4);                    // [WN][MR][2]
+    constexpr uint32_t OS = HD + 4;
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      const uint32_t r = wm * 16 + gq + 8 * x;
+      float *d = so + (wn * MR + r) * OS + 2 * tq;
+#pragma unroll
+      for (int n2 = 0; n2 < HD / 8; n2++)
+        *reinterpret_cast<float2 *>(d + 8 * n2) = make_float2(o[n2][2 * x], o[n2][2 * x + 1]);
+      if (tq == 0) {
+        sm[(wn * MR + r) * 2] = m[x];
+        sm[(wn * MR + r) * 2 + 1] = l[x];
+      }
+    }
+    __syncthreads();
+    const bool whole = tile0 == 0 && tile1 == w.tiles;
+    const uint64_t slot = 2 * cta + (begin >= unit0 ? 0 : 1);
+    for (uint32_t e = t; e < MR * (HD / 4); e += kThreads) {
+      const uint32_t r = e / (HD / 4), d = (e % (HD / 4)) * 4;
+      float M = -INFINITY;
+#pragma unroll
+      for (uint32_t y = 0; y < WN; y++) M = fmaxf(M, sm[(y * MR + r) * 2]);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float L = 0.0f;
+#pragma unroll
+      for (uint32_t y = 0; y < WN; y++) {
+        const float my = sm[(y * MR + r) * 2], wy = my == -INFINITY ? 0.0f : exp2f(my - M);
+        if (my == -INFINITY) continue;
+        const float4 f = *reinterpret_cast<const float4 *>(so + (y * MR + r) * OS + d);
+        acc.x = fmaf(f.x, wy, acc.x), acc.y = fmaf(f.y, wy, acc.y);
+        acc.z = fmaf(f.z, wy, acc.z), acc.w = fmaf(f.w, wy, acc.w);
+        L = fmaf(sm[(y * MR + r) * 2 + 1], wy, L);
+      }
+      const uint32_t rr = block * MR + r, nd = rr / p.g;
+      if (whole) {
+        if (nd < w.nodes) {
+          const float inv = L != 0.0f ? 1.0f / L : 0.0f;  // a row that sees nothing gets zeros
+          *reinterpret_cast<float4 *>(p.out + ((size_t)(w.first + nd) * p.h + kvh * p.g + rr % p.g) * HD + d) =
+              make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+        }
+      } else {
+        *reinterpret_cast<float4 *>(p.part_o + (slot * MR + r) * HD + d) = acc;
+        if (d == 0) {
+          p.part_ml[(slot * MR + r) * 2] = M;
+          p.part_ml[(slot * MR + r) * 2 + 1] = L;
+        }
+      }
+    }
+    if (!whole) {
+      // CTAs of the unit: those whose ranges hold its first and last pairs, and all between
+      const uint64_t c0 = ((unit0 + 1) * grid - 1) / all, c1 = (unit1 * grid - 1) / all;
+      uint32_t *cnt = &p.cnt[((size_t)s * hk + kvh) * p.max_blocks + block];
+      __threadfence();
+      __syncthreads();
+      if (t == 0) ticket = atomicAdd(cnt, 1u);
+      __syncthreads();
+      if (ticket == (uint32_t)(c1 - c0)) {
+        __threadfence();
+        if (t == 0) *cnt = 0;
+        for (uint32_t e = t; e < MR * (HD / 4); e += kThreads) {
+          const uint32_t r = e / (HD / 4), d = (e % (HD / 4)) * 4;
+          const uint32_t rr = block * MR + r, nd = rr / p.g;
+          if (nd >= w.nodes) continue;
+          float M = -INFINITY, L = 0.0f;
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (uint64_t q = c0; q <= c1; q++) {
+            // the unit is the first of CTA q's range, or the last
+            const uint64_t sl = 2 * q + (q * all / grid >= unit0 ? 0 : 1);
+            const float mq = __ldcg(&p.part_ml[(sl * MR + r) * 2]), lq = __ldcg(&p.part_ml[(sl * MR + r) * 2 + 1]);
+            const float4 f = __ldcg(reinterpret_cast<const float4 *>(p.part_o + (sl * MR + r) * HD + d));
+            if (mq == -INFINITY) continue;
+            const float M2 = fmaxf(M, mq), a = M == -INFINITY ? 0.0f : exp2f(M - M2), b = exp2f(mq - M2);
+            acc.x = acc.x * a + f.x * b, acc.y = acc.y * a + f.y * b;
+            acc.z = acc.z * a + f.z * b, acc.w = acc.w * a + f.w * b;
+            L = L * a + lq * b;
+            M = M2;
+          }
+          const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+          *reinterpret_cast<float4 *>(p.out + ((size_t)(w.first + nd) * p.h + kvh * p.g + rr % p.g) * HD + d) =
+              make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+        }
+      }
+    }
+    at = unit0 + tile1;
+  }
+}
+
+template <int HD, int WM>
+pai_status_t launch_tree(pai_b200_ctx_t *ctx, TreeParams &p) {
+  constexpr uint32_t MR = 16 * WM, WN = 4 / WM;
+  constexpr size_t stages = kStages * sizeof(Stage<HD>), join = WN * MR * (HD + 4 + 2) * sizeof(float);
+  constexpr size_t smem = stages > join ? stages : join;
+  static SmemOptIn opt;
+  pai_status_t st = b200_cuda(opt.ensure(b200_ctx_device(ctx), smem,
+                                         [](size_t b) {
+                                           return cudaFuncSetAttribute(k_attn_tree<HD, WM>,
+                                                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)b);
+                                         }),
+                              "k_attn_tree smem attribute");
+  if (st) return st;
+  p.max_blocks = (p.max_nodes * p.g + MR - 1) / MR;
+  const uint64_t units = (uint64_t)p.c.n_seq * p.c.hk * p.max_blocks;
+  if (units > 0x7FFFFFFu) return b200_fail(PAI_ERR_UNSUPPORTED, "attn_tree: %llu row tiles", (unsigned long long)units);
+  // two CTAs an SM, and no more than there can be pairs
+  const uint64_t pairs = units * (((uint64_t)p.c.max_pages * p.c.page_tokens + p.max_nodes + kTile - 1) / kTile);
+  const uint32_t grid = (uint32_t)std::min<uint64_t>(296, pairs);
+  float *scratch;
+  st = b200_ctx_scratch(ctx, 2ull * grid * MR * (HD + 2), (uint32_t)units, &scratch, &p.cnt);
+  if (st) return st;
+  p.part_o = scratch;
+  p.part_ml = scratch + 2ull * grid * MR * HD;
+  b200_launch(ctx, k_attn_tree<HD, WM>, dim3(grid), dim3(kThreads), smem, p);
+  return b200_launched(ctx, 1, "k_attn_tree");
+}
+
+template <int HD>
+pai_status_t launch_tree_hd(pai_b200_ctx_t *ctx, TreeParams &p) {
+  const uint32_t rows = p.max_nodes * p.g;
+  if (rows <= 16) return launch_tree<HD, 1>(ctx, p);
+  if (rows <= 32) return launch_tree<HD, 2>(ctx, p);
+  return launch_tree<HD, 4>(ctx, p);
+}
+
+}  // namespace
+
+extern "C" pai_status_t pai_b200_attn_tree_f16kv(pai_b200_ctx_t *ctx, const pai_b200_kv_view_t *kv, uint32_t layer,
+                                                 uint64_t h, uint64_t rows, uint32_t max_nodes, const int32_t *lens,
+                                                 const int32_t *node_off, const uint64_t *mask, const float *q,
+                                                 float *out) {
+  TreeParams p{};
+  if (!ctx) return b200_fail(PAI_ERR_INVALID_ARG, "attn_tree: NULL context");
+  pai_status_t st = kv_nodes_check(kv, "attn_tree", layer, h, rows, max_nodes, lens, node_off, p.c);
+  if (st) return st;
+  if (!q || !out) return b200_fail(PAI_ERR_INVALID_ARG, "attn_tree: NULL");
+  if (((uintptr_t)q | (uintptr_t)out) & 15)
+    return b200_fail(PAI_ERR_INVALID_ARG, "attn_tree: q and out must be 16-byte aligned");
+  if ((uintptr_t)mask & 7) return b200_fail(PAI_ERR_INVALID_ARG, "attn_tree: the mask must be 8-byte aligned");
+  if (kv->head_dim != 64 && kv->head_dim != 128)
+    return b200_fail(PAI_ERR_UNSUPPORTED, "attn_tree: head_dim %u (64 or 128)", kv->head_dim);
+  p.h = (uint32_t)h, p.g = (uint32_t)h / kv->kv_heads, p.max_nodes = max_nodes, p.words = (max_nodes + 63) / 64;
+  p.rows = rows, p.lens = lens, p.off = node_off, p.mask = mask, p.q = q, p.out = out;
+  p.scale = 1.4426950408889634f / sqrtf((float)kv->head_dim);
+  const CtxDeviceGuard on(ctx);
+  if (on.status()) return on.status();
+  return kv->head_dim == 64 ? launch_tree_hd<64>(ctx, p) : launch_tree_hd<128>(ctx, p);
+}

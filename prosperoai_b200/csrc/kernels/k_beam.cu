@@ -1,0 +1,315 @@
+// Beam search's selection: the n_out best of beams x vocabulary candidates
+// of every prompt, one launch, the logits read once.
+//
+//   score(b, t) = start_b + (x_t - m_b) - log Z_b,   Z_b = sum_t e^(x_t - m_b)
+//
+// Within a beam the order of the scores is the order of the logits, so a CTA
+// needs neither m_b nor Z_b to know which of its logits can be chosen: it
+// keeps the n_out largest of its slice (in registers), the slice's maximum
+// and its sum of exponentials. The last CTA of a prompt to finish merges:
+// m_b and Z_b of every beam from the slices in order, then the n_out best of
+// the kept logits by score. What is added up is added in a fixed order; the
+// chosen ones are ranked by (score, flat index), so nothing depends on which
+// CTA is last.
+//
+// The n_out largest of a slice: with 256 threads' maxima ranked, the n_out-th
+// of them is a bound that at least n_out values reach, and that few others
+// do; those that reach it are collected and ranked. Where more than
+// kCollect reach it (a slice of equal logits), they are taken one by one.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "../b200_internal.h"
+#include "b200_device.cuh"
+
+namespace {
+
+constexpr uint32_t kThreads = 256, kPer = 32, kSlice = kThreads * kPer;  // logits of a CTA: 32 registers a thread
+constexpr uint32_t kMaxPick = 64, kMaxBeams = 64, kCollect = 1024;
+
+struct BeamParams {
+  const float *logits, *scores;
+  const int32_t *done;
+  uint64_t stride;
+  uint32_t beams, vocab, slices, per, n_out;
+  int32_t pad;
+  float *out_scores;
+  int32_t *out_parents, *out_tokens;
+  float *top;      // scratch [row][slice]: the slice's maximum
+  float *sum;      // scratch [row][slice]: its sum of e^(x - maximum)
+  float *val;      // scratch [row][slice][n_out]: the kept logits, largest first, -inf behind them
+  uint32_t *idx;   // scratch [row][slice][n_out]: their tokens
+  uint32_t *cnt;   // counters [prompt], left at zero
+};
+
+template <typename T>
+struct Cand {
+  T v;
+  uint32_t i;
+};
+
+// (value, index): larger first, equal values by the lower index
+template <typename T>
+__device__ __forceinline__ bool before(T v, uint32_t i, T w, uint32_t j) {
+  return v > w || (v == w && i < j);
+}
+
+template <typename T>
+__device__ __forceinline__ T ninf() {
+  return -(T)INFINITY;
+}
+
+// The `pick` first of the block's candidates into out[] (shared), ranked;
+// `each` calls f(value, index) for every candidate of the calling thread, the
+// same each time; `most` is the thread's largest value. Candidates of value
+// -inf are never taken. Returns how many there are (at most pick).
+template <typename T, typename Each>
+__device__ uint32_t block_pick(uint32_t pick, T most, Each each, Cand<T> *out, Cand<T> *buf, T *maxima) {
+  __shared__ uint32_t count;
+  __shared__ T bound;
+  __shared__ Cand<T> wbest[kThreads / 32];
+  const uint32_t t = threadIdx.x;
+  __syncthreads();
+  maxima[t] = most;
+  if (t == 0) count = 0;
+  __syncthreads();
+  uint32_t rank = 0;
+#pragma unroll 8
+  for (uint32_t j = 0; j < kThreads; j++) rank += before(maxima[j], j, most, t);
+  if (rank == pick - 1) bound = most;
+  __syncthreads();
+  const T low = bound;
+  each([&](T v, uint32_t i) {
+    if (v >= low && v > ninf<T>()) {
+      const uint32_t at = atomicAdd(&count, 1u);
+      if (at < kCollect) buf[at] = Cand<T>{v, i};
+    }
+  });
+  __syncthreads();
+  const uint32_t n = count;
+  if (n <= kCollect) {
+    for (uint32_t a = t; a < n; a += kThreads) {
+      const Cand<T> me = buf[a];
+      uint32_t r = 0;
+      for (uint32_t b = 0; b < n; b++) r += before(buf[b].v, buf[b].i, me.v, me.i);
+      if (r < pick) out[r] = me;
+    }
+    __syncthreads();
+    return min(n, pick);
+  }
+  // many equal values: one after the other
+  T lv = (T)INFINITY;
+  uint32_t li = 0;
+  for (uint32_t k = 0; k < pick; k++) {
+    T bv = ninf<T>();
+    uint32_t bi = 0xFFFFFFFFu;
+    each([&](T v, uint32_t i) {
+      if ((k == 0 || before(lv, li, v, i)) && v > ninf<T>() && before(v, i, bv, bi)) bv = v, bi = i;
+    });
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const T ov = __shfl_xor_sync(0xffffffffu, bv, o);
+      const uint32_t oi = __shfl_xor_sync(0xffffffffu, bi, o);
+      if (before(ov, oi, bv, bi)) bv = ov, bi = oi;
+    }
+    if ((t & 31) == 0) wbest[t >> 5] = Cand<T>{bv, bi};
+    __syncthreads();
+    for (uint32_t w = 0; w < kThreads / 32; w++)
+      if (before(wbest[w].v, wbest[w].i, bv, bi)) bv = wbest[w].v, bi = wbest[w].i;
+    lv = bv, li = bi;
+    if (t == 0) out[k] = Cand<T>{bv, bi};
+    __syncthreads();
+  }
+  return pick;
+}
+
+__global__ void __launch_bounds__(kThreads) k_beam_select(BeamParams p) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ Cand<double> buf_d[kCollect];  // the float form's buffer is its first half
+  __shared__ Cand<double> out_d[kMaxPick];
+  __shared__ double maxima_d[kThreads];
+  __shared__ double logz[kMaxBeams], start[kMaxBeams];
+  __shared__ float topb[kMaxBeams];
+  __shared__ float redf[kThreads / 32];
+  __shared__ double redd[kThreads / 32];
+  __shared__ uint32_t ticket;
+  const uint32_t t = threadIdx.x, slice = blockIdx.x, row = blockIdx.y, prompt = row / p.beams;
+  const uint32_t M = p.n_out;
+  const uint64_t slot = (uint64_t)row * p.slices + slice;
+  const bool done = p.done && p.done[row] != 0;
+  if (!done) {
+    const uint32_t lo = slice * p.per, hi = min(p.vocab, lo + p.per);
+    const float *x = p.logits + (uint64_t)row * p.stride;
+    float v[kPer];
+    float most = -INFINITY;
+    const bool wide = (((uintptr_t)x | (lo * 4ull)) & 15) == 0;
+    // thread t has logits lo + 4t .. +3, then 1024 further on: index of v[e] = lo + (e/4) 1024 + 4t + e%4
+#pragma unroll
+    for (uint32_t e = 0; e < kPer; e += 4) {
+      const uint32_t i = lo + (e / 4) * (kThreads * 4) + 4 * t;
+      if (wide && i + 4 <= hi) {
+        const float4 f = __ldcs(reinterpret_cast<const float4 *>(x + i));
+        v[e] = f.x, v[e + 1] = f.y, v[e + 2] = f.z, v[e + 3] = f.w;
+      } else {
+#pragma unroll
+        for (uint32_t q = 0; q < 4; q++) v[e + q] = i + q < hi ? x[i + q] : -INFINITY;
+      }
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < kPer; e++) {
+      if (v[e] != v[e]) v[e] = -INFINITY;  // NaN counts as -inf
+      most = fmaxf(most, v[e]);
+    }
+    float m = warp_max(most);
+    if ((t & 31) == 0) redf[t >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < kThreads / 32; w++) m = fmaxf(m, redf[w]);
+    // the exponentials of a thread's 32 logits in 32 bits, their sums over threads in 64
+    float s = 0.0f;
+    if (m > -INFINITY) {
+#pragma unroll
+      for (uint32_t e = 0; e < kPer; e++) s += v[e] == m ? 1.0f : expf(v[e] - m);
+    }
+    double sd = s;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sd += __shfl_xor_sync(0xffffffffu, sd, o);
+    if ((t & 31) == 0) redd[t >> 5] = sd;
+    __syncthreads();
+    if (t == 0) {
+      double z = 0.0;
+      for (uint32_t w = 0; w < kThreads / 32; w++) z += redd[w];
+      p.top[slot] = m;
+      p.sum[slot] = (float)z;
+    }
+    Cand<float> *buf = reinterpret_cast<Cand<float> *>(buf_d), *out = reinterpret_cast<Cand<float> *>(out_d);
+    const uint32_t n = block_pick<float>(
+        M, most,
+        [&](auto f) {
+#pragma unroll
+          for (uint32_t e = 0; e < kPer; e++) f(v[e], lo + (e / 4) * (kThreads * 4) + 4 * t + e % 4);
+        },
+        out, buf, reinterpret_cast<float *>(maxima_d));
+    for (uint32_t k = t; k < M; k += kThreads) {
+      p.val[slot * M + k] = k < n ? out[k].v : -INFINITY;
+      p.idx[slot * M + k] = k < n ? out[k].i : 0;
+    }
+  }
+  // the last CTA of the prompt merges
+  __threadfence();
+  __syncthreads();
+  if (t == 0) ticket = atomicAdd(&p.cnt[prompt], 1u);
+  __syncthreads();
+  if (ticket != p.beams * p.slices - 1) return;
+  __threadfence();
+  const uint64_t row0 = (uint64_t)prompt * p.beams;
+  for (uint32_t b = t; b < p.beams; b += kThreads) {
+    const uint64_t r = (row0 + b) * p.slices;
+    float m = -INFINITY;
+    double z = 0.0;
+    const bool over = p.done && p.done[row0 + b] != 0;
+    if (!over) {
+      for (uint32_t k = 0; k < p.slices; k++) m = fmaxf(m, __ldcg(&p.top[r + k]));
+      for (uint32_t k = 0; k < p.slices; k++) {
+        const float mk = __ldcg(&p.top[r + k]);
+        if (mk > -INFINITY) z += (double)__ldcg(&p.sum[r + k]) * (mk == m ? 1.0 : exp((double)mk - (double)m));
+      }
+    }
+    start[b] = p.scores[row0 + b];
+    topb[b] = m;
+    logz[b] = over ? NAN : log(z);  // NaN marks a finished beam
+  }
+  __syncthreads();
+  // candidates: beam b's kept logits, or the one of a finished beam, as (score, b * vocab + token)
+  const uint32_t per = p.slices * M, all = p.beams * per;
+  auto score = [&](uint32_t c, double &sc, uint32_t &flat) {
+    const uint32_t b = c / per, k = c % per;
+    sc = ninf<double>();
+    flat = 0;
+    if (logz[b] != logz[b]) {
+      if (k == 0) {
+        sc = start[b];
+        flat = b * p.vocab + (uint32_t)p.pad;
+      }
+    } else {
+      const float x = __ldcg(&p.val[row0 * per + c]);
+      if (x > -INFINITY) {
+        sc = start[b] + ((x == topb[b] ? 0.0 : (double)x - (double)topb[b]) - logz[b]);
+        flat = b * p.vocab + __ldcg(&p.idx[row0 * per + c]);
+      }
+    }
+    if (sc != sc) sc = ninf<double>();
+  };
+  double most = ninf<double>();
+  for (uint32_t c = t; c < all; c += kThreads) {
+    double sc;
+    uint32_t flat;
+    score(c, sc, flat);
+    most = sc > most ? sc : most;
+  }
+  const uint32_t n = block_pick<double>(
+      M, most,
+      [&](auto f) {
+        for (uint32_t c = t; c < all; c += kThreads) {
+          double sc;
+          uint32_t flat;
+          score(c, sc, flat);
+          f(sc, flat);
+        }
+      },
+      out_d, buf_d, maxima_d);
+  for (uint32_t k = t; k < M; k += kThreads) {
+    const uint64_t o = (uint64_t)prompt * M + k;
+    const bool is = k < n && out_d[k].v > ninf<double>();
+    p.out_scores[o] = is ? (float)out_d[k].v : -INFINITY;
+    p.out_parents[o] = is ? (int32_t)(row0 + out_d[k].i / p.vocab) : -1;
+    p.out_tokens[o] = is ? (int32_t)(out_d[k].i % p.vocab) : p.pad;
+  }
+  if (t == 0) p.cnt[prompt] = 0;
+}
+
+}  // namespace
+
+extern "C" pai_status_t pai_b200_beam_select_f32(pai_b200_ctx_t *ctx, uint64_t prompts, uint64_t beams, uint64_t vocab,
+                                                 const float *logits, uint64_t stride, const float *scores,
+                                                 const int32_t *done, int32_t pad, uint64_t n_out, float *out_scores,
+                                                 int32_t *out_parents, int32_t *out_tokens) {
+  if (!ctx || !logits || !scores || !out_scores || !out_parents || !out_tokens)
+    return b200_fail(PAI_ERR_INVALID_ARG, "beam_select: NULL");
+  if (prompts == 0 || beams == 0 || vocab == 0 || n_out == 0)
+    return b200_fail(PAI_ERR_INVALID_ARG, "beam_select: a size is 0");
+  if (stride < vocab)
+    return b200_fail(PAI_ERR_MISMATCH, "beam_select: stride %llu below the vocabulary of %llu",
+                     (unsigned long long)stride, (unsigned long long)vocab);
+  if (pad < 0 || (uint64_t)pad >= vocab)
+    return b200_fail(PAI_ERR_INVALID_ARG, "beam_select: pad token %d outside vocab %llu", pad, (unsigned long long)vocab);
+  if (beams > kMaxBeams || n_out > kMaxPick)
+    return b200_fail(PAI_ERR_UNSUPPORTED, "beam_select: %llu beams, %llu picked (at most %u and %u)",
+                     (unsigned long long)beams, (unsigned long long)n_out, kMaxBeams, kMaxPick);
+  // flat indexes within a prompt and the grid's rows stay in 32 and 16 bits
+  if (vocab > 0x7FFFFFFFull / kMaxBeams || prompts > 65535 || prompts * beams > 65535)
+    return b200_fail(PAI_ERR_UNSUPPORTED, "beam_select: %llu prompts of %llu beams over %llu tokens",
+                     (unsigned long long)prompts, (unsigned long long)beams, (unsigned long long)vocab);
+  if ((uintptr_t)logits & 3) return b200_fail(PAI_ERR_INVALID_ARG, "beam_select: logits must be 4-byte aligned");
+  BeamParams p{};
+  p.logits = logits, p.scores = scores, p.done = done, p.stride = stride, p.pad = pad;
+  p.beams = (uint32_t)beams, p.vocab = (uint32_t)vocab, p.n_out = (uint32_t)n_out;
+  const uint64_t rows = prompts * beams;
+  p.slices = (uint32_t)((vocab + kSlice - 1) / kSlice);
+  p.per = kSlice;
+  p.out_scores = out_scores, p.out_parents = out_parents, p.out_tokens = out_tokens;
+  const CtxDeviceGuard on(ctx);
+  if (on.status()) return on.status();
+  const uint64_t slots = rows * p.slices;
+  float *scratch;
+  pai_status_t st = b200_ctx_scratch(ctx, slots * (2 + 2 * n_out), (uint32_t)prompts, &scratch, &p.cnt);
+  if (st) return st;
+  p.top = scratch;
+  p.sum = scratch + slots;
+  p.val = scratch + 2 * slots;
+  p.idx = (uint32_t *)(p.val + slots * n_out);
+  b200_launch(ctx, k_beam_select, dim3(p.slices, (uint32_t)rows), dim3(kThreads), 0, p);
+  return b200_launched(ctx, 1, "k_beam_select");
+}
