@@ -32,6 +32,7 @@
 namespace {
 
 constexpr uint32_t kTile = 64, kThreads = 128, kMaxSeqs = 1024;
+constexpr uint32_t kGrid = 296;  // two CTAs an SM
 constexpr int kStages = 3;
 constexpr float kPShift = 12.0f;
 
@@ -85,6 +86,13 @@ __device__ __forceinline__ void split_f16(float x, float y, uint32_t &hi, uint32
   lo = *reinterpret_cast<const uint32_t *>(&l);
 }
 
+// 2^x of the special function unit: 2^-22 relative, results below 2^-126 are 0
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Bits [at, at + 64) of a row of `words` 64-bit words; at may be negative.
 __device__ __forceinline__ uint64_t window(const uint64_t *m, uint32_t words, int32_t at) {
   const int32_t w = at >> 6, sh = at & 63;
@@ -118,6 +126,58 @@ struct Stage {
   __half v[kTile][HD + 8];
 };
 
+// Join the parts of a unit: CTAs c0 .. c0 + parts - 1, in order. First every row's maximum, weights 2^(m - max) and
+// sum, in shared memory `ws` [MR][parts]; then the outputs, 8 parts' loads in flight.
+template <int HD, uint32_t MR>
+__device__ __noinline__ void join_parts(const TreeParams &p, const SeqWork &w, uint32_t kvh, uint32_t block, uint64_t c0,
+                                        uint32_t parts, uint64_t unit0, uint64_t all, uint64_t grid, float *ws) {
+  const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const uint32_t rows = min(MR, w.nodes * p.g - block * MR);
+  // the unit is the first of a CTA's range, or the last; only CTA c0's range can begin before it
+  const bool late = c0 * all / grid < unit0;
+  auto slot = [&](uint32_t q) { return 2 * (c0 + q) + (q == 0 && late); };
+  float *inv = ws + MR * parts;
+  for (uint32_t r = warp; r < rows; r += kThreads / 32) {
+    float M = -INFINITY;
+    for (uint32_t q = lane; q < parts; q += 32) {
+      const float mq = __ldcg(&p.part_ml[(slot(q) * MR + r) * 2]);
+      ws[r * parts + q] = mq;
+      M = fmaxf(M, mq);
+    }
+    M = warp_max(M);
+    float L = 0.0f;
+    for (uint32_t q = lane; q < parts; q += 32) {
+      const float mq = ws[r * parts + q], e = mq == -INFINITY ? 0.0f : ex2(mq - M);
+      L += __ldcg(&p.part_ml[(slot(q) * MR + r) * 2 + 1]) * e;
+      ws[r * parts + q] = e;
+    }
+    L = warp_sum(L);
+    if (lane == 0) inv[r] = L != 0.0f ? 1.0f / L : 0.0f;
+  }
+  __syncthreads();
+  for (uint32_t e = t; e < rows * (HD / 4); e += kThreads) {
+    const uint32_t r = e / (HD / 4), d = (e % (HD / 4)) * 4;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t q0 = 0; q0 < parts; q0 += 8) {
+      float4 f[8];
+#pragma unroll
+      for (int u = 0; u < 8; u++)
+        if (q0 + u < parts) f[u] = __ldcg(reinterpret_cast<const float4 *>(p.part_o + (slot(q0 + u) * MR + r) * HD + d));
+#pragma unroll
+      for (int u = 0; u < 8; u++)
+        if (q0 + u < parts) {
+          const float y = ws[r * parts + q0 + u];
+          acc.x = fmaf(f[u].x, y, acc.x), acc.y = fmaf(f[u].y, y, acc.y);
+          acc.z = fmaf(f[u].z, y, acc.z), acc.w = fmaf(f[u].w, y, acc.w);
+        }
+    }
+    const uint32_t rr = block * MR + r;
+    const float y = inv[r];
+    *reinterpret_cast<float4 *>(p.out + ((size_t)(w.first + rr / p.g) * p.h + kvh * p.g + rr % p.g) * HD + d) =
+        make_float4(acc.x * y, acc.y * y, acc.z * y, acc.w * y);
+  }
+}
+
 // WM warps share a tile's rows (16 each), 4 / WM share its positions.
 template <int HD, int WM>
 __global__ void __launch_bounds__(kThreads, 2) k_attn_tree(TreeParams p) {
@@ -125,8 +185,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tree(TreeParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
   Stage<HD> *st = reinterpret_cast<Stage<HD> *>(smem);
   __shared__ uint64_t upto[kMaxSeqs + 1];
-  __shared__ uint64_t valid[kStages];    // positions of a stage's tile that hold a row
-  __shared__ uint64_t odd;               // its nodes with a non-finite V row
+  __shared__ int64_t where[4][kTile];             // element offsets of the rows of the next tiles, -1: none
+  __shared__ __align__(8) uint32_t valid[4][2];   // their positions that hold a row
+  __shared__ uint64_t odd;                        // nodes of a tile with a non-finite V row
   __shared__ uint32_t ticket;
   const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5, wm = warp % WM, wn = warp / WM;
   const uint32_t gq = lane >> 2, tq = lane & 3;
@@ -219,41 +280,49 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tree(TreeParams p) {
     for (int n = 0; n < HD / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 
-    auto load = [&](uint32_t tile, uint32_t slot) {
-      Stage<HD> &sg = st[slot];
-      uint32_t have = 0;  // rows of this thread's pass that exist
+    // Row offsets are looked up (page table, a division) one tile before the copies that use them, one row a
+    // thread; the copies of tile n + 2 are issued while tile n is multiplied.
+    auto find = [&](uint32_t tile) -> int64_t {
+      const uint32_t pos = tile * kTile + t;
+      return t < kTile && tile < tile1 && pos < total ? kv_row(p.c, s, pos) : -1;
+    };
+    auto note = [&](uint32_t n, int64_t at_row) {
+      if (t < kTile) {
+        where[n % 4][t] = at_row;
+        const uint32_t bits = __ballot_sync(0xffffffffu, at_row >= 0);
+        if (lane == 0) valid[n % 4][warp] = bits;
+      }
+    };
+    auto load = [&](uint32_t n) {
+      Stage<HD> &sg = st[n % kStages];
+      const int64_t *wh = where[n % 4];
 #pragma unroll
       for (uint32_t i = 0; i < kTile * CH / kThreads; i++) {
-        const uint32_t r = t / CH + i * (kThreads / CH), ch = t % CH, pos = tile * kTile + r;
-        const int64_t at_row = pos < total ? kv_row(p.c, s, pos) : -1;
+        const uint32_t r = t / CH + i * (kThreads / CH), ch = t % CH;
+        const int64_t at_row = wh[r];
         const bool ok = at_row >= 0;
         cp16(&sg.k[r][ch * 8], kp + (ok ? at_row : 0) + ch * 8, ok);
         cp16(&sg.v[r][ch * 8], vp + (ok ? at_row : 0) + ch * 8, ok);
-        have |= (ok ? 1u : 0u) << i;
-      }
-      cp_commit();
-      if (t % CH == 0) {
-        uint64_t bits = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < kTile * CH / kThreads; i++)
-          bits |= (uint64_t)((have >> i) & 1u) << (t / CH + i * (kThreads / CH));
-        atomicOr((unsigned long long *)&valid[slot], (unsigned long long)bits);
       }
     };
 
     __syncthreads();  // the stages are free
-    if (t < kStages) valid[t] = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 3; i++) note(i, find(tile0 + i));
     __syncthreads();
-    for (uint32_t i = 0; i < kStages - 1; i++) {
-      if (tile0 + i < tile1) load(tile0 + i, i); else cp_commit();
+    for (uint32_t i = 0; i < 2; i++) {
+      if (tile0 + i < tile1) load(i);
+      cp_commit();
     }
     for (uint32_t tile = tile0; tile < tile1; tile++) {
-      const uint32_t n = tile - tile0, slot = n % kStages;
+      const uint32_t n = tile - tile0;
       cp_wait<kStages - 2>();
-      __syncthreads();  // this tile has landed, and the last one's stage is free
-      if (t == 0) valid[(n + kStages - 1) % kStages] = 0;
+      __syncthreads();  // this tile has landed, the last one's stage is free, the offsets of tile n + 2 are there
+      if (tile + 2 < tile1) load(n + 2);
+      cp_commit();
+      const int64_t ahead = find(tile + 3);
       const bool drafted = (tile + 1) * kTile > w.len;  // the tile holds nodes
-      Stage<HD> &sg = st[slot];
+      Stage<HD> &sg = st[n % kStages];
       if (drafted) {
         // A non-finite V row may only reach the rows that see its node, and a weight of
         // 0 does not keep it out of a product: such elements become 0 here and are
@@ -271,10 +340,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tree(TreeParams p) {
           }
           if (bad) atomicOr((unsigned long long *)&odd, 1ull << (e / CH));
         }
+        __syncthreads();
       }
-      __syncthreads();
-      if (tile + kStages - 1 < tile1) load(tile + kStages - 1, (n + kStages - 1) % kStages); else cp_commit();
-      const uint64_t rows_ok = valid[slot];
+      const uint64_t rows_ok = *reinterpret_cast<const uint64_t *>(valid[n % 4]);
+      const bool masked = drafted || rows_ok != ~0ull;
       uint64_t sees[2] = {rows_ok, rows_ok};
       if (drafted) {
         const int32_t base = (int32_t)(tile * kTile - w.len);  // node of the tile's first position
@@ -310,8 +379,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tree(TreeParams p) {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           const int x = e >> 1;
-          const uint32_t j = (wn * NT + nt) * 8 + 2 * tq + (e & 1);
-          sc[nt][e] = (sees[x] >> j) & 1 ? sc[nt][e] * factor[x] : -INFINITY;
+          sc[nt][e] *= factor[x];
+          if (masked) {
+            const uint32_t j = (wn * NT + nt) * 8 + 2 * tq + (e & 1);
+            if (!((sees[x] >> j) & 1)) sc[nt][e] = -INFINITY;
+          }
           mt[x] = fmaxf(mt[x], sc[nt][e]);
         }
       float corr[2], sub[2];
@@ -320,43 +392,45 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tree(TreeParams p) {
         mt[x] = fmaxf(mt[x], __shfl_xor_sync(0xffffffffu, mt[x], 1));
         mt[x] = fmaxf(mt[x], __shfl_xor_sync(0xffffffffu, mt[x], 2));
         const float mn = fmaxf(m[x], mt[x]);
-        corr[x] = m[x] == mn ? 1.0f : exp2f(m[x] - mn);
+        corr[x] = m[x] == mn ? 1.0f : ex2(m[x] - mn);
         m[x] = mn;
         sub[x] = mn == -INFINITY ? 0.0f : mn - kPShift;
         l[x] *= corr[x];
       }
-      if (__any_sync(0xffffffffu, corr[0] != 1.0f || corr[1] != 1.0f)) {
+      // weights as A fragments
+      uint32_t ph[NT / 2][4], pl[NT / 2][4];
 #pragma unroll
-        for (int n2 = 0; n2 < HD / 8; n2++) {
-          o[n2][0] *= corr[0];
-          o[n2][1] *= corr[0];
-          o[n2][2] *= corr[1];
-          o[n2][3] *= corr[1];
-        }
-      }
-      // weights as A fragments; O += P V
-#pragma unroll
-      for (uint32_t ks = 0; ks < NT / 2; ks++) {
-        uint32_t ph[4], pl[4];
+      for (uint32_t ks = 0; ks < NT / 2; ks++)
 #pragma unroll
         for (int y = 0; y < 2; y++) {
           float pv[4];
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            pv[e] = exp2f(sc[2 * ks + y][e] - sub[e >> 1]);
+            pv[e] = ex2(sc[2 * ks + y][e] - sub[e >> 1]);
             l[e >> 1] += pv[e];
           }
-          split_f16(pv[0], pv[1], ph[2 * y], pl[2 * y]);
-          split_f16(pv[2], pv[3], ph[2 * y + 1], pl[2 * y + 1]);
+          split_f16(pv[0], pv[1], ph[ks][2 * y], pl[ks][2 * y]);
+          split_f16(pv[2], pv[3], ph[ks][2 * y + 1], pl[ks][2 * y + 1]);
         }
+      // O = O corr + P V. The tensor cores cut off what an accumulator cannot hold, always towards zero: over
+      // thousands of tiles that adds up (5e-5 of the output at 32768 positions). So they sum one tile, from
+      // zero, and the tiles are added by rounding additions (2e-7).
 #pragma unroll
-        for (int n2 = 0; n2 < HD / 16; n2++) {
+      for (int n2 = 0; n2 < HD / 16; n2++) {
+        float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (uint32_t ks = 0; ks < NT / 2; ks++) {
           uint32_t b[4];
           ldsm4t(b, &sg.v[wn * (NT * 8) + 16 * ks + (lane & 15)][16 * n2 + 8 * (lane >> 4)]);
-          mma_f16(o[2 * n2], ph, b[0], b[1]);
-          mma_f16(o[2 * n2], pl, b[0], b[1]);
-          mma_f16(o[2 * n2 + 1], ph, b[2], b[3]);
-          mma_f16(o[2 * n2 + 1], pl, b[2], b[3]);
+          mma_f16(d0, ph[ks], b[0], b[1]);
+          mma_f16(d1, ph[ks], b[2], b[3]);
+          mma_f16(d0, pl[ks], b[0], b[1]);
+          mma_f16(d1, pl[ks], b[2], b[3]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          o[2 * n2][e] = fmaf(o[2 * n2][e], corr[e >> 1], d0[e]);
+          o[2 * n2 + 1][e] = fmaf(o[2 * n2 + 1][e], corr[e >> 1], d1[e]);
         }
       }
       if (drafted && odd) {
@@ -376,6 +450,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tree(TreeParams p) {
           }
         }
       }
+      note(n + 3, ahead);
     }
     cp_wait<0>();
     // row sums: each of a row's 4 threads holds a part
@@ -413,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tree(TreeParams p) {
       float L = 0.0f;
 #pragma unroll
       for (uint32_t y = 0; y < WN; y++) {
-        const float my = sm[(y * MR + r) * 2], wy = my == -INFINITY ? 0.0f : exp2f(my - M);
+        const float my = sm[(y * MR + r) * 2], wy = my == -INFINITY ? 0.0f : ex2(my - M);
         if (my == -INFINITY) continue;
         const float4 f = *reinterpret_cast<const float4 *>(so + (y * MR + r) * OS + d);
         acc.x = fmaf(f.x, wy, acc.x), acc.y = fmaf(f.y, wy, acc.y);
@@ -446,28 +521,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tree(TreeParams p) {
       if (ticket == (uint32_t)(c1 - c0)) {
         __threadfence();
         if (t == 0) *cnt = 0;
-        for (uint32_t e = t; e < MR * (HD / 4); e += kThreads) {
-          const uint32_t r = e / (HD / 4), d = (e % (HD / 4)) * 4;
-          const uint32_t rr = block * MR + r, nd = rr / p.g;
-          if (nd >= w.nodes) continue;
-          float M = -INFINITY, L = 0.0f;
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (uint64_t q = c0; q <= c1; q++) {
-            // the unit is the first of CTA q's range, or the last
-            const uint64_t sl = 2 * q + (q * all / grid >= unit0 ? 0 : 1);
-            const float mq = __ldcg(&p.part_ml[(sl * MR + r) * 2]), lq = __ldcg(&p.part_ml[(sl * MR + r) * 2 + 1]);
-            const float4 f = __ldcg(reinterpret_cast<const float4 *>(p.part_o + (sl * MR + r) * HD + d));
-            if (mq == -INFINITY) continue;
-            const float M2 = fmaxf(M, mq), a = M == -INFINITY ? 0.0f : exp2f(M - M2), b = exp2f(mq - M2);
-            acc.x = acc.x * a + f.x * b, acc.y = acc.y * a + f.y * b;
-            acc.z = acc.z * a + f.z * b, acc.w = acc.w * a + f.w * b;
-            L = L * a + lq * b;
-            M = M2;
-          }
-          const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-          *reinterpret_cast<float4 *>(p.out + ((size_t)(w.first + nd) * p.h + kvh * p.g + rr % p.g) * HD + d) =
-              make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-        }
+        join_parts<HD, MR>(p, w, kvh, block, c0, (uint32_t)(c1 - c0 + 1), unit0, all, grid, reinterpret_cast<float *>(smem));
       }
     }
     at = unit0 + tile1;
@@ -478,7 +532,8 @@ template <int HD, int WM>
 pai_status_t launch_tree(pai_b200_ctx_t *ctx, TreeParams &p) {
   constexpr uint32_t MR = 16 * WM, WN = 4 / WM;
   constexpr size_t stages = kStages * sizeof(Stage<HD>), join = WN * MR * (HD + 4 + 2) * sizeof(float);
-  constexpr size_t smem = stages > join ? stages : join;
+  constexpr size_t weights = MR * (kGrid + 1) * sizeof(float);  // of the parts of one unit
+  constexpr size_t smem = std::max(stages, std::max(join, weights));
   static SmemOptIn opt;
   pai_status_t st = b200_cuda(opt.ensure(b200_ctx_device(ctx), smem,
                                          [](size_t b) {
@@ -492,7 +547,7 @@ pai_status_t launch_tree(pai_b200_ctx_t *ctx, TreeParams &p) {
   if (units > 0x7FFFFFFu) return b200_fail(PAI_ERR_UNSUPPORTED, "attn_tree: %llu row tiles", (unsigned long long)units);
   // two CTAs an SM, and no more than there can be pairs
   const uint64_t pairs = units * (((uint64_t)p.c.max_pages * p.c.page_tokens + p.max_nodes + kTile - 1) / kTile);
-  const uint32_t grid = (uint32_t)std::min<uint64_t>(296, pairs);
+  const uint32_t grid = (uint32_t)std::min<uint64_t>(kGrid, pairs);
   float *scratch;
   st = b200_ctx_scratch(ctx, 2ull * grid * MR * (HD + 2), (uint32_t)units, &scratch, &p.cnt);
   if (st) return st;
