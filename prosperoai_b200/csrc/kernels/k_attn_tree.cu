@@ -47,6 +47,9 @@ struct TreeParams {
   float *part_o;   // scratch [2 gridDim.x][MR][hd]
   float *part_ml;  // scratch [2 gridDim.x][MR][2]
   uint32_t *cnt;   // counters [n_seq][kv head][row tile], left at zero
+  uint32_t *units; // scratch [n_seq][kv head][row tile][2]: parts of a unit, slot of the first
+  uint32_t *err;
+  uint64_t wait_ns;
   float scale;     // log2(e) / sqrt(hd)
 };
 
@@ -109,14 +112,50 @@ __device__ __forceinline__ uint64_t low_bits(int64_t n) {
 struct SeqWork {
   uint32_t len, nodes, first, blocks, tiles;
 };
-template <uint32_t MR>
+template <uint32_t MR, uint32_t KT>
 __device__ __forceinline__ SeqWork seq_work(const TreeParams &p, uint32_t s) {
   SeqWork w;
   w.nodes = kv_nodes(p.off, s, p.rows, p.max_nodes, &w.first);
   w.len = kv_len(p.c, p.lens, s);
   w.blocks = (w.nodes * p.g + MR - 1) / MR;
-  w.tiles = (w.len + w.nodes + kTile - 1) / kTile;
+  w.tiles = (w.len + w.nodes + KT - 1) / KT;
   return w;
+}
+
+// upto[s]: (unit, tile) pairs of the sequences before s. Every thread of the block calls it; a barrier must follow.
+template <uint32_t MR, uint32_t KT, uint32_t THREADS>
+__device__ __forceinline__ void pairs_before(const TreeParams &p, uint64_t *upto) {
+  const uint32_t n_seq = p.c.n_seq, lane = threadIdx.x & 31;
+  for (uint32_t s = threadIdx.x; s < n_seq; s += THREADS) {
+    const SeqWork w = seq_work<MR, KT>(p, s);
+    upto[s + 1] = (uint64_t)w.blocks * w.tiles * p.c.hk;
+  }
+  if (threadIdx.x == 0) upto[0] = 0;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    uint64_t sum = 0;
+    for (uint32_t s0 = 0; s0 < n_seq; s0 += 32) {
+      const uint32_t s = s0 + lane;
+      uint64_t x = s < n_seq ? upto[s + 1] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= (uint32_t)o) x += y;
+      }
+      x += sum;
+      if (s < n_seq) upto[s + 1] = x;
+      sum = __shfl_sync(0xffffffffu, x, 31);
+    }
+  }
+}
+
+// 2^-e (down) that brings a row's largest element `top` into [1, 2), and 2^e; 1 for a row of zeros, subnormals or
+// infinities.
+__device__ __forceinline__ void row_scale(float top, float &down, float &up) {
+  const uint32_t ex = __float_as_uint(top) >> 23;
+  const bool turn = ex >= 1 && ex <= 252;
+  down = turn ? __uint_as_float((254 - ex) << 23) : 1.0f;
+  up = turn ? __uint_as_float(ex << 23) : 1.0f;
 }
 
 // Shared memory of a stage: K then V rows, padded so that the eight rows of an ldmatrix lie in different banks.
@@ -195,28 +234,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tree(TreeParams p) {
   pdl_trigger();
   pdl_wait();
 
-  // pairs before each sequence
-  for (uint32_t s = t; s < n_seq; s += kThreads) {
-    const SeqWork w = seq_work<MR>(p, s);
-    upto[s + 1] = (uint64_t)w.blocks * w.tiles * hk;
-  }
-  if (t == 0) upto[0] = 0;
-  __syncthreads();
-  if (warp == 0) {
-    uint64_t sum = 0;
-    for (uint32_t s0 = 0; s0 < n_seq; s0 += 32) {
-      const uint32_t s = s0 + lane;
-      uint64_t x = s < n_seq ? upto[s + 1] : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= (uint32_t)o) x += y;
-      }
-      x += sum;
-      if (s < n_seq) upto[s + 1] = x;
-      sum = __shfl_sync(0xffffffffu, x, 31);
-    }
-  }
+  pairs_before<MR, kTile, kThreads>(p, upto);
   __syncthreads();
   const uint64_t all = upto[n_seq], cta = blockIdx.x, grid = gridDim.x < all ? gridDim.x : all;
   if (cta >= grid) return;  // every CTA of the cut has at least one pair
@@ -231,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tree(TreeParams p) {
 
   while (at < end) {
     while (upto[s + 1] <= at) s++;
-    const SeqWork w = seq_work<MR>(p, s);
+    const SeqWork w = seq_work<MR, kTile>(p, s);
     const uint64_t unit = (at - upto[s]) / w.tiles, unit0 = upto[s] + unit * w.tiles, unit1 = unit0 + w.tiles;
     const uint32_t kvh = (uint32_t)(unit / w.blocks), block = (uint32_t)(unit % w.blocks);
     const uint32_t tile0 = (uint32_t)(at - unit0), tile1 = (uint32_t)((end < unit1 ? end : unit1) - unit0);
@@ -261,11 +279,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tree(TreeParams p) {
         }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // 2^-e brings the row's largest element into [1, 2); a row of zeros, subnormals or infinities stays
-      const uint32_t ex = __float_as_uint(top) >> 23;
-      const bool turn = ex >= 1 && ex <= 252;
-      const float down = turn ? __uint_as_float((254 - ex) << 23) : 1.0f;
-      factor[x] = p.scale * (turn ? __uint_as_float(ex << 23) : 1.0f);
+      float down, up;
+      row_scale(top, down, up);
+      factor[x] = p.scale * up;
 #pragma unroll
       for (int k = 0; k < HD / 16; k++)
 #pragma unroll
@@ -528,6 +544,585 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tree(TreeParams p) {
   }
 }
 
+// ---- more than 32 rows: tcgen05 --------------------------------------------------------------
+//
+// The same sums for row tiles of 128 on the fifth-generation tensor cores, one CTA an SM. Key tiles of 128
+// positions; S = Q K^T and the tile's P V go to TMEM, with K, V and Q (both fp16 parts) in shared memory in the
+// 128-byte swizzle and P (both parts) written over S. P V reads V as it lies, hd contiguous (an MN-major B).
+//   warps 0-3, 4-7   softmax of every other key tile, a row a thread: maximum, weights, and the tile's P V added
+//                    to its running output in registers; the two halves join when the unit ends
+//   warp 8           issues the MMAs: Q K^T of tile i + 1 before P V of tile i, so that they overlap the softmax
+//   warps 12-13      copy K tiles, 14-15 V tiles (16 bytes a copy: pages may be of any size), and look up the pages
+// Registers: 512 threads at 128; setmaxnreg gives the softmax warps 200 and leaves 56 to the others (256 * 200 +
+// 256 * 56 = 65536, what the block was launched with).
+constexpr uint32_t kTcThreads = 512, kTcRows = 128, kTcTile = 128, kTcGrid = 148;
+
+__device__ __forceinline__ uint64_t desc_k(uint32_t saddr) {  // K-major, 128-byte swizzle, 8-row groups of 1024 bytes
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)1u << 16 | (uint64_t)(1024u >> 4) << 32 | (uint64_t)1u << 46 |
+         (uint64_t)2u << 61;
+}
+__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t block) {
+  // MN-major: 64-element blocks of the contiguous dimension `block` bytes apart, 8-row groups of 1024 bytes
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)(block >> 4) << 16 | (uint64_t)(1024u >> 4) << 32 |
+         (uint64_t)1u << 46 | (uint64_t)2u << 61;
+}
+// kind::f16: fp16 A and B, fp32 sums, M = 128, N = n; b_mn: B is MN-major
+__host__ __device__ constexpr uint32_t idesc_f16(uint32_t n, bool b_mn) {
+  return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint64_t *bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_ld32(uint32_t at, float (&v)[32]) {
+  uint32_t *r = reinterpret_cast<uint32_t *>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(at));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tc_st32(uint32_t at, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(at)
+      : "memory");
+}
+template <int ID, int N>
+__device__ __forceinline__ void named_sync() {
+  asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory");
+}
+
+// One CTA's run over the (unit, tile) pairs: the part of each unit that lies in it, in order.
+struct Segment {
+  SeqWork w;
+  uint64_t unit0;
+  uint32_t s, kvh, block, tile0, tile1;
+  __device__ __forceinline__ bool whole() const { return tile0 == 0 && tile1 == w.tiles; }
+};
+struct Walk {
+  uint64_t at, end;
+  uint32_t s;
+};
+template <uint32_t MR, uint32_t KT>
+__device__ __forceinline__ bool next_segment(const TreeParams &p, const uint64_t *upto, Walk &k, Segment &g) {
+  if (k.at >= k.end) return false;
+  while (upto[k.s + 1] <= k.at) k.s++;
+  g.s = k.s;
+  g.w = seq_work<MR, KT>(p, k.s);
+  const uint64_t unit = (k.at - upto[k.s]) / g.w.tiles;
+  g.unit0 = upto[k.s] + unit * g.w.tiles;
+  g.kvh = (uint32_t)(unit / g.w.blocks), g.block = (uint32_t)(unit % g.w.blocks);
+  const uint64_t unit1 = g.unit0 + g.w.tiles;
+  g.tile0 = (uint32_t)(k.at - g.unit0), g.tile1 = (uint32_t)((k.end < unit1 ? k.end : unit1) - g.unit0);
+  k.at = g.unit0 + g.tile1;
+  return true;
+}
+
+template <int HD>
+struct TcSmem {
+  static constexpr uint32_t kBlock = 128 * 128;             // 128 rows of 64 dims: 16 KB
+  static constexpr uint32_t kTileBytes = HD / 64 * kBlock;  // a K or V tile, or one part of Q
+  uint8_t q[2][kTileBytes];
+  uint8_t kt[2][kTileBytes];
+  uint8_t vt[2][kTileBytes];
+  int64_t where[2][2][kTcTile];  // [K, V copiers][tile parity]
+  uint32_t valid[8][4];          // positions of a tile that hold a row; a tile's words are read long before 8 tiles on
+  uint32_t odd[8][4];            // its nodes with a non-finite V row
+  float factor[kTcRows];
+  float ml[2][kTcRows][2];
+  uint64_t upto[kMaxSeqs + 1];
+  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], ofull[2], qfull, drain;
+  uint32_t tmem;
+};
+
+template <int HD>
+__global__ void __launch_bounds__(kTcThreads, 1) k_attn_tree_tc(TreeParams p) {
+  using Smem = TcSmem<HD>;
+  extern __shared__ __align__(16) uint8_t raw[];
+  Smem &sm = *reinterpret_cast<Smem *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  constexpr uint32_t CH = HD / 8, BL = Smem::kBlock;
+  const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  pdl_trigger();
+  if (t == 0) {
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&sm.kfull[i], 64);
+      mbar_init(&sm.vfull[i], 64);
+      mbar_init(&sm.kempty[i], 1);
+      mbar_init(&sm.vempty[i], 1);
+      mbar_init(&sm.sfull[i], 1);
+      mbar_init(&sm.pfull[i], 4);
+      mbar_init(&sm.ofull[i], 1);
+    }
+    mbar_init(&sm.qfull, 8);
+    mbar_init(&sm.drain, 1);
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  pdl_wait();
+  pairs_before<kTcRows, kTcTile, kTcThreads>(p, sm.upto);
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = sm.tmem;
+  const uint64_t all = sm.upto[p.c.n_seq], cta = blockIdx.x, grid = gridDim.x < all ? gridDim.x : all;
+  Walk walk;
+  walk.at = cta < grid ? cta * all / grid : 0;
+  walk.end = cta < grid ? (cta + 1) * all / grid : 0;
+  walk.s = 0;
+  const uint64_t begin = walk.at;
+  Segment g;
+  bool ok = true;
+  // after a wait has run out a role goes on without waiting or copying, so that the barriers among its own threads
+  // still meet; the error word tells the host
+  auto wait = [&](uint64_t *bar, uint32_t parity) {
+    if (ok && !mbar_wait(bar, parity & 1u, p.wait_ns)) {
+      ok = false;
+      atomicExch(p.err, 1u);
+    }
+  };
+
+  if (warp >= 12) {
+    // ---- copiers: 64 threads for K, 64 for V ----
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    const bool is_v = warp >= 14;
+    const uint32_t e = t - (is_v ? 448 : 384), ch = e % CH, r0 = e / CH;
+    uint64_t *full = is_v ? sm.vfull : sm.kfull, *empty = is_v ? sm.vempty : sm.kempty;
+    uint32_t i = 0;  // tiles of the run so far
+    uint32_t held = 0, held_len = 0;  // the tile before, not yet handed over: its first position, committed positions
+    bool holding = false;
+    auto hand_over = [&](uint32_t n) {
+      // tile n has landed (this thread's copies)
+      if (is_v && held + kTcTile > held_len) {
+        // it holds nodes: non-finite elements become 0 and are added by the softmax warps to the rows that see them
+        for (uint32_t r = r0; r < kTcTile; r += 64 / CH) {
+          uint4 *c4 = reinterpret_cast<uint4 *>(sm.vt[n & 1] + (ch / 8) * BL + r * 128 + (((ch % 8) ^ (r & 7)) << 4));
+          uint4 v = *c4;
+          uint32_t *cw = reinterpret_cast<uint32_t *>(&v);
+          bool bad = false;
+#pragma unroll
+          for (int x = 0; x < 4; x++) {
+            if ((cw[x] & 0x7C00u) == 0x7C00u) cw[x] &= 0xFFFF0000u, bad = true;
+            if ((cw[x] & 0x7C000000u) == 0x7C000000u) cw[x] &= 0xFFFFu, bad = true;
+          }
+          if (bad) {
+            *c4 = v;
+            atomicOr(&sm.odd[n & 7][r / 32], 1u << (r % 32));
+          }
+        }
+      }
+      fence_proxy_async();
+      mbar_arrive(&full[n & 1]);
+    };
+    while (next_segment<kTcRows, kTcTile>(p, sm.upto, walk, g)) {
+      const uint32_t total = g.w.len + g.w.nodes;
+      const __half *src = (is_v ? p.c.v : p.c.k) + (size_t)g.kvh * p.c.head_stride;
+      for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
+        int64_t *wh = sm.where[is_v][i & 1];
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+          const uint32_t r = e + 64 * x, pos = tile * kTcTile + r;
+          const int64_t at_row = pos < total ? kv_row(p.c, g.s, pos) : -1;
+          wh[r] = at_row;
+          const uint32_t bits = __ballot_sync(0xffffffffu, at_row >= 0);
+          if (lane == 0) {
+            if (is_v) sm.odd[i & 7][r / 32] = 0; else sm.valid[i & 7][r / 32] = bits;
+          }
+        }
+        if (is_v) named_sync<3, 64>(); else named_sync<2, 64>();
+        if (i >= 2) wait(&empty[i & 1], (i >> 1) - 1);
+        if (ok) {
+          uint8_t *dst = (is_v ? sm.vt : sm.kt)[i & 1] + (ch / 8) * BL;
+#pragma unroll 8
+          for (uint32_t r = r0; r < kTcTile; r += 64 / CH) {
+            const int64_t at_row = wh[r];
+            const bool there = at_row >= 0;
+            cp16(dst + r * 128 + (((ch % 8) ^ (r & 7)) << 4), src + (there ? at_row : 0) + ch * 8, there);
+          }
+        }
+        cp_commit();
+        if (holding) {
+          cp_wait<1>();
+          hand_over(i - 1);
+        }
+        holding = true, held = tile * kTcTile, held_len = g.w.len;
+      }
+    }
+    cp_wait<0>();
+    if (holding) hand_over(i - 1);
+  } else if (warp >= 8) {
+    // ---- MMA issue ----
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 8 && lane == 0) {
+      const uint32_t q0 = smem_u32(sm.q[0]), q1 = smem_u32(sm.q[1]);
+      uint32_t i = 0, seg = 0;
+      auto scores = [&](uint32_t n) {  // S = Q K^T of tile n: both parts of Q
+        wait(&sm.kfull[n & 1], n >> 1);
+        tc_after();
+        if (!ok) return;
+        const uint32_t kb = smem_u32(sm.kt[n & 1]), d = tmem + 128 * (n & 1);
+#pragma unroll
+        for (uint32_t k = 0; k < HD / 16; k++) {
+          const uint32_t off = (k / 4) * BL + (k % 4) * 32;
+          tc_mma_ss(d, desc_k(q0 + off), desc_k(kb + off), idesc_f16(kTcTile, false), k > 0);
+          tc_mma_ss(d, desc_k(q1 + off), desc_k(kb + off), idesc_f16(kTcTile, false), true);
+        }
+        tc_commit(&sm.sfull[n & 1]);
+        tc_commit(&sm.kempty[n & 1]);
+      };
+      while (next_segment<kTcRows, kTcTile>(p, sm.upto, walk, g)) {
+        wait(&sm.qfull, seg++);
+        const uint32_t n = g.tile1 - g.tile0;
+        scores(i);
+        for (uint32_t j = 0; j < n; j++, i++) {
+          if (j + 1 < n) scores(i + 1);
+          wait(&sm.pfull[i & 1], i >> 1);
+          wait(&sm.vfull[i & 1], i >> 1);
+          tc_after();
+          if (ok) {  // this tile's P V, from zero: the sum over tiles is made in registers, where it is rounded
+            const uint32_t vb = smem_u32(sm.vt[i & 1]), a = tmem + 128 * (i & 1), d = tmem + 256 + 128 * (i & 1);
+#pragma unroll
+            for (uint32_t k = 0; k < kTcTile / 16; k++) {
+              const uint64_t b = desc_mn(vb + k * 2048, BL);
+              const uint32_t at = a + 32 * (k / 2) + 8 * (k % 2);
+              tc_mma_ts(d, at, b, idesc_f16(HD, true), k > 0);
+              tc_mma_ts(d, at + 16, b, idesc_f16(HD, true), true);
+            }
+            tc_commit(&sm.ofull[i & 1]);
+            tc_commit(&sm.vempty[i & 1]);
+          }
+        }
+      }
+      // the MMAs in flight end before TMEM is given back
+      tc_commit(&sm.drain);
+      ok = true;
+      wait(&sm.drain, 0);
+    }
+    __syncwarp();
+  } else {
+    // ---- softmax: warpgroup wg has every other tile, a thread a row ----
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    const uint32_t wg = warp >> 2, r = t & 127;
+    const uint32_t lanes = (warp & 3) * 32 << 16;
+    uint32_t i = 0;
+    while (next_segment<kTcRows, kTcTile>(p, sm.upto, walk, g)) {
+      const uint32_t rows = min(kTcRows, g.w.nodes * p.g - g.block * kTcRows);
+      // Q into shared memory, a power of two and two fp16 parts a row; the last segment's products are done
+      {
+        constexpr uint32_t LR = HD / 4, RW = 32 / LR;  // lanes of a row, rows of a warp's access
+        const uint32_t d4 = lane % LR;
+        for (uint32_t b0 = 0; b0 < 16; b0 += 4 * RW) {
+          float4 f[4];
+#pragma unroll
+          for (uint32_t u = 0; u < 4; u++) {
+            const uint32_t rl = warp * 16 + b0 + u * RW + lane / LR, rr = g.block * kTcRows + rl, nd = rr / p.g;
+            f[u] = rl < rows ? *reinterpret_cast<const float4 *>(
+                                   p.q + ((size_t)(g.w.first + nd) * p.h + g.kvh * p.g + rr % p.g) * HD + 4 * d4)
+                             : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+#pragma unroll
+          for (uint32_t u = 0; u < 4; u++) {
+            const uint32_t rl = warp * 16 + b0 + u * RW + lane / LR;
+            float top = fmaxf(fmaxf(fabsf(f[u].x), fabsf(f[u].y)), fmaxf(fabsf(f[u].z), fabsf(f[u].w)));
+#pragma unroll
+            for (uint32_t o = LR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            float down, up;
+            row_scale(top, down, up);
+            uint2 hi, lo;
+            split_f16(f[u].x * down, f[u].y * down, hi.x, lo.x);
+            split_f16(f[u].z * down, f[u].w * down, hi.y, lo.y);
+            const uint32_t at = (d4 / 16) * BL + rl * 128 + (((d4 % 16) / 2 ^ (rl & 7)) << 4) + (d4 & 1) * 8;
+            *reinterpret_cast<uint2 *>(sm.q[0] + at) = hi;
+            *reinterpret_cast<uint2 *>(sm.q[1] + at) = lo;
+            if (d4 == 0) sm.factor[rl] = p.scale * up;
+          }
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.qfull);
+        named_sync<1, 256>();
+      }
+      const float factor = sm.factor[r];
+      const bool work = (warp & 3) * 32 < rows;  // a warp whose rows are all past the last one keeps step only
+      const uint32_t rr = g.block * kTcRows + r, nd = rr / p.g;
+      const bool live = r < rows;
+      float o[HD], m = -INFINITY, l = 0.0f;
+#pragma unroll
+      for (int d = 0; d < HD; d++) o[d] = 0.0f;
+      for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
+        if ((i & 1) != wg) continue;
+        const uint32_t sa = tmem + lanes + 128 * wg, oa = tmem + lanes + 256 + 128 * wg;
+        wait(&sm.sfull[wg], i >> 1);
+        __syncwarp();
+        tc_after();
+        float corr = 1.0f;
+        uint64_t sees[2];
+        bool masked = false;
+        if (work) {
+          const bool drafted = (tile + 1) * kTcTile > g.w.len;
+#pragma unroll
+          for (int x = 0; x < 2; x++)
+            sees[x] = (uint64_t)sm.valid[i & 7][2 * x] | (uint64_t)sm.valid[i & 7][2 * x + 1] << 32;
+          masked = drafted || (sees[0] & sees[1]) != ~0ull;
+          if (drafted) {
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+              const int32_t base = (int32_t)(tile * kTcTile + 64 * x - g.w.len);
+              uint64_t b = low_bits(-(int64_t)base);
+              if (live)
+                b |= p.mask ? window(p.mask + (size_t)(g.w.first + nd) * p.words, p.words, base) & ~low_bits(-(int64_t)base)
+                            : low_bits((int64_t)nd + 1 - base);
+              sees[x] &= b;
+            }
+          }
+          float top = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            float v[32];
+            tc_ld32(sa + 32 * c, v);
+            if (masked) {
+              const uint32_t bits = (uint32_t)(sees[c / 2] >> (32 * (c & 1)));
+#pragma unroll
+              for (int e = 0; e < 32; e++)
+                if (!((bits >> e) & 1)) v[e] = -INFINITY;
+            }
+#pragma unroll
+            for (int e = 0; e < 32; e++) top = fmaxf(top, v[e]);
+          }
+          const float mn = fmaxf(m, top * factor);
+          corr = m == mn ? 1.0f : ex2(m - mn);
+          m = mn;
+          const float sub = mn == -INFINITY ? 0.0f : mn - kPShift;
+          l *= corr;
+          float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            float v[32];
+            tc_ld32(sa + 32 * c, v);
+            if (masked) {
+              const uint32_t bits = (uint32_t)(sees[c / 2] >> (32 * (c & 1)));
+#pragma unroll
+              for (int e = 0; e < 32; e++)
+                if (!((bits >> e) & 1)) v[e] = -INFINITY;
+            }
+            uint32_t w[32];  // 16 words of parts, 16 of remainders
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float p0 = ex2(fmaf(v[e], factor, -sub)), p1 = ex2(fmaf(v[e + 1], factor, -sub));
+              part[(e / 2) & 3] += p0 + p1;
+              split_f16(p0, p1, w[e / 2], w[16 + e / 2]);
+            }
+            tc_st32(sa + 32 * c, w);
+          }
+          l += (part[0] + part[1]) + (part[2] + part[3]);
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        }
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.pfull[wg]);
+        wait(&sm.ofull[wg], i >> 1);
+        __syncwarp();
+        tc_after();
+        if (work) {
+#pragma unroll
+          for (int c = 0; c < HD / 32; c++) {
+            float v[32];
+            tc_ld32(oa + 32 * c, v);
+#pragma unroll
+            for (int e = 0; e < 32; e++) o[32 * c + e] = fmaf(o[32 * c + e], corr, v[e]);
+          }
+          if (masked) {
+            // non-finite V elements of nodes that this row sees
+#pragma unroll 1
+            for (int x = 0; x < 4; x++)
+#pragma unroll 1
+              for (uint32_t left = sm.odd[i & 7][x] & (uint32_t)(sees[x / 2] >> (32 * (x & 1))); left; left &= left - 1) {
+                const int64_t at_row = kv_row(p.c, g.s, tile * kTcTile + 32 * x + __ffs(left) - 1);
+                const __half2 *vr = reinterpret_cast<const __half2 *>(p.c.v + (size_t)g.kvh * p.c.head_stride + at_row);
+#pragma unroll
+                for (int d = 0; d < HD / 2; d++) {
+                  const float2 f = __half22float2(vr[d]);
+                  if (!isfinite(f.x)) o[2 * d] += f.x;
+                  if (!isfinite(f.y)) o[2 * d + 1] += f.y;
+                }
+              }
+          }
+        }
+        __syncwarp();
+        tc_before();
+      }
+      // join the two warpgroups' halves of the tiles: each gives the other half of the dims, over Q
+      named_sync<1, 256>();
+      float *give = reinterpret_cast<float *>(wg ? sm.q[0] : sm.q[1]);        // [HD / 2][128]
+      const float *take = reinterpret_cast<const float *>(wg ? sm.q[1] : sm.q[0]);
+      sm.ml[wg][r][0] = m;
+      sm.ml[wg][r][1] = l;
+      // wg 0 keeps dims 0 .. HD/2 - 1, wg 1 the others
+      if (wg) {
+#pragma unroll
+        for (int d = 0; d < HD / 2; d++) give[d * 128 + r] = o[d];
+      } else {
+#pragma unroll
+        for (int d = 0; d < HD / 2; d++) give[d * 128 + r] = o[HD / 2 + d];
+      }
+      named_sync<1, 256>();
+      const float m2 = sm.ml[1 - wg][r][0], M = fmaxf(m, m2);
+      const float w1 = m == -INFINITY ? 0.0f : ex2(m - M), w2 = m2 == -INFINITY ? 0.0f : ex2(m2 - M);
+      const float L = wg ? sm.ml[0][r][1] * w2 + l * w1 : l * w1 + sm.ml[1][r][1] * w2;
+      const bool whole = g.whole();
+      const uint64_t slot = 2 * cta + (begin >= g.unit0 ? 0 : 1);
+      const float scale = whole ? (L != 0.0f ? 1.0f / L : 0.0f) : 1.0f;
+      // whole units go to their rows of out; parts lie [hd / 4][row] float4
+      float *dst = whole ? p.out + ((size_t)(g.w.first + (live ? nd : 0)) * p.h + g.kvh * p.g + rr % p.g) * HD + wg * (HD / 2)
+                         : p.part_o + ((slot * (HD / 4) + wg * (HD / 8)) * kTcRows + r) * 4;
+      const uint32_t step = whole ? 4 : 4 * kTcRows;
+      if (live) {
+#pragma unroll
+        for (int d = 0; d < HD / 2; d += 4) {
+          float f[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float mine = wg ? o[HD / 2 + d + e] : o[d + e];
+            f[e] = ((m == -INFINITY ? 0.0f : mine * w1) + (m2 == -INFINITY ? 0.0f : take[(d + e) * 128 + r] * w2)) * scale;
+          }
+          *reinterpret_cast<float4 *>(dst + (size_t)(d / 4) * step) = make_float4(f[0], f[1], f[2], f[3]);
+        }
+        if (!whole && wg == 0) {
+          p.part_ml[(slot * kTcRows + r) * 2] = M;
+          p.part_ml[(slot * kTcRows + r) * 2 + 1] = L;
+        }
+      }
+      if (g.tile0 == 0 && t == 0) {
+        // for the joining kernel: which CTAs hold parts of the unit (0 parts: none, it is whole)
+        const uint64_t c0 = ((g.unit0 + 1) * grid - 1) / all, c1 = ((g.unit0 + g.w.tiles) * grid - 1) / all;
+        uint32_t *u = p.units + 2 * (((size_t)g.s * p.c.hk + g.kvh) * p.max_blocks + g.block);
+        u[0] = whole ? 0 : (uint32_t)(c1 - c0 + 1);
+        u[1] = (uint32_t)(2 * c0 + (c0 * all / grid < g.unit0 ? 1 : 0));  // the first part's slot; the others' are even
+      }
+      named_sync<1, 256>();  // Q may be written again
+    }
+  }
+  tc_before();
+  __syncthreads();
+  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+}
+
+// Join the parts of the units that several CTAs shared: CTA (unit, 8 rows), a thread 4 dims of a row.
+constexpr uint32_t kJoinRows = 8;
+template <int HD>
+__global__ void __launch_bounds__(kJoinRows * HD / 4) k_attn_tree_join(TreeParams p) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ float ws[kJoinRows][kTcGrid];
+  __shared__ float inv[kJoinRows];
+  const uint32_t unit = blockIdx.x, block = unit % p.max_blocks, kvh = unit / p.max_blocks % p.c.hk;
+  const uint32_t s = unit / p.max_blocks / p.c.hk, row0 = blockIdx.y * kJoinRows, t = threadIdx.x;
+  const SeqWork w = seq_work<kTcRows, kTcTile>(p, s);
+  if (block >= w.blocks) return;
+  const uint32_t rows = min(kTcRows, w.nodes * p.g - block * kTcRows);
+  const uint32_t parts = min(p.units[2 * unit], kTcGrid), first = p.units[2 * unit + 1];
+  if (parts == 0 || row0 >= rows) return;
+  auto slot = [&](uint32_t q) -> size_t { return q == 0 ? first : (first & ~1u) + 2 * q; };
+  const uint32_t n = min(kJoinRows, rows - row0), warps = kJoinRows * HD / 128, lane = t & 31;
+  for (uint32_t r = t >> 5; r < n; r += warps) {
+    float M = -INFINITY;
+    for (uint32_t q = lane; q < parts; q += 32) {
+      ws[r][q] = p.part_ml[(slot(q) * kTcRows + row0 + r) * 2];
+      M = fmaxf(M, ws[r][q]);
+    }
+    M = warp_max(M);
+    float L = 0.0f;
+    for (uint32_t q = lane; q < parts; q += 32) {
+      const float e = ws[r][q] == -INFINITY ? 0.0f : ex2(ws[r][q] - M);
+      L = fmaf(p.part_ml[(slot(q) * kTcRows + row0 + r) * 2 + 1], e, L);
+      ws[r][q] = e;
+    }
+    L = warp_sum(L);
+    if (lane == 0) inv[r] = L != 0.0f ? 1.0f / L : 0.0f;
+  }
+  __syncthreads();
+  const uint32_t r = t % kJoinRows, d4 = t / kJoinRows;
+  if (r >= n) return;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (uint32_t q0 = 0; q0 < parts; q0 += 8) {
+    float4 f[8];
+#pragma unroll
+    for (int u = 0; u < 8; u++)
+      if (q0 + u < parts)
+        f[u] = *reinterpret_cast<const float4 *>(p.part_o + ((slot(q0 + u) * (HD / 4) + d4) * kTcRows + row0 + r) * 4);
+#pragma unroll
+    for (int u = 0; u < 8; u++)
+      if (q0 + u < parts) {
+        const float y = ws[r][q0 + u];
+        acc.x = fmaf(f[u].x, y, acc.x), acc.y = fmaf(f[u].y, y, acc.y);
+        acc.z = fmaf(f[u].z, y, acc.z), acc.w = fmaf(f[u].w, y, acc.w);
+      }
+  }
+  const uint32_t rr = block * kTcRows + row0 + r;
+  const float y = inv[r];
+  *reinterpret_cast<float4 *>(p.out + ((size_t)(w.first + rr / p.g) * p.h + kvh * p.g + rr % p.g) * HD + 4 * d4) =
+      make_float4(acc.x * y, acc.y * y, acc.z * y, acc.w * y);
+}
+
+template <int HD>
+pai_status_t launch_tree_tc(pai_b200_ctx_t *ctx, TreeParams &p) {
+  constexpr size_t smem = sizeof(TcSmem<HD>) + 1024;
+  static SmemOptIn opt;
+  pai_status_t st = b200_cuda(opt.ensure(b200_ctx_device(ctx), smem,
+                                         [](size_t b) {
+                                           return cudaFuncSetAttribute(k_attn_tree_tc<HD>,
+                                                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)b);
+                                         }),
+                              "k_attn_tree_tc smem attribute");
+  if (st) return st;
+  p.max_blocks = (p.max_nodes * p.g + kTcRows - 1) / kTcRows;
+  const uint64_t units = (uint64_t)p.c.n_seq * p.c.hk * p.max_blocks;
+  if (units > 0x7FFFFFFu) return b200_fail(PAI_ERR_UNSUPPORTED, "attn_tree: %llu row tiles", (unsigned long long)units);
+  const uint64_t pairs = units * (((uint64_t)p.c.max_pages * p.c.page_tokens + p.max_nodes + kTcTile - 1) / kTcTile);
+  const uint32_t grid = (uint32_t)std::min<uint64_t>(kTcGrid, pairs);
+  float *scratch;
+  const uint64_t slots = 2ull * grid;
+  st = b200_ctx_scratch(ctx, slots * kTcRows * (HD + 2) + 2 * units, 1, &scratch, &p.cnt);
+  if (st) return st;
+  p.part_o = scratch;
+  p.part_ml = scratch + slots * kTcRows * HD;
+  p.units = (uint32_t *)(p.part_ml + slots * kTcRows * 2);
+  b200_launch(ctx, k_attn_tree_tc<HD>, dim3(grid), dim3(kTcThreads), smem, p);
+  // the joining kernel is resident before this one ends, and waits for it
+  const int pdl = b200_ctx_pdl(ctx);
+  b200_ctx_set_pdl(ctx, 1);
+  b200_launch(ctx, k_attn_tree_join<HD>, dim3((uint32_t)units, kTcRows / kJoinRows), dim3(kJoinRows * HD / 4), 0, p);
+  b200_ctx_set_pdl(ctx, pdl);
+  return b200_launched(ctx, 2, "k_attn_tree_tc");
+}
+
 template <int HD, int WM>
 pai_status_t launch_tree(pai_b200_ctx_t *ctx, TreeParams &p) {
   constexpr uint32_t MR = 16 * WM, WN = 4 / WM;
@@ -562,7 +1157,7 @@ pai_status_t launch_tree_hd(pai_b200_ctx_t *ctx, TreeParams &p) {
   const uint32_t rows = p.max_nodes * p.g;
   if (rows <= 16) return launch_tree<HD, 1>(ctx, p);
   if (rows <= 32) return launch_tree<HD, 2>(ctx, p);
-  return launch_tree<HD, 4>(ctx, p);
+  return launch_tree_tc<HD>(ctx, p);
 }
 
 }  // namespace
@@ -583,6 +1178,7 @@ extern "C" pai_status_t pai_b200_attn_tree_f16kv(pai_b200_ctx_t *ctx, const pai_
     return b200_fail(PAI_ERR_UNSUPPORTED, "attn_tree: head_dim %u (64 or 128)", kv->head_dim);
   p.h = (uint32_t)h, p.g = (uint32_t)h / kv->kv_heads, p.max_nodes = max_nodes, p.words = (max_nodes + 63) / 64;
   p.rows = rows, p.lens = lens, p.off = node_off, p.mask = mask, p.q = q, p.out = out;
+  p.err = b200_ctx_errflag(ctx), p.wait_ns = b200_ctx_wait_ns(ctx);
   p.scale = 1.4426950408889634f / sqrtf((float)kv->head_dim);
   const CtxDeviceGuard on(ctx);
   if (on.status()) return on.status();
