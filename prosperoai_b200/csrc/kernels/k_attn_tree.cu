@@ -20,6 +20,8 @@
 // remainder and multiplied twice, with fp32 sums: 22 bits of each, so that
 // the products are as exact as fp32 ones. The weights carry a factor 2^12
 // that keeps the remainders of small ones above fp16's smallest step.
+#include <cuda.h>  // CUtensorMap and its enums (types only; the encoder comes from the runtime)
+#include <cudaTypedefs.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -50,6 +52,7 @@ struct TreeParams {
   uint32_t *units; // scratch [n_seq][kv head][row tile][2]: parts of a unit, slot of the first
   uint32_t *err;
   uint64_t wait_ns;
+  uint32_t chunk;  // tcgen05 form: positions of one tensor copy
   float scale;     // log2(e) / sqrt(hd)
 };
 
@@ -549,10 +552,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tree(TreeParams p) {
 // The same sums for row tiles of 128 on the fifth-generation tensor cores, one CTA an SM. Key tiles of 128
 // positions; S = Q K^T and the tile's P V go to TMEM, with K, V and Q (both fp16 parts) in shared memory in the
 // 128-byte swizzle and P (both parts) written over S. P V reads V as it lies, hd contiguous (an MN-major B).
-//   warps 0-3, 4-7   softmax of every other key tile, a row a thread: maximum, weights, and the tile's P V added
-//                    to its running output in registers; the two halves join when the unit ends
+//   warps 0-3, 4-7   softmax, a row a thread: the first four have a tile's positions 0-63, the others 64-127; the
+//                    row's maximum goes through shared memory. Then the P V of the tile before, which ran
+//                    meanwhile, is added to the running output in registers, half of the dims each.
 //   warp 8           issues the MMAs: Q K^T of tile i + 1 before P V of tile i, so that they overlap the softmax
-//   warps 12-13      copy K tiles, 14-15 V tiles (16 bytes a copy: pages may be of any size), and look up the pages
+//   warp 12, 13      copy the K and the V tiles by tensor copies, a page or a share of one at a time (p.chunk
+//                    positions: the largest power of two up to 128 that divides the page size)
+//   warps 14-15      take non-finite elements out of V tiles that hold nodes
 // Registers: 512 threads at 128; setmaxnreg gives the softmax warps 200 and leaves 56 to the others (256 * 200 +
 // 256 * 56 = 65536, what the block was launched with).
 constexpr uint32_t kTcThreads = 512, kTcRows = 128, kTcTile = 128, kTcGrid = 148;
@@ -570,28 +576,46 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t block) {
 __host__ __device__ constexpr uint32_t idesc_f16(uint32_t n, bool b_mn) {
   return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((128u >> 4) << 24);
 }
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+// Issued by the one lane that has `leader` set; the whole warp runs the loop around it, so that descriptors stay in
+// uniform registers.
+__device__ __forceinline__ void tc_mma_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add), "r"(leader)
       : "memory");
 }
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void tc_mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add), "r"(leader)
       : "memory");
 }
-__device__ __forceinline__ void tc_commit(uint64_t *bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+__device__ __forceinline__ void tc_commit(uint32_t leader, uint64_t *bar) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)),
+      "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t is;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(is));
+  return is;
+}
+// [64 dims] x [chunk positions] of one kv head of one page; coordinates outside the planes read zeros
+__device__ __forceinline__ void tma_load(void *dst, const CUtensorMap *map, uint32_t dim, uint32_t row, uint32_t head,
+                                         uint32_t page, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(dim), "r"(row), "r"(head), "r"(page), "r"(smem_u32(bar))
+      : "memory");
 }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_ld32(uint32_t at, float (&v)[32]) {
-  uint32_t *r = reinterpret_cast<uint32_t *>(v);
+__device__ __forceinline__ void tc_ld32(uint32_t at, uint32_t *r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
       "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -600,8 +624,8 @@ __device__ __forceinline__ void tc_ld32(uint32_t at, float (&v)[32]) {
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(at));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void tc_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_st32(uint32_t at, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
@@ -650,32 +674,34 @@ struct TcSmem {
   uint8_t q[2][kTileBytes];
   uint8_t kt[2][kTileBytes];
   uint8_t vt[2][kTileBytes];
-  int64_t where[2][2][kTcTile];  // [K, V copiers][tile parity]
   uint32_t valid[8][4];          // positions of a tile that hold a row; a tile's words are read long before 8 tiles on
   uint32_t odd[8][4];            // its nodes with a non-finite V row
   float factor[kTcRows];
-  float ml[2][kTcRows][2];
+  float top[2][2][kTcRows];      // [tile parity][warpgroup]: maxima of a row's halves
+  float ml[2][kTcRows];
   uint64_t upto[kMaxSeqs + 1];
-  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], ofull[2], qfull, drain;
+  uint64_t kfull[2], kempty[2], vfull[2], vclean[2], vempty[2], sfull[2], pfull[2], ofull[2], qfull, drain;
   uint32_t tmem;
 };
 
 template <int HD>
-__global__ void __launch_bounds__(kTcThreads, 1) k_attn_tree_tc(TreeParams p) {
+__global__ void __launch_bounds__(kTcThreads, 1)
+    k_attn_tree_tc(TreeParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using Smem = TcSmem<HD>;
   extern __shared__ __align__(16) uint8_t raw[];
   Smem &sm = *reinterpret_cast<Smem *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-  constexpr uint32_t CH = HD / 8, BL = Smem::kBlock;
+  constexpr uint32_t BL = Smem::kBlock;
   const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
   pdl_trigger();
   if (t == 0) {
     for (int i = 0; i < 2; i++) {
-      mbar_init(&sm.kfull[i], 64);
-      mbar_init(&sm.vfull[i], 64);
+      mbar_init(&sm.kfull[i], 1);
+      mbar_init(&sm.vfull[i], 1);
+      mbar_init(&sm.vclean[i], 64);
       mbar_init(&sm.kempty[i], 1);
       mbar_init(&sm.vempty[i], 1);
       mbar_init(&sm.sfull[i], 1);
-      mbar_init(&sm.pfull[i], 4);
+      mbar_init(&sm.pfull[i], 8);
       mbar_init(&sm.ofull[i], 1);
     }
     mbar_init(&sm.qfull, 8);
@@ -709,22 +735,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tree_tc(TreeParams p) {
     }
   };
 
-  if (warp >= 12) {
-    // ---- copiers: 64 threads for K, 64 for V ----
+  if (warp >= 14) {
+    // ---- cleaners: the V rows of tiles that hold nodes ----
+    // A non-finite V row may only reach the rows that see its node, and a weight of 0 does not keep it out of a
+    // product: such elements (those of stale rows behind the last node too) become 0 here, and the softmax warps add
+    // them to the rows that see them.
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    const bool is_v = warp >= 14;
-    const uint32_t e = t - (is_v ? 448 : 384), ch = e % CH, r0 = e / CH;
-    uint64_t *full = is_v ? sm.vfull : sm.kfull, *empty = is_v ? sm.vempty : sm.kempty;
-    uint32_t i = 0;  // tiles of the run so far
-    uint32_t held = 0, held_len = 0;  // the tile before, not yet handed over: its first position, committed positions
-    bool holding = false;
-    auto hand_over = [&](uint32_t n) {
-      // tile n has landed (this thread's copies)
-      if (is_v && held + kTcTile > held_len) {
-        // it holds nodes: non-finite elements become 0 and are added by the softmax warps to the rows that see them
-        for (uint32_t r = r0; r < kTcTile; r += 64 / CH) {
-          uint4 *c4 = reinterpret_cast<uint4 *>(sm.vt[n & 1] + (ch / 8) * BL + r * 128 + (((ch % 8) ^ (r & 7)) << 4));
-          uint4 v = *c4;
+    const uint32_t e = t - 448;
+    constexpr uint32_t CH = HD / 8;
+    uint32_t i = 0;
+    while (next_segment<kTcRows, kTcTile>(p, sm.upto, walk, g))
+      for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
+        if ((tile + 1) * kTcTile <= g.w.len) continue;
+        wait(&sm.vfull[i & 1], i >> 1);
+        if (e < 4) sm.odd[i & 7][e] = 0;  // tile i - 8 is long folded: this one's copy waited for P V of tile i - 2
+        named_sync<2, 64>();
+        for (uint32_t c = e; c < kTcTile * CH; c += 64) {
+          const uint32_t r = c / CH, ch = c % CH;
+          uint4 *at = reinterpret_cast<uint4 *>(sm.vt[i & 1] + (ch / 8) * BL + r * 128 + (((ch % 8) ^ (r & 7)) << 4));
+          uint4 v = *at;
           uint32_t *cw = reinterpret_cast<uint32_t *>(&v);
           bool bad = false;
 #pragma unroll
@@ -733,105 +762,144 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tree_tc(TreeParams p) {
             if ((cw[x] & 0x7C000000u) == 0x7C000000u) cw[x] &= 0xFFFFu, bad = true;
           }
           if (bad) {
-            *c4 = v;
-            atomicOr(&sm.odd[n & 7][r / 32], 1u << (r % 32));
+            *at = v;
+            atomicOr(&sm.odd[i & 7][r / 32], 1u << (r % 32));
           }
         }
+        fence_proxy_async();
+        mbar_arrive(&sm.vclean[i & 1]);
       }
-      fence_proxy_async();
-      mbar_arrive(&full[n & 1]);
-    };
+  } else if (warp >= 12) {
+    // ---- copies: warp 12 the K tiles, 13 the V tiles; a lane a chunk of p.chunk positions, which lie in one page ----
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    const bool is_v = warp == 13;
+    const CUtensorMap *map = is_v ? &vmap : &kmap;
+    uint64_t *full = is_v ? sm.vfull : sm.kfull, *empty = is_v ? sm.vempty : sm.kempty;
+    const uint32_t chunks = kTcTile / p.chunk, chunk = p.chunk, P = p.c.page_tokens;
+    uint32_t i = 0;  // tiles of the run so far
     while (next_segment<kTcRows, kTcTile>(p, sm.upto, walk, g)) {
       const uint32_t total = g.w.len + g.w.nodes;
-      const __half *src = (is_v ? p.c.v : p.c.k) + (size_t)g.kvh * p.c.head_stride;
+      // where the lane's chunk of a tile lies: page (n_pages for a hole, which reads zeros), first row; -1: behind the
+      // last position, not copied
+      int32_t page, row;
+      auto find = [&](uint32_t tile) {
+        const uint32_t pos = tile * kTcTile + lane * chunk;
+        page = -1, row = 0;
+        if (lane < chunks && tile < g.tile1 && pos < total) {
+          const uint32_t pg = pos / P;
+          uint32_t x = p.c.n_pages;
+          if (pg < p.c.max_pages) x = p.c.table ? (uint32_t)p.c.table[(size_t)g.s * p.c.max_pages + pg] : g.s;
+          page = (int32_t)min(x, p.c.n_pages);
+          row = (int32_t)(pos - pg * P);
+        }
+      };
+      find(g.tile0);
       for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
-        int64_t *wh = sm.where[is_v][i & 1];
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-          const uint32_t r = e + 64 * x, pos = tile * kTcTile + r;
-          const int64_t at_row = pos < total ? kv_row(p.c, g.s, pos) : -1;
-          wh[r] = at_row;
-          const uint32_t bits = __ballot_sync(0xffffffffu, at_row >= 0);
-          if (lane == 0) {
-            if (is_v) sm.odd[i & 7][r / 32] = 0; else sm.valid[i & 7][r / 32] = bits;
-          }
-        }
-        if (is_v) named_sync<3, 64>(); else named_sync<2, 64>();
+        const int32_t at = page, r = row;
+        find(tile + 1);  // the next tile's table entries come while this one is copied
+        const uint32_t copied = __ballot_sync(0xffffffffu, at >= 0);
         if (i >= 2) wait(&empty[i & 1], (i >> 1) - 1);
+        __syncwarp();
+        if (!is_v) {
+          const uint32_t there = __ballot_sync(0xffffffffu, at >= 0 && at < (int32_t)p.c.n_pages);
+          if (lane < 4) {  // the word of positions 32 lane .. + 31
+            const uint32_t cap = min(total, p.c.max_pages * P), pos = tile * kTcTile + 32 * lane;
+            uint32_t bits = 0;
+            if (chunk >= 32) {
+              bits = (there >> (32 * lane / chunk)) & 1 ? 0xFFFFFFFFu : 0u;
+            } else {
+              for (uint32_t c = 0; c < 32 / chunk; c++)
+                if ((there >> (32 / chunk * lane + c)) & 1) bits |= ((1u << chunk) - 1) << (c * chunk);
+            }
+            sm.valid[i & 7][lane] = bits & (uint32_t)low_bits((int64_t)cap - pos);
+          }
+          __syncwarp();
+        }
         if (ok) {
-          uint8_t *dst = (is_v ? sm.vt : sm.kt)[i & 1] + (ch / 8) * BL;
-#pragma unroll 8
-          for (uint32_t r = r0; r < kTcTile; r += 64 / CH) {
-            const int64_t at_row = wh[r];
-            const bool there = at_row >= 0;
-            cp16(dst + r * 128 + (((ch % 8) ^ (r & 7)) << 4), src + (there ? at_row : 0) + ch * 8, there);
+          uint8_t *dst = (is_v ? sm.vt : sm.kt)[i & 1] + lane * chunk * 128;
+          if (lane == 0) mbar_expect_tx(&full[i & 1], __popc(copied) * chunk * HD * 2);
+          __syncwarp();
+          if (at >= 0) {
+#pragma unroll
+            for (uint32_t b = 0; b < HD / 64; b++) tma_load(dst + b * BL, map, 64 * b, r, g.kvh, at, &full[i & 1]);
           }
         }
-        cp_commit();
-        if (holding) {
-          cp_wait<1>();
-          hand_over(i - 1);
-        }
-        holding = true, held = tile * kTcTile, held_len = g.w.len;
+        __syncwarp();
       }
     }
-    cp_wait<0>();
-    if (holding) hand_over(i - 1);
+    // the last copies land before the block ends, whatever became of the others
+    ok = true;
+    if (i >= 2) wait(&full[i & 1], (i - 2) >> 1);
+    if (i >= 1) wait(&full[(i - 1) & 1], (i - 1) >> 1);
   } else if (warp >= 8) {
     // ---- MMA issue ----
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 8 && lane == 0) {
-      const uint32_t q0 = smem_u32(sm.q[0]), q1 = smem_u32(sm.q[1]);
-      uint32_t i = 0, seg = 0;
+    if (warp == 8) {
+      const uint32_t leader = elect_one();
+      const uint64_t qd = desc_k(smem_u32(sm.q[0])), kd = desc_k(smem_u32(sm.kt[0])), vd = desc_mn(smem_u32(sm.vt[0]), BL);
+      constexpr uint64_t kPart = Smem::kTileBytes >> 4;  // from one part of Q, or one tile, to the next, in 16 bytes
+      uint32_t i = 0, seg = 0, cleaned[2] = {0, 0};
       auto scores = [&](uint32_t n) {  // S = Q K^T of tile n: both parts of Q
         wait(&sm.kfull[n & 1], n >> 1);
         tc_after();
-        if (!ok) return;
-        const uint32_t kb = smem_u32(sm.kt[n & 1]), d = tmem + 128 * (n & 1);
+        const uint64_t kb = kd + (n & 1) * kPart;
+        const uint32_t d = tmem + 128 * (n & 1);
+        if (ok) {
 #pragma unroll
-        for (uint32_t k = 0; k < HD / 16; k++) {
-          const uint32_t off = (k / 4) * BL + (k % 4) * 32;
-          tc_mma_ss(d, desc_k(q0 + off), desc_k(kb + off), idesc_f16(kTcTile, false), k > 0);
-          tc_mma_ss(d, desc_k(q1 + off), desc_k(kb + off), idesc_f16(kTcTile, false), true);
+          for (uint32_t k = 0; k < HD / 16; k++) {
+            const uint64_t off = ((k / 4) * BL + (k % 4) * 32) >> 4;
+            tc_mma_ss(leader, d, qd + off, kb + off, idesc_f16(kTcTile, false), k > 0);
+            tc_mma_ss(leader, d, qd + kPart + off, kb + off, idesc_f16(kTcTile, false), true);
+          }
+          tc_commit(leader, &sm.sfull[n & 1]);
+          tc_commit(leader, &sm.kempty[n & 1]);
         }
-        tc_commit(&sm.sfull[n & 1]);
-        tc_commit(&sm.kempty[n & 1]);
+        __syncwarp();
       };
       while (next_segment<kTcRows, kTcTile>(p, sm.upto, walk, g)) {
         wait(&sm.qfull, seg++);
-        const uint32_t n = g.tile1 - g.tile0;
         scores(i);
-        for (uint32_t j = 0; j < n; j++, i++) {
-          if (j + 1 < n) scores(i + 1);
+        for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
+          if (tile + 1 < g.tile1) scores(i + 1);
           wait(&sm.pfull[i & 1], i >> 1);
           wait(&sm.vfull[i & 1], i >> 1);
+          if ((tile + 1) * kTcTile > g.w.len) wait(&sm.vclean[i & 1], i & 1 ? cleaned[1]++ : cleaned[0]++);
           tc_after();
+          const uint64_t vb = vd + (i & 1) * kPart;
+          const uint32_t a = tmem + 128 * (i & 1), d = tmem + 256 + 128 * (i & 1);
           if (ok) {  // this tile's P V, from zero: the sum over tiles is made in registers, where it is rounded
-            const uint32_t vb = smem_u32(sm.vt[i & 1]), a = tmem + 128 * (i & 1), d = tmem + 256 + 128 * (i & 1);
 #pragma unroll
             for (uint32_t k = 0; k < kTcTile / 16; k++) {
-              const uint64_t b = desc_mn(vb + k * 2048, BL);
               const uint32_t at = a + 32 * (k / 2) + 8 * (k % 2);
-              tc_mma_ts(d, at, b, idesc_f16(HD, true), k > 0);
-              tc_mma_ts(d, at + 16, b, idesc_f16(HD, true), true);
+              tc_mma_ts(leader, d, at, vb + k * (2048 >> 4), idesc_f16(HD, true), k > 0);
+              tc_mma_ts(leader, d, at + 16, vb + k * (2048 >> 4), idesc_f16(HD, true), true);
             }
-            tc_commit(&sm.ofull[i & 1]);
-            tc_commit(&sm.vempty[i & 1]);
+            tc_commit(leader, &sm.ofull[i & 1]);
+            tc_commit(leader, &sm.vempty[i & 1]);
           }
+          __syncwarp();
         }
       }
       // the MMAs in flight end before TMEM is given back
-      tc_commit(&sm.drain);
+      tc_commit(leader, &sm.drain);
       ok = true;
       wait(&sm.drain, 0);
+      __syncwarp();
     }
-    __syncwarp();
   } else {
-    // ---- softmax: warpgroup wg has every other tile, a thread a row ----
+    // ---- softmax: a thread a row, warpgroup wg half of the positions and half of the dims ----
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     const uint32_t wg = warp >> 2, r = t & 127;
     const uint32_t lanes = (warp & 3) * 32 << 16;
     uint32_t i = 0;
+    // which of the 64 positions from node `base` (negative: committed) on a row of node `nd` may see
+    auto seen = [&](uint32_t base32, bool live, uint32_t nd, uint32_t first) -> uint64_t {
+      const int32_t base = (int32_t)base32;
+      const uint64_t past = low_bits(-(int64_t)base);
+      if (!live) return past;
+      if (!p.mask) return low_bits((int64_t)nd + 1 - base);
+      return past | (window(p.mask + (size_t)(first + nd) * p.words, p.words, base) & ~past);
+    };
     while (next_segment<kTcRows, kTcTile>(p, sm.upto, walk, g)) {
       const uint32_t rows = min(kTcRows, g.w.nodes * p.g - g.block * kTcRows);
       // Q into shared memory, a power of two and two fp16 parts a row; the last segment's products are done
@@ -873,101 +941,34 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tree_tc(TreeParams p) {
       const bool work = (warp & 3) * 32 < rows;  // a warp whose rows are all past the last one keeps step only
       const uint32_t rr = g.block * kTcRows + r, nd = rr / p.g;
       const bool live = r < rows;
-      float o[HD], m = -INFINITY, l = 0.0f;
+      float o[HD / 2], m = -INFINITY, l = 0.0f, corr = 1.0f;
 #pragma unroll
-      for (int d = 0; d < HD; d++) o[d] = 0.0f;
-      for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
-        if ((i & 1) != wg) continue;
-        const uint32_t sa = tmem + lanes + 128 * wg, oa = tmem + lanes + 256 + 128 * wg;
-        wait(&sm.sfull[wg], i >> 1);
-        __syncwarp();
-        tc_after();
-        float corr = 1.0f;
-        uint64_t sees[2];
-        bool masked = false;
-        if (work) {
-          const bool drafted = (tile + 1) * kTcTile > g.w.len;
-#pragma unroll
-          for (int x = 0; x < 2; x++)
-            sees[x] = (uint64_t)sm.valid[i & 7][2 * x] | (uint64_t)sm.valid[i & 7][2 * x + 1] << 32;
-          masked = drafted || (sees[0] & sees[1]) != ~0ull;
-          if (drafted) {
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-              const int32_t base = (int32_t)(tile * kTcTile + 64 * x - g.w.len);
-              uint64_t b = low_bits(-(int64_t)base);
-              if (live)
-                b |= p.mask ? window(p.mask + (size_t)(g.w.first + nd) * p.words, p.words, base) & ~low_bits(-(int64_t)base)
-                            : low_bits((int64_t)nd + 1 - base);
-              sees[x] &= b;
-            }
-          }
-          float top = -INFINITY;
-#pragma unroll
-          for (int c = 0; c < 4; c++) {
-            float v[32];
-            tc_ld32(sa + 32 * c, v);
-            if (masked) {
-              const uint32_t bits = (uint32_t)(sees[c / 2] >> (32 * (c & 1)));
-#pragma unroll
-              for (int e = 0; e < 32; e++)
-                if (!((bits >> e) & 1)) v[e] = -INFINITY;
-            }
-#pragma unroll
-            for (int e = 0; e < 32; e++) top = fmaxf(top, v[e]);
-          }
-          const float mn = fmaxf(m, top * factor);
-          corr = m == mn ? 1.0f : ex2(m - mn);
-          m = mn;
-          const float sub = mn == -INFINITY ? 0.0f : mn - kPShift;
-          l *= corr;
-          float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < 4; c++) {
-            float v[32];
-            tc_ld32(sa + 32 * c, v);
-            if (masked) {
-              const uint32_t bits = (uint32_t)(sees[c / 2] >> (32 * (c & 1)));
-#pragma unroll
-              for (int e = 0; e < 32; e++)
-                if (!((bits >> e) & 1)) v[e] = -INFINITY;
-            }
-            uint32_t w[32];  // 16 words of parts, 16 of remainders
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float p0 = ex2(fmaf(v[e], factor, -sub)), p1 = ex2(fmaf(v[e + 1], factor, -sub));
-              part[(e / 2) & 3] += p0 + p1;
-              split_f16(p0, p1, w[e / 2], w[16 + e / 2]);
-            }
-            tc_st32(sa + 32 * c, w);
-          }
-          l += (part[0] + part[1]) + (part[2] + part[3]);
-          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-        }
-        tc_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.pfull[wg]);
-        wait(&sm.ofull[wg], i >> 1);
+      for (int d = 0; d < HD / 2; d++) o[d] = 0.0f;
+      // add the P V of tile n (the n-th of the run) to this thread's half of the dims; `tile` its number in the unit
+      auto fold = [&](uint32_t n, uint32_t tile, uint64_t sees0, uint64_t sees1) {
+        wait(&sm.ofull[n & 1], n >> 1);
         __syncwarp();
         tc_after();
         if (work) {
+          const uint32_t oa = tmem + lanes + 256 + 128 * (n & 1) + wg * (HD / 2);
+          uint32_t v[HD / 2];
 #pragma unroll
-          for (int c = 0; c < HD / 32; c++) {
-            float v[32];
-            tc_ld32(oa + 32 * c, v);
+          for (int c = 0; c < HD / 64; c++) tc_ld32(oa + 32 * c, v + 32 * c);
+          tc_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 32; e++) o[32 * c + e] = fmaf(o[32 * c + e], corr, v[e]);
-          }
-          if (masked) {
+          for (int d = 0; d < HD / 2; d++) o[d] = fmaf(o[d], corr, __uint_as_float(v[d]));
+          if ((tile + 1) * kTcTile > g.w.len) {
             // non-finite V elements of nodes that this row sees
 #pragma unroll 1
             for (int x = 0; x < 4; x++)
 #pragma unroll 1
-              for (uint32_t left = sm.odd[i & 7][x] & (uint32_t)(sees[x / 2] >> (32 * (x & 1))); left; left &= left - 1) {
+              for (uint32_t left = sm.odd[n & 7][x] & (uint32_t)((x < 2 ? sees0 : sees1) >> (32 * (x & 1))); left;
+                   left &= left - 1) {
                 const int64_t at_row = kv_row(p.c, g.s, tile * kTcTile + 32 * x + __ffs(left) - 1);
-                const __half2 *vr = reinterpret_cast<const __half2 *>(p.c.v + (size_t)g.kvh * p.c.head_stride + at_row);
+                const __half2 *vr =
+                    reinterpret_cast<const __half2 *>(p.c.v + (size_t)g.kvh * p.c.head_stride + at_row + wg * (HD / 2));
 #pragma unroll
-                for (int d = 0; d < HD / 2; d++) {
+                for (int d = 0; d < HD / 4; d++) {
                   const float2 f = __half22float2(vr[d]);
                   if (!isfinite(f.x)) o[2 * d] += f.x;
                   if (!isfinite(f.y)) o[2 * d + 1] += f.y;
@@ -977,25 +978,79 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tree_tc(TreeParams p) {
         }
         __syncwarp();
         tc_before();
-      }
-      // join the two warpgroups' halves of the tiles: each gives the other half of the dims, over Q
-      named_sync<1, 256>();
-      float *give = reinterpret_cast<float *>(wg ? sm.q[0] : sm.q[1]);        // [HD / 2][128]
-      const float *take = reinterpret_cast<const float *>(wg ? sm.q[1] : sm.q[0]);
-      sm.ml[wg][r][0] = m;
-      sm.ml[wg][r][1] = l;
-      // wg 0 keeps dims 0 .. HD/2 - 1, wg 1 the others
-      if (wg) {
+      };
+      uint64_t sees0 = 0, sees1 = 0;  // of the tile that is folded next
+      for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
+        const uint32_t sa = tmem + lanes + 128 * (i & 1) + 64 * wg;
+        wait(&sm.sfull[i & 1], i >> 1);
+        __syncwarp();
+        tc_after();
+        float corr1 = 1.0f;
+        uint64_t now0 = 0, now1 = 0;
+        if (work) {
+          uint32_t v[64];
+          tc_ld32(sa, v);
+          tc_ld32(sa + 32, v + 32);
+          const bool drafted = (tile + 1) * kTcTile > g.w.len;
+          const uint64_t ok0 = (uint64_t)sm.valid[i & 7][0] | (uint64_t)sm.valid[i & 7][1] << 32;
+          const uint64_t ok1 = (uint64_t)sm.valid[i & 7][2] | (uint64_t)sm.valid[i & 7][3] << 32;
+          const bool masked = drafted || (ok0 & ok1) != ~0ull;
+          now0 = ok0, now1 = ok1;
+          if (drafted) {
+            now0 &= seen(tile * kTcTile - g.w.len, live, nd, g.w.first);
+            now1 &= seen(tile * kTcTile + 64 - g.w.len, live, nd, g.w.first);
+          }
+          tc_ld_wait();
+          if (masked) {
+            const uint64_t bits = wg ? now1 : now0;
+            const uint32_t b0 = (uint32_t)bits, b1 = (uint32_t)(bits >> 32);
 #pragma unroll
-        for (int d = 0; d < HD / 2; d++) give[d * 128 + r] = o[d];
-      } else {
+            for (int e = 0; e < 64; e++)
+              if (!(((e < 32 ? b0 : b1) >> (e & 31)) & 1)) v[e] = 0xFF800000u;  // -inf
+          }
+          float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int d = 0; d < HD / 2; d++) give[d * 128 + r] = o[HD / 2 + d];
+          for (int e = 0; e < 64; e += 8)
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+              t4[u] = fmaxf(t4[u], fmaxf(__uint_as_float(v[e + 2 * u]), __uint_as_float(v[e + 2 * u + 1])));
+          float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+          // the row's other 64 positions are the other warpgroup's
+          sm.top[i & 1][wg][r] = top;
+          asm volatile("bar.sync %0, 64;" ::"r"(4 + (warp & 3)) : "memory");
+          top = fmaxf(top, sm.top[i & 1][1 - wg][r]);
+          const float mn = fmaxf(m, top * factor);
+          corr1 = m == mn ? 1.0f : ex2(m - mn);
+          m = mn;
+          const float sub = mn == -INFINITY ? 0.0f : mn - kPShift;
+          float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 2; c++) {
+            uint32_t w[32];  // 16 words of parts, 16 of remainders
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float p0 = ex2(fmaf(__uint_as_float(v[32 * c + e]), factor, -sub));
+              const float p1 = ex2(fmaf(__uint_as_float(v[32 * c + e + 1]), factor, -sub));
+              part[(e / 2) & 3] += p0 + p1;
+              split_f16(p0, p1, w[e / 2], w[16 + e / 2]);
+            }
+            tc_st32(sa + 32 * c, w);
+          }
+          l = l * corr1 + ((part[0] + part[1]) + (part[2] + part[3]));
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        }
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.pfull[i & 1]);
+        // the tile before, whose P V ran meanwhile
+        if (tile > g.tile0) fold(i - 1, tile - 1, sees0, sees1);
+        corr = corr1, sees0 = now0, sees1 = now1;
       }
+      fold(i - 1, g.tile1 - 1, sees0, sees1);
+      // the two halves' sums of weights
+      sm.ml[wg][r] = l;
       named_sync<1, 256>();
-      const float m2 = sm.ml[1 - wg][r][0], M = fmaxf(m, m2);
-      const float w1 = m == -INFINITY ? 0.0f : ex2(m - M), w2 = m2 == -INFINITY ? 0.0f : ex2(m2 - M);
-      const float L = wg ? sm.ml[0][r][1] * w2 + l * w1 : l * w1 + sm.ml[1][r][1] * w2;
+      const float L = sm.ml[0][r] + sm.ml[1][r];
       const bool whole = g.whole();
       const uint64_t slot = 2 * cta + (begin >= g.unit0 ? 0 : 1);
       const float scale = whole ? (L != 0.0f ? 1.0f / L : 0.0f) : 1.0f;
@@ -1005,17 +1060,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tree_tc(TreeParams p) {
       const uint32_t step = whole ? 4 : 4 * kTcRows;
       if (live) {
 #pragma unroll
-        for (int d = 0; d < HD / 2; d += 4) {
-          float f[4];
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const float mine = wg ? o[HD / 2 + d + e] : o[d + e];
-            f[e] = ((m == -INFINITY ? 0.0f : mine * w1) + (m2 == -INFINITY ? 0.0f : take[(d + e) * 128 + r] * w2)) * scale;
-          }
-          *reinterpret_cast<float4 *>(dst + (size_t)(d / 4) * step) = make_float4(f[0], f[1], f[2], f[3]);
-        }
+        for (int d = 0; d < HD / 2; d += 4)
+          *reinterpret_cast<float4 *>(dst + (size_t)(d / 4) * step) =
+              make_float4(o[d] * scale, o[d + 1] * scale, o[d + 2] * scale, o[d + 3] * scale);
         if (!whole && wg == 0) {
-          p.part_ml[(slot * kTcRows + r) * 2] = M;
+          p.part_ml[(slot * kTcRows + r) * 2] = m;
           p.part_ml[(slot * kTcRows + r) * 2 + 1] = L;
         }
       }
@@ -1026,7 +1075,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_attn_tree_tc(TreeParams p) {
         u[0] = whole ? 0 : (uint32_t)(c1 - c0 + 1);
         u[1] = (uint32_t)(2 * c0 + (c0 * all / grid < g.unit0 ? 1 : 0));  // the first part's slot; the others' are even
       }
-      named_sync<1, 256>();  // Q may be written again
+      named_sync<1, 256>();  // Q and the sums may be written again
     }
   }
   tc_before();
@@ -1091,8 +1140,21 @@ __global__ void __launch_bounds__(kJoinRows * HD / 4) k_attn_tree_join(TreeParam
       make_float4(acc.x * y, acc.y * y, acc.z * y, acc.w * y);
 }
 
+// Tensor map of a layer's plane: [page][kv head][position][64 dims of hd], boxes of `chunk` positions, 128-byte swizzle.
+bool plane_map(const TreeParams &p, const __half *plane, CUtensorMap *map) {
+  const auto encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(b200_tensor_map_encoder());
+  if (!encode) return false;
+  const cuuint64_t dims[4] = {p.c.hd, p.c.page_tokens, p.c.hk, p.c.n_pages};
+  const cuuint64_t row = p.c.hd * 2ull;  // a stride along a dimension of one is never used
+  const cuuint64_t strides[3] = {row, p.c.hk > 1 ? p.c.head_stride * 2 : row, p.c.n_pages > 1 ? p.c.page_stride * 2 : row};
+  const cuuint32_t box[4] = {64, p.chunk, 1, 1}, estr[4] = {1, 1, 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<__half *>(plane), dims, strides, box, estr,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int HD>
-pai_status_t launch_tree_tc(pai_b200_ctx_t *ctx, TreeParams &p) {
+pai_status_t launch_tree_tc(pai_b200_ctx_t *ctx, TreeParams &p, const CUtensorMap &kmap, const CUtensorMap &vmap) {
   constexpr size_t smem = sizeof(TcSmem<HD>) + 1024;
   static SmemOptIn opt;
   pai_status_t st = b200_cuda(opt.ensure(b200_ctx_device(ctx), smem,
@@ -1114,7 +1176,7 @@ pai_status_t launch_tree_tc(pai_b200_ctx_t *ctx, TreeParams &p) {
   p.part_o = scratch;
   p.part_ml = scratch + slots * kTcRows * HD;
   p.units = (uint32_t *)(p.part_ml + slots * kTcRows * 2);
-  b200_launch(ctx, k_attn_tree_tc<HD>, dim3(grid), dim3(kTcThreads), smem, p);
+  b200_launch(ctx, k_attn_tree_tc<HD>, dim3(grid), dim3(kTcThreads), smem, p, kmap, vmap);
   // the joining kernel is resident before this one ends, and waits for it
   const int pdl = b200_ctx_pdl(ctx);
   b200_ctx_set_pdl(ctx, 1);
@@ -1154,10 +1216,16 @@ pai_status_t launch_tree(pai_b200_ctx_t *ctx, TreeParams &p) {
 
 template <int HD>
 pai_status_t launch_tree_hd(pai_b200_ctx_t *ctx, TreeParams &p) {
+  // tensor copies take whole shares of a page, a power of two of at least 8 positions
+  p.chunk = 128;
+  if (p.c.table)
+    while (p.chunk > 8 && p.c.page_tokens % p.chunk) p.chunk /= 2;
+  CUtensorMap kmap, vmap;
+  if ((!p.c.table || p.c.page_tokens % p.chunk == 0) && plane_map(p, p.c.k, &kmap) && plane_map(p, p.c.v, &vmap))
+    return launch_tree_tc<HD>(ctx, p, kmap, vmap);
   const uint32_t rows = p.max_nodes * p.g;
   if (rows <= 16) return launch_tree<HD, 1>(ctx, p);
-  if (rows <= 32) return launch_tree<HD, 2>(ctx, p);
-  return launch_tree_tc<HD>(ctx, p);
+  return launch_tree<HD, 4>(ctx, p);
 }
 
 }  // namespace

@@ -163,7 +163,8 @@ SHAPES = [
     ([300], [33], 100, 6, 2, 128), ([70, 0, 1000, 5], [5, 0, 17, 9], 64, 16, 2, 128), ([129, 40], [65, 20], 16, 8, 8, 64),
     ([90], [130], 32, 4, 1, 128), ([37, 500], [1, 64], 0, 32, 8, 128), ([5000], [8], 128, 8, 2, 128),
     ([3000, 2, 777, 64, 0, 1500, 31, 900], [4, 1, 7, 16, 2, 1, 12, 3], 128, 10, 2, 128), ([17], [31], 1, 2, 1, 64),
-    ([40], [20], 16, 64, 1, 128),
+    ([40], [20], 16, 64, 1, 128), ([333, 20], [40, 9], 24, 4, 2, 128), ([250], [5], 8, 8, 2, 64), ([1000], [6], 0, 6, 2, 128),
+    ([260, 131], [70, 3], 20, 8, 2, 128), ([127, 128, 129, 255], [1, 1, 1, 1], 256, 8, 8, 128),
 ]
 
 
