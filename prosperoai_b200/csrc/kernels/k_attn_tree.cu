@@ -552,16 +552,16 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tree(TreeParams p) {
 // The same sums for row tiles of 128 on the fifth-generation tensor cores, one CTA an SM. Key tiles of 128
 // positions; S = Q K^T and the tile's P V go to TMEM, with K, V and Q (both fp16 parts) in shared memory in the
 // 128-byte swizzle and P (both parts) written over S. P V reads V as it lies, hd contiguous (an MN-major B).
-//   warps 0-3, 4-7   softmax, a row a thread: the first four have a tile's positions 0-63, the others 64-127; the
-//                    row's maximum goes through shared memory. Then the P V of the tile before, which ran
-//                    meanwhile, is added to the running output in registers, half of the dims each.
-//   warp 8           issues the MMAs: Q K^T of tile i + 1 before P V of tile i, so that they overlap the softmax
-//   warp 12, 13      copy the K and the V tiles by tensor copies, a page or a share of one at a time (p.chunk
+//   warps 0-3, 4-7   softmax of every other key tile, a row a thread: maximum and weights
+//   warps 8-11       add the tiles' P V to the running output in registers, a row a thread
+//   warp 12          issues the MMAs: Q K^T of tile i + 1 before P V of tile i, so that they overlap the softmax
+//   warp 13, 14      copy the K and the V tiles by tensor copies, a page or a share of one at a time (p.chunk
 //                    positions: the largest power of two up to 128 that divides the page size)
-//   warps 14-15      take non-finite elements out of V tiles that hold nodes
-// Registers: 512 threads at 128; setmaxnreg gives the softmax warps 200 and leaves 56 to the others (256 * 200 +
-// 256 * 56 = 65536, what the block was launched with).
-constexpr uint32_t kTcThreads = 512, kTcRows = 128, kTcTile = 128, kTcGrid = 148;
+//   warp 15          takes non-finite elements out of V tiles that hold nodes
+// Registers: 512 threads at 128; setmaxnreg gives the softmax warps 136, the folding ones 184 and leaves 56 to the
+// others (256 * 136 + 128 * 184 + 128 * 56 = 65536, what the block was launched with).
+// Calls of at most 32 rows a kv head take row tiles of 32: Q is then small enough for a third K and V tile in flight.
+constexpr uint32_t kTcThreads = 512, kTcTile = 128, kTcGrid = 148;
 
 __device__ __forceinline__ uint64_t desc_k(uint32_t saddr) {  // K-major, 128-byte swizzle, 8-row groups of 1024 bytes
   return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)1u << 16 | (uint64_t)(1024u >> 4) << 32 | (uint64_t)1u << 46 |
@@ -625,19 +625,37 @@ __device__ __forceinline__ void tc_ld32(uint32_t at, uint32_t *r) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(at));
 }
-__device__ __forceinline__ void tc_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tc_st32(uint32_t at, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tc_ld16(uint32_t at, uint32_t (&r)[16]) {  // and wait for it
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
-      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(at)
+      : "memory");
+}
+// Wait for the loads; the words pass through, so that nothing that uses them is moved before the wait.
+__device__ __forceinline__ void tc_ld_wait(uint32_t *r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13])
+               :
+               : "memory");
+  asm volatile("" : "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+                    "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27])
+               :: "memory");
+  asm volatile("" : "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t at, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
       "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
-      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(at)
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(at)
       : "memory");
 }
 template <int ID, int N>
 __device__ __forceinline__ void named_sync() {
+  __syncwarp();
   asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory");
 }
 
@@ -667,53 +685,62 @@ __device__ __forceinline__ bool next_segment(const TreeParams &p, const uint64_t
   return true;
 }
 
-template <int HD>
+template <int HD, uint32_t MR, uint32_t NS>
 struct TcSmem {
-  static constexpr uint32_t kBlock = 128 * 128;             // 128 rows of 64 dims: 16 KB
-  static constexpr uint32_t kTileBytes = HD / 64 * kBlock;  // a K or V tile, or one part of Q
-  uint8_t q[2][kTileBytes];
-  uint8_t kt[2][kTileBytes];
-  uint8_t vt[2][kTileBytes];
-  uint32_t valid[8][4];          // positions of a tile that hold a row; a tile's words are read long before 8 tiles on
-  uint32_t odd[8][4];            // its nodes with a non-finite V row
-  float factor[kTcRows];
-  float top[2][2][kTcRows];      // [tile parity][warpgroup]: maxima of a row's halves
-  float ml[2][kTcRows];
+  static constexpr uint32_t kBlock = kTcTile * 128;         // a tile's 64 dims: 16 KB
+  static constexpr uint32_t kTileBytes = HD / 64 * kBlock;  // a K or V tile
+  static constexpr uint32_t kQBlock = MR * 128, kQBytes = HD / 64 * kQBlock;  // one part of Q
+  // With MR below 128 the MMAs read 128 rows all the same: what follows Q, for rows that nobody reads.
+  uint8_t q[2][kQBytes];
+  uint8_t kt[NS][kTileBytes];
+  uint8_t vt[NS][kTileBytes];
+  // Words and rows of a tile are read long before the tile that takes their place: fold(i) frees the TMEM of P V of
+  // tile i + 2, so no warp is more than a few tiles ahead of it.
+  uint32_t valid[8][4];       // positions of a tile that hold a row
+  uint32_t odd[8][4];         // its nodes with a non-finite V row
+  float mrow[4][MR];          // [tile]: the maximum that a row's weights of this tile are relative to
+  float ml[4][2][MR][2];      // [segment][warpgroup]: a row's maximum and sum of weights
+  float factor[MR];
   uint64_t upto[kMaxSeqs + 1];
-  uint64_t kfull[2], kempty[2], vfull[2], vclean[2], vempty[2], sfull[2], pfull[2], ofull[2], qfull, drain;
+  uint64_t kfull[NS], kempty[NS], vfull[NS], vclean[NS], vempty[NS], sfull[2], pfull[2], ofull[2], ofree[2], lfull[4],
+      qfull, drain;
   uint32_t tmem;
 };
 
-template <int HD>
+template <int HD, uint32_t MR, uint32_t NS>
 __global__ void __launch_bounds__(kTcThreads, 1)
     k_attn_tree_tc(TreeParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
-  using Smem = TcSmem<HD>;
+  using Smem = TcSmem<HD, MR, NS>;
   extern __shared__ __align__(16) uint8_t raw[];
   Smem &sm = *reinterpret_cast<Smem *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   constexpr uint32_t BL = Smem::kBlock;
   const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
   pdl_trigger();
   if (t == 0) {
-    for (int i = 0; i < 2; i++) {
+    for (uint32_t i = 0; i < NS; i++) {
       mbar_init(&sm.kfull[i], 1);
       mbar_init(&sm.vfull[i], 1);
-      mbar_init(&sm.vclean[i], 64);
+      mbar_init(&sm.vclean[i], 32);
       mbar_init(&sm.kempty[i], 1);
       mbar_init(&sm.vempty[i], 1);
+    }
+    for (int i = 0; i < 2; i++) {
       mbar_init(&sm.sfull[i], 1);
-      mbar_init(&sm.pfull[i], 8);
+      mbar_init(&sm.pfull[i], 4);
       mbar_init(&sm.ofull[i], 1);
+      mbar_init(&sm.ofree[i], 4);
     }
     mbar_init(&sm.qfull, 8);
+    for (int i = 0; i < 4; i++) mbar_init(&sm.lfull[i], 8);
     mbar_init(&sm.drain, 1);
     fence_mbar_init();
   }
-  if (warp == 8) {
+  if (warp == 12) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   pdl_wait();
-  pairs_before<kTcRows, kTcTile, kTcThreads>(p, sm.upto);
+  pairs_before<MR, kTcTile, kTcThreads>(p, sm.upto);
   tc_before();
   __syncthreads();
   tc_after();
@@ -734,148 +761,164 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       atomicExch(p.err, 1u);
     }
   };
+  // which of the 64 positions from node `base32` (negative: committed) on a row of node `nd` may see
+  auto seen = [&](uint32_t base32, bool live, uint32_t nd, uint32_t first) -> uint64_t {
+    const int32_t base = (int32_t)base32;
+    const uint64_t past = low_bits(-(int64_t)base);
+    if (!live) return past;
+    if (!p.mask) return low_bits((int64_t)nd + 1 - base);
+    return past | (window(p.mask + (size_t)(first + nd) * p.words, p.words, base) & ~past);
+  };
 
-  if (warp >= 14) {
-    // ---- cleaners: the V rows of tiles that hold nodes ----
-    // A non-finite V row may only reach the rows that see its node, and a weight of 0 does not keep it out of a
-    // product: such elements (those of stale rows behind the last node too) become 0 here, and the softmax warps add
-    // them to the rows that see them.
+  if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    const uint32_t e = t - 448;
-    constexpr uint32_t CH = HD / 8;
-    uint32_t i = 0;
-    while (next_segment<kTcRows, kTcTile>(p, sm.upto, walk, g))
-      for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
-        if ((tile + 1) * kTcTile <= g.w.len) continue;
-        wait(&sm.vfull[i & 1], i >> 1);
-        if (e < 4) sm.odd[i & 7][e] = 0;  // tile i - 8 is long folded: this one's copy waited for P V of tile i - 2
-        named_sync<2, 64>();
-        for (uint32_t c = e; c < kTcTile * CH; c += 64) {
-          const uint32_t r = c / CH, ch = c % CH;
-          uint4 *at = reinterpret_cast<uint4 *>(sm.vt[i & 1] + (ch / 8) * BL + r * 128 + (((ch % 8) ^ (r & 7)) << 4));
-          uint4 v = *at;
-          uint32_t *cw = reinterpret_cast<uint32_t *>(&v);
-          bool bad = false;
+    if (warp == 15) {
+      // ---- cleaner: V tiles on their way to the MMAs, the rows of those that hold nodes ----
+      // (It hands every tile over: a barrier that it watched for some phases only could be two phases on.)
+      // A non-finite V row may only reach the rows that see its node, and a weight of 0 does not keep it out of a
+      // product: such elements (those of stale rows behind the last node too) become 0 here, and the folding warps
+      // add them to the rows that see them.
+      constexpr uint32_t CH = HD / 8;
+      uint32_t i = 0;
+      while (next_segment<MR, kTcTile>(p, sm.upto, walk, g))
+        for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
+          const uint32_t sl = i % NS;
+          wait(&sm.vfull[sl], i / NS);
+          if ((tile + 1) * kTcTile <= g.w.len) {
+            mbar_arrive(&sm.vclean[sl]);
+            continue;
+          }
+          uint32_t any[4] = {0, 0, 0, 0};
+          // a lane has rows lane, lane + 32, ..: its rows of a word are one bit each
 #pragma unroll
-          for (int x = 0; x < 4; x++) {
-            if ((cw[x] & 0x7C00u) == 0x7C00u) cw[x] &= 0xFFFF0000u, bad = true;
-            if ((cw[x] & 0x7C000000u) == 0x7C000000u) cw[x] &= 0xFFFFu, bad = true;
-          }
-          if (bad) {
-            *at = v;
-            atomicOr(&sm.odd[i & 7][r / 32], 1u << (r % 32));
-          }
-        }
-        fence_proxy_async();
-        mbar_arrive(&sm.vclean[i & 1]);
-      }
-  } else if (warp >= 12) {
-    // ---- copies: warp 12 the K tiles, 13 the V tiles; a lane a chunk of p.chunk positions, which lie in one page ----
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    const bool is_v = warp == 13;
-    const CUtensorMap *map = is_v ? &vmap : &kmap;
-    uint64_t *full = is_v ? sm.vfull : sm.kfull, *empty = is_v ? sm.vempty : sm.kempty;
-    const uint32_t chunks = kTcTile / p.chunk, chunk = p.chunk, P = p.c.page_tokens;
-    uint32_t i = 0;  // tiles of the run so far
-    while (next_segment<kTcRows, kTcTile>(p, sm.upto, walk, g)) {
-      const uint32_t total = g.w.len + g.w.nodes;
-      // where the lane's chunk of a tile lies: page (n_pages for a hole, which reads zeros), first row; -1: behind the
-      // last position, not copied
-      int32_t page, row;
-      auto find = [&](uint32_t tile) {
-        const uint32_t pos = tile * kTcTile + lane * chunk;
-        page = -1, row = 0;
-        if (lane < chunks && tile < g.tile1 && pos < total) {
-          const uint32_t pg = pos / P;
-          uint32_t x = p.c.n_pages;
-          if (pg < p.c.max_pages) x = p.c.table ? (uint32_t)p.c.table[(size_t)g.s * p.c.max_pages + pg] : g.s;
-          page = (int32_t)min(x, p.c.n_pages);
-          row = (int32_t)(pos - pg * P);
-        }
-      };
-      find(g.tile0);
-      for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
-        const int32_t at = page, r = row;
-        find(tile + 1);  // the next tile's table entries come while this one is copied
-        const uint32_t copied = __ballot_sync(0xffffffffu, at >= 0);
-        if (i >= 2) wait(&empty[i & 1], (i >> 1) - 1);
-        __syncwarp();
-        if (!is_v) {
-          const uint32_t there = __ballot_sync(0xffffffffu, at >= 0 && at < (int32_t)p.c.n_pages);
-          if (lane < 4) {  // the word of positions 32 lane .. + 31
-            const uint32_t cap = min(total, p.c.max_pages * P), pos = tile * kTcTile + 32 * lane;
-            uint32_t bits = 0;
-            if (chunk >= 32) {
-              bits = (there >> (32 * lane / chunk)) & 1 ? 0xFFFFFFFFu : 0u;
-            } else {
-              for (uint32_t c = 0; c < 32 / chunk; c++)
-                if ((there >> (32 / chunk * lane + c)) & 1) bits |= ((1u << chunk) - 1) << (c * chunk);
+          for (uint32_t x = 0; x < 4; x++) {
+            const uint32_t r = 32 * x + lane;
+            bool bad = false;
+#pragma unroll 4
+            for (uint32_t ch = 0; ch < CH; ch++) {
+              uint4 *at = reinterpret_cast<uint4 *>(sm.vt[sl] + (ch / 8) * BL + r * 128 + (((ch % 8) ^ (r & 7)) << 4));
+              uint4 v = *at;
+              uint32_t *cw = reinterpret_cast<uint32_t *>(&v);
+              bool here = false;
+#pragma unroll
+              for (int y = 0; y < 4; y++) {
+                if ((cw[y] & 0x7C00u) == 0x7C00u) cw[y] &= 0xFFFF0000u, here = true;
+                if ((cw[y] & 0x7C000000u) == 0x7C000000u) cw[y] &= 0xFFFFu, here = true;
+              }
+              if (here) *at = v;
+              bad |= here;
             }
-            sm.valid[i & 7][lane] = bits & (uint32_t)low_bits((int64_t)cap - pos);
+            any[x] = __ballot_sync(0xffffffffu, bad);
           }
-          __syncwarp();
+          if (lane < 4) sm.odd[i & 7][lane] = lane == 0 ? any[0] : lane == 1 ? any[1] : lane == 2 ? any[2] : any[3];
+          fence_proxy_async();
+          mbar_arrive(&sm.vclean[sl]);
         }
-        if (ok) {
-          uint8_t *dst = (is_v ? sm.vt : sm.kt)[i & 1] + lane * chunk * 128;
-          if (lane == 0) mbar_expect_tx(&full[i & 1], __popc(copied) * chunk * HD * 2);
+    } else if (warp >= 13) {
+      // ---- copies: warp 13 the K tiles, 14 the V tiles; a lane a chunk of p.chunk positions, which lie in one page ----
+      const bool is_v = warp == 14;
+      const CUtensorMap *map = is_v ? &vmap : &kmap;
+      uint64_t *full = is_v ? sm.vfull : sm.kfull, *empty = is_v ? sm.vempty : sm.kempty;
+      const uint32_t chunks = kTcTile / p.chunk, chunk = p.chunk, P = p.c.page_tokens;
+      uint32_t i = 0;  // tiles of the run so far
+      while (next_segment<MR, kTcTile>(p, sm.upto, walk, g)) {
+        const uint32_t total = g.w.len + g.w.nodes;
+        // where the lane's chunk of a tile lies: page (n_pages for a hole, which reads zeros), first row; -1: behind
+        // the last position, not copied
+        int32_t page, row;
+        auto find = [&](uint32_t tile) {
+          const uint32_t pos = tile * kTcTile + lane * chunk;
+          page = -1, row = 0;
+          if (lane < chunks && tile < g.tile1 && pos < total) {
+            const uint32_t pg = pos / P;
+            uint32_t x = p.c.n_pages;
+            if (pg < p.c.max_pages) x = p.c.table ? (uint32_t)p.c.table[(size_t)g.s * p.c.max_pages + pg] : g.s;
+            page = (int32_t)min(x, p.c.n_pages);
+            row = (int32_t)(pos - pg * P);
+          }
+        };
+        find(g.tile0);
+        for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
+          const uint32_t sl = i % NS;
+          const int32_t at = page, r = row;
+          find(tile + 1);  // the next tile's table entries come while this one is copied
+          const uint32_t copied = __ballot_sync(0xffffffffu, at >= 0);
+          const uint32_t there = __ballot_sync(0xffffffffu, at >= 0 && at < (int32_t)p.c.n_pages);
+          if (i >= NS) wait(&empty[sl], i / NS - 1);
           __syncwarp();
-          if (at >= 0) {
+          if (!is_v) {
+            if (lane < 4) {  // the word of positions 32 lane .. + 31
+              const uint32_t cap = min(total, p.c.max_pages * P), pos = tile * kTcTile + 32 * lane;
+              uint32_t bits = 0;
+              if (chunk >= 32) {
+                bits = (there >> (32 * lane / chunk)) & 1 ? 0xFFFFFFFFu : 0u;
+              } else {
+                for (uint32_t c = 0; c < 32 / chunk; c++)
+                  if ((there >> (32 / chunk * lane + c)) & 1) bits |= ((1u << chunk) - 1) << (c * chunk);
+              }
+              sm.valid[i & 7][lane] = bits & (uint32_t)low_bits((int64_t)cap - pos);
+            }
+            __syncwarp();
+          }
+          if (ok) {
+            uint8_t *dst = (is_v ? sm.vt : sm.kt)[sl] + lane * chunk * 128;
+            if (lane == 0) mbar_expect_tx(&full[sl], __popc(copied) * chunk * HD * 2);
+            __syncwarp();
+            if (at >= 0) {
 #pragma unroll
-            for (uint32_t b = 0; b < HD / 64; b++) tma_load(dst + b * BL, map, 64 * b, r, g.kvh, at, &full[i & 1]);
+              for (uint32_t b = 0; b < HD / 64; b++) tma_load(dst + b * BL, map, 64 * b, r, g.kvh, at, &full[sl]);
+            }
           }
+          __syncwarp();
         }
-        __syncwarp();
       }
-    }
-    // the last copies land before the block ends, whatever became of the others
-    ok = true;
-    if (i >= 2) wait(&full[i & 1], (i - 2) >> 1);
-    if (i >= 1) wait(&full[(i - 1) & 1], (i - 1) >> 1);
-  } else if (warp >= 8) {
-    // ---- MMA issue ----
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 8) {
+      // the last copies land before the block ends, whatever became of the others
+      ok = true;
+      for (uint32_t n = i < NS ? 0 : i - NS; n < i; n++) wait(&full[n % NS], n / NS);
+    } else {
+      // ---- MMA issue ----
       const uint32_t leader = elect_one();
       const uint64_t qd = desc_k(smem_u32(sm.q[0])), kd = desc_k(smem_u32(sm.kt[0])), vd = desc_mn(smem_u32(sm.vt[0]), BL);
-      constexpr uint64_t kPart = Smem::kTileBytes >> 4;  // from one part of Q, or one tile, to the next, in 16 bytes
-      uint32_t i = 0, seg = 0, cleaned[2] = {0, 0};
+      constexpr uint64_t kTileStep = Smem::kTileBytes >> 4, kQStep = Smem::kQBytes >> 4;  // in 16 bytes
+      uint32_t i = 0, seg = 0;
       auto scores = [&](uint32_t n) {  // S = Q K^T of tile n: both parts of Q
-        wait(&sm.kfull[n & 1], n >> 1);
+        wait(&sm.kfull[n % NS], n / NS);
         tc_after();
-        const uint64_t kb = kd + (n & 1) * kPart;
+        const uint64_t kb = kd + (n % NS) * kTileStep;
         const uint32_t d = tmem + 128 * (n & 1);
         if (ok) {
 #pragma unroll
           for (uint32_t k = 0; k < HD / 16; k++) {
-            const uint64_t off = ((k / 4) * BL + (k % 4) * 32) >> 4;
-            tc_mma_ss(leader, d, qd + off, kb + off, idesc_f16(kTcTile, false), k > 0);
-            tc_mma_ss(leader, d, qd + kPart + off, kb + off, idesc_f16(kTcTile, false), true);
+            const uint64_t qo = ((k / 4) * Smem::kQBlock + (k % 4) * 32) >> 4, ko = ((k / 4) * BL + (k % 4) * 32) >> 4;
+            tc_mma_ss(leader, d, qd + qo, kb + ko, idesc_f16(kTcTile, false), k > 0);
+            tc_mma_ss(leader, d, qd + kQStep + qo, kb + ko, idesc_f16(kTcTile, false), true);
           }
           tc_commit(leader, &sm.sfull[n & 1]);
-          tc_commit(leader, &sm.kempty[n & 1]);
+          tc_commit(leader, &sm.kempty[n % NS]);
         }
         __syncwarp();
       };
-      while (next_segment<kTcRows, kTcTile>(p, sm.upto, walk, g)) {
+      while (next_segment<MR, kTcTile>(p, sm.upto, walk, g)) {
         wait(&sm.qfull, seg++);
         scores(i);
         for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
+          const uint32_t sl = i % NS;
           if (tile + 1 < g.tile1) scores(i + 1);
+          if (i >= 2) wait(&sm.ofree[i & 1], (i >> 1) - 1);
           wait(&sm.pfull[i & 1], i >> 1);
-          wait(&sm.vfull[i & 1], i >> 1);
-          if ((tile + 1) * kTcTile > g.w.len) wait(&sm.vclean[i & 1], i & 1 ? cleaned[1]++ : cleaned[0]++);
+          wait(&sm.vclean[sl], i / NS);
           tc_after();
-          const uint64_t vb = vd + (i & 1) * kPart;
+          const uint64_t vb = vd + sl * kTileStep;
           const uint32_t a = tmem + 128 * (i & 1), d = tmem + 256 + 128 * (i & 1);
           if (ok) {  // this tile's P V, from zero: the sum over tiles is made in registers, where it is rounded
 #pragma unroll
             for (uint32_t k = 0; k < kTcTile / 16; k++) {
-              const uint32_t at = a + 32 * (k / 2) + 8 * (k % 2);
+              const uint32_t at = a + 16 * k;  // 8 words of parts, 8 of remainders
               tc_mma_ts(leader, d, at, vb + k * (2048 >> 4), idesc_f16(HD, true), k > 0);
-              tc_mma_ts(leader, d, at + 16, vb + k * (2048 >> 4), idesc_f16(HD, true), true);
+              tc_mma_ts(leader, d, at + 8, vb + k * (2048 >> 4), idesc_f16(HD, true), true);
             }
             tc_commit(leader, &sm.ofull[i & 1]);
-            tc_commit(leader, &sm.vempty[i & 1]);
+            tc_commit(leader, &sm.vempty[sl]);
           }
           __syncwarp();
         }
@@ -886,38 +929,126 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       wait(&sm.drain, 0);
       __syncwarp();
     }
+  } else if (warp >= 8) {
+    // ---- fold: P V of the tiles, in order, into a row's running output; a thread a row ----
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    const uint32_t r = t & 127, lanes = (warp & 3) * 32 << 16;
+    uint32_t i = 0, seg = 0;
+    while (next_segment<MR, kTcTile>(p, sm.upto, walk, g)) {
+      const uint32_t rows = min(MR, g.w.nodes * p.g - g.block * MR);
+      const bool work = (warp & 3) * 32 < rows;  // a warp whose rows are all past the last one keeps step only
+      const uint32_t rr = g.block * MR + r, nd = rr / p.g;
+      const bool live = r < rows;
+      float o[HD], M = -INFINITY;
+#pragma unroll
+      for (int d = 0; d < HD; d++) o[d] = 0.0f;
+      for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
+        wait(&sm.ofull[i & 1], i >> 1);
+        __syncwarp();
+        tc_after();
+        if (work) {
+          // the weights of even and odd tiles are relative to maxima of their own
+          const float mt = sm.mrow[i & 3][r], mn = fmaxf(M, mt);
+          const float a = M == mn ? 1.0f : ex2(M - mn), b = mt == mn ? 1.0f : ex2(mt - mn);
+          M = mn;
+          const uint32_t oa = tmem + lanes + 256 + 128 * (i & 1);
+          const bool plain = __all_sync(0xffffffffu, a == 1.0f && b == 1.0f);
+#pragma unroll
+          for (int c = 0; c < HD / 16; c++) {
+            uint32_t v[16];
+            tc_ld16(oa + 16 * c, v);
+            if (plain) {
+#pragma unroll
+              for (int d = 0; d < 16; d++) o[16 * c + d] += __uint_as_float(v[d]);
+            } else {
+#pragma unroll
+              for (int d = 0; d < 16; d++) o[16 * c + d] = fmaf(o[16 * c + d], a, __uint_as_float(v[d]) * b);
+            }
+          }
+        }
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.ofree[i & 1]);
+        if (work && (tile + 1) * kTcTile > g.w.len) {
+          // non-finite V elements of nodes that this row sees
+#pragma unroll 1
+          for (int x = 0; x < 4; x++) {
+            uint32_t left = sm.odd[i & 7][x] & sm.valid[i & 7][x];
+            if (left) left &= (uint32_t)(seen(tile * kTcTile + 32 * x - g.w.len, live, nd, g.w.first));
+#pragma unroll 1
+            for (; left; left &= left - 1) {
+              const int64_t at_row = kv_row(p.c, g.s, tile * kTcTile + 32 * x + __ffs(left) - 1);
+              const __half2 *vr = reinterpret_cast<const __half2 *>(p.c.v + (size_t)g.kvh * p.c.head_stride + at_row);
+#pragma unroll
+              for (int d = 0; d < HD / 2; d++) {
+                const float2 f = __half22float2(vr[d]);
+                if (!isfinite(f.x)) o[2 * d] += f.x;
+                if (!isfinite(f.y)) o[2 * d + 1] += f.y;
+              }
+            }
+          }
+          __syncwarp();
+        }
+      }
+      wait(&sm.lfull[seg & 3], seg >> 2);  // the softmax warps may be two segments ahead, never four
+      __syncwarp();
+      const bool whole = g.whole();
+      if (live) {
+        float L = 0.0f;
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+          const float my = sm.ml[seg & 3][y][r][0];
+          if (my != -INFINITY) L = fmaf(sm.ml[seg & 3][y][r][1], my == M ? 1.0f : ex2(my - M), L);
+        }
+        const uint64_t slot = 2 * cta + (begin >= g.unit0 ? 0 : 1);
+        const float scale = whole ? (L != 0.0f ? 1.0f / L : 0.0f) : 1.0f;  // a row that sees nothing gets zeros
+        // whole units go to their rows of out; parts lie [hd / 4][row] float4
+        float *dst = whole ? p.out + ((size_t)(g.w.first + nd) * p.h + g.kvh * p.g + rr % p.g) * HD
+                           : p.part_o + (slot * (HD / 4) * MR + r) * 4;
+        const uint32_t step = whole ? 4 : 4 * MR;
+#pragma unroll
+        for (int d = 0; d < HD; d += 4)
+          *reinterpret_cast<float4 *>(dst + (size_t)(d / 4) * step) =
+              make_float4(o[d] * scale, o[d + 1] * scale, o[d + 2] * scale, o[d + 3] * scale);
+        if (!whole) {
+          p.part_ml[(slot * MR + r) * 2] = M;
+          p.part_ml[(slot * MR + r) * 2 + 1] = L;
+        }
+      }
+      if (g.tile0 == 0 && r == 0) {
+        // for the joining kernel: how many CTAs hold parts of the unit (0: it is whole), and the first one's slot
+        const uint64_t c0 = ((g.unit0 + 1) * grid - 1) / all, c1 = ((g.unit0 + g.w.tiles) * grid - 1) / all;
+        uint32_t *u = p.units + 2 * (((size_t)g.s * p.c.hk + g.kvh) * p.max_blocks + g.block);
+        u[0] = whole ? 0 : (uint32_t)(c1 - c0 + 1);
+        u[1] = (uint32_t)(2 * c0 + (c0 * all / grid < g.unit0 ? 1 : 0));
+      }
+      seg++;
+    }
   } else {
-    // ---- softmax: a thread a row, warpgroup wg half of the positions and half of the dims ----
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    // ---- softmax: warpgroup wg has every other tile of the run, a thread a row ----
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
     const uint32_t wg = warp >> 2, r = t & 127;
-    const uint32_t lanes = (warp & 3) * 32 << 16;
-    uint32_t i = 0;
-    // which of the 64 positions from node `base` (negative: committed) on a row of node `nd` may see
-    auto seen = [&](uint32_t base32, bool live, uint32_t nd, uint32_t first) -> uint64_t {
-      const int32_t base = (int32_t)base32;
-      const uint64_t past = low_bits(-(int64_t)base);
-      if (!live) return past;
-      if (!p.mask) return low_bits((int64_t)nd + 1 - base);
-      return past | (window(p.mask + (size_t)(first + nd) * p.words, p.words, base) & ~past);
-    };
-    while (next_segment<kTcRows, kTcTile>(p, sm.upto, walk, g)) {
-      const uint32_t rows = min(kTcRows, g.w.nodes * p.g - g.block * kTcRows);
+    const uint32_t sa = tmem + ((warp & 3) * 32 << 16) + 128 * wg;
+    uint32_t i = 0, seg = 0;
+    while (next_segment<MR, kTcTile>(p, sm.upto, walk, g)) {
+      const uint32_t rows = min(MR, g.w.nodes * p.g - g.block * MR);
       // Q into shared memory, a power of two and two fp16 parts a row; the last segment's products are done
       {
-        constexpr uint32_t LR = HD / 4, RW = 32 / LR;  // lanes of a row, rows of a warp's access
+        constexpr uint32_t LR = HD / 4, RW = 32 / LR, WR = MR / 8;  // lanes of a row, rows of an access, rows of a warp
+        constexpr uint32_t UN = WR / RW < 4 ? WR / RW : 4;
         const uint32_t d4 = lane % LR;
-        for (uint32_t b0 = 0; b0 < 16; b0 += 4 * RW) {
-          float4 f[4];
+        for (uint32_t b0 = 0; b0 < WR; b0 += UN * RW) {
+          float4 f[UN];
 #pragma unroll
-          for (uint32_t u = 0; u < 4; u++) {
-            const uint32_t rl = warp * 16 + b0 + u * RW + lane / LR, rr = g.block * kTcRows + rl, nd = rr / p.g;
+          for (uint32_t u = 0; u < UN; u++) {
+            const uint32_t rl = warp * WR + b0 + u * RW + lane / LR, rr = g.block * MR + rl;
             f[u] = rl < rows ? *reinterpret_cast<const float4 *>(
-                                   p.q + ((size_t)(g.w.first + nd) * p.h + g.kvh * p.g + rr % p.g) * HD + 4 * d4)
+                                   p.q + ((size_t)(g.w.first + rr / p.g) * p.h + g.kvh * p.g + rr % p.g) * HD + 4 * d4)
                              : make_float4(0.f, 0.f, 0.f, 0.f);
           }
 #pragma unroll
-          for (uint32_t u = 0; u < 4; u++) {
-            const uint32_t rl = warp * 16 + b0 + u * RW + lane / LR;
+          for (uint32_t u = 0; u < UN; u++) {
+            const uint32_t rl = warp * WR + b0 + u * RW + lane / LR;
             float top = fmaxf(fmaxf(fabsf(f[u].x), fabsf(f[u].y)), fmaxf(fabsf(f[u].z), fabsf(f[u].w)));
 #pragma unroll
             for (uint32_t o = LR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -926,7 +1057,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             uint2 hi, lo;
             split_f16(f[u].x * down, f[u].y * down, hi.x, lo.x);
             split_f16(f[u].z * down, f[u].w * down, hi.y, lo.y);
-            const uint32_t at = (d4 / 16) * BL + rl * 128 + (((d4 % 16) / 2 ^ (rl & 7)) << 4) + (d4 & 1) * 8;
+            const uint32_t at = (d4 / 16) * Smem::kQBlock + rl * 128 + (((d4 % 16) / 2 ^ (rl & 7)) << 4) + (d4 & 1) * 8;
             *reinterpret_cast<uint2 *>(sm.q[0] + at) = hi;
             *reinterpret_cast<uint2 *>(sm.q[1] + at) = lo;
             if (d4 == 0) sm.factor[rl] = p.scale * up;
@@ -937,155 +1068,99 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (lane == 0) mbar_arrive(&sm.qfull);
         named_sync<1, 256>();
       }
-      const float factor = sm.factor[r];
-      const bool work = (warp & 3) * 32 < rows;  // a warp whose rows are all past the last one keeps step only
-      const uint32_t rr = g.block * kTcRows + r, nd = rr / p.g;
-      const bool live = r < rows;
-      float o[HD / 2], m = -INFINITY, l = 0.0f, corr = 1.0f;
-#pragma unroll
-      for (int d = 0; d < HD / 2; d++) o[d] = 0.0f;
-      // add the P V of tile n (the n-th of the run) to this thread's half of the dims; `tile` its number in the unit
-      auto fold = [&](uint32_t n, uint32_t tile, uint64_t sees0, uint64_t sees1) {
-        wait(&sm.ofull[n & 1], n >> 1);
-        __syncwarp();
-        tc_after();
-        if (work) {
-          const uint32_t oa = tmem + lanes + 256 + 128 * (n & 1) + wg * (HD / 2);
-          uint32_t v[HD / 2];
-#pragma unroll
-          for (int c = 0; c < HD / 64; c++) tc_ld32(oa + 32 * c, v + 32 * c);
-          tc_ld_wait();
-#pragma unroll
-          for (int d = 0; d < HD / 2; d++) o[d] = fmaf(o[d], corr, __uint_as_float(v[d]));
-          if ((tile + 1) * kTcTile > g.w.len) {
-            // non-finite V elements of nodes that this row sees
-#pragma unroll 1
-            for (int x = 0; x < 4; x++)
-#pragma unroll 1
-              for (uint32_t left = sm.odd[n & 7][x] & (uint32_t)((x < 2 ? sees0 : sees1) >> (32 * (x & 1))); left;
-                   left &= left - 1) {
-                const int64_t at_row = kv_row(p.c, g.s, tile * kTcTile + 32 * x + __ffs(left) - 1);
-                const __half2 *vr =
-                    reinterpret_cast<const __half2 *>(p.c.v + (size_t)g.kvh * p.c.head_stride + at_row + wg * (HD / 2));
-#pragma unroll
-                for (int d = 0; d < HD / 4; d++) {
-                  const float2 f = __half22float2(vr[d]);
-                  if (!isfinite(f.x)) o[2 * d] += f.x;
-                  if (!isfinite(f.y)) o[2 * d + 1] += f.y;
-                }
-              }
-          }
-        }
-        __syncwarp();
-        tc_before();
-      };
-      uint64_t sees0 = 0, sees1 = 0;  // of the tile that is folded next
+      const bool work = (warp & 3) * 32 < rows, live = r < rows;
+      const float factor = work ? sm.factor[r] : 0.0f;
+      const uint32_t nd = (g.block * MR + r) / p.g;
+      float m = -INFINITY, l = 0.0f;
       for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
-        const uint32_t sa = tmem + lanes + 128 * (i & 1) + 64 * wg;
-        wait(&sm.sfull[i & 1], i >> 1);
+        if ((i & 1) != wg) continue;
+        wait(&sm.sfull[wg], i >> 1);
         __syncwarp();
         tc_after();
-        float corr1 = 1.0f;
-        uint64_t now0 = 0, now1 = 0;
         if (work) {
-          uint32_t v[64];
-          tc_ld32(sa, v);
-          tc_ld32(sa + 32, v + 32);
+          // Two passes over the scores in steps of 64, rolled: unrolled over the tile, the code of the three
+          // warps that share a scheduler outgrew the instruction cache (4 of 14 stalled warps waited for
+          // instructions, and a tile took 4000 cycles).
           const bool drafted = (tile + 1) * kTcTile > g.w.len;
-          const uint64_t ok0 = (uint64_t)sm.valid[i & 7][0] | (uint64_t)sm.valid[i & 7][1] << 32;
-          const uint64_t ok1 = (uint64_t)sm.valid[i & 7][2] | (uint64_t)sm.valid[i & 7][3] << 32;
-          const bool masked = drafted || (ok0 & ok1) != ~0ull;
-          now0 = ok0, now1 = ok1;
-          if (drafted) {
-            now0 &= seen(tile * kTcTile - g.w.len, live, nd, g.w.first);
-            now1 &= seen(tile * kTcTile + 64 - g.w.len, live, nd, g.w.first);
-          }
-          tc_ld_wait();
-          if (masked) {
-            const uint64_t bits = wg ? now1 : now0;
-            const uint32_t b0 = (uint32_t)bits, b1 = (uint32_t)(bits >> 32);
-#pragma unroll
-            for (int e = 0; e < 64; e++)
-              if (!(((e < 32 ? b0 : b1) >> (e & 31)) & 1)) v[e] = 0xFF800000u;  // -inf
-          }
+          const uint32_t *ok4 = sm.valid[i & 7];
+          const bool masked = drafted || (ok4[0] & ok4[1] & ok4[2] & ok4[3]) != ~0u;
           float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+          for (uint32_t h = 0; h < 128; h += 64) {
+            uint32_t v[64];
+            tc_ld32(sa + h, v);
+            tc_ld32(sa + h + 32, v + 32);
+            tc_ld_wait(v);
+            tc_ld_wait(v + 32);
+            if (masked) {  // unseen positions become -inf, for the second pass too
+              uint64_t see = (uint64_t)ok4[h / 32] | (uint64_t)ok4[h / 32 + 1] << 32;
+              if (drafted) see &= seen(tile * kTcTile + h - g.w.len, live, nd, g.w.first);
+              const uint32_t b0 = (uint32_t)see, b1 = (uint32_t)(see >> 32);
 #pragma unroll
-          for (int e = 0; e < 64; e += 8)
+              for (int e = 0; e < 64; e++)
+                if (!(((e < 32 ? b0 : b1) >> (e & 31)) & 1)) v[e] = 0xFF800000u;
 #pragma unroll
-            for (int u = 0; u < 4; u++)
-              t4[u] = fmaxf(t4[u], fmaxf(__uint_as_float(v[e + 2 * u]), __uint_as_float(v[e + 2 * u + 1])));
-          float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
-          // the row's other 64 positions are the other warpgroup's
-          sm.top[i & 1][wg][r] = top;
-          asm volatile("bar.sync %0, 64;" ::"r"(4 + (warp & 3)) : "memory");
-          top = fmaxf(top, sm.top[i & 1][1 - wg][r]);
-          const float mn = fmaxf(m, top * factor);
-          corr1 = m == mn ? 1.0f : ex2(m - mn);
+              for (int e = 0; e < 64; e += 16) tc_st16(sa + h + e, v + e);
+            }
+#pragma unroll
+            for (int e = 0; e < 64; e += 8)
+#pragma unroll
+              for (int u = 0; u < 4; u++)
+                t4[u] = fmaxf(t4[u], fmaxf(__uint_as_float(v[e + 2 * u]), __uint_as_float(v[e + 2 * u + 1])));
+          }
+          if (masked) asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          const float mn = fmaxf(m, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * factor);
+          const float corr = m == mn ? 1.0f : ex2(m - mn);
           m = mn;
+          sm.mrow[i & 3][r] = mn;
+          __syncwarp();
           const float sub = mn == -INFINITY ? 0.0f : mn - kPShift;
           float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+          for (uint32_t h = 0; h < 128; h += 64) {  // the weights, over the scores
+            uint32_t v[64];
+            tc_ld32(sa + h, v);
+            tc_ld32(sa + h + 32, v + 32);
+            tc_ld_wait(v);
+            tc_ld_wait(v + 32);
 #pragma unroll
-          for (int c = 0; c < 2; c++) {
-            uint32_t w[32];  // 16 words of parts, 16 of remainders
+            for (int c = 0; c < 64; c += 16) {
+              uint32_t w[16];  // 8 words of parts, 8 of remainders
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float p0 = ex2(fmaf(__uint_as_float(v[32 * c + e]), factor, -sub));
-              const float p1 = ex2(fmaf(__uint_as_float(v[32 * c + e + 1]), factor, -sub));
-              part[(e / 2) & 3] += p0 + p1;
-              split_f16(p0, p1, w[e / 2], w[16 + e / 2]);
+              for (int e = 0; e < 16; e += 2) {
+                const float p0 = ex2(fmaf(__uint_as_float(v[c + e]), factor, -sub));
+                const float p1 = ex2(fmaf(__uint_as_float(v[c + e + 1]), factor, -sub));
+                part[(e / 2) & 3] += p0 + p1;
+                split_f16(p0, p1, w[e / 2], w[8 + e / 2]);
+              }
+              tc_st16(sa + h + c, w);
             }
-            tc_st32(sa + 32 * c, w);
           }
-          l = l * corr1 + ((part[0] + part[1]) + (part[2] + part[3]));
+          l = l * corr + ((part[0] + part[1]) + (part[2] + part[3]));
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         }
         tc_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.pfull[i & 1]);
-        // the tile before, whose P V ran meanwhile
-        if (tile > g.tile0) fold(i - 1, tile - 1, sees0, sees1);
-        corr = corr1, sees0 = now0, sees1 = now1;
+        if (lane == 0) mbar_arrive(&sm.pfull[wg]);
       }
-      fold(i - 1, g.tile1 - 1, sees0, sees1);
-      // the two halves' sums of weights
-      sm.ml[wg][r] = l;
-      named_sync<1, 256>();
-      const float L = sm.ml[0][r] + sm.ml[1][r];
-      const bool whole = g.whole();
-      const uint64_t slot = 2 * cta + (begin >= g.unit0 ? 0 : 1);
-      const float scale = whole ? (L != 0.0f ? 1.0f / L : 0.0f) : 1.0f;
-      // whole units go to their rows of out; parts lie [hd / 4][row] float4
-      float *dst = whole ? p.out + ((size_t)(g.w.first + (live ? nd : 0)) * p.h + g.kvh * p.g + rr % p.g) * HD + wg * (HD / 2)
-                         : p.part_o + ((slot * (HD / 4) + wg * (HD / 8)) * kTcRows + r) * 4;
-      const uint32_t step = whole ? 4 : 4 * kTcRows;
-      if (live) {
-#pragma unroll
-        for (int d = 0; d < HD / 2; d += 4)
-          *reinterpret_cast<float4 *>(dst + (size_t)(d / 4) * step) =
-              make_float4(o[d] * scale, o[d + 1] * scale, o[d + 2] * scale, o[d + 3] * scale);
-        if (!whole && wg == 0) {
-          p.part_ml[(slot * kTcRows + r) * 2] = m;
-          p.part_ml[(slot * kTcRows + r) * 2 + 1] = L;
-        }
+      if (work) {
+        sm.ml[seg & 3][wg][r][0] = m;
+        sm.ml[seg & 3][wg][r][1] = l;
       }
-      if (g.tile0 == 0 && t == 0) {
-        // for the joining kernel: which CTAs hold parts of the unit (0 parts: none, it is whole)
-        const uint64_t c0 = ((g.unit0 + 1) * grid - 1) / all, c1 = ((g.unit0 + g.w.tiles) * grid - 1) / all;
-        uint32_t *u = p.units + 2 * (((size_t)g.s * p.c.hk + g.kvh) * p.max_blocks + g.block);
-        u[0] = whole ? 0 : (uint32_t)(c1 - c0 + 1);
-        u[1] = (uint32_t)(2 * c0 + (c0 * all / grid < g.unit0 ? 1 : 0));  // the first part's slot; the others' are even
-      }
-      named_sync<1, 256>();  // Q and the sums may be written again
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.lfull[seg & 3]);
+      named_sync<1, 256>();  // every score of the segment has been read: Q may be written again
+      seg++;
     }
   }
   tc_before();
   __syncthreads();
-  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
 // Join the parts of the units that several CTAs shared: CTA (unit, 8 rows), a thread 4 dims of a row.
 constexpr uint32_t kJoinRows = 8;
-template <int HD>
+template <int HD, uint32_t MR>
 __global__ void __launch_bounds__(kJoinRows * HD / 4) k_attn_tree_join(TreeParams p) {
   pdl_trigger();
   pdl_wait();
@@ -1093,9 +1168,9 @@ __global__ void __launch_bounds__(kJoinRows * HD / 4) k_attn_tree_join(TreeParam
   __shared__ float inv[kJoinRows];
   const uint32_t unit = blockIdx.x, block = unit % p.max_blocks, kvh = unit / p.max_blocks % p.c.hk;
   const uint32_t s = unit / p.max_blocks / p.c.hk, row0 = blockIdx.y * kJoinRows, t = threadIdx.x;
-  const SeqWork w = seq_work<kTcRows, kTcTile>(p, s);
+  const SeqWork w = seq_work<MR, kTcTile>(p, s);
   if (block >= w.blocks) return;
-  const uint32_t rows = min(kTcRows, w.nodes * p.g - block * kTcRows);
+  const uint32_t rows = min(MR, w.nodes * p.g - block * MR);
   const uint32_t parts = min(p.units[2 * unit], kTcGrid), first = p.units[2 * unit + 1];
   if (parts == 0 || row0 >= rows) return;
   auto slot = [&](uint32_t q) -> size_t { return q == 0 ? first : (first & ~1u) + 2 * q; };
@@ -1103,14 +1178,14 @@ __global__ void __launch_bounds__(kJoinRows * HD / 4) k_attn_tree_join(TreeParam
   for (uint32_t r = t >> 5; r < n; r += warps) {
     float M = -INFINITY;
     for (uint32_t q = lane; q < parts; q += 32) {
-      ws[r][q] = p.part_ml[(slot(q) * kTcRows + row0 + r) * 2];
+      ws[r][q] = p.part_ml[(slot(q) * MR + row0 + r) * 2];
       M = fmaxf(M, ws[r][q]);
     }
     M = warp_max(M);
     float L = 0.0f;
     for (uint32_t q = lane; q < parts; q += 32) {
       const float e = ws[r][q] == -INFINITY ? 0.0f : ex2(ws[r][q] - M);
-      L = fmaf(p.part_ml[(slot(q) * kTcRows + row0 + r) * 2 + 1], e, L);
+      L = fmaf(p.part_ml[(slot(q) * MR + row0 + r) * 2 + 1], e, L);
       ws[r][q] = e;
     }
     L = warp_sum(L);
@@ -1125,7 +1200,7 @@ __global__ void __launch_bounds__(kJoinRows * HD / 4) k_attn_tree_join(TreeParam
 #pragma unroll
     for (int u = 0; u < 8; u++)
       if (q0 + u < parts)
-        f[u] = *reinterpret_cast<const float4 *>(p.part_o + ((slot(q0 + u) * (HD / 4) + d4) * kTcRows + row0 + r) * 4);
+        f[u] = *reinterpret_cast<const float4 *>(p.part_o + ((slot(q0 + u) * (HD / 4) + d4) * MR + row0 + r) * 4);
 #pragma unroll
     for (int u = 0; u < 8; u++)
       if (q0 + u < parts) {
@@ -1134,7 +1209,7 @@ __global__ void __launch_bounds__(kJoinRows * HD / 4) k_attn_tree_join(TreeParam
         acc.z = fmaf(f[u].z, y, acc.z), acc.w = fmaf(f[u].w, y, acc.w);
       }
   }
-  const uint32_t rr = block * kTcRows + row0 + r;
+  const uint32_t rr = block * MR + row0 + r;
   const float y = inv[r];
   *reinterpret_cast<float4 *>(p.out + ((size_t)(w.first + rr / p.g) * p.h + kvh * p.g + rr % p.g) * HD + 4 * d4) =
       make_float4(acc.x * y, acc.y * y, acc.z * y, acc.w * y);
@@ -1153,34 +1228,34 @@ bool plane_map(const TreeParams &p, const __half *plane, CUtensorMap *map) {
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int HD>
+template <int HD, uint32_t MR, uint32_t NS>
 pai_status_t launch_tree_tc(pai_b200_ctx_t *ctx, TreeParams &p, const CUtensorMap &kmap, const CUtensorMap &vmap) {
-  constexpr size_t smem = sizeof(TcSmem<HD>) + 1024;
+  constexpr size_t smem = sizeof(TcSmem<HD, MR, NS>) + 1024;
   static SmemOptIn opt;
   pai_status_t st = b200_cuda(opt.ensure(b200_ctx_device(ctx), smem,
                                          [](size_t b) {
-                                           return cudaFuncSetAttribute(k_attn_tree_tc<HD>,
+                                           return cudaFuncSetAttribute(k_attn_tree_tc<HD, MR, NS>,
                                                                        cudaFuncAttributeMaxDynamicSharedMemorySize, (int)b);
                                          }),
                               "k_attn_tree_tc smem attribute");
   if (st) return st;
-  p.max_blocks = (p.max_nodes * p.g + kTcRows - 1) / kTcRows;
+  p.max_blocks = (p.max_nodes * p.g + MR - 1) / MR;
   const uint64_t units = (uint64_t)p.c.n_seq * p.c.hk * p.max_blocks;
   if (units > 0x7FFFFFFu) return b200_fail(PAI_ERR_UNSUPPORTED, "attn_tree: %llu row tiles", (unsigned long long)units);
   const uint64_t pairs = units * (((uint64_t)p.c.max_pages * p.c.page_tokens + p.max_nodes + kTcTile - 1) / kTcTile);
   const uint32_t grid = (uint32_t)std::min<uint64_t>(kTcGrid, pairs);
   float *scratch;
   const uint64_t slots = 2ull * grid;
-  st = b200_ctx_scratch(ctx, slots * kTcRows * (HD + 2) + 2 * units, 1, &scratch, &p.cnt);
+  st = b200_ctx_scratch(ctx, slots * MR * (HD + 2) + 2 * units, 1, &scratch, &p.cnt);
   if (st) return st;
   p.part_o = scratch;
-  p.part_ml = scratch + slots * kTcRows * HD;
-  p.units = (uint32_t *)(p.part_ml + slots * kTcRows * 2);
-  b200_launch(ctx, k_attn_tree_tc<HD>, dim3(grid), dim3(kTcThreads), smem, p, kmap, vmap);
+  p.part_ml = scratch + slots * MR * HD;
+  p.units = (uint32_t *)(p.part_ml + slots * MR * 2);
+  b200_launch(ctx, k_attn_tree_tc<HD, MR, NS>, dim3(grid), dim3(kTcThreads), smem, p, kmap, vmap);
   // the joining kernel is resident before this one ends, and waits for it
   const int pdl = b200_ctx_pdl(ctx);
   b200_ctx_set_pdl(ctx, 1);
-  b200_launch(ctx, k_attn_tree_join<HD>, dim3((uint32_t)units, kTcRows / kJoinRows), dim3(kJoinRows * HD / 4), 0, p);
+  b200_launch(ctx, k_attn_tree_join<HD, MR>, dim3((uint32_t)units, MR / kJoinRows), dim3(kJoinRows * HD / 4), 0, p);
   b200_ctx_set_pdl(ctx, pdl);
   return b200_launched(ctx, 2, "k_attn_tree_tc");
 }
@@ -1216,14 +1291,14 @@ pai_status_t launch_tree(pai_b200_ctx_t *ctx, TreeParams &p) {
 
 template <int HD>
 pai_status_t launch_tree_hd(pai_b200_ctx_t *ctx, TreeParams &p) {
+  const uint32_t rows = p.max_nodes * p.g;
   // tensor copies take whole shares of a page, a power of two of at least 8 positions
   p.chunk = 128;
   if (p.c.table)
     while (p.chunk > 8 && p.c.page_tokens % p.chunk) p.chunk /= 2;
   CUtensorMap kmap, vmap;
   if ((!p.c.table || p.c.page_tokens % p.chunk == 0) && plane_map(p, p.c.k, &kmap) && plane_map(p, p.c.v, &vmap))
-    return launch_tree_tc<HD>(ctx, p, kmap, vmap);
-  const uint32_t rows = p.max_nodes * p.g;
+    return rows <= 32 ? launch_tree_tc<HD, 32, 3>(ctx, p, kmap, vmap) : launch_tree_tc<HD, 128, 2>(ctx, p, kmap, vmap);
   if (rows <= 16) return launch_tree<HD, 1>(ctx, p);
   return launch_tree<HD, 4>(ctx, p);
 }
