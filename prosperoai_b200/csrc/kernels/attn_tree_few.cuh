@@ -1,0 +1,346 @@
+// Tree attention of at most 32 rows a kv head (decoding, small trees): bound by the cache's bytes.
+//
+// The operands change places, so that the tensor cores and the softmax do the rows' work and not that of 128 rows:
+//   S^T = K Q^T      M = 128 positions, N = 64: the 32 rows' fp16 parts, then their remainders
+//   O^T = V^T P^T    M = 128 dims (V as it lies, hd contiguous: an MN-major A), N = 64 likewise, K = 128 positions
+// A softmax thread has a position and all rows: the weights of a tile need no exchange as long as no row's maximum
+// grows by more than 2^3 (they are relative to a maximum that may be that much too small: fp16 holds 2^15.99, and the
+// weights carry 2^12). Only when some row's does, in a sequence's first tiles, are the rows' maxima taken over the
+// tile, by a reduction that leaves lane r with row r. The sums of weights stay in the threads, one a row and
+// position, until a unit ends.
+//   warps 0-3   softmax; the weights go to shared memory, 128 bytes a position, as an MN-major B
+//   warps 4-7   add the tiles' O^T to the running output, a thread a dim, the rows in registers
+//   warp 8      issues the MMAs (8 + 8 of 48 cycles of shared memory a tile); 9, 10 copy K and V; 11 cleans V
+// With row tiles as A (attn_tree_many.cuh) 8 sequences of one row x 4 heads at 16384 positions took 134 us: 128 rows'
+// MMAs, and one warp of four with a row to work on.
+#pragma once
+#include "attn_tree_tc.cuh"
+
+namespace {
+
+constexpr uint32_t kFewThreads = 384, kFewRows = 32, kFewK = 3, kFewV = 2;
+
+template <int HD>
+struct FewSmem {
+  static constexpr uint32_t kBlock = kTcTile * 128;         // a tile's 64 dims: 16 KB
+  static constexpr uint32_t kTileBytes = HD / 64 * kBlock;  // a K or V tile
+  static constexpr uint32_t kQBlock = 64 * 128;             // 64 dims of the rows' parts and remainders
+  uint8_t q[HD / 64 * kQBlock];
+  uint8_t kt[kFewK][kTileBytes];
+  uint8_t vt[kFewV][kTileBytes];
+  uint8_t pt[2][kTcTile * 128];  // weights: [position][32 rows' parts, 32 rows' remainders]
+  // Words of a tile are read long before the tile that takes their place: P V of a tile waits for the tile before the
+  // last to be folded, so no warp is more than a few tiles ahead of another.
+  uint32_t valid[8][4];  // positions of a tile that hold a row
+  uint32_t odd[8][4];    // its nodes with a non-finite V row
+  uint32_t grew[8];      // whether the tile's weights are relative to new maxima
+  float corr[8][kFewRows];  // then: 2^(old - new)
+  float factor[kFewRows], sub[kFewRows];
+  float wmax[4][kFewRows];
+  float lsum[4][4][kFewRows], msum[4][kFewRows];  // [segment][warp]: sums of weights; maxima
+  uint64_t upto[kMaxSeqs + 1];
+  uint64_t kfull[kFewK], kempty[kFewK], vfull[kFewV], vclean[kFewV], vempty[kFewV], sfull[2], pfull[2], ofull[2], ofree[2],
+      lfull[4], qfull, drain;
+  uint32_t tmem;
+};
+
+// Lane r gets the reduction over the lanes of v[r]: 31 exchanges for 32 values.
+template <typename F>
+__device__ __forceinline__ float reduce_rows(float (&v)[32], F f) {
+  const uint32_t lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int j = 0; j < o; j++) {
+      const bool up = lane & o;
+      const float mine = up ? v[j + o] : v[j], other = up ? v[j] : v[j + o];
+      v[j] = f(mine, __shfl_xor_sync(0xffffffffu, other, o));
+    }
+  return v[0];
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kFewThreads, 1)
+    k_attn_tree_few(TreeParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+  using Smem = FewSmem<HD>;
+  extern __shared__ __align__(16) uint8_t raw[];
+  Smem &sm = *reinterpret_cast<Smem *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  constexpr uint32_t BL = Smem::kBlock;
+  const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  pdl_trigger();
+  if (t == 0) {
+    for (uint32_t i = 0; i < kFewK; i++) {
+      mbar_init(&sm.kfull[i], 1);
+      mbar_init(&sm.kempty[i], 1);
+    }
+    for (uint32_t i = 0; i < kFewV; i++) {
+      mbar_init(&sm.vfull[i], 1);
+      mbar_init(&sm.vclean[i], 1);
+      mbar_init(&sm.vempty[i], 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&sm.sfull[i], 1);
+      mbar_init(&sm.pfull[i], 4);
+      mbar_init(&sm.ofull[i], 1);
+      mbar_init(&sm.ofree[i], 4);
+    }
+    for (int i = 0; i < 4; i++) mbar_init(&sm.lfull[i], 4);
+    mbar_init(&sm.qfull, 4);
+    mbar_init(&sm.drain, 1);
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(256));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  pdl_wait();
+  pairs_before<kFewRows, kTcTile, kFewThreads>(p, sm.upto);
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = sm.tmem;  // columns 0, 64: S^T of even and odd tiles; 128, 192: O^T
+  const uint64_t all = sm.upto[p.c.n_seq], cta = blockIdx.x, grid = gridDim.x < all ? gridDim.x : all;
+  Walk walk = walk_of(p, sm.upto, grid);
+  const uint64_t begin = walk.at;
+  Segment g;
+  Waiter wait{p.wait_ns, p.err};
+  uint32_t i = 0, seg = 0;  // tiles and segments of the run so far
+
+  if (warp == 9) {
+    copy_tiles<HD, kFewRows, kFewK>(p, &kmap, sm.upto, walk, sm.kt[0], sm.kfull, sm.kempty, sm.valid);
+  } else if (warp == 10) {
+    copy_tiles<HD, kFewRows, kFewV>(p, &vmap, sm.upto, walk, sm.vt[0], sm.vfull, sm.vempty, nullptr);
+  } else if (warp == 11) {
+    clean_tiles<HD, kFewRows, kFewV>(p, sm.upto, walk, sm.vt[0], sm.vfull, sm.vclean, sm.odd);
+  } else if (warp == 8) {
+    // ---- MMA issue ----
+    const uint32_t leader = elect_one();
+    const uint64_t qd = desc_k(smem_u32(sm.q)), kd = desc_k(smem_u32(sm.kt[0]));
+    const uint64_t vd = desc_mn(smem_u32(sm.vt[0]), BL), pd = desc_mn(smem_u32(sm.pt[0]), 0);
+    constexpr uint64_t kStep = Smem::kTileBytes >> 4, kPStep = (kTcTile * 128) >> 4;  // in 16 bytes
+    auto scores = [&](uint32_t n) {  // S^T of tile n
+      wait(&sm.kfull[n % kFewK], n / kFewK);
+      tc_after();
+      const uint64_t kb = kd + (n % kFewK) * kStep;
+      if (wait.ok) {
+#pragma unroll
+        for (uint32_t k = 0; k < HD / 16; k++)
+          tc_mma_ss(leader, tmem + 64 * (n & 1), kb + (((k / 4) * BL + (k % 4) * 32) >> 4),
+                    qd + (((k / 4) * Smem::kQBlock + (k % 4) * 32) >> 4), idesc_f16(64, false), k > 0);
+        tc_commit(leader, &sm.sfull[n & 1]);
+        tc_commit(leader, &sm.kempty[n % kFewK]);
+      }
+      __syncwarp();
+    };
+    while (next_segment<kFewRows, kTcTile>(p, sm.upto, walk, g)) {
+      wait(&sm.qfull, seg++);
+      scores(i);
+      for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
+        if (tile + 1 < g.tile1) scores(i + 1);
+        if (i >= 2) wait(&sm.ofree[i & 1], (i >> 1) - 1);
+        wait(&sm.vclean[i % kFewV], i / kFewV);
+        wait(&sm.pfull[i & 1], i >> 1);
+        tc_after();
+        const uint64_t vb = vd + (i % kFewV) * kStep, pb = pd + (i & 1) * kPStep;
+        if (wait.ok) {  // this tile's O^T, from zero: the sum over tiles is made in registers, where it is rounded
+#pragma unroll
+          for (uint32_t k = 0; k < kTcTile / 16; k++)
+            tc_mma_ss(leader, tmem + 128 + 64 * (i & 1), vb + k * (2048 >> 4), pb + k * (2048 >> 4),
+                      idesc_f16(64, true, true), k > 0);
+          tc_commit(leader, &sm.ofull[i & 1]);
+          tc_commit(leader, &sm.vempty[i % kFewV]);
+        }
+        __syncwarp();
+      }
+    }
+    // the MMAs in flight end before TMEM is given back
+    tc_commit(leader, &sm.drain);
+    wait.ok = true;
+    wait(&sm.drain, 0);
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ---- fold: a thread a dim (with hd 64 the upper half of the lanes has none) ----
+    const uint32_t d = t - 128, lanes = (warp & 3) * 32 << 16;
+    const bool live = d < HD;
+    while (next_segment<kFewRows, kTcTile>(p, sm.upto, walk, g)) {
+      const uint32_t rows = min(kFewRows, g.w.nodes * p.g - g.block * kFewRows);
+      float o[32];
+#pragma unroll
+      for (int r = 0; r < 32; r++) o[r] = 0.0f;
+      for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
+        wait(&sm.ofull[i & 1], i >> 1);
+        __syncwarp();
+        tc_after();
+        uint32_t v[64];
+        tc_ld32(tmem + lanes + 128 + 64 * (i & 1), v);
+        tc_ld32(tmem + lanes + 160 + 64 * (i & 1), v + 32);
+        if (sm.grew[i & 7]) {
+#pragma unroll
+          for (int r = 0; r < 32; r++) o[r] *= sm.corr[i & 7][r];
+        }
+        tc_ld_wait(v);
+        tc_ld_wait(v + 32);
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.ofree[i & 1]);
+#pragma unroll
+        for (int r = 0; r < 32; r++) o[r] += __uint_as_float(v[r]) + __uint_as_float(v[32 + r]);
+        if ((tile + 1) * kTcTile > g.w.len && live) {
+          // non-finite V elements of nodes, for the rows that see them
+#pragma unroll 1
+          for (int x = 0; x < 4; x++)
+#pragma unroll 1
+            for (uint32_t left = sm.odd[i & 7][x] & sm.valid[i & 7][x]; left; left &= left - 1) {
+              const uint32_t pos = tile * kTcTile + 32 * x + __ffs(left) - 1;
+              const float f = __half2float(p.c.v[(size_t)g.kvh * p.c.head_stride + kv_row(p.c, g.s, pos) + d]);
+              if (isfinite(f)) continue;
+#pragma unroll
+              for (int r = 0; r < 32; r++)
+                if ((uint32_t)r < rows && (seen(p, pos - g.w.len, true, (g.block * kFewRows + r) / p.g, g.w.first) & 1))
+                  o[r] += f;
+            }
+        }
+        __syncwarp();
+      }
+      wait(&sm.lfull[seg & 3], seg >> 2);  // the softmax warps may be two segments ahead, never four
+      __syncwarp();
+      const bool whole = g.whole();
+      const uint64_t slot = 2 * cta + (begin >= g.unit0 ? 0 : 1);
+#pragma unroll
+      for (int r = 0; r < 32; r++) {
+        if ((uint32_t)r >= rows) continue;
+        const float *ls = &sm.lsum[seg & 3][0][r];
+        const float L = (ls[0] + ls[kFewRows]) + (ls[2 * kFewRows] + ls[3 * kFewRows]);
+        const uint32_t rr = g.block * kFewRows + r;
+        if (whole) {  // a row that sees nothing gets zeros
+          if (live)
+            p.out[((size_t)(g.w.first + rr / p.g) * p.h + g.kvh * p.g + rr % p.g) * HD + d] = L != 0.0f ? o[r] * (1.0f / L) : 0.0f;
+        } else {
+          if (live) p.part_o[(slot * kFewRows + r) * HD + d] = o[r];
+          if (d == 0) {
+            p.part_ml[(slot * kFewRows + r) * 2] = sm.msum[seg & 3][r];
+            p.part_ml[(slot * kFewRows + r) * 2 + 1] = L;
+          }
+        }
+      }
+      if (g.tile0 == 0 && d == 0) note_unit(p, g, all, grid);
+      seg++;
+    }
+  } else {
+    // ---- softmax: a thread a position ----
+    constexpr float kNone = -1e30f, kFull = 15.5f;  // no maximum yet; the largest exponent that weights may have
+    while (next_segment<kFewRows, kTcTile>(p, sm.upto, walk, g)) {
+      const uint32_t rows = min(kFewRows, g.w.nodes * p.g - g.block * kFewRows), groups = (rows + 7) / 8;
+      // every score of the last segment has been read, so its products are done: Q may be written
+      put_queries<HD, kFewRows, 4>(p, g, rows, warp, sm.q, Smem::kQBlock, kFewRows * 128, sm.factor);
+      if (t < kFewRows) sm.sub[t] = kNone;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.qfull);
+      named_sync<1, 128>();
+      float m = -INFINITY;  // of row `lane`
+      float l[32];
+#pragma unroll
+      for (int r = 0; r < 32; r++) l[r] = 0.0f;
+      for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
+        const uint32_t sa = tmem + ((warp & 3) * 32 << 16) + 64 * (i & 1);
+        wait(&sm.sfull[i & 1], i >> 1);
+        __syncwarp();
+        tc_after();
+        float s[32];
+        {
+          uint32_t v[64];
+          tc_ld32(sa, v);
+          tc_ld32(sa + 32, v + 32);
+          tc_ld_wait(v);
+          tc_ld_wait(v + 32);
+#pragma unroll
+          for (int r = 0; r < 32; r++) s[r] = __uint_as_float(v[r]) + __uint_as_float(v[32 + r]);
+        }
+        const bool there = (sm.valid[i & 7][warp] >> lane) & 1;
+        const uint32_t pos = tile * kTcTile + t;
+#pragma unroll
+        for (int r = 0; r < 32; r += 4) {
+          const float4 f = *reinterpret_cast<const float4 *>(&sm.factor[r]);
+          s[r] = there ? s[r] * f.x : -INFINITY;
+          s[r + 1] = there ? s[r + 1] * f.y : -INFINITY;
+          s[r + 2] = there ? s[r + 2] * f.z : -INFINITY;
+          s[r + 3] = there ? s[r + 3] * f.w : -INFINITY;
+        }
+        if ((tile + 1) * kTcTile > g.w.len && pos >= g.w.len) {  // a node: for the rows that see it
+#pragma unroll
+          for (int r = 0; r < 32; r++)
+            if ((uint32_t)r < rows && !(seen(p, pos - g.w.len, true, (g.block * kFewRows + r) / p.g, g.w.first) & 1))
+              s[r] = -INFINITY;
+        }
+        __syncwarp();
+        // exponents relative to the rows' maxima so far
+        float top = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 32; r += 4) {
+          const float4 u = *reinterpret_cast<const float4 *>(&sm.sub[r]);
+          if ((uint32_t)r < rows)
+            top = fmaxf(fmaxf(top, fmaxf(s[r] - u.x, s[r + 1] - u.y)), fmaxf(s[r + 2] - u.z, s[r + 3] - u.w));
+        }
+        uint32_t any;
+        asm volatile(
+            "{\n .reg .pred p, q;\n setp.ne.u32 q, %1, 0;\n bar.red.or.pred p, 1, 128, q;\n selp.u32 %0, 1, 0, p;\n}\n"
+            : "=r"(any)
+            : "r"((uint32_t)(top > kFull))
+            : "memory");
+        if (any) {
+          float x[32];
+#pragma unroll
+          for (int r = 0; r < 32; r++) x[r] = s[r];
+          sm.wmax[warp][lane] = reduce_rows(x, [](float a, float b) { return fmaxf(a, b); });
+          named_sync<1, 128>();
+          const float mn = fmaxf(fmaxf(fmaxf(m, sm.wmax[0][lane]), fmaxf(sm.wmax[1][lane], sm.wmax[2][lane])), sm.wmax[3][lane]);
+          const float corr = m == mn ? 1.0f : ex2(m - mn);
+          m = mn;
+          if (warp == 0) {
+            sm.sub[lane] = mn == -INFINITY ? kNone : mn - kPShift;
+            sm.corr[i & 7][lane] = corr;
+          }
+#pragma unroll
+          for (int r = 0; r < 32; r++) l[r] *= __shfl_sync(0xffffffffu, corr, r);
+          named_sync<1, 128>();
+        }
+        if (t == 0) sm.grew[i & 7] = any;
+        // weights, in groups of 8 rows, to the position's 128 bytes (16 of parts and 16 of remainders a group)
+        uint8_t *dst = sm.pt[i & 1] + t * 128;
+#pragma unroll
+        for (uint32_t gr = 0; gr < 4; gr++) {
+          if (gr >= groups) continue;
+          uint4 hi, lo;
+          uint32_t *hw = reinterpret_cast<uint32_t *>(&hi), *lw = reinterpret_cast<uint32_t *>(&lo);
+#pragma unroll
+          for (uint32_t e = 0; e < 8; e += 2) {
+            const uint32_t r = 8 * gr + e;
+            const float2 u = *reinterpret_cast<const float2 *>(&sm.sub[r]);
+            const float p0 = ex2(s[r] - u.x), p1 = ex2(s[r + 1] - u.y);
+            l[r] += p0;
+            l[r + 1] += p1;
+            split_f16(p0, p1, hw[e / 2], lw[e / 2]);
+          }
+          *reinterpret_cast<uint4 *>(dst + ((gr ^ (t & 7)) << 4)) = hi;
+          *reinterpret_cast<uint4 *>(dst + (((4 + gr) ^ (t & 7)) << 4)) = lo;
+        }
+        fence_proxy_async();
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.pfull[i & 1]);
+      }
+      // lane r: the warp's sum of row r
+      sm.lsum[seg & 3][warp][lane] = reduce_rows(l, [](float a, float b) { return a + b; });
+      if (warp == 0) sm.msum[seg & 3][lane] = m;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.lfull[seg & 3]);
+      named_sync<1, 128>();  // the factors and maxima may be written again
+      seg++;
+    }
+  }
+  tc_before();
+  __syncthreads();
+  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256));
+}
+
+}  // namespace

@@ -1,0 +1,294 @@
+// Tree attention of more than 32 rows a kv head: row tiles of 128.
+//
+// S = Q K^T (M = 128 rows, N = 128 positions, both fp16 parts of Q) and the tile's P V go to TMEM; P (both parts) is
+// written over S and is the A operand of P V, V, as it lies with hd contiguous, an MN-major B.
+//   warps 0-3, 4-7   softmax, a row a thread: the first four have a tile's positions 0-63, the others 64-127; the
+//                    row's maximum goes through shared memory. Then the P V of the tile before, which ran
+//                    meanwhile, is added to the running output in registers, half of the dims each.
+//   warp 8           issues the MMAs: Q K^T of tile i + 1 before P V of tile i, so that they overlap the softmax
+//   warps 12-14      K copies, V copies, cleaning
+// Registers: 512 threads at 128; setmaxnreg gives the softmax warps 200 and leaves 56 to the others (256 * 200 +
+// 256 * 56 = 65536, what the block was launched with).
+#pragma once
+#include "attn_tree_tc.cuh"
+
+namespace {
+
+constexpr uint32_t kManyThreads = 512, kManyRows = 128;
+
+template <int HD>
+struct ManySmem {
+  static constexpr uint32_t kBlock = 128 * 128;             // 128 rows of 64 dims: 16 KB
+  static constexpr uint32_t kTileBytes = HD / 64 * kBlock;  // a K or V tile, or one part of Q
+  uint8_t q[2][kTileBytes];
+  uint8_t kt[2][kTileBytes];
+  uint8_t vt[2][kTileBytes];
+  uint32_t valid[8][4];          // positions of a tile that hold a row; a tile's words are read long before 8 tiles on
+  uint32_t odd[8][4];            // its nodes with a non-finite V row
+  float factor[kManyRows];
+  float top[2][2][kManyRows];      // [tile parity][warpgroup]: maxima of a row's halves
+  float ml[2][kManyRows];
+  uint64_t upto[kMaxSeqs + 1];
+  uint64_t kfull[2], kempty[2], vfull[2], vclean[2], vempty[2], sfull[2], pfull[2], ofull[2], qfull, drain;
+  uint32_t tmem;
+};
+
+template <int HD>
+__global__ void __launch_bounds__(kManyThreads, 1)
+    k_attn_tree_many(TreeParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+  using Smem = ManySmem<HD>;
+  extern __shared__ __align__(16) uint8_t raw[];
+  Smem &sm = *reinterpret_cast<Smem *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  constexpr uint32_t BL = Smem::kBlock;
+  const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  pdl_trigger();
+  if (t == 0) {
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&sm.kfull[i], 1);
+      mbar_init(&sm.vfull[i], 1);
+      mbar_init(&sm.vclean[i], 1);
+      mbar_init(&sm.kempty[i], 1);
+      mbar_init(&sm.vempty[i], 1);
+      mbar_init(&sm.sfull[i], 1);
+      mbar_init(&sm.pfull[i], 8);
+      mbar_init(&sm.ofull[i], 1);
+    }
+    mbar_init(&sm.qfull, 8);
+    mbar_init(&sm.drain, 1);
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  pdl_wait();
+  pairs_before<kManyRows, kTcTile, kManyThreads>(p, sm.upto);
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = sm.tmem;
+  const uint64_t all = sm.upto[p.c.n_seq], cta = blockIdx.x, grid = gridDim.x < all ? gridDim.x : all;
+  Walk walk = walk_of(p, sm.upto, grid);
+  const uint64_t begin = walk.at;
+  Segment g;
+  Waiter wait{p.wait_ns, p.err};
+
+  if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 12)
+      copy_tiles<HD, kManyRows, 2>(p, &kmap, sm.upto, walk, sm.kt[0], sm.kfull, sm.kempty, sm.valid);
+    else if (warp == 13)
+      copy_tiles<HD, kManyRows, 2>(p, &vmap, sm.upto, walk, sm.vt[0], sm.vfull, sm.vempty, nullptr);
+    else if (warp == 14)
+      clean_tiles<HD, kManyRows, 2>(p, sm.upto, walk, sm.vt[0], sm.vfull, sm.vclean, sm.odd);
+  } else if (warp >= 8) {
+    // ---- MMA issue ----
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 8) {
+      const uint32_t leader = elect_one();
+      const uint64_t qd = desc_k(smem_u32(sm.q[0])), kd = desc_k(smem_u32(sm.kt[0])), vd = desc_mn(smem_u32(sm.vt[0]), BL);
+      constexpr uint64_t kPart = Smem::kTileBytes >> 4;  // from one part of Q, or one tile, to the next, in 16 bytes
+      uint32_t i = 0, seg = 0;
+      auto scores = [&](uint32_t n) {  // S = Q K^T of tile n: both parts of Q
+        wait(&sm.kfull[n & 1], n >> 1);
+        tc_after();
+        const uint64_t kb = kd + (n & 1) * kPart;
+        const uint32_t d = tmem + 128 * (n & 1);
+        if (wait.ok) {
+#pragma unroll
+          for (uint32_t k = 0; k < HD / 16; k++) {
+            const uint64_t off = ((k / 4) * BL + (k % 4) * 32) >> 4;
+            tc_mma_ss(leader, d, qd + off, kb + off, idesc_f16(kTcTile, false), k > 0);
+            tc_mma_ss(leader, d, qd + kPart + off, kb + off, idesc_f16(kTcTile, false), true);
+          }
+          tc_commit(leader, &sm.sfull[n & 1]);
+          tc_commit(leader, &sm.kempty[n & 1]);
+        }
+        __syncwarp();
+      };
+      while (next_segment<kManyRows, kTcTile>(p, sm.upto, walk, g)) {
+        wait(&sm.qfull, seg++);
+        scores(i);
+        for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
+          if (tile + 1 < g.tile1) scores(i + 1);
+          wait(&sm.pfull[i & 1], i >> 1);
+          wait(&sm.vclean[i & 1], i >> 1);
+          tc_after();
+          const uint64_t vb = vd + (i & 1) * kPart;
+          const uint32_t a = tmem + 128 * (i & 1), d = tmem + 256 + 128 * (i & 1);
+          if (wait.ok) {  // this tile's P V, from zero: the sum over tiles is made in registers, where it is rounded
+#pragma unroll
+            for (uint32_t k = 0; k < kTcTile / 16; k++) {
+              const uint32_t at = a + 32 * (k / 2) + 8 * (k % 2);
+              tc_mma_ts(leader, d, at, vb + k * (2048 >> 4), idesc_f16(HD, true), k > 0);
+              tc_mma_ts(leader, d, at + 16, vb + k * (2048 >> 4), idesc_f16(HD, true), true);
+            }
+            tc_commit(leader, &sm.ofull[i & 1]);
+            tc_commit(leader, &sm.vempty[i & 1]);
+          }
+          __syncwarp();
+        }
+      }
+      // the MMAs in flight end before TMEM is given back
+      tc_commit(leader, &sm.drain);
+      wait.ok = true;
+      wait(&sm.drain, 0);
+      __syncwarp();
+    }
+  } else {
+    // ---- softmax: a thread a row, warpgroup wg half of the positions and half of the dims ----
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    const uint32_t wg = warp >> 2, r = t & 127;
+    const uint32_t lanes = (warp & 3) * 32 << 16;
+    uint32_t i = 0;
+    while (next_segment<kManyRows, kTcTile>(p, sm.upto, walk, g)) {
+      const uint32_t rows = min(kManyRows, g.w.nodes * p.g - g.block * kManyRows);
+      // the last segment's products are done: Q may be written
+      put_queries<HD, kManyRows, 8>(p, g, rows, warp, sm.q[0], BL, Smem::kTileBytes, sm.factor);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.qfull);
+      named_sync<1, 256>();
+      const float factor = sm.factor[r];
+      const bool work = (warp & 3) * 32 < rows;  // a warp whose rows are all past the last one keeps step only
+      const uint32_t rr = g.block * kManyRows + r, nd = rr / p.g;
+      const bool live = r < rows;
+      float o[HD / 2], m = -INFINITY, l = 0.0f, corr = 1.0f;
+#pragma unroll
+      for (int d = 0; d < HD / 2; d++) o[d] = 0.0f;
+      // add the P V of tile n (the n-th of the run) to this thread's half of the dims; `tile` its number in the unit
+      auto fold = [&](uint32_t n, uint32_t tile, uint64_t sees0, uint64_t sees1) {
+        wait(&sm.ofull[n & 1], n >> 1);
+        __syncwarp();
+        tc_after();
+        if (work) {
+          const uint32_t oa = tmem + lanes + 256 + 128 * (n & 1) + wg * (HD / 2);
+          uint32_t v[HD / 2];
+#pragma unroll
+          for (int c = 0; c < HD / 64; c++) tc_ld32(oa + 32 * c, v + 32 * c);
+#pragma unroll
+          for (int c = 0; c < HD / 64; c++) tc_ld_wait(v + 32 * c);
+#pragma unroll
+          for (int d = 0; d < HD / 2; d++) o[d] = fmaf(o[d], corr, __uint_as_float(v[d]));
+          if ((tile + 1) * kTcTile > g.w.len) {
+            // non-finite V elements of nodes that this row sees
+#pragma unroll 1
+            for (int x = 0; x < 4; x++)
+#pragma unroll 1
+              for (uint32_t left = sm.odd[n & 7][x] & (uint32_t)((x < 2 ? sees0 : sees1) >> (32 * (x & 1))); left;
+                   left &= left - 1) {
+                const int64_t at_row = kv_row(p.c, g.s, tile * kTcTile + 32 * x + __ffs(left) - 1);
+                const __half2 *vr =
+                    reinterpret_cast<const __half2 *>(p.c.v + (size_t)g.kvh * p.c.head_stride + at_row + wg * (HD / 2));
+#pragma unroll
+                for (int d = 0; d < HD / 4; d++) {
+                  const float2 f = __half22float2(vr[d]);
+                  if (!isfinite(f.x)) o[2 * d] += f.x;
+                  if (!isfinite(f.y)) o[2 * d + 1] += f.y;
+                }
+              }
+          }
+        }
+        __syncwarp();
+        tc_before();
+      };
+      uint64_t sees0 = 0, sees1 = 0;  // of the tile that is folded next
+      for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
+        const uint32_t sa = tmem + lanes + 128 * (i & 1) + 64 * wg;
+        wait(&sm.sfull[i & 1], i >> 1);
+        __syncwarp();
+        tc_after();
+        float corr1 = 1.0f;
+        uint64_t now0 = 0, now1 = 0;
+        if (work) {
+          uint32_t v[64];
+          tc_ld32(sa, v);
+          tc_ld32(sa + 32, v + 32);
+          const bool drafted = (tile + 1) * kTcTile > g.w.len;
+          const uint64_t ok0 = (uint64_t)sm.valid[i & 7][0] | (uint64_t)sm.valid[i & 7][1] << 32;
+          const uint64_t ok1 = (uint64_t)sm.valid[i & 7][2] | (uint64_t)sm.valid[i & 7][3] << 32;
+          const bool masked = drafted || (ok0 & ok1) != ~0ull;
+          now0 = ok0, now1 = ok1;
+          if (drafted) {
+            now0 &= seen(p, tile * kTcTile - g.w.len, live, nd, g.w.first);
+            now1 &= seen(p, tile * kTcTile + 64 - g.w.len, live, nd, g.w.first);
+          }
+          tc_ld_wait(v);
+          tc_ld_wait(v + 32);
+          if (masked) {
+            const uint64_t bits = wg ? now1 : now0;
+            const uint32_t b0 = (uint32_t)bits, b1 = (uint32_t)(bits >> 32);
+#pragma unroll
+            for (int e = 0; e < 64; e++)
+              if (!(((e < 32 ? b0 : b1) >> (e & 31)) & 1)) v[e] = 0xFF800000u;  // -inf
+          }
+          float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int e = 0; e < 64; e += 8)
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+              t4[u] = fmaxf(t4[u], fmaxf(__uint_as_float(v[e + 2 * u]), __uint_as_float(v[e + 2 * u + 1])));
+          float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+          // the row's other 64 positions are the other warpgroup's
+          sm.top[i & 1][wg][r] = top;
+          __syncwarp();
+          asm volatile("bar.sync %0, 64;" ::"r"(4 + (warp & 3)) : "memory");
+          top = fmaxf(top, sm.top[i & 1][1 - wg][r]);
+          const float mn = fmaxf(m, top * factor);
+          corr1 = m == mn ? 1.0f : ex2(m - mn);
+          m = mn;
+          const float sub = mn == -INFINITY ? 0.0f : mn - kPShift;
+          float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 2; c++) {
+            uint32_t w[32];  // 16 words of parts, 16 of remainders
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float p0 = ex2(fmaf(__uint_as_float(v[32 * c + e]), factor, -sub));
+              const float p1 = ex2(fmaf(__uint_as_float(v[32 * c + e + 1]), factor, -sub));
+              part[(e / 2) & 3] += p0 + p1;
+              split_f16(p0, p1, w[e / 2], w[16 + e / 2]);
+            }
+            tc_st32(sa + 32 * c, w);
+          }
+          l = l * corr1 + ((part[0] + part[1]) + (part[2] + part[3]));
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        }
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.pfull[i & 1]);
+        // the tile before, whose P V ran meanwhile
+        if (tile > g.tile0) fold(i - 1, tile - 1, sees0, sees1);
+        corr = corr1, sees0 = now0, sees1 = now1;
+      }
+      fold(i - 1, g.tile1 - 1, sees0, sees1);
+      // the two halves' sums of weights
+      sm.ml[wg][r] = l;
+      named_sync<1, 256>();
+      const float L = sm.ml[0][r] + sm.ml[1][r];
+      const bool whole = g.whole();
+      const uint64_t slot = 2 * cta + (begin >= g.unit0 ? 0 : 1);
+      const float scale = whole ? (L != 0.0f ? 1.0f / L : 0.0f) : 1.0f;
+      // whole units go to their rows of out; parts lie [hd / 4][row] float4
+      float *dst = whole ? p.out + ((size_t)(g.w.first + (live ? nd : 0)) * p.h + g.kvh * p.g + rr % p.g) * HD + wg * (HD / 2)
+                         : p.part_o + ((slot * (HD / 4) + wg * (HD / 8)) * kManyRows + r) * 4;
+      const uint32_t step = whole ? 4 : 4 * kManyRows;
+      if (live) {
+#pragma unroll
+        for (int d = 0; d < HD / 2; d += 4)
+          *reinterpret_cast<float4 *>(dst + (size_t)(d / 4) * step) =
+              make_float4(o[d] * scale, o[d + 1] * scale, o[d + 2] * scale, o[d + 3] * scale);
+        if (!whole && wg == 0) {
+          p.part_ml[(slot * kManyRows + r) * 2] = m;
+          p.part_ml[(slot * kManyRows + r) * 2 + 1] = L;
+        }
+      }
+      if (g.tile0 == 0 && t == 0) note_unit(p, g, all, grid);
+      named_sync<1, 256>();  // Q and the sums may be written again
+    }
+  }
+  tc_before();
+  __syncthreads();
+  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+}
+
+}  // namespace

@@ -1,0 +1,381 @@
+// Tree attention on the fifth-generation tensor cores (tcgen05): what its two kernels share.
+//
+// Key tiles of 128 positions, whatever the rows: K and V come by tensor copies (TMA) in the 128-byte swizzle, a page or
+// a share of one at a time; products go to TMEM. Both kernels are one CTA an SM and keep their roles in warps of their
+// own, which meet at mbarriers; every wait is bounded.
+#pragma once
+#include <cuda.h>  // CUtensorMap and its enums (types only; the encoder comes from the runtime)
+
+#include "attn_tree.cuh"
+
+namespace {
+
+constexpr uint32_t kTcTile = 128, kTcGrid = 148;
+
+__device__ __forceinline__ uint64_t desc_k(uint32_t saddr) {  // K-major, 128-byte swizzle, 8-row groups of 1024 bytes
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)1u << 16 | (uint64_t)(1024u >> 4) << 32 | (uint64_t)1u << 46 |
+         (uint64_t)2u << 61;
+}
+__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t block) {
+  // MN-major: 64-element blocks of the contiguous dimension `block` bytes apart, 8-row groups of 1024 bytes
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)(block >> 4) << 16 | (uint64_t)(1024u >> 4) << 32 |
+         (uint64_t)1u << 46 | (uint64_t)2u << 61;
+}
+// kind::f16: fp16 A and B, fp32 sums, M = 128, N = n; a_mn, b_mn: that operand is MN-major
+__host__ __device__ constexpr uint32_t idesc_f16(uint32_t n, bool b_mn, bool a_mn = false) {
+  return (1u << 4) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+// Issued by the one lane that has `leader` set; the whole warp runs the loop around it, so that descriptors stay in
+// uniform registers.
+__device__ __forceinline__ void tc_mma_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint32_t leader, uint64_t *bar) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)),
+      "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t is;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(is));
+  return is;
+}
+// [64 dims] x [chunk positions] of one kv head of one page; coordinates outside the planes read zeros
+__device__ __forceinline__ void tma_load(void *dst, const CUtensorMap *map, uint32_t dim, uint32_t row, uint32_t head,
+                                         uint32_t page, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(dim), "r"(row), "r"(head), "r"(page), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_ld32(uint32_t at, uint32_t *r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(at));
+}
+// Wait for the loads; the words pass through, so that nothing that uses them is moved before the wait.
+__device__ __forceinline__ void tc_ld_wait(uint32_t *r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13])
+               :
+               : "memory");
+  asm volatile("" : "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+                    "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27])
+               :: "memory");
+  asm volatile("" : "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
+}
+__device__ __forceinline__ void tc_st32(uint32_t at, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(at)
+      : "memory");
+}
+template <int ID, int N>
+__device__ __forceinline__ void named_sync() {
+  __syncwarp();
+  asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory");
+}
+
+// One CTA's run over the (unit, tile) pairs: the part of each unit that lies in it, in order.
+struct Segment {
+  SeqWork w;
+  uint64_t unit0;
+  uint32_t s, kvh, block, tile0, tile1;
+  __device__ __forceinline__ bool whole() const { return tile0 == 0 && tile1 == w.tiles; }
+};
+struct Walk {
+  uint64_t at, end;
+  uint32_t s;
+};
+template <uint32_t MR, uint32_t KT>
+__device__ __forceinline__ bool next_segment(const TreeParams &p, const uint64_t *upto, Walk &k, Segment &g) {
+  if (k.at >= k.end) return false;
+  while (upto[k.s + 1] <= k.at) k.s++;
+  g.s = k.s;
+  g.w = seq_work<MR, KT>(p, k.s);
+  const uint64_t unit = (k.at - upto[k.s]) / g.w.tiles;
+  g.unit0 = upto[k.s] + unit * g.w.tiles;
+  g.kvh = (uint32_t)(unit / g.w.blocks), g.block = (uint32_t)(unit % g.w.blocks);
+  const uint64_t unit1 = g.unit0 + g.w.tiles;
+  g.tile0 = (uint32_t)(k.at - g.unit0), g.tile1 = (uint32_t)((k.end < unit1 ? k.end : unit1) - g.unit0);
+  k.at = g.unit0 + g.tile1;
+  return true;
+}
+
+// Which of the 64 positions from node `base32` (negative: committed) on a row of node `nd` may see.
+__device__ __forceinline__ uint64_t seen(const TreeParams &p, uint32_t base32, bool live, uint32_t nd, uint32_t first) {
+  const int32_t base = (int32_t)base32;
+  const uint64_t past = low_bits(-(int64_t)base);
+  if (!live) return past;
+  if (!p.mask) return low_bits((int64_t)nd + 1 - base);
+  return past | (window(p.mask + (size_t)(first + nd) * p.words, p.words, base) & ~past);
+}
+
+// A bounded wait that a role makes. After one has run out the role goes on without waiting or copying, so that the
+// barriers among its own threads still meet; the error word tells the host.
+struct Waiter {
+  uint64_t limit_ns;
+  uint32_t *err;
+  bool ok = true;
+  __device__ __forceinline__ void operator()(uint64_t *bar, uint32_t parity) {
+    if (ok && !mbar_wait(bar, parity & 1u, limit_ns)) {
+      ok = false;
+      atomicExch(err, 1u);
+    }
+  }
+};
+
+// The run of this CTA.
+__device__ __forceinline__ Walk walk_of(const TreeParams &p, const uint64_t *upto, uint64_t grid) {
+  const uint64_t all = upto[p.c.n_seq], cta = blockIdx.x;
+  Walk k;
+  k.at = cta < grid ? cta * all / grid : 0;
+  k.end = cta < grid ? (cta + 1) * all / grid : 0;
+  k.s = 0;
+  return k;
+}
+
+// Copies, one warp for all K tiles or all V tiles: a lane a chunk of p.chunk positions, which lie in one page. With
+// `valid` (K) it also notes which positions of a tile hold a row. `slots` tiles are in flight.
+template <int HD, uint32_t MR, uint32_t SLOTS>
+__device__ __forceinline__ void copy_tiles(const TreeParams &p, const CUtensorMap *map, const uint64_t *upto, Walk walk,
+                                           uint8_t *slot0, uint64_t *full, uint64_t *empty, uint32_t (*valid)[4]) {
+  constexpr uint32_t BL = kTcTile * 128, BYTES = HD / 64 * BL;
+  const uint32_t lane = threadIdx.x & 31, chunks = kTcTile / p.chunk, chunk = p.chunk, P = p.c.page_tokens;
+  Waiter wait{p.wait_ns, p.err};
+  Segment g;
+  uint32_t i = 0;  // tiles of the run so far
+  while (next_segment<MR, kTcTile>(p, upto, walk, g)) {
+    const uint32_t total = g.w.len + g.w.nodes;
+    // where the lane's chunk of a tile lies: page (n_pages for a hole, which reads zeros), first row; -1: behind the
+    // last position, not copied
+    int32_t page, row;
+    auto find = [&](uint32_t tile) {
+      const uint32_t pos = tile * kTcTile + lane * chunk;
+      page = -1, row = 0;
+      if (lane < chunks && tile < g.tile1 && pos < total) {
+        const uint32_t pg = pos / P;
+        uint32_t x = p.c.n_pages;
+        if (pg < p.c.max_pages) x = p.c.table ? (uint32_t)p.c.table[(size_t)g.s * p.c.max_pages + pg] : g.s;
+        page = (int32_t)min(x, p.c.n_pages);
+        row = (int32_t)(pos - pg * P);
+      }
+    };
+    find(g.tile0);
+    for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
+      const uint32_t sl = i % SLOTS;
+      const int32_t at = page, r = row;
+      find(tile + 1);  // the next tile's table entries come while this one is copied
+      const uint32_t copied = __ballot_sync(0xffffffffu, at >= 0);
+      const uint32_t there = __ballot_sync(0xffffffffu, at >= 0 && at < (int32_t)p.c.n_pages);
+      if (i >= SLOTS) wait(&empty[sl], i / SLOTS - 1);
+      __syncwarp();
+      if (valid) {
+        if (lane < 4) {  // the word of positions 32 lane .. + 31
+          const uint32_t cap = min(total, p.c.max_pages * P), pos = tile * kTcTile + 32 * lane;
+          uint32_t bits = 0;
+          if (chunk >= 32) {
+            bits = (there >> (32 * lane / chunk)) & 1 ? 0xFFFFFFFFu : 0u;
+          } else {
+            for (uint32_t c = 0; c < 32 / chunk; c++)
+              if ((there >> (32 / chunk * lane + c)) & 1) bits |= ((1u << chunk) - 1) << (c * chunk);
+          }
+          valid[i & 7][lane] = bits & (uint32_t)low_bits((int64_t)cap - pos);
+        }
+        __syncwarp();
+      }
+      if (wait.ok) {
+        uint8_t *dst = slot0 + sl * BYTES + lane * chunk * 128;
+        if (lane == 0) mbar_expect_tx(&full[sl], __popc(copied) * chunk * HD * 2);
+        __syncwarp();
+        if (at >= 0) {
+#pragma unroll
+          for (uint32_t b = 0; b < HD / 64; b++) tma_load(dst + b * BL, map, 64 * b, r, g.kvh, at, &full[sl]);
+        }
+      }
+      __syncwarp();
+    }
+  }
+  // the last copies land before the block ends, whatever became of the others
+  wait.ok = true;
+  for (uint32_t n = i < SLOTS ? 0 : i - SLOTS; n < i; n++) wait(&full[n % SLOTS], n / SLOTS);
+}
+
+// One warp hands the V tiles on to the MMAs, after it has looked at the rows of those that hold nodes: a non-finite V
+// row may only reach the rows that see its node, and a weight of 0 does not keep it out of a product. Such elements
+// (those of stale rows behind the last node too) become 0 here, and `odd` tells where; they are added later to the rows
+// that see them. (Every tile is handed on: a barrier that was watched for some phases only could be two phases on.)
+template <int HD, uint32_t MR, uint32_t SLOTS>
+__device__ __forceinline__ void clean_tiles(const TreeParams &p, const uint64_t *upto, Walk walk, uint8_t *slot0,
+                                            uint64_t *full, uint64_t *clean, uint32_t (*odd)[4]) {
+  constexpr uint32_t BL = kTcTile * 128, BYTES = HD / 64 * BL, CH = HD / 8;
+  const uint32_t lane = threadIdx.x & 31;
+  Waiter wait{p.wait_ns, p.err};
+  Segment g;
+  uint32_t i = 0;
+  while (next_segment<MR, kTcTile>(p, upto, walk, g))
+    for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
+      const uint32_t sl = i % SLOTS;
+      wait(&full[sl], i / SLOTS);
+      __syncwarp();
+      if ((tile + 1) * kTcTile > g.w.len) {
+#pragma unroll 1
+        for (uint32_t x = 0; x < 4; x++) {  // a lane has a row of each 32
+          const uint32_t r = 32 * x + lane;
+          bool bad = false;
+#pragma unroll 4
+          for (uint32_t ch = 0; ch < CH; ch++) {
+            uint4 *at = reinterpret_cast<uint4 *>(slot0 + sl * BYTES + (ch / 8) * BL + r * 128 + (((ch % 8) ^ (r & 7)) << 4));
+            uint4 v = *at;
+            uint32_t *cw = reinterpret_cast<uint32_t *>(&v);
+            bool here = false;
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+              if ((cw[y] & 0x7C00u) == 0x7C00u) cw[y] &= 0xFFFF0000u, here = true;
+              if ((cw[y] & 0x7C000000u) == 0x7C000000u) cw[y] &= 0xFFFFu, here = true;
+            }
+            if (here) *at = v;
+            bad |= here;
+          }
+          const uint32_t word = __ballot_sync(0xffffffffu, bad);
+          if (lane == 0) odd[i & 7][x] = word;
+        }
+        fence_proxy_async();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&clean[sl]);
+    }
+}
+
+// Query rows into shared memory as a K-major operand [64 dims][rows][128 bytes], a power of two and two fp16 parts a
+// row: warp `w` of WARPS has MR / WARPS rows; the remainders lie `rem` bytes behind the parts.
+template <int HD, uint32_t MR, uint32_t WARPS>
+__device__ __forceinline__ void put_queries(const TreeParams &p, const Segment &g, uint32_t rows, uint32_t w, uint8_t *q,
+                                            uint32_t block, uint32_t rem, float *factor) {
+  constexpr uint32_t LR = HD / 4, RW = 32 / LR, WR = MR / WARPS;  // lanes of a row, rows of an access, rows of a warp
+  constexpr uint32_t UN = WR / RW < 4 ? WR / RW : 4;
+  const uint32_t lane = threadIdx.x & 31, d4 = lane % LR;
+#pragma unroll 1
+  for (uint32_t b0 = 0; b0 < WR; b0 += UN * RW) {
+    float4 f[UN];
+#pragma unroll
+    for (uint32_t u = 0; u < UN; u++) {
+      const uint32_t rl = w * WR + b0 + u * RW + lane / LR, rr = g.block * MR + rl;
+      f[u] = rl < rows ? *reinterpret_cast<const float4 *>(
+                             p.q + ((size_t)(g.w.first + rr / p.g) * p.h + g.kvh * p.g + rr % p.g) * HD + 4 * d4)
+                       : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < UN; u++) {
+      const uint32_t rl = w * WR + b0 + u * RW + lane / LR;
+      float top = fmaxf(fmaxf(fabsf(f[u].x), fabsf(f[u].y)), fmaxf(fabsf(f[u].z), fabsf(f[u].w)));
+#pragma unroll
+      for (uint32_t o = LR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      float down, up;
+      row_scale(top, down, up);
+      uint2 hi, lo;
+      split_f16(f[u].x * down, f[u].y * down, hi.x, lo.x);
+      split_f16(f[u].z * down, f[u].w * down, hi.y, lo.y);
+      const uint32_t at = (d4 / 16) * block + rl * 128 + (((d4 % 16) / 2 ^ (rl & 7)) << 4) + (d4 & 1) * 8;
+      *reinterpret_cast<uint2 *>(q + at) = hi;
+      *reinterpret_cast<uint2 *>(q + rem + at) = lo;
+      if (d4 == 0) factor[rl] = p.scale * up;
+    }
+  }
+  fence_proxy_async();
+}
+
+// For the joining kernel: how many CTAs hold parts of the unit (0: it is whole), and the first one's slot.
+__device__ __forceinline__ void note_unit(const TreeParams &p, const Segment &g, uint64_t all, uint64_t grid) {
+  const uint64_t c0 = ((g.unit0 + 1) * grid - 1) / all, c1 = ((g.unit0 + g.w.tiles) * grid - 1) / all;
+  uint32_t *u = p.units + 2 * (((size_t)g.s * p.c.hk + g.kvh) * p.max_blocks + g.block);
+  u[0] = g.whole() ? 0 : (uint32_t)(c1 - c0 + 1);
+  u[1] = (uint32_t)(2 * c0 + (c0 * all / grid < g.unit0 ? 1 : 0));
+}
+
+// Join the parts of the units that several CTAs shared: CTA (unit, 8 rows), a thread 4 dims of a row. Parts lie
+// [row][hd] (BY_ROW) or [hd / 4][row] float4, as the kernels have them.
+constexpr uint32_t kJoinRows = 8;
+template <int HD, uint32_t MR, bool BY_ROW>
+__global__ void __launch_bounds__(kJoinRows * HD / 4) k_attn_tree_join(TreeParams p) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ float ws[kJoinRows][kTcGrid];
+  __shared__ float inv[kJoinRows];
+  const uint32_t unit = blockIdx.x, block = unit % p.max_blocks, kvh = unit / p.max_blocks % p.c.hk;
+  const uint32_t s = unit / p.max_blocks / p.c.hk, row0 = blockIdx.y * kJoinRows, t = threadIdx.x;
+  const SeqWork w = seq_work<MR, kTcTile>(p, s);
+  if (block >= w.blocks) return;
+  const uint32_t rows = min(MR, w.nodes * p.g - block * MR);
+  const uint32_t parts = min(p.units[2 * unit], kTcGrid), first = p.units[2 * unit + 1];
+  if (parts == 0 || row0 >= rows) return;
+  auto slot = [&](uint32_t q) -> size_t { return q == 0 ? first : (first & ~1u) + 2 * q; };
+  const uint32_t n = min(kJoinRows, rows - row0), warps = kJoinRows * HD / 128, lane = t & 31;
+  for (uint32_t r = t >> 5; r < n; r += warps) {
+    float M = -INFINITY;
+    for (uint32_t q = lane; q < parts; q += 32) {
+      ws[r][q] = p.part_ml[(slot(q) * MR + row0 + r) * 2];
+      M = fmaxf(M, ws[r][q]);
+    }
+    M = warp_max(M);
+    float L = 0.0f;
+    for (uint32_t q = lane; q < parts; q += 32) {
+      const float e = ws[r][q] == -INFINITY ? 0.0f : ex2(ws[r][q] - M);
+      L = fmaf(p.part_ml[(slot(q) * MR + row0 + r) * 2 + 1], e, L);
+      ws[r][q] = e;
+    }
+    L = warp_sum(L);
+    if (lane == 0) inv[r] = L != 0.0f ? 1.0f / L : 0.0f;
+  }
+  __syncthreads();
+  const uint32_t r = BY_ROW ? t / (HD / 4) : t % kJoinRows, d4 = BY_ROW ? t % (HD / 4) : t / kJoinRows;
+  if (r >= n) return;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (uint32_t q0 = 0; q0 < parts; q0 += 8) {
+    float4 f[8];
+#pragma unroll
+    for (int u = 0; u < 8; u++)
+      if (q0 + u < parts)
+        f[u] = *reinterpret_cast<const float4 *>(p.part_o + (BY_ROW ? (slot(q0 + u) * MR + row0 + r) * HD + 4 * d4
+                                                                          : ((slot(q0 + u) * (HD / 4) + d4) * MR + row0 + r) * 4));
+#pragma unroll
+    for (int u = 0; u < 8; u++)
+      if (q0 + u < parts) {
+        const float y = ws[r][q0 + u];
+        acc.x = fmaf(f[u].x, y, acc.x), acc.y = fmaf(f[u].y, y, acc.y);
+        acc.z = fmaf(f[u].z, y, acc.z), acc.w = fmaf(f[u].w, y, acc.w);
+      }
+  }
+  const uint32_t rr = block * MR + row0 + r;
+  const float y = inv[r];
+  *reinterpret_cast<float4 *>(p.out + ((size_t)(w.first + rr / p.g) * p.h + kvh * p.g + rr % p.g) * HD + 4 * d4) =
+      make_float4(acc.x * y, acc.y * y, acc.z * y, acc.w * y);
+}
+
+}  // namespace

@@ -1,26 +1,10 @@
-// Attention of drafted nodes over a cache view (pai_b200_attn_tree_f16kv).
+// Attention of drafted nodes over a cache view (pai_b200_attn_tree_f16kv): the choice of kernel, and the form that
+// takes any page size.
 //
-// A sequence's query rows are its nodes times the G = h / kv_heads query heads
-// that share a kv head, in tiles of MR rows. Every row tile of every kv head
-// ("unit") goes over the same keys: the committed positions, then the nodes
-// themselves, in tiles of kTile positions, with one running softmax.
-//
-//   s_j = (q . k_j) / sqrt(hd) if row sees j, else -inf
-//   m = max s_j, l = sum e^(s_j - m), o = sum e^(s_j - m) v_j / l
-//
-// Work split: the (unit, tile) pairs of all sequences, in order, are cut into
-// gridDim.x even ranges, whatever the lengths are (they are known on the
-// device only). A CTA writes the units that lie in its range to `out`, and
-// (o, m, l) of a unit that it shares to scratch; the last CTA of such a unit
-// joins the parts in order, so that the result does not depend on which CTA
-// is last.
-//
-// Arithmetic: K and V are fp16 as stored. q, scaled by a power of two for
-// each row, and the softmax weights are split into an fp16 part and an fp16
-// remainder and multiplied twice, with fp32 sums: 22 bits of each, so that
-// the products are as exact as fp32 ones. The weights carry a factor 2^12
-// that keeps the remainders of small ones above fp16's smallest step.
-#include <cuda.h>  // CUtensorMap and its enums (types only; the encoder comes from the runtime)
+//   attn_tree_few.cuh    at most 32 rows (nodes x query heads of a kv head) of a sequence: decoding, small trees
+//   attn_tree_many.cuh   more rows
+//   k_attn_tree (here)   where tensor copies cannot fetch the cache: page sizes that no power of two from 8 divides
+//                        (a page of 8 n positions is fetched in shares), strides beyond a tensor map's
 #include <cudaTypedefs.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -28,33 +12,21 @@
 #include <algorithm>
 
 #include "../b200_internal.h"
+#include "attn_tree.cuh"
+#include "attn_tree_few.cuh"
+#include "attn_tree_many.cuh"
+#include "attn_tree_tc.cuh"
 #include "b200_device.cuh"
 #include "kv_view.cuh"
 
 namespace {
 
-constexpr uint32_t kTile = 64, kThreads = 128, kMaxSeqs = 1024;
+// ---- any page size: mma.sync -----------------------------------------------------------------
+//
+// Tiles of kTile positions by 16-byte asynchronous copies, row by row, so that a page may end anywhere.
+constexpr uint32_t kTile = 64, kThreads = 128;
 constexpr uint32_t kGrid = 296;  // two CTAs an SM
 constexpr int kStages = 3;
-constexpr float kPShift = 12.0f;
-
-struct TreeParams {
-  KvDev c;
-  uint32_t h, g, max_nodes, words, max_blocks;  // g: query heads of a kv head; max_blocks: row tiles of a sequence
-  uint64_t rows;
-  const int32_t *lens, *off;
-  const uint64_t *mask;
-  const float *q;
-  float *out;
-  float *part_o;   // scratch [2 gridDim.x][MR][hd]
-  float *part_ml;  // scratch [2 gridDim.x][MR][2]
-  uint32_t *cnt;   // counters [n_seq][kv head][row tile], left at zero
-  uint32_t *units; // scratch [n_seq][kv head][row tile][2]: parts of a unit, slot of the first
-  uint32_t *err;
-  uint64_t wait_ns;
-  uint32_t chunk;  // tcgen05 form: positions of one tensor copy
-  float scale;     // log2(e) / sqrt(hd)
-};
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -83,84 +55,6 @@ template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-// (x, y) -> packed fp16 parts and packed fp16 remainders
-__device__ __forceinline__ void split_f16(float x, float y, uint32_t &hi, uint32_t &lo) {
-  const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
-  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
-  hi = *reinterpret_cast<const uint32_t *>(&h);
-  lo = *reinterpret_cast<const uint32_t *>(&l);
-}
-
-// 2^x of the special function unit: 2^-22 relative, results below 2^-126 are 0
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Bits [at, at + 64) of a row of `words` 64-bit words; at may be negative.
-__device__ __forceinline__ uint64_t window(const uint64_t *m, uint32_t words, int32_t at) {
-  const int32_t w = at >> 6, sh = at & 63;
-  const uint64_t a = w >= 0 && w < (int32_t)words ? m[w] : 0;
-  const uint64_t b = w + 1 >= 0 && w + 1 < (int32_t)words ? m[w + 1] : 0;
-  return sh ? (a >> sh) | (b << (64 - sh)) : a;
-}
-// The lowest n bits (n below 0: none; above 63: all).
-__device__ __forceinline__ uint64_t low_bits(int64_t n) {
-  return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1;
-}
-
-// One sequence's share of the work.
-struct SeqWork {
-  uint32_t len, nodes, first, blocks, tiles;
-};
-template <uint32_t MR, uint32_t KT>
-__device__ __forceinline__ SeqWork seq_work(const TreeParams &p, uint32_t s) {
-  SeqWork w;
-  w.nodes = kv_nodes(p.off, s, p.rows, p.max_nodes, &w.first);
-  w.len = kv_len(p.c, p.lens, s);
-  w.blocks = (w.nodes * p.g + MR - 1) / MR;
-  w.tiles = (w.len + w.nodes + KT - 1) / KT;
-  return w;
-}
-
-// upto[s]: (unit, tile) pairs of the sequences before s. Every thread of the block calls it; a barrier must follow.
-template <uint32_t MR, uint32_t KT, uint32_t THREADS>
-__device__ __forceinline__ void pairs_before(const TreeParams &p, uint64_t *upto) {
-  const uint32_t n_seq = p.c.n_seq, lane = threadIdx.x & 31;
-  for (uint32_t s = threadIdx.x; s < n_seq; s += THREADS) {
-    const SeqWork w = seq_work<MR, KT>(p, s);
-    upto[s + 1] = (uint64_t)w.blocks * w.tiles * p.c.hk;
-  }
-  if (threadIdx.x == 0) upto[0] = 0;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    uint64_t sum = 0;
-    for (uint32_t s0 = 0; s0 < n_seq; s0 += 32) {
-      const uint32_t s = s0 + lane;
-      uint64_t x = s < n_seq ? upto[s + 1] : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= (uint32_t)o) x += y;
-      }
-      x += sum;
-      if (s < n_seq) upto[s + 1] = x;
-      sum = __shfl_sync(0xffffffffu, x, 31);
-    }
-  }
-}
-
-// 2^-e (down) that brings a row's largest element `top` into [1, 2), and 2^e; 1 for a row of zeros, subnormals or
-// infinities.
-__device__ __forceinline__ void row_scale(float top, float &down, float &up) {
-  const uint32_t ex = __float_as_uint(top) >> 23;
-  const bool turn = ex >= 1 && ex <= 252;
-  down = turn ? __uint_as_float((254 - ex) << 23) : 1.0f;
-  up = turn ? __uint_as_float(ex << 23) : 1.0f;
-}
-
 // Shared memory of a stage: K then V rows, padded so that the eight rows of an ldmatrix lie in different banks.
 template <int HD>
 struct Stage {
@@ -547,674 +441,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tree(TreeParams p) {
   }
 }
 
-// ---- more than 32 rows: tcgen05 --------------------------------------------------------------
-//
-// The same sums for row tiles of 128 on the fifth-generation tensor cores, one CTA an SM. Key tiles of 128
-// positions; S = Q K^T and the tile's P V go to TMEM, with K, V and Q (both fp16 parts) in shared memory in the
-// 128-byte swizzle and P (both parts) written over S. P V reads V as it lies, hd contiguous (an MN-major B).
-//   warps 0-3, 4-7   softmax of every other key tile, a row a thread: maximum and weights
-//   warps 8-11       add the tiles' P V to the running output in registers, a row a thread
-//   warp 12          issues the MMAs: Q K^T of tile i + 1 before P V of tile i, so that they overlap the softmax
-//   warp 13, 14      copy the K and the V tiles by tensor copies, a page or a share of one at a time (p.chunk
-//                    positions: the largest power of two up to 128 that divides the page size)
-//   warp 15          takes non-finite elements out of V tiles that hold nodes
-// Registers: 512 threads at 128; setmaxnreg gives the softmax warps 136, the folding ones 184 and leaves 56 to the
-// others (256 * 136 + 128 * 184 + 128 * 56 = 65536, what the block was launched with).
-// Calls of at most 32 rows a kv head take row tiles of 32: Q is then small enough for a third K and V tile in flight.
-constexpr uint32_t kTcThreads = 512, kTcTile = 128, kTcGrid = 148;
-
-__device__ __forceinline__ uint64_t desc_k(uint32_t saddr) {  // K-major, 128-byte swizzle, 8-row groups of 1024 bytes
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)1u << 16 | (uint64_t)(1024u >> 4) << 32 | (uint64_t)1u << 46 |
-         (uint64_t)2u << 61;
-}
-__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t block) {
-  // MN-major: 64-element blocks of the contiguous dimension `block` bytes apart, 8-row groups of 1024 bytes
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)(block >> 4) << 16 | (uint64_t)(1024u >> 4) << 32 |
-         (uint64_t)1u << 46 | (uint64_t)2u << 61;
-}
-// kind::f16: fp16 A and B, fp32 sums, M = 128, N = n; b_mn: B is MN-major
-__host__ __device__ constexpr uint32_t idesc_f16(uint32_t n, bool b_mn) {
-  return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((128u >> 4) << 24);
-}
-// Issued by the one lane that has `leader` set; the whole warp runs the loop around it, so that descriptors stay in
-// uniform registers.
-__device__ __forceinline__ void tc_mma_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-  asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
-      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add), "r"(leader)
-      : "memory");
-}
-__device__ __forceinline__ void tc_mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-  asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
-      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add), "r"(leader)
-      : "memory");
-}
-__device__ __forceinline__ void tc_commit(uint32_t leader, uint64_t *bar) {
-  asm volatile(
-      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
-      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)),
-      "r"(leader)
-      : "memory");
-}
-__device__ __forceinline__ uint32_t elect_one() {
-  uint32_t is;
-  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(is));
-  return is;
-}
-// [64 dims] x [chunk positions] of one kv head of one page; coordinates outside the planes read zeros
-__device__ __forceinline__ void tma_load(void *dst, const CUtensorMap *map, uint32_t dim, uint32_t row, uint32_t head,
-                                         uint32_t page, uint64_t *bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
-      "[%6];" ::"r"(smem_u32(dst)),
-      "l"(map), "r"(dim), "r"(row), "r"(head), "r"(page), "r"(smem_u32(bar))
-      : "memory");
-}
-__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_ld32(uint32_t at, uint32_t *r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(at));
-}
-__device__ __forceinline__ void tc_ld16(uint32_t at, uint32_t (&r)[16]) {  // and wait for it
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(at)
-      : "memory");
-}
-// Wait for the loads; the words pass through, so that nothing that uses them is moved before the wait.
-__device__ __forceinline__ void tc_ld_wait(uint32_t *r) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13])
-               :
-               : "memory");
-  asm volatile("" : "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
-                    "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27])
-               :: "memory");
-  asm volatile("" : "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
-}
-__device__ __forceinline__ void tc_st16(uint32_t at, const uint32_t *r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
-      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(at)
-      : "memory");
-}
-template <int ID, int N>
-__device__ __forceinline__ void named_sync() {
-  __syncwarp();
-  asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory");
-}
-
-// One CTA's run over the (unit, tile) pairs: the part of each unit that lies in it, in order.
-struct Segment {
-  SeqWork w;
-  uint64_t unit0;
-  uint32_t s, kvh, block, tile0, tile1;
-  __device__ __forceinline__ bool whole() const { return tile0 == 0 && tile1 == w.tiles; }
-};
-struct Walk {
-  uint64_t at, end;
-  uint32_t s;
-};
-template <uint32_t MR, uint32_t KT>
-__device__ __forceinline__ bool next_segment(const TreeParams &p, const uint64_t *upto, Walk &k, Segment &g) {
-  if (k.at >= k.end) return false;
-  while (upto[k.s + 1] <= k.at) k.s++;
-  g.s = k.s;
-  g.w = seq_work<MR, KT>(p, k.s);
-  const uint64_t unit = (k.at - upto[k.s]) / g.w.tiles;
-  g.unit0 = upto[k.s] + unit * g.w.tiles;
-  g.kvh = (uint32_t)(unit / g.w.blocks), g.block = (uint32_t)(unit % g.w.blocks);
-  const uint64_t unit1 = g.unit0 + g.w.tiles;
-  g.tile0 = (uint32_t)(k.at - g.unit0), g.tile1 = (uint32_t)((k.end < unit1 ? k.end : unit1) - g.unit0);
-  k.at = g.unit0 + g.tile1;
-  return true;
-}
-
-template <int HD, uint32_t MR, uint32_t NS>
-struct TcSmem {
-  static constexpr uint32_t kBlock = kTcTile * 128;         // a tile's 64 dims: 16 KB
-  static constexpr uint32_t kTileBytes = HD / 64 * kBlock;  // a K or V tile
-  static constexpr uint32_t kQBlock = MR * 128, kQBytes = HD / 64 * kQBlock;  // one part of Q
-  // With MR below 128 the MMAs read 128 rows all the same: what follows Q, for rows that nobody reads.
-  uint8_t q[2][kQBytes];
-  uint8_t kt[NS][kTileBytes];
-  uint8_t vt[NS][kTileBytes];
-  // Words and rows of a tile are read long before the tile that takes their place: fold(i) frees the TMEM of P V of
-  // tile i + 2, so no warp is more than a few tiles ahead of it.
-  uint32_t valid[8][4];       // positions of a tile that hold a row
-  uint32_t odd[8][4];         // its nodes with a non-finite V row
-  float mrow[4][MR];          // [tile]: the maximum that a row's weights of this tile are relative to
-  float ml[4][2][MR][2];      // [segment][warpgroup]: a row's maximum and sum of weights
-  float factor[MR];
-  uint64_t upto[kMaxSeqs + 1];
-  uint64_t kfull[NS], kempty[NS], vfull[NS], vclean[NS], vempty[NS], sfull[2], pfull[2], ofull[2], ofree[2], lfull[4],
-      qfull, drain;
-  uint32_t tmem;
-};
-
-template <int HD, uint32_t MR, uint32_t NS>
-__global__ void __launch_bounds__(kTcThreads, 1)
-    k_attn_tree_tc(TreeParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
-  using Smem = TcSmem<HD, MR, NS>;
-  extern __shared__ __align__(16) uint8_t raw[];
-  Smem &sm = *reinterpret_cast<Smem *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-  constexpr uint32_t BL = Smem::kBlock;
-  const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  pdl_trigger();
-  if (t == 0) {
-    for (uint32_t i = 0; i < NS; i++) {
-      mbar_init(&sm.kfull[i], 1);
-      mbar_init(&sm.vfull[i], 1);
-      mbar_init(&sm.vclean[i], 32);
-      mbar_init(&sm.kempty[i], 1);
-      mbar_init(&sm.vempty[i], 1);
-    }
-    for (int i = 0; i < 2; i++) {
-      mbar_init(&sm.sfull[i], 1);
-      mbar_init(&sm.pfull[i], 4);
-      mbar_init(&sm.ofull[i], 1);
-      mbar_init(&sm.ofree[i], 4);
-    }
-    mbar_init(&sm.qfull, 8);
-    for (int i = 0; i < 4; i++) mbar_init(&sm.lfull[i], 8);
-    mbar_init(&sm.drain, 1);
-    fence_mbar_init();
-  }
-  if (warp == 12) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  }
-  pdl_wait();
-  pairs_before<MR, kTcTile, kTcThreads>(p, sm.upto);
-  tc_before();
-  __syncthreads();
-  tc_after();
-  const uint32_t tmem = sm.tmem;
-  const uint64_t all = sm.upto[p.c.n_seq], cta = blockIdx.x, grid = gridDim.x < all ? gridDim.x : all;
-  Walk walk;
-  walk.at = cta < grid ? cta * all / grid : 0;
-  walk.end = cta < grid ? (cta + 1) * all / grid : 0;
-  walk.s = 0;
-  const uint64_t begin = walk.at;
-  Segment g;
-  bool ok = true;
-  // after a wait has run out a role goes on without waiting or copying, so that the barriers among its own threads
-  // still meet; the error word tells the host
-  auto wait = [&](uint64_t *bar, uint32_t parity) {
-    if (ok && !mbar_wait(bar, parity & 1u, p.wait_ns)) {
-      ok = false;
-      atomicExch(p.err, 1u);
-    }
-  };
-  // which of the 64 positions from node `base32` (negative: committed) on a row of node `nd` may see
-  auto seen = [&](uint32_t base32, bool live, uint32_t nd, uint32_t first) -> uint64_t {
-    const int32_t base = (int32_t)base32;
-    const uint64_t past = low_bits(-(int64_t)base);
-    if (!live) return past;
-    if (!p.mask) return low_bits((int64_t)nd + 1 - base);
-    return past | (window(p.mask + (size_t)(first + nd) * p.words, p.words, base) & ~past);
-  };
-
-  if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 15) {
-      // ---- cleaner: V tiles on their way to the MMAs, the rows of those that hold nodes ----
-      // (It hands every tile over: a barrier that it watched for some phases only could be two phases on.)
-      // A non-finite V row may only reach the rows that see its node, and a weight of 0 does not keep it out of a
-      // product: such elements (those of stale rows behind the last node too) become 0 here, and the folding warps
-      // add them to the rows that see them.
-      constexpr uint32_t CH = HD / 8;
-      uint32_t i = 0;
-      while (next_segment<MR, kTcTile>(p, sm.upto, walk, g))
-        for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
-          const uint32_t sl = i % NS;
-          wait(&sm.vfull[sl], i / NS);
-          if ((tile + 1) * kTcTile <= g.w.len) {
-            mbar_arrive(&sm.vclean[sl]);
-            continue;
-          }
-          uint32_t any[4] = {0, 0, 0, 0};
-          // a lane has rows lane, lane + 32, ..: its rows of a word are one bit each
-#pragma unroll
-          for (uint32_t x = 0; x < 4; x++) {
-            const uint32_t r = 32 * x + lane;
-            bool bad = false;
-#pragma unroll 4
-            for (uint32_t ch = 0; ch < CH; ch++) {
-              uint4 *at = reinterpret_cast<uint4 *>(sm.vt[sl] + (ch / 8) * BL + r * 128 + (((ch % 8) ^ (r & 7)) << 4));
-              uint4 v = *at;
-              uint32_t *cw = reinterpret_cast<uint32_t *>(&v);
-              bool here = false;
-#pragma unroll
-              for (int y = 0; y < 4; y++) {
-                if ((cw[y] & 0x7C00u) == 0x7C00u) cw[y] &= 0xFFFF0000u, here = true;
-                if ((cw[y] & 0x7C000000u) == 0x7C000000u) cw[y] &= 0xFFFFu, here = true;
-              }
-              if (here) *at = v;
-              bad |= here;
-            }
-            any[x] = __ballot_sync(0xffffffffu, bad);
-          }
-          if (lane < 4) sm.odd[i & 7][lane] = lane == 0 ? any[0] : lane == 1 ? any[1] : lane == 2 ? any[2] : any[3];
-          fence_proxy_async();
-          mbar_arrive(&sm.vclean[sl]);
-        }
-    } else if (warp >= 13) {
-      // ---- copies: warp 13 the K tiles, 14 the V tiles; a lane a chunk of p.chunk positions, which lie in one page ----
-      const bool is_v = warp == 14;
-      const CUtensorMap *map = is_v ? &vmap : &kmap;
-      uint64_t *full = is_v ? sm.vfull : sm.kfull, *empty = is_v ? sm.vempty : sm.kempty;
-      const uint32_t chunks = kTcTile / p.chunk, chunk = p.chunk, P = p.c.page_tokens;
-      uint32_t i = 0;  // tiles of the run so far
-      while (next_segment<MR, kTcTile>(p, sm.upto, walk, g)) {
-        const uint32_t total = g.w.len + g.w.nodes;
-        // where the lane's chunk of a tile lies: page (n_pages for a hole, which reads zeros), first row; -1: behind
-        // the last position, not copied
-        int32_t page, row;
-        auto find = [&](uint32_t tile) {
-          const uint32_t pos = tile * kTcTile + lane * chunk;
-          page = -1, row = 0;
-          if (lane < chunks && tile < g.tile1 && pos < total) {
-            const uint32_t pg = pos / P;
-            uint32_t x = p.c.n_pages;
-            if (pg < p.c.max_pages) x = p.c.table ? (uint32_t)p.c.table[(size_t)g.s * p.c.max_pages + pg] : g.s;
-            page = (int32_t)min(x, p.c.n_pages);
-            row = (int32_t)(pos - pg * P);
-          }
-        };
-        find(g.tile0);
-        for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
-          const uint32_t sl = i % NS;
-          const int32_t at = page, r = row;
-          find(tile + 1);  // the next tile's table entries come while this one is copied
-          const uint32_t copied = __ballot_sync(0xffffffffu, at >= 0);
-          const uint32_t there = __ballot_sync(0xffffffffu, at >= 0 && at < (int32_t)p.c.n_pages);
-          if (i >= NS) wait(&empty[sl], i / NS - 1);
-          __syncwarp();
-          if (!is_v) {
-            if (lane < 4) {  // the word of positions 32 lane .. + 31
-              const uint32_t cap = min(total, p.c.max_pages * P), pos = tile * kTcTile + 32 * lane;
-              uint32_t bits = 0;
-              if (chunk >= 32) {
-                bits = (there >> (32 * lane / chunk)) & 1 ? 0xFFFFFFFFu : 0u;
-              } else {
-                for (uint32_t c = 0; c < 32 / chunk; c++)
-                  if ((there >> (32 / chunk * lane + c)) & 1) bits |= ((1u << chunk) - 1) << (c * chunk);
-              }
-              sm.valid[i & 7][lane] = bits & (uint32_t)low_bits((int64_t)cap - pos);
-            }
-            __syncwarp();
-          }
-          if (ok) {
-            uint8_t *dst = (is_v ? sm.vt : sm.kt)[sl] + lane * chunk * 128;
-            if (lane == 0) mbar_expect_tx(&full[sl], __popc(copied) * chunk * HD * 2);
-            __syncwarp();
-            if (at >= 0) {
-#pragma unroll
-              for (uint32_t b = 0; b < HD / 64; b++) tma_load(dst + b * BL, map, 64 * b, r, g.kvh, at, &full[sl]);
-            }
-          }
-          __syncwarp();
-        }
-      }
-      // the last copies land before the block ends, whatever became of the others
-      ok = true;
-      for (uint32_t n = i < NS ? 0 : i - NS; n < i; n++) wait(&full[n % NS], n / NS);
-    } else {
-      // ---- MMA issue ----
-      const uint32_t leader = elect_one();
-      const uint64_t qd = desc_k(smem_u32(sm.q[0])), kd = desc_k(smem_u32(sm.kt[0])), vd = desc_mn(smem_u32(sm.vt[0]), BL);
-      constexpr uint64_t kTileStep = Smem::kTileBytes >> 4, kQStep = Smem::kQBytes >> 4;  // in 16 bytes
-      uint32_t i = 0, seg = 0;
-      auto scores = [&](uint32_t n) {  // S = Q K^T of tile n: both parts of Q
-        wait(&sm.kfull[n % NS], n / NS);
-        tc_after();
-        const uint64_t kb = kd + (n % NS) * kTileStep;
-        const uint32_t d = tmem + 128 * (n & 1);
-        if (ok) {
-#pragma unroll
-          for (uint32_t k = 0; k < HD / 16; k++) {
-            const uint64_t qo = ((k / 4) * Smem::kQBlock + (k % 4) * 32) >> 4, ko = ((k / 4) * BL + (k % 4) * 32) >> 4;
-            tc_mma_ss(leader, d, qd + qo, kb + ko, idesc_f16(kTcTile, false), k > 0);
-            tc_mma_ss(leader, d, qd + kQStep + qo, kb + ko, idesc_f16(kTcTile, false), true);
-          }
-          tc_commit(leader, &sm.sfull[n & 1]);
-          tc_commit(leader, &sm.kempty[n % NS]);
-        }
-        __syncwarp();
-      };
-      while (next_segment<MR, kTcTile>(p, sm.upto, walk, g)) {
-        wait(&sm.qfull, seg++);
-        scores(i);
-        for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
-          const uint32_t sl = i % NS;
-          if (tile + 1 < g.tile1) scores(i + 1);
-          if (i >= 2) wait(&sm.ofree[i & 1], (i >> 1) - 1);
-          wait(&sm.pfull[i & 1], i >> 1);
-          wait(&sm.vclean[sl], i / NS);
-          tc_after();
-          const uint64_t vb = vd + sl * kTileStep;
-          const uint32_t a = tmem + 128 * (i & 1), d = tmem + 256 + 128 * (i & 1);
-          if (ok) {  // this tile's P V, from zero: the sum over tiles is made in registers, where it is rounded
-#pragma unroll
-            for (uint32_t k = 0; k < kTcTile / 16; k++) {
-              const uint32_t at = a + 16 * k;  // 8 words of parts, 8 of remainders
-              tc_mma_ts(leader, d, at, vb + k * (2048 >> 4), idesc_f16(HD, true), k > 0);
-              tc_mma_ts(leader, d, at + 8, vb + k * (2048 >> 4), idesc_f16(HD, true), true);
-            }
-            tc_commit(leader, &sm.ofull[i & 1]);
-            tc_commit(leader, &sm.vempty[sl]);
-          }
-          __syncwarp();
-        }
-      }
-      // the MMAs in flight end before TMEM is given back
-      tc_commit(leader, &sm.drain);
-      ok = true;
-      wait(&sm.drain, 0);
-      __syncwarp();
-    }
-  } else if (warp >= 8) {
-    // ---- fold: P V of the tiles, in order, into a row's running output; a thread a row ----
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
-    const uint32_t r = t & 127, lanes = (warp & 3) * 32 << 16;
-    uint32_t i = 0, seg = 0;
-    while (next_segment<MR, kTcTile>(p, sm.upto, walk, g)) {
-      const uint32_t rows = min(MR, g.w.nodes * p.g - g.block * MR);
-      const bool work = (warp & 3) * 32 < rows;  // a warp whose rows are all past the last one keeps step only
-      const uint32_t rr = g.block * MR + r, nd = rr / p.g;
-      const bool live = r < rows;
-      float o[HD], M = -INFINITY;
-#pragma unroll
-      for (int d = 0; d < HD; d++) o[d] = 0.0f;
-      for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
-        wait(&sm.ofull[i & 1], i >> 1);
-        __syncwarp();
-        tc_after();
-        if (work) {
-          // the weights of even and odd tiles are relative to maxima of their own
-          const float mt = sm.mrow[i & 3][r], mn = fmaxf(M, mt);
-          const float a = M == mn ? 1.0f : ex2(M - mn), b = mt == mn ? 1.0f : ex2(mt - mn);
-          M = mn;
-          const uint32_t oa = tmem + lanes + 256 + 128 * (i & 1);
-          const bool plain = __all_sync(0xffffffffu, a == 1.0f && b == 1.0f);
-#pragma unroll
-          for (int c = 0; c < HD / 16; c++) {
-            uint32_t v[16];
-            tc_ld16(oa + 16 * c, v);
-            if (plain) {
-#pragma unroll
-              for (int d = 0; d < 16; d++) o[16 * c + d] += __uint_as_float(v[d]);
-            } else {
-#pragma unroll
-              for (int d = 0; d < 16; d++) o[16 * c + d] = fmaf(o[16 * c + d], a, __uint_as_float(v[d]) * b);
-            }
-          }
-        }
-        tc_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.ofree[i & 1]);
-        if (work && (tile + 1) * kTcTile > g.w.len) {
-          // non-finite V elements of nodes that this row sees
-#pragma unroll 1
-          for (int x = 0; x < 4; x++) {
-            uint32_t left = sm.odd[i & 7][x] & sm.valid[i & 7][x];
-            if (left) left &= (uint32_t)(seen(tile * kTcTile + 32 * x - g.w.len, live, nd, g.w.first));
-#pragma unroll 1
-            for (; left; left &= left - 1) {
-              const int64_t at_row = kv_row(p.c, g.s, tile * kTcTile + 32 * x + __ffs(left) - 1);
-              const __half2 *vr = reinterpret_cast<const __half2 *>(p.c.v + (size_t)g.kvh * p.c.head_stride + at_row);
-#pragma unroll
-              for (int d = 0; d < HD / 2; d++) {
-                const float2 f = __half22float2(vr[d]);
-                if (!isfinite(f.x)) o[2 * d] += f.x;
-                if (!isfinite(f.y)) o[2 * d + 1] += f.y;
-              }
-            }
-          }
-          __syncwarp();
-        }
-      }
-      wait(&sm.lfull[seg & 3], seg >> 2);  // the softmax warps may be two segments ahead, never four
-      __syncwarp();
-      const bool whole = g.whole();
-      if (live) {
-        float L = 0.0f;
-#pragma unroll
-        for (int y = 0; y < 2; y++) {
-          const float my = sm.ml[seg & 3][y][r][0];
-          if (my != -INFINITY) L = fmaf(sm.ml[seg & 3][y][r][1], my == M ? 1.0f : ex2(my - M), L);
-        }
-        const uint64_t slot = 2 * cta + (begin >= g.unit0 ? 0 : 1);
-        const float scale = whole ? (L != 0.0f ? 1.0f / L : 0.0f) : 1.0f;  // a row that sees nothing gets zeros
-        // whole units go to their rows of out; parts lie [hd / 4][row] float4
-        float *dst = whole ? p.out + ((size_t)(g.w.first + nd) * p.h + g.kvh * p.g + rr % p.g) * HD
-                           : p.part_o + (slot * (HD / 4) * MR + r) * 4;
-        const uint32_t step = whole ? 4 : 4 * MR;
-#pragma unroll
-        for (int d = 0; d < HD; d += 4)
-          *reinterpret_cast<float4 *>(dst + (size_t)(d / 4) * step) =
-              make_float4(o[d] * scale, o[d + 1] * scale, o[d + 2] * scale, o[d + 3] * scale);
-        if (!whole) {
-          p.part_ml[(slot * MR + r) * 2] = M;
-          p.part_ml[(slot * MR + r) * 2 + 1] = L;
-        }
-      }
-      if (g.tile0 == 0 && r == 0) {
-        // for the joining kernel: how many CTAs hold parts of the unit (0: it is whole), and the first one's slot
-        const uint64_t c0 = ((g.unit0 + 1) * grid - 1) / all, c1 = ((g.unit0 + g.w.tiles) * grid - 1) / all;
-        uint32_t *u = p.units + 2 * (((size_t)g.s * p.c.hk + g.kvh) * p.max_blocks + g.block);
-        u[0] = whole ? 0 : (uint32_t)(c1 - c0 + 1);
-        u[1] = (uint32_t)(2 * c0 + (c0 * all / grid < g.unit0 ? 1 : 0));
-      }
-      seg++;
-    }
-  } else {
-    // ---- softmax: warpgroup wg has every other tile of the run, a thread a row ----
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
-    const uint32_t wg = warp >> 2, r = t & 127;
-    const uint32_t sa = tmem + ((warp & 3) * 32 << 16) + 128 * wg;
-    uint32_t i = 0, seg = 0;
-    while (next_segment<MR, kTcTile>(p, sm.upto, walk, g)) {
-      const uint32_t rows = min(MR, g.w.nodes * p.g - g.block * MR);
-      // Q into shared memory, a power of two and two fp16 parts a row; the last segment's products are done
-      {
-        constexpr uint32_t LR = HD / 4, RW = 32 / LR, WR = MR / 8;  // lanes of a row, rows of an access, rows of a warp
-        constexpr uint32_t UN = WR / RW < 4 ? WR / RW : 4;
-        const uint32_t d4 = lane % LR;
-        for (uint32_t b0 = 0; b0 < WR; b0 += UN * RW) {
-          float4 f[UN];
-#pragma unroll
-          for (uint32_t u = 0; u < UN; u++) {
-            const uint32_t rl = warp * WR + b0 + u * RW + lane / LR, rr = g.block * MR + rl;
-            f[u] = rl < rows ? *reinterpret_cast<const float4 *>(
-                                   p.q + ((size_t)(g.w.first + rr / p.g) * p.h + g.kvh * p.g + rr % p.g) * HD + 4 * d4)
-                             : make_float4(0.f, 0.f, 0.f, 0.f);
-          }
-#pragma unroll
-          for (uint32_t u = 0; u < UN; u++) {
-            const uint32_t rl = warp * WR + b0 + u * RW + lane / LR;
-            float top = fmaxf(fmaxf(fabsf(f[u].x), fabsf(f[u].y)), fmaxf(fabsf(f[u].z), fabsf(f[u].w)));
-#pragma unroll
-            for (uint32_t o = LR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            float down, up;
-            row_scale(top, down, up);
-            uint2 hi, lo;
-            split_f16(f[u].x * down, f[u].y * down, hi.x, lo.x);
-            split_f16(f[u].z * down, f[u].w * down, hi.y, lo.y);
-            const uint32_t at = (d4 / 16) * Smem::kQBlock + rl * 128 + (((d4 % 16) / 2 ^ (rl & 7)) << 4) + (d4 & 1) * 8;
-            *reinterpret_cast<uint2 *>(sm.q[0] + at) = hi;
-            *reinterpret_cast<uint2 *>(sm.q[1] + at) = lo;
-            if (d4 == 0) sm.factor[rl] = p.scale * up;
-          }
-        }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.qfull);
-        named_sync<1, 256>();
-      }
-      const bool work = (warp & 3) * 32 < rows, live = r < rows;
-      const float factor = work ? sm.factor[r] : 0.0f;
-      const uint32_t nd = (g.block * MR + r) / p.g;
-      float m = -INFINITY, l = 0.0f;
-      for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
-        if ((i & 1) != wg) continue;
-        wait(&sm.sfull[wg], i >> 1);
-        __syncwarp();
-        tc_after();
-        if (work) {
-          // Two passes over the scores in steps of 64, rolled: unrolled over the tile, the code of the three
-          // warps that share a scheduler outgrew the instruction cache (4 of 14 stalled warps waited for
-          // instructions, and a tile took 4000 cycles).
-          const bool drafted = (tile + 1) * kTcTile > g.w.len;
-          const uint32_t *ok4 = sm.valid[i & 7];
-          const bool masked = drafted || (ok4[0] & ok4[1] & ok4[2] & ok4[3]) != ~0u;
-          float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-          for (uint32_t h = 0; h < 128; h += 64) {
-            uint32_t v[64];
-            tc_ld32(sa + h, v);
-            tc_ld32(sa + h + 32, v + 32);
-            tc_ld_wait(v);
-            tc_ld_wait(v + 32);
-            if (masked) {  // unseen positions become -inf, for the second pass too
-              uint64_t see = (uint64_t)ok4[h / 32] | (uint64_t)ok4[h / 32 + 1] << 32;
-              if (drafted) see &= seen(tile * kTcTile + h - g.w.len, live, nd, g.w.first);
-              const uint32_t b0 = (uint32_t)see, b1 = (uint32_t)(see >> 32);
-#pragma unroll
-              for (int e = 0; e < 64; e++)
-                if (!(((e < 32 ? b0 : b1) >> (e & 31)) & 1)) v[e] = 0xFF800000u;
-#pragma unroll
-              for (int e = 0; e < 64; e += 16) tc_st16(sa + h + e, v + e);
-            }
-#pragma unroll
-            for (int e = 0; e < 64; e += 8)
-#pragma unroll
-              for (int u = 0; u < 4; u++)
-                t4[u] = fmaxf(t4[u], fmaxf(__uint_as_float(v[e + 2 * u]), __uint_as_float(v[e + 2 * u + 1])));
-          }
-          if (masked) asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-          const float mn = fmaxf(m, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * factor);
-          const float corr = m == mn ? 1.0f : ex2(m - mn);
-          m = mn;
-          sm.mrow[i & 3][r] = mn;
-          __syncwarp();
-          const float sub = mn == -INFINITY ? 0.0f : mn - kPShift;
-          float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-          for (uint32_t h = 0; h < 128; h += 64) {  // the weights, over the scores
-            uint32_t v[64];
-            tc_ld32(sa + h, v);
-            tc_ld32(sa + h + 32, v + 32);
-            tc_ld_wait(v);
-            tc_ld_wait(v + 32);
-#pragma unroll
-            for (int c = 0; c < 64; c += 16) {
-              uint32_t w[16];  // 8 words of parts, 8 of remainders
-#pragma unroll
-              for (int e = 0; e < 16; e += 2) {
-                const float p0 = ex2(fmaf(__uint_as_float(v[c + e]), factor, -sub));
-                const float p1 = ex2(fmaf(__uint_as_float(v[c + e + 1]), factor, -sub));
-                part[(e / 2) & 3] += p0 + p1;
-                split_f16(p0, p1, w[e / 2], w[8 + e / 2]);
-              }
-              tc_st16(sa + h + c, w);
-            }
-          }
-          l = l * corr + ((part[0] + part[1]) + (part[2] + part[3]));
-          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-        }
-        tc_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.pfull[wg]);
-      }
-      if (work) {
-        sm.ml[seg & 3][wg][r][0] = m;
-        sm.ml[seg & 3][wg][r][1] = l;
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.lfull[seg & 3]);
-      named_sync<1, 256>();  // every score of the segment has been read: Q may be written again
-      seg++;
-    }
-  }
-  tc_before();
-  __syncthreads();
-  if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
-}
-
-// Join the parts of the units that several CTAs shared: CTA (unit, 8 rows), a thread 4 dims of a row.
-constexpr uint32_t kJoinRows = 8;
-template <int HD, uint32_t MR>
-__global__ void __launch_bounds__(kJoinRows * HD / 4) k_attn_tree_join(TreeParams p) {
-  pdl_trigger();
-  pdl_wait();
-  __shared__ float ws[kJoinRows][kTcGrid];
-  __shared__ float inv[kJoinRows];
-  const uint32_t unit = blockIdx.x, block = unit % p.max_blocks, kvh = unit / p.max_blocks % p.c.hk;
-  const uint32_t s = unit / p.max_blocks / p.c.hk, row0 = blockIdx.y * kJoinRows, t = threadIdx.x;
-  const SeqWork w = seq_work<MR, kTcTile>(p, s);
-  if (block >= w.blocks) return;
-  const uint32_t rows = min(MR, w.nodes * p.g - block * MR);
-  const uint32_t parts = min(p.units[2 * unit], kTcGrid), first = p.units[2 * unit + 1];
-  if (parts == 0 || row0 >= rows) return;
-  auto slot = [&](uint32_t q) -> size_t { return q == 0 ? first : (first & ~1u) + 2 * q; };
-  const uint32_t n = min(kJoinRows, rows - row0), warps = kJoinRows * HD / 128, lane = t & 31;
-  for (uint32_t r = t >> 5; r < n; r += warps) {
-    float M = -INFINITY;
-    for (uint32_t q = lane; q < parts; q += 32) {
-      ws[r][q] = p.part_ml[(slot(q) * MR + row0 + r) * 2];
-      M = fmaxf(M, ws[r][q]);
-    }
-    M = warp_max(M);
-    float L = 0.0f;
-    for (uint32_t q = lane; q < parts; q += 32) {
-      const float e = ws[r][q] == -INFINITY ? 0.0f : ex2(ws[r][q] - M);
-      L = fmaf(p.part_ml[(slot(q) * MR + row0 + r) * 2 + 1], e, L);
-      ws[r][q] = e;
-    }
-    L = warp_sum(L);
-    if (lane == 0) inv[r] = L != 0.0f ? 1.0f / L : 0.0f;
-  }
-  __syncthreads();
-  const uint32_t r = t % kJoinRows, d4 = t / kJoinRows;
-  if (r >= n) return;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (uint32_t q0 = 0; q0 < parts; q0 += 8) {
-    float4 f[8];
-#pragma unroll
-    for (int u = 0; u < 8; u++)
-      if (q0 + u < parts)
-        f[u] = *reinterpret_cast<const float4 *>(p.part_o + ((slot(q0 + u) * (HD / 4) + d4) * MR + row0 + r) * 4);
-#pragma unroll
-    for (int u = 0; u < 8; u++)
-      if (q0 + u < parts) {
-        const float y = ws[r][q0 + u];
-        acc.x = fmaf(f[u].x, y, acc.x), acc.y = fmaf(f[u].y, y, acc.y);
-        acc.z = fmaf(f[u].z, y, acc.z), acc.w = fmaf(f[u].w, y, acc.w);
-      }
-  }
-  const uint32_t rr = block * MR + row0 + r;
-  const float y = inv[r];
-  *reinterpret_cast<float4 *>(p.out + ((size_t)(w.first + rr / p.g) * p.h + kvh * p.g + rr % p.g) * HD + 4 * d4) =
-      make_float4(acc.x * y, acc.y * y, acc.z * y, acc.w * y);
-}
-
 // Tensor map of a layer's plane: [page][kv head][position][64 dims of hd], boxes of `chunk` positions, 128-byte swizzle.
 bool plane_map(const TreeParams &p, const __half *plane, CUtensorMap *map) {
   const auto encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(b200_tensor_map_encoder());
@@ -1228,16 +454,17 @@ bool plane_map(const TreeParams &p, const __half *plane, CUtensorMap *map) {
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int HD, uint32_t MR, uint32_t NS>
-pai_status_t launch_tree_tc(pai_b200_ctx_t *ctx, TreeParams &p, const CUtensorMap &kmap, const CUtensorMap &vmap) {
-  constexpr size_t smem = sizeof(TcSmem<HD, MR, NS>) + 1024;
+// The tcgen05 kernels: `kern` with `smem` bytes and row tiles of MR, then the joining kernel.
+template <int HD, uint32_t MR, bool BY_ROW>
+pai_status_t launch_tc(pai_b200_ctx_t *ctx, TreeParams &p, void (*kern)(TreeParams, CUtensorMap, CUtensorMap),
+                       uint32_t threads, size_t smem, const CUtensorMap &kmap, const CUtensorMap &vmap) {
   static SmemOptIn opt;
   pai_status_t st = b200_cuda(opt.ensure(b200_ctx_device(ctx), smem,
-                                         [](size_t b) {
-                                           return cudaFuncSetAttribute(k_attn_tree_tc<HD, MR, NS>,
+                                         [kern](size_t b) {
+                                           return cudaFuncSetAttribute((const void *)kern,
                                                                        cudaFuncAttributeMaxDynamicSharedMemorySize, (int)b);
                                          }),
-                              "k_attn_tree_tc smem attribute");
+                              "attn_tree smem attribute");
   if (st) return st;
   p.max_blocks = (p.max_nodes * p.g + MR - 1) / MR;
   const uint64_t units = (uint64_t)p.c.n_seq * p.c.hk * p.max_blocks;
@@ -1251,13 +478,13 @@ pai_status_t launch_tree_tc(pai_b200_ctx_t *ctx, TreeParams &p, const CUtensorMa
   p.part_o = scratch;
   p.part_ml = scratch + slots * MR * HD;
   p.units = (uint32_t *)(p.part_ml + slots * MR * 2);
-  b200_launch(ctx, k_attn_tree_tc<HD, MR, NS>, dim3(grid), dim3(kTcThreads), smem, p, kmap, vmap);
+  b200_launch(ctx, kern, dim3(grid), dim3(threads), smem, p, kmap, vmap);
   // the joining kernel is resident before this one ends, and waits for it
   const int pdl = b200_ctx_pdl(ctx);
   b200_ctx_set_pdl(ctx, 1);
-  b200_launch(ctx, k_attn_tree_join<HD, MR>, dim3((uint32_t)units, MR / kJoinRows), dim3(kJoinRows * HD / 4), 0, p);
+  b200_launch(ctx, k_attn_tree_join<HD, MR, BY_ROW>, dim3((uint32_t)units, MR / kJoinRows), dim3(kJoinRows * HD / 4), 0, p);
   b200_ctx_set_pdl(ctx, pdl);
-  return b200_launched(ctx, 2, "k_attn_tree_tc");
+  return b200_launched(ctx, 2, "k_attn_tree");
 }
 
 template <int HD, int WM>
@@ -1298,7 +525,10 @@ pai_status_t launch_tree_hd(pai_b200_ctx_t *ctx, TreeParams &p) {
     while (p.chunk > 8 && p.c.page_tokens % p.chunk) p.chunk /= 2;
   CUtensorMap kmap, vmap;
   if ((!p.c.table || p.c.page_tokens % p.chunk == 0) && plane_map(p, p.c.k, &kmap) && plane_map(p, p.c.v, &vmap))
-    return rows <= 32 ? launch_tree_tc<HD, 32, 3>(ctx, p, kmap, vmap) : launch_tree_tc<HD, 128, 2>(ctx, p, kmap, vmap);
+    return rows <= kFewRows ? launch_tc<HD, kFewRows, true>(ctx, p, k_attn_tree_few<HD>, kFewThreads,
+                                                            sizeof(FewSmem<HD>) + 1024, kmap, vmap)
+                            : launch_tc<HD, kManyRows, false>(ctx, p, k_attn_tree_many<HD>, kManyThreads,
+                                                              sizeof(ManySmem<HD>) + 1024, kmap, vmap);
   if (rows <= 16) return launch_tree<HD, 1>(ctx, p);
   return launch_tree<HD, 4>(ctx, p);
 }
