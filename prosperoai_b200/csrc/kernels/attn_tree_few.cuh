@@ -18,7 +18,7 @@
 
 namespace {
 
-constexpr uint32_t kFewThreads = 384, kFewRows = 32, kFewK = 3, kFewV = 2;
+constexpr uint32_t kFewThreads = 384, kFewRows = 32, kFewK = 3, kFewV = 2, kFewWaves = 4;
 
 template <int HD>
 struct FewSmem {
@@ -38,7 +38,8 @@ struct FewSmem {
   float factor[kFewRows], sub[kFewRows];
   float wmax[4][kFewRows];
   float lsum[4][4][kFewRows], msum[4][kFewRows];  // [segment][warp]: sums of weights; maxima
-  uint64_t upto[kMaxSeqs + 1];
+  uint32_t upto[kMaxSeqs + 1];
+  Ring ring;
   uint64_t kfull[kFewK], kempty[kFewK], vfull[kFewV], vclean[kFewV], vempty[kFewV], sfull[2], pfull[2], ofull[2], ofree[2],
       lfull[4], qfull, drain;
   uint32_t tmem;
@@ -87,6 +88,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     for (int i = 0; i < 4; i++) mbar_init(&sm.lfull[i], 4);
     mbar_init(&sm.qfull, 4);
     mbar_init(&sm.drain, 1);
+    for (uint32_t i = 0; i < kRing; i++) mbar_init(&sm.ring.full[i], 1);
     fence_mbar_init();
   }
   if (warp == 8) {
@@ -94,24 +96,21 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   pdl_wait();
-  pairs_before<kFewRows, kTcTile, kFewThreads>(p, sm.upto);
+  pairs_before32<kFewRows, kFewThreads>(p, sm.upto);
   tc_before();
   __syncthreads();
   tc_after();
   const uint32_t tmem = sm.tmem;  // columns 0, 64: S^T of even and odd tiles; 128, 192: O^T
-  const uint64_t all = sm.upto[p.c.n_seq], cta = blockIdx.x, grid = gridDim.x < all ? gridDim.x : all;
-  Walk walk = walk_of(p, sm.upto, grid);
-  const uint64_t begin = walk.at;
   Segment g;
   Waiter wait{p.wait_ns, p.err};
   uint32_t i = 0, seg = 0;  // tiles and segments of the run so far
 
   if (warp == 9) {
-    copy_tiles<HD, kFewRows, kFewK>(p, &kmap, sm.upto, walk, sm.kt[0], sm.kfull, sm.kempty, sm.valid);
+    copy_tiles<HD, kFewRows, kFewK, true>(p, &kmap, sm.upto, sm.ring, kFewWaves, sm.kt[0], sm.kfull, sm.kempty, sm.valid);
   } else if (warp == 10) {
-    copy_tiles<HD, kFewRows, kFewV>(p, &vmap, sm.upto, walk, sm.vt[0], sm.vfull, sm.vempty, nullptr);
+    copy_tiles<HD, kFewRows, kFewV, false>(p, &vmap, sm.upto, sm.ring, 0, sm.vt[0], sm.vfull, sm.vempty, nullptr);
   } else if (warp == 11) {
-    clean_tiles<HD, kFewRows, kFewV>(p, sm.upto, walk, sm.vt[0], sm.vfull, sm.vclean, sm.odd);
+    clean_tiles<HD, kFewV>(p, sm.ring, sm.vt[0], sm.vfull, sm.vclean, sm.odd);
   } else if (warp == 8) {
     // ---- MMA issue ----
     const uint32_t leader = elect_one();
@@ -132,8 +131,8 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       }
       __syncwarp();
     };
-    while (next_segment<kFewRows, kTcTile>(p, sm.upto, walk, g)) {
-      wait(&sm.qfull, seg++);
+    for (; next_segment(sm.ring, seg, wait, g); seg++) {
+      wait(&sm.qfull, seg);
       scores(i);
       for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
         if (tile + 1 < g.tile1) scores(i + 1);
@@ -162,8 +161,8 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     // ---- fold: a thread a dim (with hd 64 the upper half of the lanes has none) ----
     const uint32_t d = t - 128, lanes = (warp & 3) * 32 << 16;
     const bool live = d < HD;
-    while (next_segment<kFewRows, kTcTile>(p, sm.upto, walk, g)) {
-      const uint32_t rows = min(kFewRows, g.w.nodes * p.g - g.block * kFewRows);
+    for (; next_segment(sm.ring, seg, wait, g); seg++) {
+      const uint32_t rows = min(kFewRows, g.nodes * p.g - g.block * kFewRows);
       float o[32];
 #pragma unroll
       for (int r = 0; r < 32; r++) o[r] = 0.0f;
@@ -185,7 +184,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
         if (lane == 0) mbar_arrive(&sm.ofree[i & 1]);
 #pragma unroll
         for (int r = 0; r < 32; r++) o[r] += __uint_as_float(v[r]) + __uint_as_float(v[32 + r]);
-        if ((tile + 1) * kTcTile > g.w.len && live) {
+        if ((tile + 1) * kTcTile > g.len && live) {
           // non-finite V elements of nodes, for the rows that see them
 #pragma unroll 1
           for (int x = 0; x < 4; x++)
@@ -196,7 +195,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
               if (isfinite(f)) continue;
 #pragma unroll
               for (int r = 0; r < 32; r++)
-                if ((uint32_t)r < rows && (seen(p, pos - g.w.len, true, (g.block * kFewRows + r) / p.g, g.w.first) & 1))
+                if ((uint32_t)r < rows && (seen(p, pos - g.len, true, (g.block * kFewRows + r) / p.g, g.first) & 1))
                   o[r] += f;
             }
         }
@@ -205,7 +204,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       wait(&sm.lfull[seg & 3], seg >> 2);  // the softmax warps may be two segments ahead, never four
       __syncwarp();
       const bool whole = g.whole();
-      const uint64_t slot = 2 * cta + (begin >= g.unit0 ? 0 : 1);
+      const size_t slot = g.slot;
 #pragma unroll
       for (int r = 0; r < 32; r++) {
         if ((uint32_t)r >= rows) continue;
@@ -214,7 +213,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
         const uint32_t rr = g.block * kFewRows + r;
         if (whole) {  // a row that sees nothing gets zeros
           if (live)
-            p.out[((size_t)(g.w.first + rr / p.g) * p.h + g.kvh * p.g + rr % p.g) * HD + d] = L != 0.0f ? o[r] * (1.0f / L) : 0.0f;
+            p.out[((size_t)(g.first + rr / p.g) * p.h + g.kvh * p.g + rr % p.g) * HD + d] = L != 0.0f ? o[r] * (1.0f / L) : 0.0f;
         } else {
           if (live) p.part_o[(slot * kFewRows + r) * HD + d] = o[r];
           if (d == 0) {
@@ -223,14 +222,13 @@ __global__ void __launch_bounds__(kFewThreads, 1)
           }
         }
       }
-      if (g.tile0 == 0 && d == 0) note_unit(p, g, all, grid);
-      seg++;
+      if (g.tile0 == 0 && d == 0) note_unit(p, g);
     }
   } else {
     // ---- softmax: a thread a position ----
     constexpr float kNone = -1e30f, kFull = 15.5f;  // no maximum yet; the largest exponent that weights may have
-    while (next_segment<kFewRows, kTcTile>(p, sm.upto, walk, g)) {
-      const uint32_t rows = min(kFewRows, g.w.nodes * p.g - g.block * kFewRows), groups = (rows + 7) / 8;
+    for (; next_segment<1, 128>(sm.ring, seg, wait, g); seg++) {
+      const uint32_t rows = min(kFewRows, g.nodes * p.g - g.block * kFewRows), groups = (rows + 7) / 8;
       // every score of the last segment has been read, so its products are done: Q may be written
       put_queries<HD, kFewRows, 4>(p, g, rows, warp, sm.q, Smem::kQBlock, kFewRows * 128, sm.factor);
       if (t < kFewRows) sm.sub[t] = kNone;
@@ -266,10 +264,10 @@ __global__ void __launch_bounds__(kFewThreads, 1)
           s[r + 2] = there ? s[r + 2] * f.z : -INFINITY;
           s[r + 3] = there ? s[r + 3] * f.w : -INFINITY;
         }
-        if ((tile + 1) * kTcTile > g.w.len && pos >= g.w.len) {  // a node: for the rows that see it
+        if ((tile + 1) * kTcTile > g.len && pos >= g.len) {  // a node: for the rows that see it
 #pragma unroll
           for (int r = 0; r < 32; r++)
-            if ((uint32_t)r < rows && !(seen(p, pos - g.w.len, true, (g.block * kFewRows + r) / p.g, g.w.first) & 1))
+            if ((uint32_t)r < rows && !(seen(p, pos - g.len, true, (g.block * kFewRows + r) / p.g, g.first) & 1))
               s[r] = -INFINITY;
         }
         __syncwarp();
@@ -335,11 +333,11 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.lfull[seg & 3]);
       named_sync<1, 128>();  // the factors and maxima may be written again
-      seg++;
     }
   }
   tc_before();
   __syncthreads();
+  if (t == 0) leave(p);
   if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256));
 }
 

@@ -14,7 +14,7 @@
 
 namespace {
 
-constexpr uint32_t kManyThreads = 512, kManyRows = 128;
+constexpr uint32_t kManyThreads = 512, kManyRows = 128, kManyWaves = 2;
 
 template <int HD>
 struct ManySmem {
@@ -28,7 +28,8 @@ struct ManySmem {
   float factor[kManyRows];
   float top[2][2][kManyRows];      // [tile parity][warpgroup]: maxima of a row's halves
   float ml[2][kManyRows];
-  uint64_t upto[kMaxSeqs + 1];
+  uint32_t upto[kMaxSeqs + 1];
+  Ring ring;
   uint64_t kfull[2], kempty[2], vfull[2], vclean[2], vempty[2], sfull[2], pfull[2], ofull[2], qfull, drain;
   uint32_t tmem;
 };
@@ -55,6 +56,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     }
     mbar_init(&sm.qfull, 8);
     mbar_init(&sm.drain, 1);
+    for (uint32_t i = 0; i < kRing; i++) mbar_init(&sm.ring.full[i], 1);
     fence_mbar_init();
   }
   if (warp == 8) {
@@ -62,25 +64,22 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   pdl_wait();
-  pairs_before<kManyRows, kTcTile, kManyThreads>(p, sm.upto);
+  pairs_before32<kManyRows, kManyThreads>(p, sm.upto);
   tc_before();
   __syncthreads();
   tc_after();
   const uint32_t tmem = sm.tmem;
-  const uint64_t all = sm.upto[p.c.n_seq], cta = blockIdx.x, grid = gridDim.x < all ? gridDim.x : all;
-  Walk walk = walk_of(p, sm.upto, grid);
-  const uint64_t begin = walk.at;
   Segment g;
   Waiter wait{p.wait_ns, p.err};
 
   if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 12)
-      copy_tiles<HD, kManyRows, 2>(p, &kmap, sm.upto, walk, sm.kt[0], sm.kfull, sm.kempty, sm.valid);
+      copy_tiles<HD, kManyRows, 2, true>(p, &kmap, sm.upto, sm.ring, kManyWaves, sm.kt[0], sm.kfull, sm.kempty, sm.valid);
     else if (warp == 13)
-      copy_tiles<HD, kManyRows, 2>(p, &vmap, sm.upto, walk, sm.vt[0], sm.vfull, sm.vempty, nullptr);
+      copy_tiles<HD, kManyRows, 2, false>(p, &vmap, sm.upto, sm.ring, 0, sm.vt[0], sm.vfull, sm.vempty, nullptr);
     else if (warp == 14)
-      clean_tiles<HD, kManyRows, 2>(p, sm.upto, walk, sm.vt[0], sm.vfull, sm.vclean, sm.odd);
+      clean_tiles<HD, 2>(p, sm.ring, sm.vt[0], sm.vfull, sm.vclean, sm.odd);
   } else if (warp >= 8) {
     // ---- MMA issue ----
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -106,8 +105,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         }
         __syncwarp();
       };
-      while (next_segment<kManyRows, kTcTile>(p, sm.upto, walk, g)) {
-        wait(&sm.qfull, seg++);
+      for (; next_segment(sm.ring, seg, wait, g); seg++) {
+        wait(&sm.qfull, seg);
         scores(i);
         for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
           if (tile + 1 < g.tile1) scores(i + 1);
@@ -141,8 +140,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     const uint32_t wg = warp >> 2, r = t & 127;
     const uint32_t lanes = (warp & 3) * 32 << 16;
     uint32_t i = 0;
-    while (next_segment<kManyRows, kTcTile>(p, sm.upto, walk, g)) {
-      const uint32_t rows = min(kManyRows, g.w.nodes * p.g - g.block * kManyRows);
+    for (uint32_t seg = 0; next_segment<1, 256>(sm.ring, seg, wait, g); seg++) {
+      const uint32_t rows = min(kManyRows, g.nodes * p.g - g.block * kManyRows);
       // the last segment's products are done: Q may be written
       put_queries<HD, kManyRows, 8>(p, g, rows, warp, sm.q[0], BL, Smem::kTileBytes, sm.factor);
       __syncwarp();
@@ -169,7 +168,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           for (int c = 0; c < HD / 64; c++) tc_ld_wait(v + 32 * c);
 #pragma unroll
           for (int d = 0; d < HD / 2; d++) o[d] = fmaf(o[d], corr, __uint_as_float(v[d]));
-          if ((tile + 1) * kTcTile > g.w.len) {
+          if ((tile + 1) * kTcTile > g.len) {
             // non-finite V elements of nodes that this row sees
 #pragma unroll 1
             for (int x = 0; x < 4; x++)
@@ -203,14 +202,14 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           uint32_t v[64];
           tc_ld32(sa, v);
           tc_ld32(sa + 32, v + 32);
-          const bool drafted = (tile + 1) * kTcTile > g.w.len;
+          const bool drafted = (tile + 1) * kTcTile > g.len;
           const uint64_t ok0 = (uint64_t)sm.valid[i & 7][0] | (uint64_t)sm.valid[i & 7][1] << 32;
           const uint64_t ok1 = (uint64_t)sm.valid[i & 7][2] | (uint64_t)sm.valid[i & 7][3] << 32;
           const bool masked = drafted || (ok0 & ok1) != ~0ull;
           now0 = ok0, now1 = ok1;
           if (drafted) {
-            now0 &= seen(p, tile * kTcTile - g.w.len, live, nd, g.w.first);
-            now1 &= seen(p, tile * kTcTile + 64 - g.w.len, live, nd, g.w.first);
+            now0 &= seen(p, tile * kTcTile - g.len, live, nd, g.first);
+            now1 &= seen(p, tile * kTcTile + 64 - g.len, live, nd, g.first);
           }
           tc_ld_wait(v);
           tc_ld_wait(v + 32);
@@ -266,10 +265,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       named_sync<1, 256>();
       const float L = sm.ml[0][r] + sm.ml[1][r];
       const bool whole = g.whole();
-      const uint64_t slot = 2 * cta + (begin >= g.unit0 ? 0 : 1);
+      const size_t slot = g.slot;
       const float scale = whole ? (L != 0.0f ? 1.0f / L : 0.0f) : 1.0f;
       // whole units go to their rows of out; parts lie [hd / 4][row] float4
-      float *dst = whole ? p.out + ((size_t)(g.w.first + (live ? nd : 0)) * p.h + g.kvh * p.g + rr % p.g) * HD + wg * (HD / 2)
+      float *dst = whole ? p.out + ((size_t)(g.first + (live ? nd : 0)) * p.h + g.kvh * p.g + rr % p.g) * HD + wg * (HD / 2)
                          : p.part_o + ((slot * (HD / 4) + wg * (HD / 8)) * kManyRows + r) * 4;
       const uint32_t step = whole ? 4 : 4 * kManyRows;
       if (live) {
@@ -282,12 +281,13 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           p.part_ml[(slot * kManyRows + r) * 2 + 1] = L;
         }
       }
-      if (g.tile0 == 0 && t == 0) note_unit(p, g, all, grid);
+      if (g.tile0 == 0 && t == 0) note_unit(p, g);
       named_sync<1, 256>();  // Q and the sums may be written again
     }
   }
   tc_before();
   __syncthreads();
+  if (t == 0) leave(p);
   if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 

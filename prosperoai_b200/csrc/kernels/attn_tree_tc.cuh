@@ -10,7 +10,7 @@
 
 namespace {
 
-constexpr uint32_t kTcTile = 128, kTcGrid = 148;
+constexpr uint32_t kTcTile = 128, kTcGrid = 148, kRing = 16;
 
 __device__ __forceinline__ uint64_t desc_k(uint32_t saddr) {  // K-major, 128-byte swizzle, 8-row groups of 1024 bytes
   return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)1u << 16 | (uint64_t)(1024u >> 4) << 32 | (uint64_t)1u << 46 |
@@ -102,30 +102,48 @@ __device__ __forceinline__ void named_sync() {
   asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory");
 }
 
-// One CTA's run over the (unit, tile) pairs: the part of each unit that lies in it, in order.
+// A part of a unit: what the roles of a CTA work through, in order. `tile1` 0: there are no more.
 struct Segment {
-  SeqWork w;
-  uint64_t unit0;
-  uint32_t s, kvh, block, tile0, tile1;
-  __device__ __forceinline__ bool whole() const { return tile0 == 0 && tile1 == w.tiles; }
+  uint32_t s, kvh, block, tile0, tile1, tiles;  // sequence, unit, key tiles of the part and of the unit
+  uint32_t len, nodes, first;                   // the sequence's committed positions, nodes, first row
+  uint32_t slot;                                // where a part is put
+  uint32_t parts, slot0;                        // chunks that share the unit, slot of the first of its parts
+  __device__ __forceinline__ bool whole() const { return tile0 == 0 && tile1 == tiles; }
 };
-struct Walk {
-  uint64_t at, end;
-  uint32_t s;
+// The warp that copies K walks over the pairs and hands the segments to the other roles through a ring: the divisions
+// and lookups of a step are made once, and ahead. (A role is at most a few tiles behind it, never kRing segments.)
+struct Ring {
+  Segment seg[kRing];
+  uint64_t full[kRing];
 };
-template <uint32_t MR, uint32_t KT>
-__device__ __forceinline__ bool next_segment(const TreeParams &p, const uint64_t *upto, Walk &k, Segment &g) {
-  if (k.at >= k.end) return false;
-  while (upto[k.s + 1] <= k.at) k.s++;
-  g.s = k.s;
-  g.w = seq_work<MR, KT>(p, k.s);
-  const uint64_t unit = (k.at - upto[k.s]) / g.w.tiles;
-  g.unit0 = upto[k.s] + unit * g.w.tiles;
-  g.kvh = (uint32_t)(unit / g.w.blocks), g.block = (uint32_t)(unit % g.w.blocks);
-  const uint64_t unit1 = g.unit0 + g.w.tiles;
-  g.tile0 = (uint32_t)(k.at - g.unit0), g.tile1 = (uint32_t)((k.end < unit1 ? k.end : unit1) - g.unit0);
-  k.at = g.unit0 + g.tile1;
-  return true;
+
+// upto[s]: (unit, tile) pairs of the sequences before s (the caller bounds their sum). Every thread of the block calls
+// it; a barrier must follow.
+template <uint32_t MR, uint32_t THREADS>
+__device__ __forceinline__ void pairs_before32(const TreeParams &p, uint32_t *upto) {
+  const uint32_t n_seq = p.c.n_seq, lane = threadIdx.x & 31;
+  for (uint32_t s = threadIdx.x; s < n_seq; s += THREADS) {
+    const SeqWork w = seq_work<MR, kTcTile>(p, s);
+    upto[s + 1] = w.blocks * w.tiles * p.c.hk;
+  }
+  if (threadIdx.x == 0) upto[0] = 0;
+  if (n_seq <= 1) return;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    uint32_t sum = 0;
+    for (uint32_t s0 = 0; s0 < n_seq; s0 += 32) {
+      const uint32_t s = s0 + lane;
+      uint32_t x = s < n_seq ? upto[s + 1] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= (uint32_t)o) x += y;
+      }
+      x += sum;
+      if (s < n_seq) upto[s + 1] = x;
+      sum = __shfl_sync(0xffffffffu, x, 31);
+    }
+  }
 }
 
 // Which of the 64 positions from node `base32` (negative: committed) on a row of node `nd` may see.
@@ -151,28 +169,112 @@ struct Waiter {
   }
 };
 
-// The run of this CTA.
-__device__ __forceinline__ Walk walk_of(const TreeParams &p, const uint64_t *upto, uint64_t grid) {
-  const uint64_t all = upto[p.c.n_seq], cta = blockIdx.x;
-  Walk k;
-  k.at = cta < grid ? cta * all / grid : 0;
-  k.end = cta < grid ? (cta + 1) * all / grid : 0;
-  k.s = 0;
-  return k;
+// Whether all threads of a role say so: a warp, or THREADS that meet at barrier BAR.
+template <int BAR, int THREADS>
+__device__ __forceinline__ bool all_of(bool mine) {
+  if (THREADS == 32) return __all_sync(0xffffffffu, mine);
+  uint32_t all;
+  __syncwarp();
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 q, %1, 0;\n bar.red.and.pred p, %2, %3, q;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(all)
+      : "r"((uint32_t)mine), "n"(BAR), "n"(THREADS)
+      : "memory");
+  return all;
+}
+// The n-th segment of the CTA; false behind the last. After a wait has run out anywhere in the role, all of it stops
+// here.
+template <int BAR = 0, int THREADS = 32>
+__device__ __forceinline__ bool next_segment(Ring &ring, uint32_t n, Waiter &wait, Segment &g) {
+  wait(&ring.full[n % kRing], n / kRing);
+  g = ring.seg[n % kRing];
+  return all_of<BAR, THREADS>(wait.ok) && g.tile1 != 0;
 }
 
-// Copies, one warp for all K tiles or all V tiles: a lane a chunk of p.chunk positions, which lie in one page. With
-// `valid` (K) it also notes which positions of a tile hold a row. `slots` tiles are in flight.
-template <int HD, uint32_t MR, uint32_t SLOTS>
-__device__ __forceinline__ void copy_tiles(const TreeParams &p, const CUtensorMap *map, const uint64_t *upto, Walk walk,
-                                           uint8_t *slot0, uint64_t *full, uint64_t *empty, uint32_t (*valid)[4]) {
+// The cut of the pairs into chunks of `size`. SMs do not read memory equally fast: with one even range for each, the
+// slowest of 148 took 112 us where the fastest took 66 (8 sequences of one token at 16384 positions). So there are up to
+// `waves` chunks for each CTA, of four tiles at least: its first is its own, the others are taken from a counter as they
+// come. Parts are numbered by chunks, so that who computes one changes nothing.
+__device__ __forceinline__ uint32_t chunk_size(uint32_t all, uint32_t waves) {
+  const uint32_t g = gridDim.x, w = min(max(all / (4 * g), 1u), waves);
+  return all <= g ? 1 : (all + g * w - 1) / (g * w);
+}
+// The leading role: yields the CTA's segments and hands them on.
+struct Lead {
+  uint32_t all, size, chunks, at = 0, end = 0, s = 0, n = 0;
+  uint32_t chunk = 0, ahead = 0;
+  bool begun = false;
+  template <uint32_t MR>
+  __device__ __forceinline__ bool next(const TreeParams &p, const uint32_t *upto, Ring &ring, Segment &g) {
+    const uint32_t lane = threadIdx.x & 31;
+    if (at >= end) {
+      chunk = begun ? __shfl_sync(0xffffffffu, ahead, 0) : blockIdx.x;
+      begun = true;
+      if (chunk < chunks) {
+        // asked now, needed when the chunk ends
+        ahead = 0xFFFFFFFFu;
+        if (lane == 0 && chunks > gridDim.x) ahead = gridDim.x + atomicAdd(p.cnt, 1u);
+        at = chunk * size;
+        end = min(at + size, all);
+        uint32_t lo = 0;
+        for (uint32_t hi = p.c.n_seq; lo < hi;) {  // the sequence of the first pair
+          const uint32_t mid = (lo + hi) / 2;
+          if (upto[mid + 1] <= at) lo = mid + 1; else hi = mid;
+        }
+        s = lo;
+      }
+    }
+    g.tile1 = 0;
+    if (at < end) {
+      while (upto[s + 1] <= at) s++;
+      const SeqWork w = seq_work<MR, kTcTile>(p, s);
+      const uint32_t unit = (at - upto[s]) / w.tiles, unit0 = upto[s] + unit * w.tiles, unit1 = unit0 + w.tiles;
+      g.s = s, g.kvh = unit / w.blocks, g.block = unit % w.blocks;
+      g.tile0 = at - unit0, g.tile1 = min(end, unit1) - unit0, g.tiles = w.tiles;
+      g.len = w.len, g.nodes = w.nodes, g.first = w.first;
+      g.slot = 2 * chunk + (chunk * size >= unit0 ? 0 : 1);  // the chunk's first part of a unit, or its last
+      const uint32_t c0 = unit0 / size, c1 = (unit1 - 1) / size;
+      g.parts = c1 - c0 + 1;
+      g.slot0 = 2 * c0 + (c0 * size >= unit0 ? 0 : 1);
+      at = unit0 + g.tile1;
+    }
+    if (lane == 0) {
+      ring.seg[n % kRing] = g;
+      mbar_arrive(&ring.full[n % kRing]);
+    }
+    n++;
+    return g.tile1 != 0;
+  }
+};
+// One thread of every CTA, when its roles are done: the last leaves the counters at zero.
+__device__ __forceinline__ void leave(const TreeParams &p) {
+  __threadfence();
+  if (atomicAdd(p.cnt + 1, 1u) == gridDim.x - 1) {
+    p.cnt[0] = 0;
+    p.cnt[1] = 0;
+  }
+}
+
+// Copies, one warp for all K tiles or all V tiles: a lane a chunk of p.chunk positions, which lie in one page. The warp
+// of K (LEADS) also hands out the segments, and notes in `valid` which positions of a tile hold a row. SLOTS tiles are
+// in flight.
+template <int HD, uint32_t MR, uint32_t SLOTS, bool LEADS>
+__device__ __forceinline__ void copy_tiles(const TreeParams &p, const CUtensorMap *map, const uint32_t *upto, Ring &ring,
+                                           uint32_t waves, uint8_t *slot0, uint64_t *full, uint64_t *empty,
+                                           uint32_t (*valid)[4]) {
   constexpr uint32_t BL = kTcTile * 128, BYTES = HD / 64 * BL;
   const uint32_t lane = threadIdx.x & 31, chunks = kTcTile / p.chunk, chunk = p.chunk, P = p.c.page_tokens;
   Waiter wait{p.wait_ns, p.err};
+  Lead lead;
+  if (LEADS) {
+    lead.all = upto[p.c.n_seq];
+    lead.size = chunk_size(lead.all, waves);
+    lead.chunks = (lead.all + lead.size - 1) / lead.size;
+  }
   Segment g;
-  uint32_t i = 0;  // tiles of the run so far
-  while (next_segment<MR, kTcTile>(p, upto, walk, g)) {
-    const uint32_t total = g.w.len + g.w.nodes;
+  uint32_t i = 0;  // tiles so far
+  for (uint32_t n = 0; LEADS ? lead.next<MR>(p, upto, ring, g) : next_segment(ring, n, wait, g); n++) {
+    const uint32_t total = g.len + g.nodes;
     // where the lane's chunk of a tile lies: page (n_pages for a hole, which reads zeros), first row; -1: behind the
     // last position, not copied
     int32_t page, row;
@@ -196,7 +298,7 @@ __device__ __forceinline__ void copy_tiles(const TreeParams &p, const CUtensorMa
       const uint32_t there = __ballot_sync(0xffffffffu, at >= 0 && at < (int32_t)p.c.n_pages);
       if (i >= SLOTS) wait(&empty[sl], i / SLOTS - 1);
       __syncwarp();
-      if (valid) {
+      if (LEADS) {
         if (lane < 4) {  // the word of positions 32 lane .. + 31
           const uint32_t cap = min(total, p.c.max_pages * P), pos = tile * kTcTile + 32 * lane;
           uint32_t bits = 0;
@@ -231,20 +333,20 @@ __device__ __forceinline__ void copy_tiles(const TreeParams &p, const CUtensorMa
 // row may only reach the rows that see its node, and a weight of 0 does not keep it out of a product. Such elements
 // (those of stale rows behind the last node too) become 0 here, and `odd` tells where; they are added later to the rows
 // that see them. (Every tile is handed on: a barrier that was watched for some phases only could be two phases on.)
-template <int HD, uint32_t MR, uint32_t SLOTS>
-__device__ __forceinline__ void clean_tiles(const TreeParams &p, const uint64_t *upto, Walk walk, uint8_t *slot0,
-                                            uint64_t *full, uint64_t *clean, uint32_t (*odd)[4]) {
+template <int HD, uint32_t SLOTS>
+__device__ __forceinline__ void clean_tiles(const TreeParams &p, Ring &ring, uint8_t *slot0, uint64_t *full, uint64_t *clean,
+                                            uint32_t (*odd)[4]) {
   constexpr uint32_t BL = kTcTile * 128, BYTES = HD / 64 * BL, CH = HD / 8;
   const uint32_t lane = threadIdx.x & 31;
   Waiter wait{p.wait_ns, p.err};
   Segment g;
   uint32_t i = 0;
-  while (next_segment<MR, kTcTile>(p, upto, walk, g))
+  for (uint32_t n = 0; next_segment(ring, n, wait, g); n++)
     for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
       const uint32_t sl = i % SLOTS;
       wait(&full[sl], i / SLOTS);
       __syncwarp();
-      if ((tile + 1) * kTcTile > g.w.len) {
+      if ((tile + 1) * kTcTile > g.len) {
 #pragma unroll 1
         for (uint32_t x = 0; x < 4; x++) {  // a lane has a row of each 32
           const uint32_t r = 32 * x + lane;
@@ -288,7 +390,7 @@ __device__ __forceinline__ void put_queries(const TreeParams &p, const Segment &
     for (uint32_t u = 0; u < UN; u++) {
       const uint32_t rl = w * WR + b0 + u * RW + lane / LR, rr = g.block * MR + rl;
       f[u] = rl < rows ? *reinterpret_cast<const float4 *>(
-                             p.q + ((size_t)(g.w.first + rr / p.g) * p.h + g.kvh * p.g + rr % p.g) * HD + 4 * d4)
+                             p.q + ((size_t)(g.first + rr / p.g) * p.h + g.kvh * p.g + rr % p.g) * HD + 4 * d4)
                        : make_float4(0.f, 0.f, 0.f, 0.f);
     }
 #pragma unroll
@@ -311,29 +413,28 @@ __device__ __forceinline__ void put_queries(const TreeParams &p, const Segment &
   fence_proxy_async();
 }
 
-// For the joining kernel: how many CTAs hold parts of the unit (0: it is whole), and the first one's slot.
-__device__ __forceinline__ void note_unit(const TreeParams &p, const Segment &g, uint64_t all, uint64_t grid) {
-  const uint64_t c0 = ((g.unit0 + 1) * grid - 1) / all, c1 = ((g.unit0 + g.w.tiles) * grid - 1) / all;
+// For the joining kernel: how many chunks hold parts of the unit (0: it is whole), and the first one's slot.
+__device__ __forceinline__ void note_unit(const TreeParams &p, const Segment &g) {
   uint32_t *u = p.units + 2 * (((size_t)g.s * p.c.hk + g.kvh) * p.max_blocks + g.block);
-  u[0] = g.whole() ? 0 : (uint32_t)(c1 - c0 + 1);
-  u[1] = (uint32_t)(2 * c0 + (c0 * all / grid < g.unit0 ? 1 : 0));
+  u[0] = g.whole() ? 0 : g.parts;
+  u[1] = g.slot0;
 }
 
-// Join the parts of the units that several CTAs shared: CTA (unit, 8 rows), a thread 4 dims of a row. Parts lie
+// Join the parts of the units that several chunks shared: CTA (unit, 8 rows), a thread 4 dims of a row. Parts lie
 // [row][hd] (BY_ROW) or [hd / 4][row] float4, as the kernels have them.
 constexpr uint32_t kJoinRows = 8;
-template <int HD, uint32_t MR, bool BY_ROW>
+template <int HD, uint32_t MR, uint32_t PARTS, bool BY_ROW>
 __global__ void __launch_bounds__(kJoinRows * HD / 4) k_attn_tree_join(TreeParams p) {
   pdl_trigger();
   pdl_wait();
-  __shared__ float ws[kJoinRows][kTcGrid];
+  __shared__ float ws[kJoinRows][PARTS];
   __shared__ float inv[kJoinRows];
   const uint32_t unit = blockIdx.x, block = unit % p.max_blocks, kvh = unit / p.max_blocks % p.c.hk;
   const uint32_t s = unit / p.max_blocks / p.c.hk, row0 = blockIdx.y * kJoinRows, t = threadIdx.x;
   const SeqWork w = seq_work<MR, kTcTile>(p, s);
   if (block >= w.blocks) return;
   const uint32_t rows = min(MR, w.nodes * p.g - block * MR);
-  const uint32_t parts = min(p.units[2 * unit], kTcGrid), first = p.units[2 * unit + 1];
+  const uint32_t parts = min(p.units[2 * unit], PARTS), first = p.units[2 * unit + 1];
   if (parts == 0 || row0 >= rows) return;
   auto slot = [&](uint32_t q) -> size_t { return q == 0 ? first : (first & ~1u) + 2 * q; };
   const uint32_t n = min(kJoinRows, rows - row0), warps = kJoinRows * HD / 128, lane = t & 31;
