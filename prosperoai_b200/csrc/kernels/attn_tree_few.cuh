@@ -6,7 +6,7 @@
 // A softmax thread has a position and all rows: the weights of a tile need no exchange as long as no row's maximum
 // grows by more than 2^3 (they are relative to a maximum that may be that much too small: fp16 holds 2^15.99, and the
 // weights carry 2^12). Only when some row's does, in a sequence's first tiles, are the rows' maxima taken over the
-// tile, by a reduction that leaves lane r with row r. The sums of weights stay in the threads, one a row and
+// tile. The sums of weights stay in the threads, one a row and
 // position, until a unit ends.
 //   warps 0-3   softmax; the weights go to shared memory, 128 bytes a position, as an MN-major B
 //   warps 4-7   add the tiles' O^T to the running output, a thread a dim, the rows in registers
@@ -18,7 +18,7 @@
 
 namespace {
 
-constexpr uint32_t kFewThreads = 384, kFewRows = 32, kFewK = 3, kFewV = 2, kFewWaves = 4;
+constexpr uint32_t kFewThreads = 384, kFewRows = 32, kFewK = 3, kFewV = 2;
 
 template <int HD>
 struct FewSmem {
@@ -58,6 +58,13 @@ __device__ __forceinline__ float reduce_rows(float (&v)[32], F f) {
       v[j] = f(mine, __shfl_xor_sync(0xffffffffu, other, o));
     }
   return v[0];
+}
+
+// The largest of the lanes' values, NaN apart.
+__device__ __forceinline__ float warp_top(float v) {
+  float top;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(v));
+  return top;
 }
 
 template <int HD>
@@ -106,9 +113,9 @@ __global__ void __launch_bounds__(kFewThreads, 1)
   uint32_t i = 0, seg = 0;  // tiles and segments of the run so far
 
   if (warp == 9) {
-    copy_tiles<HD, kFewRows, kFewK, true>(p, &kmap, sm.upto, sm.ring, kFewWaves, sm.kt[0], sm.kfull, sm.kempty, sm.valid);
+    copy_tiles<HD, kFewRows, kFewK, true>(p, &kmap, sm.upto, sm.ring, sm.kt[0], sm.kfull, sm.kempty, sm.valid);
   } else if (warp == 10) {
-    copy_tiles<HD, kFewRows, kFewV, false>(p, &vmap, sm.upto, sm.ring, 0, sm.vt[0], sm.vfull, sm.vempty, nullptr);
+    copy_tiles<HD, kFewRows, kFewV, false>(p, &vmap, sm.upto, sm.ring, sm.vt[0], sm.vfull, sm.vempty, nullptr);
   } else if (warp == 11) {
     clean_tiles<HD, kFewV>(p, sm.ring, sm.vt[0], sm.vfull, sm.vclean, sm.odd);
   } else if (warp == 8) {
@@ -162,7 +169,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     const uint32_t d = t - 128, lanes = (warp & 3) * 32 << 16;
     const bool live = d < HD;
     for (; next_segment(sm.ring, seg, wait, g); seg++) {
-      const uint32_t rows = min(kFewRows, g.nodes * p.g - g.block * kFewRows);
+      const uint32_t rows = min(kFewRows, g.nodes * p.g - g.block * kFewRows), groups = (rows + 7) / 8;
       float o[32];
 #pragma unroll
       for (int r = 0; r < 32; r++) o[r] = 0.0f;
@@ -170,20 +177,25 @@ __global__ void __launch_bounds__(kFewThreads, 1)
         wait(&sm.ofull[i & 1], i >> 1);
         __syncwarp();
         tc_after();
-        uint32_t v[64];
-        tc_ld32(tmem + lanes + 128 + 64 * (i & 1), v);
-        tc_ld32(tmem + lanes + 160 + 64 * (i & 1), v + 32);
-        if (sm.grew[i & 7]) {
+        const bool grew = sm.grew[i & 7];
 #pragma unroll
-          for (int r = 0; r < 32; r++) o[r] *= sm.corr[i & 7][r];
+        for (uint32_t gr = 0; gr < 4; gr++) {
+          if (gr >= groups) continue;
+          uint32_t v[16];
+          tc_ld8(tmem + lanes + 128 + 64 * (i & 1) + 8 * gr, v);
+          tc_ld8(tmem + lanes + 160 + 64 * (i & 1) + 8 * gr, v + 8);
+          if (grew) {
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) o[8 * gr + e] *= sm.corr[i & 7][8 * gr + e];
+          }
+          tc_ld_wait8(v);
+          tc_ld_wait8(v + 8);
+#pragma unroll
+          for (uint32_t e = 0; e < 8; e++) o[8 * gr + e] += __uint_as_float(v[e]) + __uint_as_float(v[8 + e]);
         }
-        tc_ld_wait(v);
-        tc_ld_wait(v + 32);
         tc_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.ofree[i & 1]);
-#pragma unroll
-        for (int r = 0; r < 32; r++) o[r] += __uint_as_float(v[r]) + __uint_as_float(v[32 + r]);
         if ((tile + 1) * kTcTile > g.len && live) {
           // non-finite V elements of nodes, for the rows that see them
 #pragma unroll 1
@@ -244,41 +256,39 @@ __global__ void __launch_bounds__(kFewThreads, 1)
         wait(&sm.sfull[i & 1], i >> 1);
         __syncwarp();
         tc_after();
-        float s[32];
-        {
-          uint32_t v[64];
-          tc_ld32(sa, v);
-          tc_ld32(sa + 32, v + 32);
-          tc_ld_wait(v);
-          tc_ld_wait(v + 32);
-#pragma unroll
-          for (int r = 0; r < 32; r++) s[r] = __uint_as_float(v[r]) + __uint_as_float(v[32 + r]);
-        }
         const bool there = (sm.valid[i & 7][warp] >> lane) & 1;
         const uint32_t pos = tile * kTcTile + t;
+        const bool is_node = (tile + 1) * kTcTile > g.len && pos >= g.len;
+        // scores in powers of two, unseen ones -inf, and the largest exponent relative to the rows' maxima so far. All of
+        // it in groups of 8 rows, of which the rows' number of groups is run: code that is not run is not fetched, and
+        // instruction fetches are what these warps wait for most.
+        float s[32], top = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < 32; r += 4) {
-          const float4 f = *reinterpret_cast<const float4 *>(&sm.factor[r]);
-          s[r] = there ? s[r] * f.x : -INFINITY;
-          s[r + 1] = there ? s[r + 1] * f.y : -INFINITY;
-          s[r + 2] = there ? s[r + 2] * f.z : -INFINITY;
-          s[r + 3] = there ? s[r + 3] * f.w : -INFINITY;
-        }
-        if ((tile + 1) * kTcTile > g.len && pos >= g.len) {  // a node: for the rows that see it
+        for (uint32_t gr = 0; gr < 4; gr++) {
+          if (gr >= groups) continue;
+          uint32_t v[16];
+          tc_ld8(sa + 8 * gr, v);
+          tc_ld8(sa + 32 + 8 * gr, v + 8);
+          tc_ld_wait8(v);
+          tc_ld_wait8(v + 8);
 #pragma unroll
-          for (int r = 0; r < 32; r++)
-            if ((uint32_t)r < rows && !(seen(p, pos - g.len, true, (g.block * kFewRows + r) / p.g, g.first) & 1))
-              s[r] = -INFINITY;
+          for (uint32_t e = 0; e < 8; e += 4) {
+            const uint32_t r = 8 * gr + e;
+            const float4 f = *reinterpret_cast<const float4 *>(&sm.factor[r]);
+            const float4 u = *reinterpret_cast<const float4 *>(&sm.sub[r]);
+            s[r] = there ? (__uint_as_float(v[e]) + __uint_as_float(v[8 + e])) * f.x : -INFINITY;
+            s[r + 1] = there ? (__uint_as_float(v[e + 1]) + __uint_as_float(v[9 + e])) * f.y : -INFINITY;
+            s[r + 2] = there ? (__uint_as_float(v[e + 2]) + __uint_as_float(v[10 + e])) * f.z : -INFINITY;
+            s[r + 3] = there ? (__uint_as_float(v[e + 3]) + __uint_as_float(v[11 + e])) * f.w : -INFINITY;
+            if (is_node) {  // for the rows that see it
+#pragma unroll
+              for (uint32_t x = r; x < r + 4; x++)
+                if (x < rows && !(seen(p, pos - g.len, true, (g.block * kFewRows + x) / p.g, g.first) & 1)) s[x] = -INFINITY;
+            }
+            top = fmaxf(fmaxf(top, fmaxf(s[r] - u.x, s[r + 1] - u.y)), fmaxf(s[r + 2] - u.z, s[r + 3] - u.w));
+          }
         }
         __syncwarp();
-        // exponents relative to the rows' maxima so far
-        float top = -INFINITY;
-#pragma unroll
-        for (int r = 0; r < 32; r += 4) {
-          const float4 u = *reinterpret_cast<const float4 *>(&sm.sub[r]);
-          if ((uint32_t)r < rows)
-            top = fmaxf(fmaxf(top, fmaxf(s[r] - u.x, s[r + 1] - u.y)), fmaxf(s[r + 2] - u.z, s[r + 3] - u.w));
-        }
         uint32_t any;
         asm volatile(
             "{\n .reg .pred p, q;\n setp.ne.u32 q, %1, 0;\n bar.red.or.pred p, 1, 128, q;\n selp.u32 %0, 1, 0, p;\n}\n"
@@ -286,10 +296,17 @@ __global__ void __launch_bounds__(kFewThreads, 1)
             : "r"((uint32_t)(top > kFull))
             : "memory");
         if (any) {
-          float x[32];
+          float mine = -INFINITY;
 #pragma unroll
-          for (int r = 0; r < 32; r++) x[r] = s[r];
-          sm.wmax[warp][lane] = reduce_rows(x, [](float a, float b) { return fmaxf(a, b); });
+          for (uint32_t gr = 0; gr < 4; gr++) {
+            if (gr >= groups) continue;
+#pragma unroll
+            for (uint32_t r = 8 * gr; r < 8 * gr + 8; r++) {
+              const float x = warp_top(s[r]);
+              if (lane == r) mine = x;
+            }
+          }
+          sm.wmax[warp][lane] = mine;
           named_sync<1, 128>();
           const float mn = fmaxf(fmaxf(fmaxf(m, sm.wmax[0][lane]), fmaxf(sm.wmax[1][lane], sm.wmax[2][lane])), sm.wmax[3][lane]);
           const float corr = m == mn ? 1.0f : ex2(m - mn);
@@ -299,7 +316,11 @@ __global__ void __launch_bounds__(kFewThreads, 1)
             sm.corr[i & 7][lane] = corr;
           }
 #pragma unroll
-          for (int r = 0; r < 32; r++) l[r] *= __shfl_sync(0xffffffffu, corr, r);
+          for (uint32_t gr = 0; gr < 4; gr++) {
+            if (gr >= groups) continue;
+#pragma unroll
+            for (uint32_t r = 8 * gr; r < 8 * gr + 8; r++) l[r] *= __shfl_sync(0xffffffffu, corr, r);
+          }
           named_sync<1, 128>();
         }
         if (t == 0) sm.grew[i & 7] = any;
@@ -337,7 +358,6 @@ __global__ void __launch_bounds__(kFewThreads, 1)
   }
   tc_before();
   __syncthreads();
-  if (t == 0) leave(p);
   if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256));
 }
 

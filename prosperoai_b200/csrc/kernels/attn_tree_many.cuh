@@ -14,7 +14,7 @@
 
 namespace {
 
-constexpr uint32_t kManyThreads = 512, kManyRows = 128, kManyWaves = 2;
+constexpr uint32_t kManyThreads = 512, kManyRows = 128;
 
 template <int HD>
 struct ManySmem {
@@ -75,9 +75,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 12)
-      copy_tiles<HD, kManyRows, 2, true>(p, &kmap, sm.upto, sm.ring, kManyWaves, sm.kt[0], sm.kfull, sm.kempty, sm.valid);
+      copy_tiles<HD, kManyRows, 2, true>(p, &kmap, sm.upto, sm.ring, sm.kt[0], sm.kfull, sm.kempty, sm.valid);
     else if (warp == 13)
-      copy_tiles<HD, kManyRows, 2, false>(p, &vmap, sm.upto, sm.ring, 0, sm.vt[0], sm.vfull, sm.vempty, nullptr);
+      copy_tiles<HD, kManyRows, 2, false>(p, &vmap, sm.upto, sm.ring, sm.vt[0], sm.vfull, sm.vempty, nullptr);
     else if (warp == 14)
       clean_tiles<HD, 2>(p, sm.ring, sm.vt[0], sm.vfull, sm.vclean, sm.odd);
   } else if (warp >= 8) {
@@ -287,7 +287,6 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   }
   tc_before();
   __syncthreads();
-  if (t == 0) leave(p);
   if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 

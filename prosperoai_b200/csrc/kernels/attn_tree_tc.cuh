@@ -75,6 +75,17 @@ __device__ __forceinline__ void tc_ld32(uint32_t at, uint32_t *r) {
       : "r"(at));
 }
 // Wait for the loads; the words pass through, so that nothing that uses them is moved before the wait.
+__device__ __forceinline__ void tc_ld8(uint32_t at, uint32_t *r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(at));
+}
+__device__ __forceinline__ void tc_ld_wait8(uint32_t *r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
+               :
+               : "memory");
+}
 __device__ __forceinline__ void tc_ld_wait(uint32_t *r) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
@@ -191,39 +202,26 @@ __device__ __forceinline__ bool next_segment(Ring &ring, uint32_t n, Waiter &wai
   return all_of<BAR, THREADS>(wait.ok) && g.tile1 != 0;
 }
 
-// The cut of the pairs into chunks of `size`. SMs do not read memory equally fast: with one even range for each, the
-// slowest of 148 took 112 us where the fastest took 66 (8 sequences of one token at 16384 positions). So there are up to
-// `waves` chunks for each CTA, of four tiles at least: its first is its own, the others are taken from a counter as they
-// come. Parts are numbered by chunks, so that who computes one changes nothing.
-__device__ __forceinline__ uint32_t chunk_size(uint32_t all, uint32_t waves) {
-  const uint32_t g = gridDim.x, w = min(max(all / (4 * g), 1u), waves);
-  return all <= g ? 1 : (all + g * w - 1) / (g * w);
-}
+// The cut of the pairs into a chunk for each CTA, of `size` (the last may be shorter, and some CTAs may have none).
+// SMs do not read memory equally fast (with even chunks the slowest of 148 takes 112 us where the fastest takes 66, 8
+// sequences of one token at 16384 positions), but more and smaller chunks, taken from a counter as they come, cost more
+// than they even out: a new chunk waits for its queries and its first maxima (two for each CTA 125 us, six 142, one 109).
 // The leading role: yields the CTA's segments and hands them on.
 struct Lead {
-  uint32_t all, size, chunks, at = 0, end = 0, s = 0, n = 0;
-  uint32_t chunk = 0, ahead = 0;
-  bool begun = false;
+  uint32_t size = 1, at = 0, end = 0, s = 0, n = 0;
+  __device__ __forceinline__ void begin(const TreeParams &p, const uint32_t *upto) {
+    const uint32_t all = upto[p.c.n_seq];
+    size = max((all + gridDim.x - 1) / gridDim.x, 1u);
+    at = min(blockIdx.x * size, all);
+    end = min(at + size, all);
+    for (uint32_t hi = p.c.n_seq; s < hi;) {  // the sequence of the first pair
+      const uint32_t mid = (s + hi) / 2;
+      if (upto[mid + 1] <= at) s = mid + 1; else hi = mid;
+    }
+  }
   template <uint32_t MR>
   __device__ __forceinline__ bool next(const TreeParams &p, const uint32_t *upto, Ring &ring, Segment &g) {
-    const uint32_t lane = threadIdx.x & 31;
-    if (at >= end) {
-      chunk = begun ? __shfl_sync(0xffffffffu, ahead, 0) : blockIdx.x;
-      begun = true;
-      if (chunk < chunks) {
-        // asked now, needed when the chunk ends
-        ahead = 0xFFFFFFFFu;
-        if (lane == 0 && chunks > gridDim.x) ahead = gridDim.x + atomicAdd(p.cnt, 1u);
-        at = chunk * size;
-        end = min(at + size, all);
-        uint32_t lo = 0;
-        for (uint32_t hi = p.c.n_seq; lo < hi;) {  // the sequence of the first pair
-          const uint32_t mid = (lo + hi) / 2;
-          if (upto[mid + 1] <= at) lo = mid + 1; else hi = mid;
-        }
-        s = lo;
-      }
-    }
+    const uint32_t lane = threadIdx.x & 31, chunk = blockIdx.x;
     g.tile1 = 0;
     if (at < end) {
       while (upto[s + 1] <= at) s++;
@@ -246,31 +244,18 @@ struct Lead {
     return g.tile1 != 0;
   }
 };
-// One thread of every CTA, when its roles are done: the last leaves the counters at zero.
-__device__ __forceinline__ void leave(const TreeParams &p) {
-  __threadfence();
-  if (atomicAdd(p.cnt + 1, 1u) == gridDim.x - 1) {
-    p.cnt[0] = 0;
-    p.cnt[1] = 0;
-  }
-}
-
 // Copies, one warp for all K tiles or all V tiles: a lane a chunk of p.chunk positions, which lie in one page. The warp
 // of K (LEADS) also hands out the segments, and notes in `valid` which positions of a tile hold a row. SLOTS tiles are
 // in flight.
 template <int HD, uint32_t MR, uint32_t SLOTS, bool LEADS>
 __device__ __forceinline__ void copy_tiles(const TreeParams &p, const CUtensorMap *map, const uint32_t *upto, Ring &ring,
-                                           uint32_t waves, uint8_t *slot0, uint64_t *full, uint64_t *empty,
+                                           uint8_t *slot0, uint64_t *full, uint64_t *empty,
                                            uint32_t (*valid)[4]) {
   constexpr uint32_t BL = kTcTile * 128, BYTES = HD / 64 * BL;
   const uint32_t lane = threadIdx.x & 31, chunks = kTcTile / p.chunk, chunk = p.chunk, P = p.c.page_tokens;
   Waiter wait{p.wait_ns, p.err};
   Lead lead;
-  if (LEADS) {
-    lead.all = upto[p.c.n_seq];
-    lead.size = chunk_size(lead.all, waves);
-    lead.chunks = (lead.all + lead.size - 1) / lead.size;
-  }
+  if (LEADS) lead.begin(p, upto);
   Segment g;
   uint32_t i = 0;  // tiles so far
   for (uint32_t n = 0; LEADS ? lead.next<MR>(p, upto, ring, g) : next_segment(ring, n, wait, g); n++) {
@@ -423,18 +408,18 @@ __device__ __forceinline__ void note_unit(const TreeParams &p, const Segment &g)
 // Join the parts of the units that several chunks shared: CTA (unit, 8 rows), a thread 4 dims of a row. Parts lie
 // [row][hd] (BY_ROW) or [hd / 4][row] float4, as the kernels have them.
 constexpr uint32_t kJoinRows = 8;
-template <int HD, uint32_t MR, uint32_t PARTS, bool BY_ROW>
+template <int HD, uint32_t MR, bool BY_ROW>
 __global__ void __launch_bounds__(kJoinRows * HD / 4) k_attn_tree_join(TreeParams p) {
   pdl_trigger();
   pdl_wait();
-  __shared__ float ws[kJoinRows][PARTS];
+  __shared__ float ws[kJoinRows][kTcGrid];
   __shared__ float inv[kJoinRows];
   const uint32_t unit = blockIdx.x, block = unit % p.max_blocks, kvh = unit / p.max_blocks % p.c.hk;
   const uint32_t s = unit / p.max_blocks / p.c.hk, row0 = blockIdx.y * kJoinRows, t = threadIdx.x;
   const SeqWork w = seq_work<MR, kTcTile>(p, s);
   if (block >= w.blocks) return;
   const uint32_t rows = min(MR, w.nodes * p.g - block * MR);
-  const uint32_t parts = min(p.units[2 * unit], PARTS), first = p.units[2 * unit + 1];
+  const uint32_t parts = min(p.units[2 * unit], kTcGrid), first = p.units[2 * unit + 1];
   if (parts == 0 || row0 >= rows) return;
   auto slot = [&](uint32_t q) -> size_t { return q == 0 ? first : (first & ~1u) + 2 * q; };
   const uint32_t n = min(kJoinRows, rows - row0), warps = kJoinRows * HD / 128, lane = t & 31;

@@ -455,7 +455,7 @@ bool plane_map(const TreeParams &p, const __half *plane, CUtensorMap *map) {
 }
 
 // The tcgen05 kernels: `kern` with `smem` bytes and row tiles of MR, then the joining kernel.
-template <int HD, uint32_t MR, uint32_t WAVES, bool BY_ROW>
+template <int HD, uint32_t MR, bool BY_ROW>
 pai_status_t launch_tc(pai_b200_ctx_t *ctx, TreeParams &p, void (*kern)(TreeParams, CUtensorMap, CUtensorMap),
                        uint32_t threads, size_t smem, const CUtensorMap &kmap, const CUtensorMap &vmap) {
   static SmemOptIn opt;
@@ -474,8 +474,8 @@ pai_status_t launch_tc(pai_b200_ctx_t *ctx, TreeParams &p, void (*kern)(TreePara
     return b200_fail(PAI_ERR_UNSUPPORTED, "attn_tree: %llu tiles of rows and keys", (unsigned long long)pairs);
   const uint32_t grid = (uint32_t)std::min<uint64_t>(kTcGrid, pairs);
   float *scratch;
-  const uint64_t slots = 2ull * grid * WAVES;
-  st = b200_ctx_scratch(ctx, slots * MR * (HD + 2) + 2 * units, 2, &scratch, &p.cnt);
+  const uint64_t slots = 2ull * grid;
+  st = b200_ctx_scratch(ctx, slots * MR * (HD + 2) + 2 * units, 1, &scratch, &p.cnt);
   if (st) return st;
   p.part_o = scratch;
   p.part_ml = scratch + slots * MR * HD;
@@ -484,7 +484,7 @@ pai_status_t launch_tc(pai_b200_ctx_t *ctx, TreeParams &p, void (*kern)(TreePara
   // the joining kernel is resident before this one ends, and waits for it
   const int pdl = b200_ctx_pdl(ctx);
   b200_ctx_set_pdl(ctx, 1);
-  b200_launch(ctx, k_attn_tree_join<HD, MR, kTcGrid * WAVES, BY_ROW>, dim3((uint32_t)units, MR / kJoinRows), dim3(kJoinRows * HD / 4), 0, p);
+  b200_launch(ctx, k_attn_tree_join<HD, MR, BY_ROW>, dim3((uint32_t)units, MR / kJoinRows), dim3(kJoinRows * HD / 4), 0, p);
   b200_ctx_set_pdl(ctx, pdl);
   return b200_launched(ctx, 2, "k_attn_tree");
 }
@@ -527,9 +527,9 @@ pai_status_t launch_tree_hd(pai_b200_ctx_t *ctx, TreeParams &p) {
     while (p.chunk > 8 && p.c.page_tokens % p.chunk) p.chunk /= 2;
   CUtensorMap kmap, vmap;
   if ((!p.c.table || p.c.page_tokens % p.chunk == 0) && plane_map(p, p.c.k, &kmap) && plane_map(p, p.c.v, &vmap))
-    return rows <= kFewRows ? launch_tc<HD, kFewRows, kFewWaves, true>(ctx, p, k_attn_tree_few<HD>, kFewThreads,
+    return rows <= kFewRows ? launch_tc<HD, kFewRows, true>(ctx, p, k_attn_tree_few<HD>, kFewThreads,
                                                             sizeof(FewSmem<HD>) + 1024, kmap, vmap)
-                            : launch_tc<HD, kManyRows, kManyWaves, false>(ctx, p, k_attn_tree_many<HD>, kManyThreads,
+                            : launch_tc<HD, kManyRows, false>(ctx, p, k_attn_tree_many<HD>, kManyThreads,
                                                               sizeof(ManySmem<HD>) + 1024, kmap, vmap);
   if (rows <= 16) return launch_tree<HD, 1>(ctx, p);
   return launch_tree<HD, 4>(ctx, p);
