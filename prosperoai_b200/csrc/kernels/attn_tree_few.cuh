@@ -12,7 +12,9 @@
 //   warps 4-7   add the tiles' O^T to the running output, a thread a dim, the rows in registers
 //   warp 8      issues the MMAs (8 + 8 of 48 cycles of shared memory a tile); 9, 10 copy K and V; 11 cleans V
 // With row tiles as A (attn_tree_many.cuh) 8 sequences of one row x 4 heads at 16384 positions took 134 us: 128 rows'
-// MMAs, and one warp of four with a row to work on.
+// MMAs, and one warp of four with a row to work on. RG, the groups of 8 rows that a softmax and a folding thread have, is
+// a compile-time value: with 1 for 8 rows that took 101 us, with 4 and three of them idle 125 (these warps wait for
+// instructions more than for anything else).
 #pragma once
 #include "attn_tree_tc.cuh"
 
@@ -45,21 +47,6 @@ struct FewSmem {
   uint32_t tmem;
 };
 
-// Lane r gets the reduction over the lanes of v[r]: 31 exchanges for 32 values.
-template <typename F>
-__device__ __forceinline__ float reduce_rows(float (&v)[32], F f) {
-  const uint32_t lane = threadIdx.x & 31;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-    for (int j = 0; j < o; j++) {
-      const bool up = lane & o;
-      const float mine = up ? v[j + o] : v[j], other = up ? v[j] : v[j + o];
-      v[j] = f(mine, __shfl_xor_sync(0xffffffffu, other, o));
-    }
-  return v[0];
-}
-
 // The largest of the lanes' values, NaN apart.
 __device__ __forceinline__ float warp_top(float v) {
   float top;
@@ -67,7 +54,7 @@ __device__ __forceinline__ float warp_top(float v) {
   return top;
 }
 
-template <int HD>
+template <int HD, uint32_t RG>
 __global__ void __launch_bounds__(kFewThreads, 1)
     k_attn_tree_few(TreeParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using Smem = FewSmem<HD>;
@@ -169,21 +156,24 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     const uint32_t d = t - 128, lanes = (warp & 3) * 32 << 16;
     const bool live = d < HD;
     for (; next_segment(sm.ring, seg, wait, g); seg++) {
-      const uint32_t rows = min(kFewRows, g.nodes * p.g - g.block * kFewRows), groups = (rows + 7) / 8;
-      float o[32];
+      const uint32_t rows = min(kFewRows, g.nodes * p.g - g.block * kFewRows);
+      float o[8 * RG];
 #pragma unroll
-      for (int r = 0; r < 32; r++) o[r] = 0.0f;
+      for (uint32_t r = 0; r < 8 * RG; r++) o[r] = 0.0f;
       for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
         wait(&sm.ofull[i & 1], i >> 1);
         __syncwarp();
         tc_after();
         const bool grew = sm.grew[i & 7];
+        uint32_t w[16 * RG];
 #pragma unroll
-        for (uint32_t gr = 0; gr < 4; gr++) {
-          if (gr >= groups) continue;
-          uint32_t v[16];
-          tc_ld8(tmem + lanes + 128 + 64 * (i & 1) + 8 * gr, v);
-          tc_ld8(tmem + lanes + 160 + 64 * (i & 1) + 8 * gr, v + 8);
+        for (uint32_t gr = 0; gr < RG; gr++) {
+          tc_ld8(tmem + lanes + 128 + 64 * (i & 1) + 8 * gr, w + 16 * gr);
+          tc_ld8(tmem + lanes + 160 + 64 * (i & 1) + 8 * gr, w + 16 * gr + 8);
+        }
+#pragma unroll
+        for (uint32_t gr = 0; gr < RG; gr++) {
+          uint32_t *v = w + 16 * gr;
           if (grew) {
 #pragma unroll
             for (uint32_t e = 0; e < 8; e++) o[8 * gr + e] *= sm.corr[i & 7][8 * gr + e];
@@ -206,8 +196,8 @@ __global__ void __launch_bounds__(kFewThreads, 1)
               const float f = __half2float(p.c.v[(size_t)g.kvh * p.c.head_stride + kv_row(p.c, g.s, pos) + d]);
               if (isfinite(f)) continue;
 #pragma unroll
-              for (int r = 0; r < 32; r++)
-                if ((uint32_t)r < rows && (seen(p, pos - g.len, true, (g.block * kFewRows + r) / p.g, g.first) & 1))
+              for (uint32_t r = 0; r < 8 * RG; r++)
+                if (r < rows && (seen(p, pos - g.len, true, (g.block * kFewRows + r) / p.g, g.first) & 1))
                   o[r] += f;
             }
         }
@@ -218,8 +208,8 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       const bool whole = g.whole();
       const size_t slot = g.slot;
 #pragma unroll
-      for (int r = 0; r < 32; r++) {
-        if ((uint32_t)r >= rows) continue;
+      for (uint32_t r = 0; r < 8 * RG; r++) {
+        if (r >= rows) continue;
         const float *ls = &sm.lsum[seg & 3][0][r];
         const float L = (ls[0] + ls[kFewRows]) + (ls[2 * kFewRows] + ls[3 * kFewRows]);
         const uint32_t rr = g.block * kFewRows + r;
@@ -240,7 +230,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     // ---- softmax: a thread a position ----
     constexpr float kNone = -1e30f, kFull = 15.5f;  // no maximum yet; the largest exponent that weights may have
     for (; next_segment<1, 128>(sm.ring, seg, wait, g); seg++) {
-      const uint32_t rows = min(kFewRows, g.nodes * p.g - g.block * kFewRows), groups = (rows + 7) / 8;
+      const uint32_t rows = min(kFewRows, g.nodes * p.g - g.block * kFewRows);
       // every score of the last segment has been read, so its products are done: Q may be written
       put_queries<HD, kFewRows, 4>(p, g, rows, warp, sm.q, Smem::kQBlock, kFewRows * 128, sm.factor);
       if (t < kFewRows) sm.sub[t] = kNone;
@@ -248,9 +238,9 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       if (lane == 0) mbar_arrive(&sm.qfull);
       named_sync<1, 128>();
       float m = -INFINITY;  // of row `lane`
-      float l[32];
+      float l[8 * RG];
 #pragma unroll
-      for (int r = 0; r < 32; r++) l[r] = 0.0f;
+      for (uint32_t r = 0; r < 8 * RG; r++) l[r] = 0.0f;
       for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
         const uint32_t sa = tmem + ((warp & 3) * 32 << 16) + 64 * (i & 1);
         wait(&sm.sfull[i & 1], i >> 1);
@@ -259,16 +249,17 @@ __global__ void __launch_bounds__(kFewThreads, 1)
         const bool there = (sm.valid[i & 7][warp] >> lane) & 1;
         const uint32_t pos = tile * kTcTile + t;
         const bool is_node = (tile + 1) * kTcTile > g.len && pos >= g.len;
-        // scores in powers of two, unseen ones -inf, and the largest exponent relative to the rows' maxima so far. All of
-        // it in groups of 8 rows, of which the rows' number of groups is run: code that is not run is not fetched, and
-        // instruction fetches are what these warps wait for most.
-        float s[32], top = -INFINITY;
+        // scores in powers of two, unseen ones -inf, and the largest exponent relative to the rows' maxima so far
+        float s[8 * RG], top = -INFINITY;
+        uint32_t w[16 * RG];
 #pragma unroll
-        for (uint32_t gr = 0; gr < 4; gr++) {
-          if (gr >= groups) continue;
-          uint32_t v[16];
-          tc_ld8(sa + 8 * gr, v);
-          tc_ld8(sa + 32 + 8 * gr, v + 8);
+        for (uint32_t gr = 0; gr < RG; gr++) {
+          tc_ld8(sa + 8 * gr, w + 16 * gr);
+          tc_ld8(sa + 32 + 8 * gr, w + 16 * gr + 8);
+        }
+#pragma unroll
+        for (uint32_t gr = 0; gr < RG; gr++) {
+          uint32_t *v = w + 16 * gr;
           tc_ld_wait8(v);
           tc_ld_wait8(v + 8);
 #pragma unroll
@@ -298,8 +289,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
         if (any) {
           float mine = -INFINITY;
 #pragma unroll
-          for (uint32_t gr = 0; gr < 4; gr++) {
-            if (gr >= groups) continue;
+          for (uint32_t gr = 0; gr < RG; gr++) {
 #pragma unroll
             for (uint32_t r = 8 * gr; r < 8 * gr + 8; r++) {
               const float x = warp_top(s[r]);
@@ -316,8 +306,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
             sm.corr[i & 7][lane] = corr;
           }
 #pragma unroll
-          for (uint32_t gr = 0; gr < 4; gr++) {
-            if (gr >= groups) continue;
+          for (uint32_t gr = 0; gr < RG; gr++) {
 #pragma unroll
             for (uint32_t r = 8 * gr; r < 8 * gr + 8; r++) l[r] *= __shfl_sync(0xffffffffu, corr, r);
           }
@@ -327,8 +316,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
         // weights, in groups of 8 rows, to the position's 128 bytes (16 of parts and 16 of remainders a group)
         uint8_t *dst = sm.pt[i & 1] + t * 128;
 #pragma unroll
-        for (uint32_t gr = 0; gr < 4; gr++) {
-          if (gr >= groups) continue;
+        for (uint32_t gr = 0; gr < RG; gr++) {
           uint4 hi, lo;
           uint32_t *hw = reinterpret_cast<uint32_t *>(&hi), *lw = reinterpret_cast<uint32_t *>(&lo);
 #pragma unroll
@@ -349,7 +337,13 @@ __global__ void __launch_bounds__(kFewThreads, 1)
         if (lane == 0) mbar_arrive(&sm.pfull[i & 1]);
       }
       // lane r: the warp's sum of row r
-      sm.lsum[seg & 3][warp][lane] = reduce_rows(l, [](float a, float b) { return a + b; });
+      float sum = 0.0f;
+#pragma unroll
+      for (uint32_t r = 0; r < 8 * RG; r++) {
+        const float x = warp_sum(l[r]);
+        if (lane == r) sum = x;
+      }
+      sm.lsum[seg & 3][warp][lane] = sum;
       if (warp == 0) sm.msum[seg & 3][lane] = m;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.lfull[seg & 3]);

@@ -454,8 +454,9 @@ bool plane_map(const TreeParams &p, const __half *plane, CUtensorMap *map) {
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// The tcgen05 kernels: `kern` with `smem` bytes and row tiles of MR, then the joining kernel.
-template <int HD, uint32_t MR, bool BY_ROW>
+// The tcgen05 kernels: `kern` with `smem` bytes and row tiles of MR, then the joining kernel. RG: the groups of 8 rows
+// of the kernel for few rows, 0 for that of many (it also keeps the kernels' shared-memory attributes apart).
+template <int HD, uint32_t MR, uint32_t RG>
 pai_status_t launch_tc(pai_b200_ctx_t *ctx, TreeParams &p, void (*kern)(TreeParams, CUtensorMap, CUtensorMap),
                        uint32_t threads, size_t smem, const CUtensorMap &kmap, const CUtensorMap &vmap) {
   static SmemOptIn opt;
@@ -484,7 +485,7 @@ pai_status_t launch_tc(pai_b200_ctx_t *ctx, TreeParams &p, void (*kern)(TreePara
   // the joining kernel is resident before this one ends, and waits for it
   const int pdl = b200_ctx_pdl(ctx);
   b200_ctx_set_pdl(ctx, 1);
-  b200_launch(ctx, k_attn_tree_join<HD, MR, BY_ROW>, dim3((uint32_t)units, MR / kJoinRows), dim3(kJoinRows * HD / 4), 0, p);
+  b200_launch(ctx, k_attn_tree_join<HD, MR, RG != 0>, dim3((uint32_t)units, MR / kJoinRows), dim3(kJoinRows * HD / 4), 0, p);
   b200_ctx_set_pdl(ctx, pdl);
   return b200_launched(ctx, 2, "k_attn_tree");
 }
@@ -527,10 +528,14 @@ pai_status_t launch_tree_hd(pai_b200_ctx_t *ctx, TreeParams &p) {
     while (p.chunk > 8 && p.c.page_tokens % p.chunk) p.chunk /= 2;
   CUtensorMap kmap, vmap;
   if ((!p.c.table || p.c.page_tokens % p.chunk == 0) && plane_map(p, p.c.k, &kmap) && plane_map(p, p.c.v, &vmap))
-    return rows <= kFewRows ? launch_tc<HD, kFewRows, true>(ctx, p, k_attn_tree_few<HD>, kFewThreads,
-                                                            sizeof(FewSmem<HD>) + 1024, kmap, vmap)
-                            : launch_tc<HD, kManyRows, false>(ctx, p, k_attn_tree_many<HD>, kManyThreads,
-                                                              sizeof(ManySmem<HD>) + 1024, kmap, vmap);
+  {
+    if (rows > kFewRows)
+      return launch_tc<HD, kManyRows, 0>(ctx, p, k_attn_tree_many<HD>, kManyThreads, sizeof(ManySmem<HD>) + 1024, kmap, vmap);
+    constexpr size_t smem = sizeof(FewSmem<HD>) + 1024;
+    if (rows <= 8) return launch_tc<HD, kFewRows, 1>(ctx, p, k_attn_tree_few<HD, 1>, kFewThreads, smem, kmap, vmap);
+    if (rows <= 16) return launch_tc<HD, kFewRows, 2>(ctx, p, k_attn_tree_few<HD, 2>, kFewThreads, smem, kmap, vmap);
+    return launch_tc<HD, kFewRows, 4>(ctx, p, k_attn_tree_few<HD, 4>, kFewThreads, smem, kmap, vmap);
+  }
   if (rows <= 16) return launch_tree<HD, 1>(ctx, p);
   return launch_tree<HD, 4>(ctx, p);
 }
