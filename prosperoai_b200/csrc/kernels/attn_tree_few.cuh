@@ -8,9 +8,9 @@
 // weights carry 2^12). Only when some row's does, in a sequence's first tiles, are the rows' maxima taken over the
 // tile. The sums of weights stay in the threads, one a row and
 // position, until a unit ends.
-//   warps 0-3   softmax; the weights go to shared memory, 128 bytes a position, as an MN-major B
-//   warps 4-7   add the tiles' O^T to the running output, a thread a dim, the rows in registers
-//   warp 8      issues the MMAs (8 + 8 of 48 cycles of shared memory a tile); 9, 10 copy K and V; 11 cleans V
+//   first 4 or 8 warps  softmax; the weights go to shared memory, 128 bytes a position, as an MN-major B
+//   next 4              add the tiles' O^T to the running output, a thread a dim, the rows in registers
+//   last 4              issue the MMAs (8 + 8 of 48 cycles of shared memory a tile), copy K and V, clean V
 // With row tiles as A (attn_tree_many.cuh) 8 sequences of one row x 4 heads at 16384 positions took 134 us: 128 rows'
 // MMAs, and one warp of four with a row to work on. RG, the groups of 8 rows that a softmax and a folding thread have, is
 // a compile-time value: with 1 for 8 rows that took 101 us, with 4 and three of them idle 125 (these warps wait for
@@ -20,7 +20,7 @@
 
 namespace {
 
-constexpr uint32_t kFewThreads = 384, kFewRows = 32, kFewK = 3, kFewV = 2;
+constexpr uint32_t kFewRows = 32, kFewK = 3, kFewV = 2;
 
 template <int HD>
 struct FewSmem {
@@ -35,10 +35,10 @@ struct FewSmem {
   // last to be folded, so no warp is more than a few tiles ahead of another.
   uint32_t valid[8][4];  // positions of a tile that hold a row
   uint32_t odd[8][4];    // its nodes with a non-finite V row
-  uint32_t grew[8];      // whether the tile's weights are relative to new maxima
+  uint32_t grew[8][2];   // [tile][softmax warpgroup]: whether the weights are relative to new maxima
   float corr[8][kFewRows];  // then: 2^(old - new)
   float factor[kFewRows], sub[kFewRows];
-  float wmax[4][kFewRows];
+  float wmax[2][4][kFewRows];
   float lsum[4][4][kFewRows], msum[4][kFewRows];  // [segment][warp]: sums of weights; maxima
   uint32_t upto[kMaxSeqs + 1];
   Ring ring;
@@ -47,6 +47,9 @@ struct FewSmem {
   uint32_t tmem;
 };
 
+// Threads of a block: SW warpgroups of softmax, one that folds, four warps for the other roles.
+__host__ __device__ constexpr uint32_t few_threads(uint32_t sw) { return 128 * (sw + 2); }
+
 // The largest of the lanes' values, NaN apart.
 __device__ __forceinline__ float warp_top(float v) {
   float top;
@@ -54,13 +57,13 @@ __device__ __forceinline__ float warp_top(float v) {
   return top;
 }
 
-template <int HD, uint32_t RG>
-__global__ void __launch_bounds__(kFewThreads, 1)
+template <int HD, uint32_t RG, uint32_t SW>
+__global__ void __launch_bounds__(few_threads(SW), 1)
     k_attn_tree_few(TreeParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using Smem = FewSmem<HD>;
   extern __shared__ __align__(16) uint8_t raw[];
   Smem &sm = *reinterpret_cast<Smem *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-  constexpr uint32_t BL = Smem::kBlock;
+  constexpr uint32_t BL = Smem::kBlock, FOLD = 4 * SW, MMA = FOLD + 4;  // first warps of those roles
   const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
   pdl_trigger();
   if (t == 0) {
@@ -75,22 +78,22 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     }
     for (int i = 0; i < 2; i++) {
       mbar_init(&sm.sfull[i], 1);
-      mbar_init(&sm.pfull[i], 4);
+      mbar_init(&sm.pfull[i], 4 * SW);
       mbar_init(&sm.ofull[i], 1);
       mbar_init(&sm.ofree[i], 4);
     }
-    for (int i = 0; i < 4; i++) mbar_init(&sm.lfull[i], 4);
-    mbar_init(&sm.qfull, 4);
+    for (int i = 0; i < 4; i++) mbar_init(&sm.lfull[i], 4 * SW);
+    mbar_init(&sm.qfull, 4 * SW);
     mbar_init(&sm.drain, 1);
     for (uint32_t i = 0; i < kRing; i++) mbar_init(&sm.ring.full[i], 1);
     fence_mbar_init();
   }
-  if (warp == 8) {
+  if (warp == MMA) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(256));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   pdl_wait();
-  pairs_before32<kFewRows, kFewThreads>(p, sm.upto);
+  pairs_before32<kFewRows, few_threads(SW)>(p, sm.upto);
   tc_before();
   __syncthreads();
   tc_after();
@@ -99,13 +102,13 @@ __global__ void __launch_bounds__(kFewThreads, 1)
   Waiter wait{p.wait_ns, p.err};
   uint32_t i = 0, seg = 0;  // tiles and segments of the run so far
 
-  if (warp == 9) {
+  if (warp == MMA + 1) {
     copy_tiles<HD, kFewRows, kFewK, true>(p, &kmap, sm.upto, sm.ring, sm.kt[0], sm.kfull, sm.kempty, sm.valid);
-  } else if (warp == 10) {
+  } else if (warp == MMA + 2) {
     copy_tiles<HD, kFewRows, kFewV, false>(p, &vmap, sm.upto, sm.ring, sm.vt[0], sm.vfull, sm.vempty, nullptr);
-  } else if (warp == 11) {
+  } else if (warp == MMA + 3) {
     clean_tiles<HD, kFewV>(p, sm.ring, sm.vt[0], sm.vfull, sm.vclean, sm.odd);
-  } else if (warp == 8) {
+  } else if (warp == MMA) {
     // ---- MMA issue ----
     const uint32_t leader = elect_one();
     const uint64_t qd = desc_k(smem_u32(sm.q)), kd = desc_k(smem_u32(sm.kt[0]));
@@ -151,30 +154,30 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     wait.ok = true;
     wait(&sm.drain, 0);
     __syncwarp();
-  } else if (warp >= 4) {
+  } else if (warp >= FOLD) {
     // ---- fold: a thread a dim (with hd 64 the upper half of the lanes has none) ----
-    const uint32_t d = t - 128, lanes = (warp & 3) * 32 << 16;
+    const uint32_t d = t - 32 * FOLD, lanes = (warp & 3) * 32 << 16;
     const bool live = d < HD;
+    constexpr uint32_t FR = 8 * RG * SW;  // rows
     for (; next_segment(sm.ring, seg, wait, g); seg++) {
       const uint32_t rows = min(kFewRows, g.nodes * p.g - g.block * kFewRows);
-      float o[8 * RG];
+      float o[FR];
 #pragma unroll
-      for (uint32_t r = 0; r < 8 * RG; r++) o[r] = 0.0f;
+      for (uint32_t r = 0; r < FR; r++) o[r] = 0.0f;
       for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
         wait(&sm.ofull[i & 1], i >> 1);
         __syncwarp();
         tc_after();
-        const bool grew = sm.grew[i & 7];
-        uint32_t w[16 * RG];
+        uint32_t w[2 * FR];
 #pragma unroll
-        for (uint32_t gr = 0; gr < RG; gr++) {
+        for (uint32_t gr = 0; gr < FR / 8; gr++) {
           tc_ld8(tmem + lanes + 128 + 64 * (i & 1) + 8 * gr, w + 16 * gr);
           tc_ld8(tmem + lanes + 160 + 64 * (i & 1) + 8 * gr, w + 16 * gr + 8);
         }
 #pragma unroll
-        for (uint32_t gr = 0; gr < RG; gr++) {
+        for (uint32_t gr = 0; gr < FR / 8; gr++) {
           uint32_t *v = w + 16 * gr;
-          if (grew) {
+          if (sm.grew[i & 7][gr / RG]) {
 #pragma unroll
             for (uint32_t e = 0; e < 8; e++) o[8 * gr + e] *= sm.corr[i & 7][8 * gr + e];
           }
@@ -196,8 +199,8 @@ __global__ void __launch_bounds__(kFewThreads, 1)
               const float f = __half2float(p.c.v[(size_t)g.kvh * p.c.head_stride + kv_row(p.c, g.s, pos) + d]);
               if (isfinite(f)) continue;
 #pragma unroll
-              for (uint32_t r = 0; r < 8 * RG; r++)
-                if (r < rows && (seen(p, pos - g.len, true, (g.block * kFewRows + r) / p.g, g.first) & 1))
+              for (uint32_t r = 0; r < FR; r++)
+                if (r < rows && sees_node(p, g.first, (g.block * kFewRows + r) / p.g, pos - g.len))
                   o[r] += f;
             }
         }
@@ -208,7 +211,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       const bool whole = g.whole();
       const size_t slot = g.slot;
 #pragma unroll
-      for (uint32_t r = 0; r < 8 * RG; r++) {
+      for (uint32_t r = 0; r < FR; r++) {
         if (r >= rows) continue;
         const float *ls = &sm.lsum[seg & 3][0][r];
         const float L = (ls[0] + ls[kFewRows]) + (ls[2 * kFewRows] + ls[3 * kFewRows]);
@@ -227,27 +230,28 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       if (g.tile0 == 0 && d == 0) note_unit(p, g);
     }
   } else {
-    // ---- softmax: a thread a position ----
+    // ---- softmax: a thread a position and 8 RG rows, from row0 ----
+    const uint32_t wg = warp / 4, w4 = warp & 3, row0 = 8 * RG * wg;
     constexpr float kNone = -1e30f, kFull = 15.5f;  // no maximum yet; the largest exponent that weights may have
-    for (; next_segment<1, 128>(sm.ring, seg, wait, g); seg++) {
+    for (; next_segment<1, 128 * SW>(sm.ring, seg, wait, g); seg++) {
       const uint32_t rows = min(kFewRows, g.nodes * p.g - g.block * kFewRows);
       // every score of the last segment has been read, so its products are done: Q may be written
-      put_queries<HD, kFewRows, 4>(p, g, rows, warp, sm.q, Smem::kQBlock, kFewRows * 128, sm.factor);
+      put_queries<HD, kFewRows, 4 * SW>(p, g, rows, warp, sm.q, Smem::kQBlock, kFewRows * 128, sm.factor);
       if (t < kFewRows) sm.sub[t] = kNone;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.qfull);
-      named_sync<1, 128>();
-      float m = -INFINITY;  // of row `lane`
+      named_sync<1, 128 * SW>();
+      float m = -INFINITY;  // of row row0 + lane
       float l[8 * RG];
 #pragma unroll
       for (uint32_t r = 0; r < 8 * RG; r++) l[r] = 0.0f;
       for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
-        const uint32_t sa = tmem + ((warp & 3) * 32 << 16) + 64 * (i & 1);
+        const uint32_t sa = tmem + (w4 * 32 << 16) + 64 * (i & 1) + row0;
         wait(&sm.sfull[i & 1], i >> 1);
         __syncwarp();
         tc_after();
-        const bool there = (sm.valid[i & 7][warp] >> lane) & 1;
-        const uint32_t pos = tile * kTcTile + t;
+        const bool there = (sm.valid[i & 7][w4] >> lane) & 1;
+        const uint32_t pos = tile * kTcTile + (t & 127);
         const bool is_node = (tile + 1) * kTcTile > g.len && pos >= g.len;
         // scores in powers of two, unseen ones -inf, and the largest exponent relative to the rows' maxima so far
         float s[8 * RG], top = -INFINITY;
@@ -265,8 +269,8 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 #pragma unroll
           for (uint32_t e = 0; e < 8; e += 4) {
             const uint32_t r = 8 * gr + e;
-            const float4 f = *reinterpret_cast<const float4 *>(&sm.factor[r]);
-            const float4 u = *reinterpret_cast<const float4 *>(&sm.sub[r]);
+            const float4 f = *reinterpret_cast<const float4 *>(&sm.factor[row0 + r]);
+            const float4 u = *reinterpret_cast<const float4 *>(&sm.sub[row0 + r]);
             s[r] = there ? (__uint_as_float(v[e]) + __uint_as_float(v[8 + e])) * f.x : -INFINITY;
             s[r + 1] = there ? (__uint_as_float(v[e + 1]) + __uint_as_float(v[9 + e])) * f.y : -INFINITY;
             s[r + 2] = there ? (__uint_as_float(v[e + 2]) + __uint_as_float(v[10 + e])) * f.z : -INFINITY;
@@ -274,17 +278,17 @@ __global__ void __launch_bounds__(kFewThreads, 1)
             if (is_node) {  // for the rows that see it
 #pragma unroll
               for (uint32_t x = r; x < r + 4; x++)
-                if (x < rows && !(seen(p, pos - g.len, true, (g.block * kFewRows + x) / p.g, g.first) & 1)) s[x] = -INFINITY;
+                if (row0 + x < rows && !sees_node(p, g.first, (g.block * kFewRows + row0 + x) / p.g, pos - g.len)) s[x] = -INFINITY;
             }
             top = fmaxf(fmaxf(top, fmaxf(s[r] - u.x, s[r + 1] - u.y)), fmaxf(s[r + 2] - u.z, s[r + 3] - u.w));
           }
         }
         __syncwarp();
-        uint32_t any;
+        uint32_t any;  // of this warpgroup's rows
         asm volatile(
-            "{\n .reg .pred p, q;\n setp.ne.u32 q, %1, 0;\n bar.red.or.pred p, 1, 128, q;\n selp.u32 %0, 1, 0, p;\n}\n"
+            "{\n .reg .pred p, q;\n setp.ne.u32 q, %1, 0;\n bar.red.or.pred p, %2, 128, q;\n selp.u32 %0, 1, 0, p;\n}\n"
             : "=r"(any)
-            : "r"((uint32_t)(top > kFull))
+            : "r"((uint32_t)(top > kFull)), "r"(2 + wg)
             : "memory");
         if (any) {
           float mine = -INFINITY;
@@ -296,25 +300,26 @@ __global__ void __launch_bounds__(kFewThreads, 1)
               if (lane == r) mine = x;
             }
           }
-          sm.wmax[warp][lane] = mine;
-          named_sync<1, 128>();
-          const float mn = fmaxf(fmaxf(fmaxf(m, sm.wmax[0][lane]), fmaxf(sm.wmax[1][lane], sm.wmax[2][lane])), sm.wmax[3][lane]);
+          sm.wmax[wg][w4][lane] = mine;
+          group_sync(2 + wg);
+          const float(*wm)[kFewRows] = sm.wmax[wg];
+          const float mn = fmaxf(fmaxf(fmaxf(m, wm[0][lane]), fmaxf(wm[1][lane], wm[2][lane])), wm[3][lane]);
           const float corr = m == mn ? 1.0f : ex2(m - mn);
           m = mn;
-          if (warp == 0) {
-            sm.sub[lane] = mn == -INFINITY ? kNone : mn - kPShift;
-            sm.corr[i & 7][lane] = corr;
+          if (w4 == 0 && lane < 8 * RG) {
+            sm.sub[row0 + lane] = mn == -INFINITY ? kNone : mn - kPShift;
+            sm.corr[i & 7][row0 + lane] = corr;
           }
 #pragma unroll
           for (uint32_t gr = 0; gr < RG; gr++) {
 #pragma unroll
             for (uint32_t r = 8 * gr; r < 8 * gr + 8; r++) l[r] *= __shfl_sync(0xffffffffu, corr, r);
           }
-          named_sync<1, 128>();
+          group_sync(2 + wg);
         }
-        if (t == 0) sm.grew[i & 7] = any;
+        if (w4 == 0 && lane == 0) sm.grew[i & 7][wg] = any;
         // weights, in groups of 8 rows, to the position's 128 bytes (16 of parts and 16 of remainders a group)
-        uint8_t *dst = sm.pt[i & 1] + t * 128;
+        uint8_t *dst = sm.pt[i & 1] + (t & 127) * 128;
 #pragma unroll
         for (uint32_t gr = 0; gr < RG; gr++) {
           uint4 hi, lo;
@@ -322,37 +327,40 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 #pragma unroll
           for (uint32_t e = 0; e < 8; e += 2) {
             const uint32_t r = 8 * gr + e;
-            const float2 u = *reinterpret_cast<const float2 *>(&sm.sub[r]);
+            const float2 u = *reinterpret_cast<const float2 *>(&sm.sub[row0 + r]);
             const float p0 = ex2(s[r] - u.x), p1 = ex2(s[r + 1] - u.y);
             l[r] += p0;
             l[r + 1] += p1;
             split_f16(p0, p1, hw[e / 2], lw[e / 2]);
           }
-          *reinterpret_cast<uint4 *>(dst + ((gr ^ (t & 7)) << 4)) = hi;
-          *reinterpret_cast<uint4 *>(dst + (((4 + gr) ^ (t & 7)) << 4)) = lo;
+          const uint32_t c = row0 / 8 + gr;
+          *reinterpret_cast<uint4 *>(dst + ((c ^ (t & 7)) << 4)) = hi;
+          *reinterpret_cast<uint4 *>(dst + (((4 + c) ^ (t & 7)) << 4)) = lo;
         }
         fence_proxy_async();
         tc_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.pfull[i & 1]);
       }
-      // lane r: the warp's sum of row r
+      // lane r: the warp's sum of row row0 + r
       float sum = 0.0f;
 #pragma unroll
       for (uint32_t r = 0; r < 8 * RG; r++) {
         const float x = warp_sum(l[r]);
         if (lane == r) sum = x;
       }
-      sm.lsum[seg & 3][warp][lane] = sum;
-      if (warp == 0) sm.msum[seg & 3][lane] = m;
+      if (lane < 8 * RG) {
+        sm.lsum[seg & 3][w4][row0 + lane] = sum;
+        if (w4 == 0) sm.msum[seg & 3][row0 + lane] = m;
+      }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.lfull[seg & 3]);
-      named_sync<1, 128>();  // the factors and maxima may be written again
+      named_sync<1, 128 * SW>();  // the factors and maxima may be written again
     }
   }
   tc_before();
   __syncthreads();
-  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256));
+  if (warp == MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256));
 }
 
 }  // namespace

@@ -107,6 +107,10 @@ __device__ __forceinline__ void tc_st32(uint32_t at, const uint32_t (&r)[32]) {
       "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(at)
       : "memory");
 }
+__device__ __forceinline__ void group_sync(uint32_t id) {  // of 128 threads
+  __syncwarp();
+  asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
+}
 template <int ID, int N>
 __device__ __forceinline__ void named_sync() {
   __syncwarp();
@@ -164,6 +168,12 @@ __device__ __forceinline__ uint64_t seen(const TreeParams &p, uint32_t base32, b
   if (!live) return past;
   if (!p.mask) return low_bits((int64_t)nd + 1 - base);
   return past | (window(p.mask + (size_t)(first + nd) * p.words, p.words, base) & ~past);
+}
+
+// Whether node `nd` of the sequence whose rows begin at `first` may see node n.
+__device__ __forceinline__ bool sees_node(const TreeParams &p, uint32_t first, uint32_t nd, uint32_t n) {
+  if (!p.mask) return n <= nd;
+  return n < 64 * p.words && (p.mask[(size_t)(first + nd) * p.words + n / 64] >> (n % 64)) & 1;
 }
 
 // A bounded wait that a role makes. After one has run out the role goes on without waiting or copying, so that the

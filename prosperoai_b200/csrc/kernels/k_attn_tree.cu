@@ -532,9 +532,9 @@ pai_status_t launch_tree_hd(pai_b200_ctx_t *ctx, TreeParams &p) {
     if (rows > kFewRows)
       return launch_tc<HD, kManyRows, 0>(ctx, p, k_attn_tree_many<HD>, kManyThreads, sizeof(ManySmem<HD>) + 1024, kmap, vmap);
     constexpr size_t smem = sizeof(FewSmem<HD>) + 1024;
-    if (rows <= 8) return launch_tc<HD, kFewRows, 1>(ctx, p, k_attn_tree_few<HD, 1>, kFewThreads, smem, kmap, vmap);
-    if (rows <= 16) return launch_tc<HD, kFewRows, 2>(ctx, p, k_attn_tree_few<HD, 2>, kFewThreads, smem, kmap, vmap);
-    return launch_tc<HD, kFewRows, 4>(ctx, p, k_attn_tree_few<HD, 4>, kFewThreads, smem, kmap, vmap);
+    if (rows <= 8) return launch_tc<HD, kFewRows, 1>(ctx, p, k_attn_tree_few<HD, 1, 1>, few_threads(1), smem, kmap, vmap);
+    if (rows <= 16) return launch_tc<HD, kFewRows, 2>(ctx, p, k_attn_tree_few<HD, 2, 1>, few_threads(1), smem, kmap, vmap);
+    return launch_tc<HD, kFewRows, 4>(ctx, p, k_attn_tree_few<HD, 2, 2>, few_threads(2), smem, kmap, vmap);
   }
   if (rows <= 16) return launch_tree<HD, 1>(ctx, p);
   return launch_tree<HD, 4>(ctx, p);
