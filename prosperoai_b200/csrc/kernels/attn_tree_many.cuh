@@ -218,7 +218,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             const uint32_t b0 = (uint32_t)bits, b1 = (uint32_t)(bits >> 32);
 #pragma unroll
             for (int e = 0; e < 64; e++)
-              if (!(((e < 32 ? b0 : b1) >> (e & 31)) & 1)) v[e] = 0xFF800000u;  // -inf
+              if (!(((e < 32 ? b0 : b1) >> (e & 31)) & 1)) v[e] = 0xFF800000u;  // -inf, for the second pass too
+            tc_st32(sa, v);
+            tc_st32(sa + 32, v + 32);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
           }
           float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -237,13 +240,16 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           m = mn;
           const float sub = mn == -INFINITY ? 0.0f : mn - kPShift;
           float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
+          __syncwarp();
+#pragma unroll 1
           for (int c = 0; c < 2; c++) {
-            uint32_t w[32];  // 16 words of parts, 16 of remainders
+            uint32_t x[32], w[32];  // 16 words of parts, 16 of remainders
+            tc_ld32(sa + 32 * c, x);
+            tc_ld_wait(x);
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
-              const float p0 = ex2(fmaf(__uint_as_float(v[32 * c + e]), factor, -sub));
-              const float p1 = ex2(fmaf(__uint_as_float(v[32 * c + e + 1]), factor, -sub));
+              const float p0 = ex2(fmaf(__uint_as_float(x[e]), factor, -sub));
+              const float p1 = ex2(fmaf(__uint_as_float(x[e + 1]), factor, -sub));
               part[(e / 2) & 3] += p0 + p1;
               split_f16(p0, p1, w[e / 2], w[16 + e / 2]);
             }

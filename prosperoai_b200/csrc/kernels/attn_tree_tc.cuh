@@ -97,7 +97,7 @@ __device__ __forceinline__ void tc_ld_wait(uint32_t *r) {
                :: "memory");
   asm volatile("" : "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
 }
-__device__ __forceinline__ void tc_st32(uint32_t at, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tc_st32(uint32_t at, const uint32_t *r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
       "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
