@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(few_threads(SW), 1)
   } else if (warp == MMA + 2) {
     copy_tiles<HD, kFewRows, kFewV, false>(p, &vmap, sm.upto, sm.ring, sm.vt[0], sm.vfull, sm.vempty, nullptr);
   } else if (warp == MMA + 3) {
-    clean_tiles<HD, kFewV>(p, sm.ring, sm.vt[0], sm.vfull, sm.vclean, sm.odd);
+    clean_tiles<HD, kFewV, 1>(p, sm.ring, 0, sm.vt[0], sm.vfull, sm.vclean, sm.odd);
   } else if (warp == MMA) {
     // ---- MMA issue ----
     const uint32_t leader = elect_one();

@@ -6,7 +6,7 @@
 //                    row's maximum goes through shared memory. Then the P V of the tile before, which ran
 //                    meanwhile, is added to the running output in registers, half of the dims each.
 //   warp 8           issues the MMAs: Q K^T of tile i + 1 before P V of tile i, so that they overlap the softmax
-//   warps 12-14      K copies, V copies, cleaning
+//   warps 12-15      K copies, V copies, cleaning by two
 // Registers: 512 threads at 128; setmaxnreg gives the softmax warps 200 and leaves 56 to the others (256 * 200 +
 // 256 * 56 = 65536, what the block was launched with).
 #pragma once
@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     for (int i = 0; i < 2; i++) {
       mbar_init(&sm.kfull[i], 1);
       mbar_init(&sm.vfull[i], 1);
-      mbar_init(&sm.vclean[i], 1);
+      mbar_init(&sm.vclean[i], 2);
       mbar_init(&sm.kempty[i], 1);
       mbar_init(&sm.vempty[i], 1);
       mbar_init(&sm.sfull[i], 1);
@@ -78,8 +78,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       copy_tiles<HD, kManyRows, 2, true>(p, &kmap, sm.upto, sm.ring, sm.kt[0], sm.kfull, sm.kempty, sm.valid);
     else if (warp == 13)
       copy_tiles<HD, kManyRows, 2, false>(p, &vmap, sm.upto, sm.ring, sm.vt[0], sm.vfull, sm.vempty, nullptr);
-    else if (warp == 14)
-      clean_tiles<HD, 2>(p, sm.ring, sm.vt[0], sm.vfull, sm.vclean, sm.odd);
+    else
+      clean_tiles<HD, 2, 2>(p, sm.ring, warp - 14, sm.vt[0], sm.vfull, sm.vclean, sm.odd);
   } else if (warp >= 8) {
     // ---- MMA issue ----
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");

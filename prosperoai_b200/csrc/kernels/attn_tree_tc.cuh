@@ -11,6 +11,9 @@
 namespace {
 
 constexpr uint32_t kTcTile = 128, kTcGrid = 148, kRing = 16;
+// What a unit's start costs, in tiles: its queries, first maxima and output. The cut counts them, or a CTA that gets ten
+// units of one tile each takes as long as 40 tiles of one unit (8 sequences of 5 to 5001 positions: 109 to 49 us).
+constexpr uint32_t kStart = 3;
 
 __device__ __forceinline__ uint64_t desc_k(uint32_t saddr) {  // K-major, 128-byte swizzle, 8-row groups of 1024 bytes
   return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)1u << 16 | (uint64_t)(1024u >> 4) << 32 | (uint64_t)1u << 46 |
@@ -132,14 +135,15 @@ struct Ring {
   uint64_t full[kRing];
 };
 
-// upto[s]: (unit, tile) pairs of the sequences before s (the caller bounds their sum). Every thread of the block calls
+// upto[s]: (unit, tile) pairs of the sequences before s, each unit counted with kStart tiles more than it has (the caller
+// bounds their sum). Every thread of the block calls
 // it; a barrier must follow.
 template <uint32_t MR, uint32_t THREADS>
 __device__ __forceinline__ void pairs_before32(const TreeParams &p, uint32_t *upto) {
   const uint32_t n_seq = p.c.n_seq, lane = threadIdx.x & 31;
   for (uint32_t s = threadIdx.x; s < n_seq; s += THREADS) {
     const SeqWork w = seq_work<MR, kTcTile>(p, s);
-    upto[s + 1] = w.blocks * w.tiles * p.c.hk;
+    upto[s + 1] = w.blocks * (w.tiles + kStart) * p.c.hk;
   }
   if (threadIdx.x == 0) upto[0] = 0;
   if (n_seq <= 1) return;
@@ -233,18 +237,19 @@ struct Lead {
   __device__ __forceinline__ bool next(const TreeParams &p, const uint32_t *upto, Ring &ring, Segment &g) {
     const uint32_t lane = threadIdx.x & 31, chunk = blockIdx.x;
     g.tile1 = 0;
-    if (at < end) {
+    while (at < end && g.tile1 == 0) {
       while (upto[s + 1] <= at) s++;
       const SeqWork w = seq_work<MR, kTcTile>(p, s);
-      const uint32_t unit = (at - upto[s]) / w.tiles, unit0 = upto[s] + unit * w.tiles, unit1 = unit0 + w.tiles;
+      const uint32_t span = w.tiles + kStart, unit = (at - upto[s]) / span, unit0 = upto[s] + unit * span;
+      const uint32_t unit1 = unit0 + span, real0 = unit0 + kStart, to = min(end, unit1);
       g.s = s, g.kvh = unit / w.blocks, g.block = unit % w.blocks;
-      g.tile0 = at - unit0, g.tile1 = min(end, unit1) - unit0, g.tiles = w.tiles;
+      g.tile0 = at > real0 ? at - real0 : 0, g.tile1 = to > real0 ? to - real0 : 0, g.tiles = w.tiles;
       g.len = w.len, g.nodes = w.nodes, g.first = w.first;
-      g.slot = 2 * chunk + (chunk * size >= unit0 ? 0 : 1);  // the chunk's first part of a unit, or its last
-      const uint32_t c0 = unit0 / size, c1 = (unit1 - 1) / size;
+      g.slot = 2 * chunk + (chunk * size >= real0 ? 0 : 1);  // the chunk's first part of a unit, or its last
+      const uint32_t c0 = real0 / size, c1 = (unit1 - 1) / size;
       g.parts = c1 - c0 + 1;
-      g.slot0 = 2 * c0 + (c0 * size >= unit0 ? 0 : 1);
-      at = unit0 + g.tile1;
+      g.slot0 = 2 * c0 + (c0 * size >= real0 ? 0 : 1);
+      at = to;
     }
     if (lane == 0) {
       ring.seg[n % kRing] = g;
@@ -324,13 +329,14 @@ __device__ __forceinline__ void copy_tiles(const TreeParams &p, const CUtensorMa
   for (uint32_t n = i < SLOTS ? 0 : i - SLOTS; n < i; n++) wait(&full[n % SLOTS], n / SLOTS);
 }
 
-// One warp hands the V tiles on to the MMAs, after it has looked at the rows of those that hold nodes: a non-finite V
-// row may only reach the rows that see its node, and a weight of 0 does not keep it out of a product. Such elements
-// (those of stale rows behind the last node too) become 0 here, and `odd` tells where; they are added later to the rows
-// that see them. (Every tile is handed on: a barrier that was watched for some phases only could be two phases on.)
-template <int HD, uint32_t SLOTS>
-__device__ __forceinline__ void clean_tiles(const TreeParams &p, Ring &ring, uint8_t *slot0, uint64_t *full, uint64_t *clean,
-                                            uint32_t (*odd)[4]) {
+// V tiles are handed on to the MMAs by WARPS warps (this one is `w`), after they have looked at the rows of those that
+// hold nodes: a non-finite V row may only reach the rows that see its node, and a weight of 0 does not keep it out of a
+// product. Such elements (those of stale rows behind the last node too) become 0 here, and `odd` tells where; they are
+// added later to the rows that see them. (Every tile is handed on: a barrier that was watched for some phases only could
+// be two phases on.)
+template <int HD, uint32_t SLOTS, uint32_t WARPS>
+__device__ __forceinline__ void clean_tiles(const TreeParams &p, Ring &ring, uint32_t w, uint8_t *slot0, uint64_t *full,
+                                            uint64_t *clean, uint32_t (*odd)[4]) {
   constexpr uint32_t BL = kTcTile * 128, BYTES = HD / 64 * BL, CH = HD / 8;
   const uint32_t lane = threadIdx.x & 31;
   Waiter wait{p.wait_ns, p.err};
@@ -342,23 +348,30 @@ __device__ __forceinline__ void clean_tiles(const TreeParams &p, Ring &ring, uin
       wait(&full[sl], i / SLOTS);
       __syncwarp();
       if ((tile + 1) * kTcTile > g.len) {
+        const uint32_t skip = g.len > tile * kTcTile ? g.len - tile * kTcTile : 0;  // committed rows of the tile
 #pragma unroll 1
-        for (uint32_t x = 0; x < 4; x++) {  // a lane has a row of each 32
+        for (uint32_t x = w; x < 4; x += WARPS) {  // a lane has a row of each 32
           const uint32_t r = 32 * x + lane;
           bool bad = false;
-#pragma unroll 4
-          for (uint32_t ch = 0; ch < CH; ch++) {
-            uint4 *at = reinterpret_cast<uint4 *>(slot0 + sl * BYTES + (ch / 8) * BL + r * 128 + (((ch % 8) ^ (r & 7)) << 4));
-            uint4 v = *at;
-            uint32_t *cw = reinterpret_cast<uint32_t *>(&v);
-            bool here = false;
+          if (r >= skip) {
+            uint8_t *row = slot0 + sl * BYTES + r * 128;
+#pragma unroll 8
+            for (uint32_t ch = 0; ch < CH; ch++) {
+              uint4 *at = reinterpret_cast<uint4 *>(row + (ch / 8) * BL + (((ch % 8) ^ (r & 7)) << 4));
+              uint4 v = *at;
+              // an exponent of all ones carries into the sign's place
+              const uint32_t E = 0x7C007C00u, one = 0x04000400u;
+              if ((((v.x & E) + one) | ((v.y & E) + one) | ((v.z & E) + one) | ((v.w & E) + one)) & 0x80008000u) {
+                bad = true;
+                uint32_t *cw = reinterpret_cast<uint32_t *>(&v);
 #pragma unroll
-            for (int y = 0; y < 4; y++) {
-              if ((cw[y] & 0x7C00u) == 0x7C00u) cw[y] &= 0xFFFF0000u, here = true;
-              if ((cw[y] & 0x7C000000u) == 0x7C000000u) cw[y] &= 0xFFFFu, here = true;
+                for (int y = 0; y < 4; y++) {
+                  if ((cw[y] & 0x7C00u) == 0x7C00u) cw[y] &= 0xFFFF0000u;
+                  if ((cw[y] & 0x7C000000u) == 0x7C000000u) cw[y] &= 0xFFFFu;
+                }
+                *at = v;
+              }
             }
-            if (here) *at = v;
-            bad |= here;
           }
           const uint32_t word = __ballot_sync(0xffffffffu, bad);
           if (lane == 0) odd[i & 7][x] = word;

@@ -470,7 +470,7 @@ pai_status_t launch_tc(pai_b200_ctx_t *ctx, TreeParams &p, void (*kern)(TreePara
   p.max_blocks = (p.max_nodes * p.g + MR - 1) / MR;
   const uint64_t units = (uint64_t)p.c.n_seq * p.c.hk * p.max_blocks;
   if (units > 0x7FFFFFFu) return b200_fail(PAI_ERR_UNSUPPORTED, "attn_tree: %llu row tiles", (unsigned long long)units);
-  const uint64_t pairs = units * (((uint64_t)p.c.max_pages * p.c.page_tokens + p.max_nodes + kTcTile - 1) / kTcTile);
+  const uint64_t pairs = units * (((uint64_t)p.c.max_pages * p.c.page_tokens + p.max_nodes + kTcTile - 1) / kTcTile + kStart);
   if (pairs > 0x7FFFFFFFull)  // numbered in 32 bits
     return b200_fail(PAI_ERR_UNSUPPORTED, "attn_tree: %llu tiles of rows and keys", (unsigned long long)pairs);
   const uint32_t grid = (uint32_t)std::min<uint64_t>(kTcGrid, pairs);
