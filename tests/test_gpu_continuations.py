@@ -562,9 +562,9 @@ def beam_reference(logits, scores, done, pad, n_out):
     return cand, order
 
 
-# exp of a logit: x - m is off by 2^-24 |x - m|, of which e^(x - m) is a vanishing part from 20 on: 20 * 2^-24, and expf
-# by 2^-22; 32 of them are added in 32 bits (31 * 2^-24), the slice's sum is rounded to 32 bits: 2^-18 in log Z is
-# above their sum. The score is rounded once more.
+# exp of a logit as 2^((x - m) log2 e): x - m, the product and the constant are off by 2^-24, 2^-24 and 2^-25 of |x - m|,
+# whose mean under the weights is at most log(vocab) < 12: 30 * 2^-24; 2^-22 for 2^x; 10 additions in 32 bits; the
+# slice's sum is rounded to 32 bits: 45 * 2^-24 in log Z, below 2^-18. The score is rounded once more.
 def beam_tol(s):
     return 2.0 ** -18 + 2.0 ** -24 * np.abs(s)
 
