@@ -412,6 +412,9 @@ extern "C" pai_status_t pai_b200_kv_fork_f16(pai_b200_ctx_t *ctx, const pai_b200
   p.keeper = p.used + kv->n_pages;
   p.fresh = p.keeper + kv->n_pages;
   b200_launch(ctx, k_kv_fork_plan, dim3(1), dim3(kPlanThreads), 0, p);
+  // the copying kernel is resident before the plan is done, and waits for it
+  const int pdl = b200_ctx_pdl(ctx);
+  b200_ctx_set_pdl(ctx, 1);
   const uint32_t planes = 2 * kv->n_layer;
   if (paged) {
     const uint64_t pieces = (uint64_t)kv->page_tokens * (kv->head_dim / 8) * kv->kv_heads;
@@ -427,5 +430,6 @@ extern "C" pai_status_t pai_b200_kv_fork_f16(pai_b200_ctx_t *ctx, const pai_b200
     else
       b200_launch(ctx, k_kv_fork_runs<32>, grid, dim3(kCopyThreads), 0, p.c, (const ForkCopy *)p.copies);
   }
+  b200_ctx_set_pdl(ctx, pdl);
   return b200_launched(ctx, 2, "k_kv_fork");
 }
