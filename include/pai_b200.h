@@ -758,6 +758,45 @@ pai_status_t pai_b200_session_kv_info(const pai_b200_session_t *s, pai_b200_kv_i
  * pointer; PAI_ERR_NOMEM when the positions do not fit. */
 pai_status_t pai_b200_session_kv_reserve(pai_b200_session_t *s, uint32_t tokens, uint32_t *out_pos);
 
+/* ---- session: drafted trees and beams ------------------------------------------
+ * The operators on cache views over the session's own cache. Not under
+ * tensor parallelism (PAI_ERR_UNSUPPORTED). */
+
+/* The session's cache as a view: one run of capacity positions a sequence. */
+pai_status_t pai_b200_session_kv_view(const pai_b200_session_t *s, pai_b200_kv_view_t *out);
+/* Run n drafted tokens of every sequence (tokens [batch][n], host) through
+ * the model in one pass, as nodes of a tree behind the session's position:
+ * parents[i] < i is the node that node i follows, -1 the last committed
+ * position (parents NULL: node i follows node i - 1). next[batch][n] receives
+ * the greedy token after every node. Nothing is committed: the position
+ * stays, and any later call but pai_b200_session_accept forgets the nodes.
+ * Up to 8 rows (batch x n) the layers are the decode step's GEMVs, above
+ * that the prefill's GEMM (see pai_b200_session_prefill for its precision).
+ * PAI_ERR_NOMEM when the nodes do not fit behind the position,
+ * PAI_ERR_UNSUPPORTED above 1024 nodes or 2048 rows. */
+pai_status_t pai_b200_session_verify(pai_b200_session_t *s, const int32_t *tokens, const int32_t *parents, uint32_t n,
+                                     int32_t *next);
+/* Keep a path of the nodes of the last pai_b200_session_verify: path is
+ * [batch][n_path] node indexes, from a node that follows the committed
+ * positions down the tree. The position advances by n_path, and next[batch]
+ * (host) are the tokens of the next pai_b200_session_run step.
+ * PAI_ERR_INVALID_ARG for anything that is no such path, or without a
+ * pai_b200_session_verify directly before. */
+pai_status_t pai_b200_session_accept(pai_b200_session_t *s, const int32_t *path, uint32_t n_path, const int32_t *next);
+/* One selection of a beam search over the session's sequences: the batch
+ * best continuations of the last step's (or prefill's) logits, as
+ * pai_b200_beam_select_f32 with one prompt and n_out = batch. The caches of
+ * the sequences are reordered to follow their parents, from position `first`
+ * on (below it, the sequences hold the same: a common prompt), and the chosen
+ * tokens become the next step's input. All arrays are host arrays of batch
+ * entries; done may be NULL. Before the first selection after a common prompt,
+ * give all beams but one a score of -INFINITY. A beam without a candidate
+ * (score -INFINITY, parent -1) keeps running on `pad` and stays unchosen.
+ * PAI_ERR_INVALID_ARG unless the position was last moved by a step or a
+ * prefill, and its logits were selected from once only. */
+pai_status_t pai_b200_session_beam(pai_b200_session_t *s, const float *scores, const int32_t *done, int32_t pad,
+                                   uint32_t first, float *out_scores, int32_t *out_parents, int32_t *out_tokens);
+
 #ifdef __cplusplus
 }
 #endif

@@ -183,6 +183,10 @@ SIGNATURES = {
     "pai_b200_session_step_kernels": (U32, [P]),
     "pai_b200_session_run_layers": (I32, [P, U32]),
     "pai_b200_session_kv_reserve": (I32, [P, U32, P]),
+    "pai_b200_session_kv_view": (I32, [P, P]),
+    "pai_b200_session_verify": (I32, [P, P, P, U32, P]),
+    "pai_b200_session_accept": (I32, [P, P, U32, P]),
+    "pai_b200_session_beam": (I32, [P, P, P, I32, U32, P, P, P]),
 }
 
 

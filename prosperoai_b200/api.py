@@ -447,6 +447,41 @@ class Session:
         check(load().pai_b200_session_kv_reserve(self.h, tokens, C.byref(pos)), "session_kv_reserve")
         return int(pos.value)
 
+    # --- several continuations -------------------------------------------------------------
+    def kv_view(self) -> KvView:
+        """The session's cache as a view for the operators on caches (pai_b200_session_kv_view)."""
+        kv = KvView()
+        check(load().pai_b200_session_kv_view(self.h, C.byref(kv)), "session_kv_view")
+        return kv
+
+    def verify(self, tokens, parents=None) -> np.ndarray:
+        """Run drafted tokens [batch][n] as nodes of a tree behind the position, without
+        committing them; the greedy token after every node (pai_b200_session_verify)."""
+        t = np.ascontiguousarray(tokens, np.int32).reshape(self.batch, -1)
+        par = None if parents is None else np.ascontiguousarray(parents, np.int32)
+        if par is not None and par.shape != (t.shape[1],):
+            raise ValueError(f"{t.shape[1]} nodes, {par.size} parents")
+        nxt = np.empty(t.shape, np.int32)
+        check(load().pai_b200_session_verify(self.h, t.ctypes.data, None if par is None else par.ctypes.data, t.shape[1],
+                                             nxt.ctypes.data), "session_verify")
+        return nxt
+
+    def accept(self, path, next_tokens) -> None:
+        """Keep a path [batch][n] of the verified nodes; next_tokens [batch] come next (pai_b200_session_accept)."""
+        p = np.ascontiguousarray(path, np.int32).reshape(self.batch, -1)
+        t = np.ascontiguousarray(next_tokens, np.int32).reshape(self.batch)
+        check(load().pai_b200_session_accept(self.h, p.ctypes.data, p.shape[1], t.ctypes.data), "session_accept")
+
+    def beam(self, scores, done=None, pad: int = 0, first: int = 0):
+        """Select the best continuations of the session's sequences as beams of one prompt and reorder
+        their caches: (scores, parents, tokens) of the new beams (pai_b200_session_beam)."""
+        sc = np.ascontiguousarray(scores, np.float32).reshape(self.batch)
+        dn = None if done is None else np.ascontiguousarray(done, np.int32).reshape(self.batch)
+        out = np.empty(self.batch, np.float32), np.empty(self.batch, np.int32), np.empty(self.batch, np.int32)
+        check(load().pai_b200_session_beam(self.h, sc.ctypes.data, None if dn is None else dn.ctypes.data, pad, first,
+                                           *(o.ctypes.data for o in out)), "session_beam")
+        return out
+
     def write_kv(self, layer: int, seq: int, k: np.ndarray, v: np.ndarray, pos0: int = 0) -> None:
         """Copy host fp16 rows [kv_head][positions][head_dim] into the cache of
         one layer and sequence at positions pos0.. (this rank's kv heads)."""

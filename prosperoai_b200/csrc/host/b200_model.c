@@ -418,6 +418,13 @@ struct pai_b200_session {
   int32_t *pf_tok, *pf_htok;
   void *pf_xq_buf;
   b200_xq_t pf_xq;
+  /* drafted trees and beams (allocated by the first use): rotated q rows, 8
+   * rows of logits, small arrays on the device and their pinned staging */
+  float *dr_q, *dr_logits;
+  uint8_t *dr_dev, *dr_host;
+  int32_t *dr_parents; /* host: the nodes of the last verification */
+  uint32_t dr_nodes;   /* ... and their number; 0: none that can be accepted */
+  int beam_ready;      /* the logits belong to the position, and no selection has used them */
 };
 
 /* Tensor-parallel hooks (csrc/host/b200_tp.c). */
@@ -693,6 +700,11 @@ pai_status_t pai_b200_session_destroy(pai_b200_session_t *s) {
   pai_b200_free(ctx, s->pf_tok);
   pai_b200_free(ctx, s->pf_xq_buf);
   pai_b200_host_free(ctx, s->pf_htok);
+  pai_b200_free(ctx, s->dr_q);
+  pai_b200_free(ctx, s->dr_logits);
+  pai_b200_free(ctx, s->dr_dev);
+  pai_b200_host_free(ctx, s->dr_host);
+  free(s->dr_parents);
   free(s);
   return PAI_OK;
 }
@@ -712,6 +724,8 @@ static pai_status_t kv_take(pai_b200_session_t *s, uint32_t tokens, uint32_t *fi
   if (first) *first = s->pos;
   s->pos += tokens;
   s->kv_reservations++;
+  s->dr_nodes = 0;
+  s->beam_ready = 0;
   return PAI_OK;
 }
 
@@ -751,6 +765,8 @@ pai_status_t pai_b200_session_reset(pai_b200_session_t *s) {
   if (!st) {
     s->pos = 0;
     s->kv_reservations = 0;
+    s->dr_nodes = 0;
+    s->beam_ready = 0;
   }
   return st;
 }
@@ -819,6 +835,7 @@ pai_status_t pai_b200_session_run(pai_b200_session_t *s, uint32_t steps) {
   for (uint32_t i = 0; i < steps && !st; i++) {
     st = b200_graph_launch(s->m->ctx, s->graph, s->graph_kernels);
     if (!st) st = kv_take(s, 1, NULL);
+    if (!st) s->beam_ready = 1;
   }
   return st;
 }
@@ -974,5 +991,233 @@ pai_status_t pai_b200_session_prefill(pai_b200_session_t *s, const int32_t *toke
     if (!st) st = seen(s, pai_b200_sync(ctx));
   }
   if (!st) st = pai_b200_session_get_tokens(s, next);
+  if (!st) s->beam_ready = 1;
   return seen(s, st);
+}
+
+/* ---- drafted trees and beams ------------------------------------------------------------ */
+
+#define DR_MAX_NODES 1024u
+/* Byte offsets in dr_dev and dr_host. A pass has at most PF_MAX_ROWS rows, so
+ * batch x nodes stays within the row arrays and the masks' words. */
+enum {
+  DR_LENS = 0, DR_OFF = 32, DR_NPATH = 96, DR_SCORES = 128, DR_DONE = 160, DR_OUT_SCORES = 192, DR_OUT_PARENTS = 224,
+  DR_OUT_TOKENS = 256, DR_LENS_OUT = 288, DR_GRANTED = 320,
+  DR_DEPTH = 512, DR_PATH = DR_DEPTH + 4 * PF_MAX_ROWS, DR_NEXT = DR_PATH + 4 * PF_MAX_ROWS,
+  DR_MASK = DR_NEXT + 4 * PF_MAX_ROWS, DR_BYTES = DR_MASK + 8 * PF_MAX_ROWS * (DR_MAX_NODES / 64)
+};
+
+static pai_status_t draft_alloc(pai_b200_session_t *s) {
+  pai_b200_model_t *m = s->m;
+  pai_b200_ctx_t *ctx = m->ctx;
+  pai_status_t st = prefill_alloc(s);
+  if (st || s->dr_parents) return st;
+  if (!s->dr_q) SALLOC(s->dr_q, (uint64_t)PF_MAX_ROWS * m->k_o * 4);
+  if (!s->dr_logits) SALLOC(s->dr_logits, 8ull * m->vl * 4);
+  if (!s->dr_dev) SALLOC(s->dr_dev, DR_BYTES);
+  if (!st && !s->dr_host) st = pai_b200_host_alloc(ctx, DR_BYTES, (void **)&s->dr_host);
+  if (!st) {
+    s->dr_parents = (int32_t *)malloc(DR_MAX_NODES * sizeof(int32_t));
+    if (!s->dr_parents) st = b200_fail(PAI_ERR_NOMEM, "session: host allocation");
+  }
+  return st;
+}
+
+static pai_status_t one_gpu(const pai_b200_session_t *s, const char *what) {
+  if (s->m->tp > 1) return b200_fail(PAI_ERR_UNSUPPORTED, "%s: not under tensor parallelism", what);
+  return usable(s);
+}
+
+static pai_status_t dr_up(pai_b200_session_t *s, uint32_t off, uint64_t bytes) {
+  return pai_b200_memcpy_h2d(s->m->ctx, s->dr_dev + off, s->dr_host + off, bytes);
+}
+
+pai_status_t pai_b200_session_kv_view(const pai_b200_session_t *s, pai_b200_kv_view_t *out) {
+  if (!s || !out) return b200_fail(PAI_ERR_INVALID_ARG, "session_kv_view: NULL");
+  memset(out, 0, sizeof(*out));
+  out->k = s->kc;
+  out->v = s->vc;
+  out->n_layer = s->m->cfg.n_layer;
+  out->n_seq = s->batch;
+  out->kv_heads = s->m->hkl;
+  out->head_dim = s->m->cfg.head_dim;
+  out->page_tokens = s->max_ctx;
+  out->n_pages = s->batch;
+  out->max_pages = 1;
+  out->layer_stride = s->layer_stride;
+  out->page_stride = s->seq_stride;
+  out->head_stride = (uint64_t)s->max_ctx * s->m->cfg.head_dim;
+  return PAI_OK;
+}
+
+/* The layers over `rows` drafted rows in pf_x, the nodes' K/V appended behind the position. */
+static pai_status_t draft_layers(pai_b200_session_t *s, uint32_t rows, uint32_t n) {
+  pai_b200_model_t *m = s->m;
+  pai_b200_ctx_t *ctx = m->ctx;
+  const pai_b200_model_cfg_t *c = &m->cfg;
+  const uint32_t E = c->n_embd;
+  const int32_t *lens = (const int32_t *)(s->dr_dev + DR_LENS), *off = (const int32_t *)(s->dr_dev + DR_OFF);
+  const int32_t *depth = (const int32_t *)(s->dr_dev + DR_DEPTH);
+  const uint64_t *mask = (const uint64_t *)(s->dr_dev + DR_MASK);
+  pai_b200_kv_view_t kv;
+  pai_status_t st = pai_b200_session_kv_view(s, &kv);
+  for (uint32_t l = 0; !st && l < c->n_layer; l++) {
+    st = b200_launch_rmsnorm_xq(ctx, rows, E, s->pf_x, m->attn_norm[l], c->eps, s->pf_xn, NULL);
+    if (!st) st = rows_matmul(s, c->wtype, rows, m->n_qkv, E, m->wqkv[l], s->pf_xn, s->pf_qkv, B200_EPI_STORE);
+    if (!st)
+      st = pai_b200_rope_append_f16kv(ctx, &kv, l, m->hl, rows, n, lens, off, depth, s->pf_qkv, s->cos_t, s->sin_t,
+                                      s->max_ctx, s->dr_q);
+    if (!st) st = pai_b200_attn_tree_f16kv(ctx, &kv, l, m->hl, rows, n, lens, off, mask, s->dr_q, s->pf_att);
+    if (!st) st = rows_matmul(s, c->wtype, rows, E, m->k_o, m->wo[l], s->pf_att, s->pf_x, B200_EPI_RESIDUAL);
+    if (!st) st = b200_launch_rmsnorm_xq(ctx, rows, E, s->pf_x, m->ffn_norm[l], c->eps, s->pf_xn, NULL);
+    if (!st) st = rows_matmul(s, c->wtype, rows, 2ull * m->ffl, E, m->wgu[l], s->pf_xn, s->pf_h, B200_EPI_SILU_GLU);
+    if (!st) st = rows_matmul(s, c->wtype, rows, E, m->ffl, m->wdown[l], s->pf_h, s->pf_x, B200_EPI_RESIDUAL);
+  }
+  return st;
+}
+
+pai_status_t pai_b200_session_verify(pai_b200_session_t *s, const int32_t *tokens, const int32_t *parents, uint32_t n,
+                                     int32_t *next) {
+  if (!s || !tokens || !next || n == 0) return b200_fail(PAI_ERR_INVALID_ARG, "session_verify: NULL or empty");
+  pai_b200_model_t *m = s->m;
+  pai_b200_ctx_t *ctx = m->ctx;
+  const pai_b200_model_cfg_t *c = &m->cfg;
+  const uint32_t B = s->batch, E = c->n_embd, words = (n + 63) / 64;
+  const int gemm = s->pf_gemm;
+  pai_status_t st = one_gpu(s, "session_verify");
+  if (st) return st;
+  if (n > DR_MAX_NODES || (uint64_t)B * n > PF_MAX_ROWS)
+    return b200_fail(PAI_ERR_UNSUPPORTED, "session_verify: %u nodes of %u sequences (at most %u nodes, %u rows)", n, B,
+                     DR_MAX_NODES, PF_MAX_ROWS);
+  if ((uint64_t)s->pos + n > s->max_ctx)
+    return b200_fail(PAI_ERR_NOMEM, "session_verify: %u nodes behind position %u exceed the %u-position cache", n, s->pos,
+                     s->max_ctx);
+  for (uint32_t i = 0; parents && i < n; i++)
+    if (parents[i] < -1 || parents[i] >= (int32_t)i)
+      return b200_fail(PAI_ERR_INVALID_ARG, "session_verify: node %u follows %d", i, parents[i]);
+  for (uint64_t i = 0; i < (uint64_t)B * n; i++)
+    if (tokens[i] < 0 || (uint32_t)tokens[i] >= c->vocab)
+      return b200_fail(PAI_ERR_INVALID_ARG, "session_verify: token %d outside vocab %u", tokens[i], c->vocab);
+  st = draft_alloc(s);
+  if (!st) st = seen(s, pai_b200_sync(ctx)); /* the staging may still feed earlier copies */
+  if (st) return st;
+  s->dr_nodes = 0;
+  const uint32_t rows = B * n;
+  int32_t *lens = (int32_t *)(s->dr_host + DR_LENS), *off = (int32_t *)(s->dr_host + DR_OFF);
+  int32_t *depth = (int32_t *)(s->dr_host + DR_DEPTH);
+  uint64_t *mask = (uint64_t *)(s->dr_host + DR_MASK);
+  for (uint32_t i = 0; i < n; i++) { /* a node sees its parent's nodes and itself */
+    const int32_t p = parents ? parents[i] : (int32_t)i - 1;
+    s->dr_parents[i] = p;
+    depth[i] = p < 0 ? 0 : depth[p] + 1;
+    for (uint32_t w = 0; w < words; w++) mask[(uint64_t)i * words + w] = p < 0 ? 0 : mask[(uint64_t)p * words + w];
+    mask[(uint64_t)i * words + i / 64] |= 1ull << (i % 64);
+  }
+  for (uint32_t b = 0; b < B; b++) {
+    lens[b] = (int32_t)s->pos;
+    off[b] = (int32_t)(b * n);
+    if (b == 0) continue;
+    memcpy(depth + (uint64_t)b * n, depth, n * 4ull);
+    memcpy(mask + (uint64_t)b * n * words, mask, (uint64_t)n * words * 8);
+  }
+  off[B] = (int32_t)rows;
+  memcpy(s->pf_htok, tokens, rows * 4ull);
+  st = dr_up(s, 0, DR_DEPTH + rows * 4ull);
+  if (!st) st = dr_up(s, DR_MASK, (uint64_t)rows * words * 8);
+  if (!st) st = pai_b200_memcpy_h2d(ctx, s->pf_tok, s->pf_htok, rows * 4ull);
+  if (!st) st = b200_launch_embed(ctx, c->etype, rows, c->vocab, E, m->tok_embd, s->pf_tok, s->pf_x);
+  /* Up to 8 rows one GEMV of the decode step reads the weights once, as the
+   * GEMM does, and without rounding the rows to bf16. Whole verifications of
+   * 1, 4, 8, 9 and 16 rows (8 layers of width 4096, Q4_0, 128256 tokens): GEMV
+   * 1108, 1278, 1689, 2400 and 2882 us, GEMM 1643, 1675, 1801, 1832 and 1925. */
+  if (rows <= 8) s->pf_gemm = 0;
+  if (!st) st = draft_layers(s, rows, n);
+  s->pf_gemm = gemm;
+  /* lm head and greedy token of every row, 8 rows at a time */
+  for (uint32_t r = 0; !st && r < rows; r += 8) {
+    const uint32_t g = rows - r < 8 ? rows - r : 8;
+    b200_xq_t xq = b200_xq_view(s->pf_xq_buf, g, E);
+    st = b200_launch_rmsnorm_xq(ctx, g, E, s->pf_x + (uint64_t)r * E, m->output_norm, c->eps, NULL, &xq);
+    if (!st) st = b200_launch_gemv(ctx, c->etype, g, m->vl, E, m->output, &xq, NULL, s->dr_logits, B200_EPI_STORE, NULL);
+    if (!st) st = b200_launch_argmax(ctx, g, m->vl, s->dr_logits, (int32_t *)(s->dr_dev + DR_NEXT) + r);
+  }
+  if (!st) st = pai_b200_memcpy_d2h(ctx, s->dr_host + DR_NEXT, s->dr_dev + DR_NEXT, rows * 4ull);
+  if (!st) st = seen(s, pai_b200_sync(ctx));
+  if (st) return st;
+  memcpy(next, s->dr_host + DR_NEXT, rows * 4ull);
+  s->dr_nodes = n;
+  return PAI_OK;
+}
+
+pai_status_t pai_b200_session_accept(pai_b200_session_t *s, const int32_t *path, uint32_t n_path, const int32_t *next) {
+  if (!s || !path || !next || n_path == 0) return b200_fail(PAI_ERR_INVALID_ARG, "session_accept: NULL or empty");
+  const uint32_t B = s->batch;
+  pai_b200_kv_view_t kv;
+  pai_status_t st = one_gpu(s, "session_accept");
+  if (st) return st;
+  if (n_path > s->dr_nodes) /* 0: no verification directly before */
+    return b200_fail(PAI_ERR_INVALID_ARG, "session_accept: %u of %u verified nodes", n_path, s->dr_nodes);
+  for (uint32_t b = 0; b < B; b++)
+    for (uint32_t i = 0; i < n_path; i++) {
+      const int32_t e = path[(uint64_t)b * n_path + i];
+      if (e < 0 || (uint32_t)e >= s->dr_nodes || s->dr_parents[e] != (i ? path[(uint64_t)b * n_path + i - 1] : -1))
+        return b200_fail(PAI_ERR_INVALID_ARG, "session_accept: node %d is no step %u of a path", e, i);
+    }
+  st = check_tokens(s, next);
+  if (!st) st = pai_b200_session_kv_view(s, &kv);
+  if (st) return st;
+  memcpy(s->dr_host + DR_PATH, path, (uint64_t)B * n_path * 4);
+  for (uint32_t b = 0; b < B; b++) ((int32_t *)(s->dr_host + DR_NPATH))[b] = (int32_t)n_path;
+  st = dr_up(s, DR_NPATH, B * 4ull);
+  if (!st) st = dr_up(s, DR_PATH, (uint64_t)B * n_path * 4);
+  if (!st)
+    st = pai_b200_kv_accept_f16(s->m->ctx, &kv, n_path, (const int32_t *)(s->dr_dev + DR_LENS),
+                                (const int32_t *)(s->dr_dev + DR_PATH), (const int32_t *)(s->dr_dev + DR_NPATH),
+                                (int32_t *)(s->dr_dev + DR_LENS_OUT));
+  if (!st) st = kv_take(s, n_path, NULL);
+  if (!st) st = set_device_pos(s);
+  if (!st) st = pai_b200_session_set_tokens(s, next);
+  return st ? st : seen(s, pai_b200_sync(s->m->ctx));
+}
+
+pai_status_t pai_b200_session_beam(pai_b200_session_t *s, const float *scores, const int32_t *done, int32_t pad,
+                                   uint32_t first, float *out_scores, int32_t *out_parents, int32_t *out_tokens) {
+  if (!s || !scores || !out_scores || !out_parents || !out_tokens)
+    return b200_fail(PAI_ERR_INVALID_ARG, "session_beam: NULL");
+  pai_b200_ctx_t *ctx = s->m->ctx;
+  const uint32_t B = s->batch;
+  pai_b200_kv_view_t kv;
+  pai_status_t st = one_gpu(s, "session_beam");
+  if (st) return st;
+  if (!s->beam_ready) return b200_fail(PAI_ERR_INVALID_ARG, "session_beam: no step since the last selection");
+  if (first > s->pos) return b200_fail(PAI_ERR_INVALID_ARG, "session_beam: %u common positions of %u", first, s->pos);
+  if (pad < 0 || (uint32_t)pad >= s->m->cfg.vocab)
+    return b200_fail(PAI_ERR_INVALID_ARG, "session_beam: pad token %d outside vocab %u", pad, s->m->cfg.vocab);
+  st = draft_alloc(s);
+  if (!st) st = seen(s, pai_b200_sync(ctx));
+  if (!st) st = pai_b200_session_kv_view(s, &kv);
+  if (st) return st;
+  memcpy(s->dr_host + DR_SCORES, scores, B * 4);
+  if (done) memcpy(s->dr_host + DR_DONE, done, B * 4);
+  for (uint32_t b = 0; b < B; b++) ((int32_t *)(s->dr_host + DR_LENS))[b] = (int32_t)s->pos;
+  st = dr_up(s, 0, DR_OUT_SCORES);
+  if (!st)
+    st = pai_b200_beam_select_f32(ctx, 1, B, s->m->vl, s->logits, s->m->vl, (const float *)(s->dr_dev + DR_SCORES),
+                                  done ? (const int32_t *)(s->dr_dev + DR_DONE) : NULL, pad, B,
+                                  (float *)(s->dr_dev + DR_OUT_SCORES), (int32_t *)(s->dr_dev + DR_OUT_PARENTS),
+                                  (int32_t *)(s->dr_dev + DR_OUT_TOKENS));
+  if (!st)
+    st = pai_b200_kv_fork_f16(ctx, &kv, first, (const int32_t *)(s->dr_dev + DR_LENS),
+                              (const int32_t *)(s->dr_dev + DR_OUT_PARENTS), NULL, NULL,
+                              (int32_t *)(s->dr_dev + DR_LENS_OUT), (int32_t *)(s->dr_dev + DR_GRANTED));
+  if (!st) st = pai_b200_memcpy_d2d(ctx, s->tok_in, s->dr_dev + DR_OUT_TOKENS, B * 4ull);
+  if (!st) st = pai_b200_memcpy_d2h(ctx, s->dr_host + DR_OUT_SCORES, s->dr_dev + DR_OUT_SCORES, 96);
+  if (!st) st = seen(s, pai_b200_sync(ctx));
+  if (st) return st;
+  s->beam_ready = 0;
+  s->dr_nodes = 0;
+  memcpy(out_scores, s->dr_host + DR_OUT_SCORES, B * 4);
+  memcpy(out_parents, s->dr_host + DR_OUT_PARENTS, B * 4);
+  memcpy(out_tokens, s->dr_host + DR_OUT_TOKENS, B * 4);
+  return PAI_OK;
 }

@@ -179,3 +179,13 @@ def test_page_arithmetic(tmp_path):
         want.append("0 0" if none else f"{a} {min(b - a, rows - a, most)}")
     got = subprocess.run([str(tmp_path / "rows")], input="\n".join(given), capture_output=True, text=True, check=True).stdout
     assert got.split("\n")[:-1] == want
+
+
+def test_session_refusals_without_a_session():
+    L = _native.load()
+    words = (C.c_int32 * 8)()
+    floats = (C.c_float * 8)()
+    assert L.pai_b200_session_kv_view(None, C.byref(KvView())) == INVALID
+    assert L.pai_b200_session_verify(None, words, None, 1, words) == INVALID
+    assert L.pai_b200_session_accept(None, words, 1, words) == INVALID
+    assert L.pai_b200_session_beam(None, floats, None, 0, 0, floats, words, words) == INVALID
