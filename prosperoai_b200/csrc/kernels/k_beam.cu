@@ -5,36 +5,46 @@
 //
 // Within a beam the order of the scores is the order of the logits, so a CTA
 // needs neither m_b nor Z_b to know which of its logits can be chosen: it
-// keeps the n_out largest of its slice (in registers), the slice's maximum
-// and its sum of exponentials. The last CTA of a prompt to finish merges:
-// m_b and Z_b of every beam from the slices in order, then the n_out best of
-// the kept logits by score. What is added up is added in a fixed order; the
-// chosen ones are ranked by (score, flat index), so nothing depends on which
-// CTA is last.
+// keeps the n_out largest of its slice, the slice's maximum and its sum of
+// exponentials. The last CTA of a prompt to finish merges: m_b and Z_b of
+// every beam from the slices in order, then the n_out best of the kept logits
+// by score. What is added up is added in a fixed order; the chosen ones are
+// ranked by (score, flat index), so nothing depends on which CTA is last.
 //
-// The n_out largest of a slice: every warp finds the ceil(n_out / 8)-th
-// largest of its threads' maxima; the smallest of these is a bound that at
-// least n_out values reach, and few others. Those that reach it are collected
-// and ranked (ranking all 256 maxima instead took most of 72 us at 128 rows
-// of 128256). Where more than kCollect reach it (a slice of equal logits),
-// they are taken one by one.
+// A slice is read in tiles of 4096 (16 registers a thread), the next one on
+// its way while one is worked on. The n_out best of the first tile give a bar
+// that few later logits reach; those that do go to a list of their warp, so
+// that the warps meet at the first and the last tile only. The best of a tile
+// or of the lists: every warp finds the ceil(n_out / 8)-th largest of its
+// threads' maxima; the smallest of these is a bound that at least n_out
+// values reach, and few others, which are collected and ranked.
 //
-// The exponentials are 2^((x - m) log2 e): x - m, the product and the
-// constant are off by 2.5 2^-24 |x - m|, of which the weighted mean is at
-// most that of |x - m|, log(vocab) at most; 2^-22 for the special function
-// unit; 10 additions of a thread. With the sums of threads in 64 bits, log Z
-// is off by less than 45 2^-24 at 128256 tokens.
+// 16 prompts of 8 beams of 128256, 16 kept (66 MB, 10 us): 30 us, of which the
+// reading and the exponentials 15, the first and last picks 5, the lists 4 and
+// the merge 6. One launch of 8192 logits a CTA, ranked there, took 40; a
+// barrier a tile 39; four CTAs on an SM instead of three (64 registers, which
+// spill) 33; tiles of 2048 41; three tiles ahead in shared memory 35; the
+// lists by ballots 31.
+//
+// The exponentials are 2^((x - c) log2 e) with the thread's own c, at most 2
+// below its maximum so far: x - c, the product and the constant are off by 2.5
+// 2^-24 |x - c|, and the weighted mean of |x - c| is below that of |x - m| + 4,
+// log(vocab) + 4 at most; 2^-22 each for the special function unit here and
+// where c meets the slice's maximum; 6 additions in 32 bits, the others in 64.
+// So log Z is off by less than 55 2^-24 at 128256 tokens.
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 
 #include "../b200_internal.h"
 #include "b200_device.cuh"
 
 namespace {
 
-constexpr uint32_t kThreads = 256, kPer = 32, kSlice = kThreads * kPer;  // logits of a CTA: 32 registers a thread
-constexpr uint32_t kMaxPick = 64, kMaxBeams = 64, kCollect = 1024;
+constexpr uint32_t kThreads = 256, kPer = 16, kTile = kThreads * kPer;  // logits of a CTA at a time: 16 registers a thread
+constexpr uint32_t kCtasPerSm = 3, kSms = 148;
+constexpr uint32_t kMaxPick = 64, kMaxBeams = 64, kCollect = 1024, kHold = 64;
 
 struct BeamParams {
   const float *logits, *scores;
@@ -62,6 +72,8 @@ template <typename T>
 __device__ __forceinline__ bool before(T v, uint32_t i, T w, uint32_t j) {
   return v > w || (v == w && i < j);
 }
+
+constexpr float kLog2e = 1.4426950408889634f;
 
 // 2^x of the special function unit
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -151,78 +163,151 @@ __device__ uint32_t block_pick(uint32_t pick, float most, Each each, Cand<T> *ou
   return pick;
 }
 
-__global__ void __launch_bounds__(kThreads) k_beam_select(BeamParams p) {
+// The next float above a value that is not NaN.
+__device__ __forceinline__ float above(float v) { return nextafterf(v, INFINITY); }
+
+// Keeps the M first of a warp's list of n > M entries (in order); returns the last one's value.
+__device__ __noinline__ float warp_keep(Cand<float> *list, uint32_t n, uint32_t M) {
+  const uint32_t lane = threadIdx.x & 31;
+  float lv = INFINITY;
+  for (uint32_t k = 0; k < M; k++) {  // the first of entries k .. n - 1 changes places with entry k
+    float bv = -INFINITY;
+    uint32_t bi = 0xFFFFFFFFu, at = 0;
+    for (uint32_t a = k + lane; a < n; a += 32)
+      if (before(list[a].v, list[a].i, bv, bi)) bv = list[a].v, bi = list[a].i, at = a;
+    lv = warp_top(bv);
+    const uint32_t i = __reduce_min_sync(0xffffffffu, bv == lv ? bi : 0xFFFFFFFFu);
+    if (bv == lv && bi == i) {
+      list[at] = list[k];
+      list[k] = Cand<float>{lv, i};
+    }
+    __syncwarp();
+  }
+  return lv;
+}
+
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) k_beam_select(BeamParams p) {
   pdl_trigger();
   pdl_wait();
-  __shared__ Cand<double> buf_d[kCollect];  // the float form's buffer is its first half
+  // what a pick collects (of 16 bytes in the merge), then the warps' lists
+  __shared__ __align__(16) Cand<float> shared[kCollect + kThreads / 32 * (kHold + kPer * 32)];
+  Cand<double> *buf_d = reinterpret_cast<Cand<double> *>(shared);
   __shared__ Cand<double> out_d[kMaxPick];
   __shared__ double logz[kMaxBeams], start[kMaxBeams];
   __shared__ float topb[kMaxBeams];
   __shared__ float redf[kThreads / 32];
   __shared__ double redd[kThreads / 32];
-  __shared__ uint32_t ticket;
-  const uint32_t t = threadIdx.x, slice = blockIdx.x, row = blockIdx.y, prompt = row / p.beams;
+  __shared__ uint32_t ticket, counts[kThreads / 32];
+  const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5, slice = blockIdx.x, row = blockIdx.y, prompt = row / p.beams;
   const uint32_t M = p.n_out;
   const uint64_t slot = (uint64_t)row * p.slices + slice;
   const bool done = p.done && p.done[row] != 0;
   if (!done) {
-    const uint32_t lo = slice * p.per, hi = min(p.vocab, lo + p.per);
+    Cand<float> *buf = reinterpret_cast<Cand<float> *>(shared), *list = buf + kCollect + warp * (kHold + kPer * 32);
+    Cand<float> *out = reinterpret_cast<Cand<float> *>(out_d);
+    const uint32_t begin = slice * p.per, hi = min(p.vocab, begin + p.per);
     const float *x = p.logits + (uint64_t)row * p.stride;
-    float v[kPer];
-    float most = -INFINITY;
-    const bool wide = (((uintptr_t)x | (lo * 4ull)) & 15) == 0;
-    // thread t has logits lo + 4t .. +3, then 1024 further on: index of v[e] = lo + (e/4) 1024 + 4t + e%4
+    const bool wide = ((uintptr_t)x & 15) == 0;
+    // thread t has logits lo + 4t .. +3 of a tile, then 1024 further on: v[e] is logit lo + (e/4) 1024 + 4t + e%4
+    float v[kPer], ahead[kPer];
+    auto load = [&](uint32_t lo) {
 #pragma unroll
-    for (uint32_t e = 0; e < kPer; e += 4) {
-      const uint32_t i = lo + (e / 4) * (kThreads * 4) + 4 * t;
-      if (wide && i + 4 <= hi) {
-        const float4 f = __ldcs(reinterpret_cast<const float4 *>(x + i));
-        v[e] = f.x, v[e + 1] = f.y, v[e + 2] = f.z, v[e + 3] = f.w;
-      } else {
+      for (uint32_t e = 0; e < kPer; e += 4) {
+        const uint32_t i = lo + (e / 4) * (kThreads * 4) + 4 * t;
+        if (wide && i + 4 <= hi) {
+          const float4 f = __ldcs(reinterpret_cast<const float4 *>(x + i));
+          ahead[e] = f.x, ahead[e + 1] = f.y, ahead[e + 2] = f.z, ahead[e + 3] = f.w;
+        } else {
 #pragma unroll
-        for (uint32_t q = 0; q < 4; q++) v[e + q] = i + q < hi ? x[i + q] : -INFINITY;
+          for (uint32_t q = 0; q < 4; q++) ahead[e + q] = i + q < hi ? x[i + q] : -INFINITY;
+        }
+      }
+    };
+    load(begin);
+    float m = -INFINITY;         // the thread's maximum so far
+    float c = -INFINITY;         // what its sum is relative to: m - 2 < c <= m
+    double z = 0.0;              // sum of e^(x - c)
+    float bar = -FLT_MAX;        // M logits of earlier tiles are above or equal but earlier: a later one has to reach it
+    uint32_t n = 0, held = 0;    // the slice's best at the end; entries of the warp's list
+    for (uint32_t lo = begin; lo < hi; lo += kTile) {
+      float most = -INFINITY, quad[kPer / 4];
+#pragma unroll
+      for (uint32_t e = 0; e < kPer; e++) {
+        v[e] = fmaxf(ahead[e], -INFINITY);  // drops NaN, which counts as -inf
+        quad[e / 4] = e % 4 ? fmaxf(quad[e / 4], v[e]) : v[e];
+      }
+#pragma unroll
+      for (uint32_t g = 0; g < kPer / 4; g++) most = fmaxf(most, quad[g]);
+      const bool last = hi - lo <= kTile;
+      if (!last) load(lo + kTile);
+      m = fmaxf(m, most);
+      if (most > c + 2.0f) {
+        z *= exp2_fast((c - most) * kLog2e);
+        c = most;
+      }
+      float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (c == INFINITY) {
+#pragma unroll
+        for (uint32_t e = 0; e < kPer; e++) part[e & 3] += v[e] == INFINITY ? 1.0f : 0.0f;
+      } else if (c > -INFINITY) {
+#pragma unroll
+        for (uint32_t e = 0; e < kPer; e++) part[e & 3] += exp2_fast((v[e] - c) * kLog2e);
+      }
+      z += (part[0] + part[1]) + (part[2] + part[3]);
+      if (lo != begin && !last) {  // what passes the bar joins the warp's list
+        if (!__any_sync(0xffffffffu, most >= bar)) continue;
+        if (most >= bar) {
+#pragma unroll
+          for (uint32_t e = 0; e < kPer; e++)
+            if (v[e] >= bar) list[atomicAdd(&counts[warp], 1u)] = Cand<float>{v[e], lo + (e / 4) * (kThreads * 4) + 4 * t + e % 4};
+        }
+        __syncwarp();
+        held = *(volatile uint32_t *)&counts[warp];
+        if (held > kHold) {
+          bar = above(warp_keep(list, held, M)), held = M;
+          if (lane == 0) counts[warp] = M;
+        }
+        __syncwarp();
+        continue;
+      }
+      // the M best of the lists and of this tile
+      for (uint32_t a = lane; a < held; a += 32) most = fmaxf(most, list[a].v);
+      n = block_pick<float>(
+          M, most,
+          [&](auto f) {
+#pragma unroll
+            for (uint32_t e = 0; e < kPer; e++) f(v[e], lo + (e / 4) * (kThreads * 4) + 4 * t + e % 4);
+            for (uint32_t a = lane; a < held; a += 32) f(list[a].v, list[a].i);
+          },
+          out, buf);
+      if (!last) {
+        bar = n == M ? above(out[M - 1].v) : -FLT_MAX;
+        held = n > warp ? (n - warp + kThreads / 32 - 1) / (kThreads / 32) : 0;
+        if (lane == 0) counts[warp] = held;
+        if (lane < held) list[lane] = out[lane * (kThreads / 32) + warp];
+        __syncwarp();
       }
     }
-#pragma unroll
-    for (uint32_t e = 0; e < kPer; e++) {
-      if (v[e] != v[e]) v[e] = -INFINITY;  // NaN counts as -inf
-      most = fmaxf(most, v[e]);
-    }
-    float m = warp_max(most);
-    if ((t & 31) == 0) redf[t >> 5] = m;
-    __syncthreads();
-#pragma unroll
-    for (uint32_t w = 0; w < kThreads / 32; w++) m = fmaxf(m, redf[w]);
-    // the exponentials of a thread's 32 logits in 32 bits, their sums over threads in 64
-    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (m > -INFINITY) {
-#pragma unroll
-      for (uint32_t e = 0; e < kPer; e++)
-        part[e & 3] += v[e] == m ? 1.0f : exp2_fast((v[e] - m) * 1.4426950408889634f);
-    }
-    const float s = (part[0] + part[1]) + (part[2] + part[3]);
-    double sd = s;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sd += __shfl_xor_sync(0xffffffffu, sd, o);
-    if ((t & 31) == 0) redd[t >> 5] = sd;
-    __syncthreads();
-    if (t == 0) {
-      double z = 0.0;
-      for (uint32_t w = 0; w < kThreads / 32; w++) z += redd[w];
-      p.top[slot] = m;
-      p.sum[slot] = (float)z;
-    }
-    Cand<float> *buf = reinterpret_cast<Cand<float> *>(buf_d), *out = reinterpret_cast<Cand<float> *>(out_d);
-    const uint32_t n = block_pick<float>(
-        M, most,
-        [&](auto f) {
-#pragma unroll
-          for (uint32_t e = 0; e < kPer; e++) f(v[e], lo + (e / 4) * (kThreads * 4) + 4 * t + e % 4);
-        },
-        out, buf);
     for (uint32_t k = t; k < M; k += kThreads) {
       p.val[slot * M + k] = k < n ? out[k].v : -INFINITY;
       p.idx[slot * M + k] = k < n ? out[k].i : 0;
+    }
+    const float mt = warp_top(m);
+    if ((t & 31) == 0) redf[t >> 5] = mt;
+    __syncthreads();
+    m = redf[0];
+#pragma unroll
+    for (uint32_t w = 1; w < kThreads / 32; w++) m = fmaxf(m, redf[w]);
+    if (c != m) z *= exp2_fast((c - m) * kLog2e);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+    if ((t & 31) == 0) redd[t >> 5] = z;
+    __syncthreads();
+    if (t == 0) {
+      z = 0.0;
+      for (uint32_t w = 0; w < kThreads / 32; w++) z += redd[w];
+      p.top[slot] = m;
+      p.sum[slot] = (float)z;
     }
   }
   // the last CTA of the prompt merges
@@ -233,8 +318,7 @@ __global__ void __launch_bounds__(kThreads) k_beam_select(BeamParams p) {
   if (ticket != p.beams * p.slices - 1) return;
   __threadfence();
   const uint64_t row0 = (uint64_t)prompt * p.beams;
-  for (uint32_t b = t / 32; b < p.beams; b += kThreads / 32) {  // a warp a beam, its slices in order
-    const uint32_t lane = t & 31;
+  for (uint32_t b = warp; b < p.beams; b += kThreads / 32) {  // a warp a beam, its slices in order
     const uint64_t r = (row0 + b) * p.slices;
     const bool over = p.done && p.done[row0 + b] != 0;
     float m = -INFINITY;
@@ -256,28 +340,31 @@ __global__ void __launch_bounds__(kThreads) k_beam_select(BeamParams p) {
     }
   }
   __syncthreads();
-  // candidates: beam b's kept logits, or the one of a finished beam, as (score, b * vocab + token)
+  // Candidates: beam b's kept logits, or the one of a finished beam, as (score, b * vocab + token).
+  // Candidate c is the k-th of a beam's slice, slices fastest and k slowest, and neighbours go to different warps: so
+  // every warp has a part of each beam's best, and its maxima are a bound that few others reach.
+  const uint32_t mine = (t & 31) * (kThreads / 32) + (((t >> 5) + t) & (kThreads / 32 - 1));
   const uint32_t per = p.slices * M, all = p.beams * per;
   auto score = [&](uint32_t c, double &sc, uint32_t &flat) {
-    const uint32_t b = c / per, k = c % per;
+    const uint32_t b = c / p.slices % p.beams, k = c / p.slices / p.beams, at = (b * p.slices + c % p.slices) * M + k;
     sc = ninf<double>();
     flat = 0;
     if (logz[b] != logz[b]) {
-      if (k == 0) {
+      if (at == b * per) {
         sc = start[b];
         flat = b * p.vocab + (uint32_t)p.pad;
       }
     } else {
-      const float x = __ldcg(&p.val[row0 * per + c]);
+      const float x = __ldcg(&p.val[row0 * per + at]);
       if (x > -INFINITY) {
         sc = start[b] + ((x == topb[b] ? 0.0 : (double)x - (double)topb[b]) - logz[b]);
-        flat = b * p.vocab + __ldcg(&p.idx[row0 * per + c]);
+        flat = b * p.vocab + __ldcg(&p.idx[row0 * per + at]);
       }
     }
     if (sc != sc) sc = ninf<double>();
   };
   float most = -INFINITY;
-  for (uint32_t c = t; c < all; c += kThreads) {
+  for (uint32_t c = mine; c < all; c += kThreads) {
     double sc;
     uint32_t flat;
     score(c, sc, flat);
@@ -286,7 +373,7 @@ __global__ void __launch_bounds__(kThreads) k_beam_select(BeamParams p) {
   const uint32_t n = block_pick<double>(
       M, most,
       [&](auto f) {
-        for (uint32_t c = t; c < all; c += kThreads) {
+        for (uint32_t c = mine; c < all; c += kThreads) {
           double sc;
           uint32_t flat;
           score(c, sc, flat);
@@ -331,8 +418,11 @@ extern "C" pai_status_t pai_b200_beam_select_f32(pai_b200_ctx_t *ctx, uint64_t p
   p.logits = logits, p.scores = scores, p.done = done, p.stride = stride, p.pad = pad;
   p.beams = (uint32_t)beams, p.vocab = (uint32_t)vocab, p.n_out = (uint32_t)n_out;
   const uint64_t rows = prompts * beams;
-  p.slices = (uint32_t)((vocab + kSlice - 1) / kSlice);
-  p.per = kSlice;
+  // slices of whole tiles, as many as the CTAs that the GPU holds at a time leave for a row
+  const uint64_t tiles = (vocab + kTile - 1) / kTile;
+  const uint64_t share = std::clamp<uint64_t>((uint64_t)kCtasPerSm * kSms / rows, 1, tiles);
+  p.per = (uint32_t)((tiles + share - 1) / share) * kTile;
+  p.slices = (uint32_t)((vocab + p.per - 1) / p.per);
   p.out_scores = out_scores, p.out_parents = out_parents, p.out_tokens = out_tokens;
   const CtxDeviceGuard on(ctx);
   if (on.status()) return on.status();

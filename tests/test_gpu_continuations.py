@@ -562,9 +562,10 @@ def beam_reference(logits, scores, done, pad, n_out):
     return cand, order
 
 
-# exp of a logit as 2^((x - m) log2 e): x - m, the product and the constant are off by 2^-24, 2^-24 and 2^-25 of |x - m|,
-# whose mean under the weights is at most log(vocab) < 12: 30 * 2^-24; 2^-22 for 2^x; 10 additions in 32 bits; the
-# slice's sum is rounded to 32 bits: 45 * 2^-24 in log Z, below 2^-18. The score is rounded once more.
+# exp of a logit as 2^((x - c) log2 e), c a thread's value up to 2 from its maximum: x - c, the product and the constant
+# are off by 2^-24, 2^-24 and 2^-25 of |x - c|, whose mean under the weights is at most log(vocab) + 4 < 16: 40 * 2^-24;
+# 2^-22 for 2^x, twice; 6 additions in 32 bits; the slice's sum is rounded to 32 bits: 55 * 2^-24 in log Z, below 2^-18.
+# The score is rounded once more.
 def beam_tol(s):
     return 2.0 ** -18 + 2.0 ** -24 * np.abs(s)
 
@@ -623,6 +624,37 @@ def test_beams_of_equal_scores(dev, vocab):
     scores[:, 1:] = -np.inf
     gs, gp, gt = check_beams(dev, logits, scores, None, 0, 5)
     assert gp[0].tolist() == [0] * 5
+
+
+@pytest.mark.parametrize("pick", [1, 16, 64])
+@pytest.mark.parametrize("kind", ["random", "rising", "falling", "equal", "masked", "steps", "lowest"])
+def test_beams_of_many_rows(dev, kind, pick):
+    """Rows enough that a CTA goes through a whole vocabulary: every way in which later logits meet the earlier best."""
+    prompts, beams, vocab = 150, 4, 13001
+    rng = np.random.default_rng(pick)
+    x = np.arange(vocab)
+    if kind == "random":
+        logits = rng.standard_normal((prompts, beams, vocab))
+    elif kind == "rising":
+        logits = np.broadcast_to(x / 1024.0, (prompts, beams, vocab))
+    elif kind == "falling":
+        logits = np.broadcast_to(-x / 1024.0, (prompts, beams, vocab))
+    elif kind == "equal":
+        logits = np.full((prompts, beams, vocab), -2.5)
+    elif kind == "masked":
+        logits = np.where(rng.random((prompts, beams, vocab)) < 0.002, rng.standard_normal((prompts, beams, vocab)), -np.inf)
+        logits[7] = -np.inf
+        logits[8, :, :9000] = np.nan
+        logits[9, 1, 12000:12003] = np.inf
+    elif kind == "lowest":  # masks of the type's lowest value: candidates like any others
+        lowest = np.finfo(np.float32).min
+        logits = np.where(rng.random((prompts, beams, vocab)) < 0.0002, rng.standard_normal((prompts, beams, vocab)), lowest)
+        logits[3, :, :8192] = -np.inf
+        logits[4] = np.where(x > 9000, lowest, -np.inf)
+    else:  # equal values within a tile, larger ones in the next
+        logits = np.broadcast_to((x // 4096).astype(float), (prompts, beams, vocab))
+    scores = (-rng.random((prompts, beams))).astype(np.float32)
+    check_beams(dev, np.ascontiguousarray(logits, np.float32), scores, None, 1, pick)
 
 
 def test_beams_with_masked_and_infinite_logits(dev):
