@@ -429,8 +429,11 @@ __device__ __forceinline__ void note_unit(const TreeParams &p, const Segment &g)
 }
 
 // Join the parts of the units that several chunks shared: CTA (unit, 8 rows), a thread 4 dims of a row. Parts lie
-// [row][hd] (BY_ROW) or [hd / 4][row] float4, as the kernels have them.
-constexpr uint32_t kJoinRows = 8;
+// [row][hd] (BY_ROW) or [hd / 4][row] float4, as the kernels have them. What it takes (4.7 us by itself for a row of each
+// of 64 units, 14 for 64 nodes of 8 sequences with 18 MB of parts) is the latency of loads that need one another: so the
+// first 8 parts of a row are under way while the maxima and sums are read (90.1 to 89.0 us for one token at 131072;
+// 4 or 16 parts, or 4 rows a CTA, are slower for one of few and many parts).
+constexpr uint32_t kJoinRows = 8, kJoinParts = 8;
 template <int HD, uint32_t MR, bool BY_ROW>
 __global__ void __launch_bounds__(kJoinRows * HD / 4) k_attn_tree_join(TreeParams p) {
   pdl_trigger();
@@ -439,13 +442,24 @@ __global__ void __launch_bounds__(kJoinRows * HD / 4) k_attn_tree_join(TreeParam
   __shared__ float inv[kJoinRows];
   const uint32_t unit = blockIdx.x, block = unit % p.max_blocks, kvh = unit / p.max_blocks % p.c.hk;
   const uint32_t s = unit / p.max_blocks / p.c.hk, row0 = blockIdx.y * kJoinRows, t = threadIdx.x;
+  const uint2 made = reinterpret_cast<const uint2 *>(p.units)[unit];  // on its way together with the sequence's
   const SeqWork w = seq_work<MR, kTcTile>(p, s);
   if (block >= w.blocks) return;
   const uint32_t rows = min(MR, w.nodes * p.g - block * MR);
-  const uint32_t parts = min(p.units[2 * unit], kTcGrid), first = p.units[2 * unit + 1];
+  const uint32_t parts = min(made.x, kTcGrid), first = made.y;
   if (parts == 0 || row0 >= rows) return;
   auto slot = [&](uint32_t q) -> size_t { return q == 0 ? first : (first & ~1u) + 2 * q; };
   const uint32_t n = min(kJoinRows, rows - row0), warps = kJoinRows * HD / 128, lane = t & 31;
+  const uint32_t r = BY_ROW ? t / (HD / 4) : t % kJoinRows, d4 = BY_ROW ? t % (HD / 4) : t / kJoinRows;
+  float4 f[kJoinParts];
+  auto load = [&](uint32_t q0) {
+#pragma unroll
+    for (uint32_t u = 0; u < kJoinParts; u++)
+      if (q0 + u < parts)
+        f[u] = *reinterpret_cast<const float4 *>(p.part_o + (BY_ROW ? (slot(q0 + u) * MR + row0 + r) * HD + 4 * d4
+                                                                    : ((slot(q0 + u) * (HD / 4) + d4) * MR + row0 + r) * 4));
+  };
+  if (r < n) load(0);  // together with the maxima and sums
   for (uint32_t r = t >> 5; r < n; r += warps) {
     float M = -INFINITY;
     for (uint32_t q = lane; q < parts; q += 32) {
@@ -463,23 +477,19 @@ __global__ void __launch_bounds__(kJoinRows * HD / 4) k_attn_tree_join(TreeParam
     if (lane == 0) inv[r] = L != 0.0f ? 1.0f / L : 0.0f;
   }
   __syncthreads();
-  const uint32_t r = BY_ROW ? t / (HD / 4) : t % kJoinRows, d4 = BY_ROW ? t % (HD / 4) : t / kJoinRows;
   if (r >= n) return;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (uint32_t q0 = 0; q0 < parts; q0 += 8) {
-    float4 f[8];
+  for (uint32_t q0 = 0;;) {
 #pragma unroll
-    for (int u = 0; u < 8; u++)
-      if (q0 + u < parts)
-        f[u] = *reinterpret_cast<const float4 *>(p.part_o + (BY_ROW ? (slot(q0 + u) * MR + row0 + r) * HD + 4 * d4
-                                                                          : ((slot(q0 + u) * (HD / 4) + d4) * MR + row0 + r) * 4));
-#pragma unroll
-    for (int u = 0; u < 8; u++)
+    for (uint32_t u = 0; u < kJoinParts; u++)
       if (q0 + u < parts) {
         const float y = ws[r][q0 + u];
         acc.x = fmaf(f[u].x, y, acc.x), acc.y = fmaf(f[u].y, y, acc.y);
         acc.z = fmaf(f[u].z, y, acc.z), acc.w = fmaf(f[u].w, y, acc.w);
       }
+    q0 += kJoinParts;
+    if (q0 >= parts) break;
+    load(q0);
   }
   const uint32_t rr = block * MR + row0 + r;
   const float y = inv[r];
