@@ -422,7 +422,10 @@ pai_status_t pai_b200_rope_append_f16kv(pai_b200_ctx_t *ctx, const pai_b200_kv_v
  * nothing gets zeros. Non-finite K or V rows make the rows that attend them
  * non-finite and no others. Results match fp32 arithmetic to about 1e-6
  * relative: K and V enter the tensor cores as stored, q and the softmax
- * weights as two fp16 parts each. The same call gives the same bits. */
+ * weights as two fp16 parts each. The same call gives the same bits.
+ * PAI_ERR_UNSUPPORTED when the sequences' rows and the positions that the
+ * tables allow make more than 2^31 tiles. A device wait that runs out is
+ * reported by pai_b200_sync, as everywhere. */
 pai_status_t pai_b200_attn_tree_f16kv(pai_b200_ctx_t *ctx, const pai_b200_kv_view_t *kv, uint32_t layer, uint64_t h,
                                       uint64_t rows, uint32_t max_nodes, const int32_t *lens,
                                       const int32_t *node_off, const uint64_t *mask, const float *q, float *out);

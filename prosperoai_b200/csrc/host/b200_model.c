@@ -424,6 +424,8 @@ struct pai_b200_session {
   uint8_t *dr_dev, *dr_host;
   int32_t *dr_parents; /* host: the nodes of the last verification */
   uint32_t dr_nodes;   /* ... and their number; 0: none that can be accepted */
+  pai_b200_graph_t *dr_graph; /* a verification's kernels for dr_shape nodes, once that many came twice in a row */
+  uint32_t dr_shape;
   int beam_ready;      /* the logits belong to the position, and no selection has used them */
 };
 
@@ -704,6 +706,7 @@ pai_status_t pai_b200_session_destroy(pai_b200_session_t *s) {
   pai_b200_free(ctx, s->dr_logits);
   pai_b200_free(ctx, s->dr_dev);
   pai_b200_host_free(ctx, s->dr_host);
+  pai_b200_graph_destroy(s->dr_graph);
   free(s->dr_parents);
   free(s);
   return PAI_OK;
@@ -1050,17 +1053,28 @@ pai_status_t pai_b200_session_kv_view(const pai_b200_session_t *s, pai_b200_kv_v
   return PAI_OK;
 }
 
-/* The layers over `rows` drafted rows in pf_x, the nodes' K/V appended behind the position. */
-static pai_status_t draft_layers(pai_b200_session_t *s, uint32_t rows, uint32_t n) {
+/* A verification's kernels: embedding, the layers over the drafted rows (the
+ * nodes' K/V appended behind the position), every row's greedy token. What
+ * they work on lies on the device, so a captured run serves every call of as
+ * many nodes. */
+static pai_status_t draft_kernels(pai_b200_session_t *s, uint32_t n) {
   pai_b200_model_t *m = s->m;
   pai_b200_ctx_t *ctx = m->ctx;
   const pai_b200_model_cfg_t *c = &m->cfg;
-  const uint32_t E = c->n_embd;
+  const uint32_t E = c->n_embd, rows = s->batch * n;
+  const int gemm = s->pf_gemm;
   const int32_t *lens = (const int32_t *)(s->dr_dev + DR_LENS), *off = (const int32_t *)(s->dr_dev + DR_OFF);
   const int32_t *depth = (const int32_t *)(s->dr_dev + DR_DEPTH);
   const uint64_t *mask = (const uint64_t *)(s->dr_dev + DR_MASK);
   pai_b200_kv_view_t kv;
   pai_status_t st = pai_b200_session_kv_view(s, &kv);
+  if (!st) st = b200_launch_embed(ctx, c->etype, rows, c->vocab, E, m->tok_embd, s->pf_tok, s->pf_x);
+  /* Up to 8 rows one GEMV of the decode step reads the weights once, as the
+   * GEMM does, and without rounding the rows to bf16. Whole verifications of
+   * 1, 4, 8, 9 and 16 rows (8 layers of width 4096, Q4_0, 128256 tokens), not
+   * captured: GEMV 1108, 1278, 1689, 2400 and 2882 us, GEMM 1643, 1675, 1801,
+   * 1832 and 1925. */
+  if (rows <= 8) s->pf_gemm = 0;
   for (uint32_t l = 0; !st && l < c->n_layer; l++) {
     st = b200_launch_rmsnorm_xq(ctx, rows, E, s->pf_x, m->attn_norm[l], c->eps, s->pf_xn, NULL);
     if (!st) st = rows_matmul(s, c->wtype, rows, m->n_qkv, E, m->wqkv[l], s->pf_xn, s->pf_qkv, B200_EPI_STORE);
@@ -1073,6 +1087,15 @@ static pai_status_t draft_layers(pai_b200_session_t *s, uint32_t rows, uint32_t 
     if (!st) st = rows_matmul(s, c->wtype, rows, 2ull * m->ffl, E, m->wgu[l], s->pf_xn, s->pf_h, B200_EPI_SILU_GLU);
     if (!st) st = rows_matmul(s, c->wtype, rows, E, m->ffl, m->wdown[l], s->pf_h, s->pf_x, B200_EPI_RESIDUAL);
   }
+  s->pf_gemm = gemm;
+  /* lm head and greedy token of every row, 8 rows at a time */
+  for (uint32_t r = 0; !st && r < rows; r += 8) {
+    const uint32_t g = rows - r < 8 ? rows - r : 8;
+    b200_xq_t xq = b200_xq_view(s->pf_xq_buf, g, E);
+    st = b200_launch_rmsnorm_xq(ctx, g, E, s->pf_x + (uint64_t)r * E, m->output_norm, c->eps, NULL, &xq);
+    if (!st) st = b200_launch_gemv(ctx, c->etype, g, m->vl, E, m->output, &xq, NULL, s->dr_logits, B200_EPI_STORE, NULL);
+    if (!st) st = b200_launch_argmax(ctx, g, m->vl, s->dr_logits, (int32_t *)(s->dr_dev + DR_NEXT) + r);
+  }
   return st;
 }
 
@@ -1082,8 +1105,7 @@ pai_status_t pai_b200_session_verify(pai_b200_session_t *s, const int32_t *token
   pai_b200_model_t *m = s->m;
   pai_b200_ctx_t *ctx = m->ctx;
   const pai_b200_model_cfg_t *c = &m->cfg;
-  const uint32_t B = s->batch, E = c->n_embd, words = (n + 63) / 64;
-  const int gemm = s->pf_gemm;
+  const uint32_t B = s->batch, words = (n + 63) / 64;
   pai_status_t st = one_gpu(s, "session_verify");
   if (st) return st;
   if (n > DR_MAX_NODES || (uint64_t)B * n > PF_MAX_ROWS)
@@ -1125,21 +1147,25 @@ pai_status_t pai_b200_session_verify(pai_b200_session_t *s, const int32_t *token
   st = dr_up(s, 0, DR_DEPTH + rows * 4ull);
   if (!st) st = dr_up(s, DR_MASK, (uint64_t)rows * words * 8);
   if (!st) st = pai_b200_memcpy_h2d(ctx, s->pf_tok, s->pf_htok, rows * 4ull);
-  if (!st) st = b200_launch_embed(ctx, c->etype, rows, c->vocab, E, m->tok_embd, s->pf_tok, s->pf_x);
-  /* Up to 8 rows one GEMV of the decode step reads the weights once, as the
-   * GEMM does, and without rounding the rows to bf16. Whole verifications of
-   * 1, 4, 8, 9 and 16 rows (8 layers of width 4096, Q4_0, 128256 tokens): GEMV
-   * 1108, 1278, 1689, 2400 and 2882 us, GEMM 1643, 1675, 1801, 1832 and 1925. */
-  if (rows <= 8) s->pf_gemm = 0;
-  if (!st) st = draft_layers(s, rows, n);
-  s->pf_gemm = gemm;
-  /* lm head and greedy token of every row, 8 rows at a time */
-  for (uint32_t r = 0; !st && r < rows; r += 8) {
-    const uint32_t g = rows - r < 8 ? rows - r : 8;
-    b200_xq_t xq = b200_xq_view(s->pf_xq_buf, g, E);
-    st = b200_launch_rmsnorm_xq(ctx, g, E, s->pf_x + (uint64_t)r * E, m->output_norm, c->eps, NULL, &xq);
-    if (!st) st = b200_launch_gemv(ctx, c->etype, g, m->vl, E, m->output, &xq, NULL, s->dr_logits, B200_EPI_STORE, NULL);
-    if (!st) st = b200_launch_argmax(ctx, g, m->vl, s->dr_logits, (int32_t *)(s->dr_dev + DR_NEXT) + r);
+  /* the launches of 8 layers cost 220 to 300 us more than a replay of them: 1
+   * row 1108 against 890 us, 4 rows 1278 and 1046, 16 rows 1925 and 1622 */
+  if (!st && s->dr_shape != n) {
+    pai_b200_graph_destroy(s->dr_graph);
+    s->dr_graph = NULL;
+    s->dr_shape = 0;
+    st = draft_kernels(s, n); /* sizes the scratch too */
+    if (!st) s->dr_shape = n;
+  } else if (!st) {
+    if (!s->dr_graph) {
+      st = pai_b200_graph_begin(ctx);
+      if (!st) {
+        const pai_status_t kst = draft_kernels(s, n);
+        st = pai_b200_graph_end(ctx, &s->dr_graph);
+        if (kst) st = kst;
+      }
+      if (st) s->dr_shape = 0;
+    }
+    if (!st) st = pai_b200_graph_launch(ctx, s->dr_graph);
   }
   if (!st) st = pai_b200_memcpy_d2h(ctx, s->dr_host + DR_NEXT, s->dr_dev + DR_NEXT, rows * 4ull);
   if (!st) st = seen(s, pai_b200_sync(ctx));

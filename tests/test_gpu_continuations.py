@@ -736,3 +736,103 @@ def test_drafts_and_beams_over_shared_pages(dev):
             host_lens[s] += len(p)
         dev.kv_accept(cache.view, most, lens, dev.put(path), dev.put(i32([len(p) for p in paths])), lens)
         assert lens.download(np.int32).tolist() == host_lens
+
+
+def test_a_beam_step_captured_and_replayed(dev):
+    """Selection, fork and attention as one graph: every replay works on what lies on the device then."""
+    rng = np.random.default_rng(31)
+    L = _native.load()
+    beams, vocab, hd, page = 4, 5003, 64, 16
+    lens = [20, 20, 20, 20]
+    cache = Cache(dev, rng, lens, page, 1, hd, layers=2, spare=8, max_pages=3)
+    start = dict(k=cache.k.copy(), v=cache.v.copy(), table=cache.table.copy())
+    logits, scores = dev.alloc(4 * beams * vocab), dev.alloc(4 * beams)
+    out = [dev.alloc(4 * beams) for _ in range(3)]
+    dl, grow, table2 = dev.put(i32(lens)), dev.put(i32([3] * beams)), dev.alloc(4 * beams * cache.max_pages)
+    lens2, granted = dev.alloc(4 * beams), dev.alloc(4 * beams)
+    after = KvView.from_buffer_copy(cache.view)
+    after.table = table2.ptr
+    q = rng.standard_normal((beams, 2, hd)).astype(np.float32)
+    off, dq, att = dev.put(i32(range(beams + 1))), dev.put(q), dev.alloc(q.nbytes)
+
+    def step():
+        dev.beam_select(1, beams, vocab, logits, vocab, scores, None, 0, beams, *out)
+        dev.kv_fork(cache.view, 0, dl, out[1], grow, table2, lens2, granted)
+        dev.attn_tree(after, 1, 2, beams, 1, lens2, off, None, dq, att)
+
+    logits.upload(np.zeros((beams, vocab), np.float32))
+    scores.upload(np.zeros(beams, np.float32))
+    step()  # sizes the scratch
+    dev.sync()
+    g = C.c_void_p()
+    _native.check(L.pai_b200_graph_begin(dev.ctx), "begin")
+    step()
+    _native.check(L.pai_b200_graph_end(dev.ctx, C.byref(g)), "end")
+    try:
+        for turn in range(3):
+            cache.k, cache.v, cache.table = start["k"].copy(), start["v"].copy(), start["table"].copy()
+            cache.put()
+            x = rng.standard_normal((1, beams, vocab)).astype(np.float32)
+            sc = (-rng.random((1, beams))).astype(np.float32)
+            logits.upload(x[0])
+            scores.upload(sc)
+            _native.check(L.pai_b200_graph_launch(dev.ctx, g), "launch")
+            got = out[1].download(np.int32)
+            cand, order = beam_reference(x, sc, None, 0, beams)
+            assert got.tolist() == (order[0] // vocab).tolist()
+            table, length, room, copies = fork_reference(cache, lens, got.tolist(), [3] * beams)
+            for src, dst, rows in copies:
+                for plane in (cache.k, cache.v):
+                    plane[:, dst, :, :rows * hd] = plane[:, src, :, :rows * hd]
+            assert table2.download(np.int32).reshape(beams, -1).tolist() == table
+            assert (lens2.download(np.int32).tolist(), granted.download(np.int32).tolist()) == (length, room)
+            cache.table = i32(table)
+            sees = [np.ones((1, 1), bool)] * beams
+            close(att.download(np.float32).reshape(q.shape), *attend(cache, 1, length, sees, q, 2))
+    finally:
+        dev.sync()
+        L.pai_b200_graph_destroy(g)
+
+
+def test_contexts_at_once():
+    """Two contexts, each on a thread of its own, give the bits that they give alone."""
+    import threading
+
+    from prosperoai_b200.api import Device
+
+    rng = np.random.default_rng(8)
+    shapes = [([700, 90], [1, 1]), ([260], [40])]
+    jobs = []
+    for lens, nodes in shapes:
+        d = Device(0)
+        cache = Cache(d, rng, [n + k for n, k in zip(lens, nodes)], 64, 2, 128)
+        rows = sum(nodes)
+        q = d.put(rng.standard_normal((rows, 8, 128)).astype(np.float32))
+        x = d.put(rng.standard_normal((rows, 9001)).astype(np.float32))
+        sc = d.put(np.zeros(rows, np.float32))
+        outs = [d.alloc(rows * 8 * 128 * 4)] + [d.alloc(4 * 8) for _ in range(3)]
+        off = d.put(i32(np.concatenate([[0], np.cumsum(nodes)])))
+        jobs.append((d, cache, d.put(i32(lens)), off, max(nodes), rows, q, x, sc, outs))
+
+    def work(job, times, results):
+        d, cache, lens, off, most, rows, q, x, sc, outs = job
+        for _ in range(times):
+            d.attn_tree(cache.view, 0, 8, rows, most, lens, off, None, q, outs[0])
+            d.beam_select(1, rows, 9001, x, 9001, sc, None, 0, 8, *outs[1:])
+        results.append([o.download(np.uint32) for o in outs])
+
+    alone, both = [], [[], []]
+    for job in jobs:
+        work(job, 1, alone)
+    threads = [threading.Thread(target=work, args=(job, 60, both[i])) for i, job in enumerate(jobs)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(alone, both):
+        for u, v in zip(a, b[0]):
+            np.testing.assert_array_equal(u, v)
+    for job in jobs:
+        for item in (job[1].dk, job[1].dv, job[1].dt, job[2], job[3], *job[6:9], *job[9]):
+            item.free()
+        job[0].close()

@@ -142,6 +142,31 @@ def test_drafts_of_drafts(model):
     s.close()
 
 
+@pytest.mark.parametrize("batch,n", [(1, 4), (2, 9)])
+def test_verifications_of_one_size_follow_their_inputs(model, batch, n):
+    """The second call of a size is captured and replayed from then on: tokens, trees and positions are those of each call."""
+    rng = np.random.default_rng(n)
+    vocab = model.cfg["vocab"]
+    history = rng.integers(0, vocab, (batch, 30))
+    s = Session(model, batch, 256)
+    s.prefill(history)
+    for turn in range(5):
+        draft = rng.integers(0, vocab, (batch, n))
+        parents = [-1] + [int(rng.integers(-1, i)) for i in range(1, n)] if turn else None
+        fresh = Session(model, batch, 256)
+        fresh.prefill(history[:, :30])
+        for i in range(30, history.shape[1]):
+            fresh.step(history[:, i])
+        got, want = s.verify(draft, parents), fresh.verify(draft, parents)
+        fresh.close()
+        np.testing.assert_array_equal(got, want)
+        if turn == 2:
+            s.verify(draft[:, :1])  # another size in between
+        s.step(draft[:, 0])
+        history = np.concatenate([history, draft[:, :1]], 1)
+    s.close()
+
+
 def log_softmax(x):
     x = x.astype(np.float64)
     return x - x.max(-1, keepdims=True) - np.log(np.exp(x - x.max(-1, keepdims=True)).sum(-1, keepdims=True))
