@@ -19,10 +19,10 @@
 // threads' maxima; the smallest of these is a bound that at least n_out
 // values reach, and few others, which are collected and ranked.
 //
-// 16 prompts of 8 beams of 128256, 16 kept (66 MB, 10 us): 30 us, of which the
+// 16 prompts of 8 beams of 128256, 16 kept (66 MB, 10 us): 27 us, of which the
 // reading and the exponentials 15, the first and last picks 5, the lists 4 and
-// the merge 6. One launch of 8192 logits a CTA, ranked there, took 40; a
-// barrier a tile 39; four CTAs on an SM instead of three (64 registers, which
+// the merge 3. Before the merge kept its scores in registers between its two
+// passes 30: 8192 logits a CTA, ranked there, took 40 then; a barrier a tile 39; four CTAs on an SM instead of three (64 registers, which
 // spill) 33; tiles of 2048 41; three tiles ahead in shared memory 35; the
 // lists by ballots 31.
 //
@@ -44,7 +44,7 @@ namespace {
 
 constexpr uint32_t kThreads = 256, kPer = 16, kTile = kThreads * kPer;  // logits of a CTA at a time: 16 registers a thread
 constexpr uint32_t kCtasPerSm = 3, kSms = 148;
-constexpr uint32_t kMaxPick = 64, kMaxBeams = 64, kCollect = 1024, kHold = 64;
+constexpr uint32_t kMaxPick = 64, kMaxBeams = 64, kMergeHold = 2, kCollect = 1024, kHold = 64;
 
 struct BeamParams {
   const float *logits, *scores;
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_beam_select(BeamParams
       p.idx[slot * M + k] = k < n ? out[k].i : 0;
     }
     const float mt = warp_top(m);
-    if ((t & 31) == 0) redf[t >> 5] = mt;
+    if (lane == 0) redf[warp] = mt;
     __syncthreads();
     m = redf[0];
 #pragma unroll
@@ -301,19 +301,20 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_beam_select(BeamParams
     if (c != m) z *= exp2_fast((c - m) * kLog2e);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-    if ((t & 31) == 0) redd[t >> 5] = z;
-    __syncthreads();
-    if (t == 0) {
-      z = 0.0;
-      for (uint32_t w = 0; w < kThreads / 32; w++) z += redd[w];
-      p.top[slot] = m;
-      p.sum[slot] = (float)z;
-    }
+    if (lane == 0) redd[warp] = z;
+    if (t == 0) p.top[slot] = m;
   }
   // the last CTA of the prompt merges
-  __threadfence();
   __syncthreads();
-  if (t == 0) ticket = atomicAdd(&p.cnt[prompt], 1u);
+  if (t == 0) {
+    if (!done) {
+      double z = 0.0;
+      for (uint32_t w = 0; w < kThreads / 32; w++) z += redd[w];
+      p.sum[slot] = (float)z;
+    }
+    __threadfence();  // behind the barrier: for what the whole CTA wrote
+    ticket = atomicAdd(&p.cnt[prompt], 1u);
+  }
   __syncthreads();
   if (ticket != p.beams * p.slices - 1) return;
   __threadfence();
@@ -321,20 +322,25 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_beam_select(BeamParams
   for (uint32_t b = warp; b < p.beams; b += kThreads / 32) {  // a warp a beam, its slices in order
     const uint64_t r = (row0 + b) * p.slices;
     const bool over = p.done && p.done[row0 + b] != 0;
+    const float first = p.scores[row0 + b];
     float m = -INFINITY;
     double z = 0.0;
     if (!over) {
-      for (uint32_t k = lane; k < p.slices; k += 32) m = fmaxf(m, __ldcg(&p.top[r + k]));
+      float mk = -INFINITY, sk = 0.0f;  // a lane's first slice, maximum and sum on their way at once
+      if (lane < p.slices) mk = __ldcg(&p.top[r + lane]), sk = __ldcg(&p.sum[r + lane]);
+      m = mk;
+      for (uint32_t k = lane + 32; k < p.slices; k += 32) m = fmaxf(m, __ldcg(&p.top[r + k]));
       m = warp_max(m);
-      for (uint32_t k = lane; k < p.slices; k += 32) {
-        const float mk = __ldcg(&p.top[r + k]);
-        if (mk > -INFINITY) z += (double)__ldcg(&p.sum[r + k]) * (mk == m ? 1.0 : exp((double)mk - (double)m));
+      for (uint32_t k = lane;;) {
+        if (mk > -INFINITY) z += (double)sk * (mk == m ? 1.0 : exp((double)mk - (double)m));
+        if ((k += 32) >= p.slices) break;
+        mk = __ldcg(&p.top[r + k]), sk = __ldcg(&p.sum[r + k]);
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
     }
     if (lane == 0) {
-      start[b] = p.scores[row0 + b];
+      start[b] = first;
       topb[b] = m;
       logz[b] = over ? NAN : log(z);  // NaN marks a finished beam
     }
@@ -363,8 +369,18 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_beam_select(BeamParams
     }
     if (sc != sc) sc = ninf<double>();
   };
+  // a thread's first ones stay in registers, so that their loads and divisions are made once
+  double kept[kMergeHold];
+  uint32_t flats[kMergeHold];
   float most = -INFINITY;
-  for (uint32_t c = mine; c < all; c += kThreads) {
+#pragma unroll
+  for (uint32_t u = 0; u < kMergeHold; u++) {
+    const uint32_t c = mine + u * kThreads;
+    kept[u] = ninf<double>(), flats[u] = 0;
+    if (c < all) score(c, kept[u], flats[u]);
+    most = fmaxf(most, (float)kept[u]);
+  }
+  for (uint32_t c = mine + kMergeHold * kThreads; c < all; c += kThreads) {
     double sc;
     uint32_t flat;
     score(c, sc, flat);
@@ -373,7 +389,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_beam_select(BeamParams
   const uint32_t n = block_pick<double>(
       M, most,
       [&](auto f) {
-        for (uint32_t c = mine; c < all; c += kThreads) {
+#pragma unroll
+        for (uint32_t u = 0; u < kMergeHold; u++) f(kept[u], flats[u]);
+        for (uint32_t c = mine + kMergeHold * kThreads; c < all; c += kThreads) {
           double sc;
           uint32_t flat;
           score(c, sc, flat);
