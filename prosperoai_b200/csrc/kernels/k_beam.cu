@@ -22,7 +22,8 @@
 // 16 prompts of 8 beams of 128256, 16 kept (66 MB, 10 us): 27 us, of which the
 // reading and the exponentials 15, the first and last picks 5, the lists 4 and
 // the merge 3. Before the merge kept its scores in registers between its two
-// passes 30: 8192 logits a CTA, ranked there, took 40 then; a barrier a tile 39; four CTAs on an SM instead of three (64 registers, which
+// passes it was 30; of that form, 8192 logits a CTA, ranked there, took 40; a
+// barrier a tile 39; four CTAs on an SM instead of three (64 registers, which
 // spill) 33; tiles of 2048 41; three tiles ahead in shared memory 35; the
 // lists by ballots 31.
 //
