@@ -2,19 +2,24 @@
 //
 // S = Q K^T (M = 128 rows, N = 128 positions, both fp16 parts of Q) and the tile's P V go to TMEM; P (both parts) is
 // written over S and is the A operand of P V, V, as it lies with hd contiguous, an MN-major B.
-//   warps 0-3, 4-7   softmax, a row a thread: the first four have a tile's positions 0-63, the others 64-127; the
-//                    row's maximum goes through shared memory. Then the P V of the tile before, which ran
-//                    meanwhile, is added to the running output in registers, half of the dims each.
-//   warp 8           issues the MMAs: Q K^T of tile i + 1 before P V of tile i, so that they overlap the softmax
-//   warps 12-15      K copies, V copies, cleaning by two
-// Registers: 512 threads at 128; setmaxnreg gives the softmax warps 200 and leaves 56 to the others (256 * 200 +
-// 256 * 56 = 65536, what the block was launched with).
+//   warps 0-15       softmax, a row a thread: every four of them have 32 of a tile's positions; the row's maximum goes
+//                    through shared memory. Then the P V of the tile before, which ran meanwhile, is added to the
+//                    running output in registers, 32 dims each.
+//   warp 16          issues the MMAs: Q K^T of tile i + 1 before P V of tile i, so that they overlap the softmax
+//   warps 17-19      K copies, V copies, cleaning
+// Registers: 640 threads at 96; setmaxnreg gives the softmax warps 104 and leaves 56 to the others (512 * 104 + 128 * 56
+// = 60416 of 61440, what the block was launched with).
+//
+// 8 sequences of 64 nodes x 4 heads a kv head at 32768 positions: 461-468 us on a box where it had 487-470 with 64
+// positions a thread (a second pass over the scores then, for want of registers); one tree of 16 at 4096 22.9 us, 24.7
+// then. With both parts that is 1.18 PFLOP/s, 0.72 of the dense rate in short bursts, and what the power limit leaves: the
+// same instructions on weights of random bits take 1.2 times as long, half of the products save 10 %.
 #pragma once
 #include "attn_tree_tc.cuh"
 
 namespace {
 
-constexpr uint32_t kManyThreads = 512, kManyRows = 128;
+constexpr uint32_t kManyGroups = 4, kManySoft = 128 * kManyGroups, kManyThreads = kManySoft + 128, kManyRows = 128;
 
 template <int HD>
 struct ManySmem {
@@ -26,8 +31,8 @@ struct ManySmem {
   uint32_t valid[8][4];          // positions of a tile that hold a row; a tile's words are read long before 8 tiles on
   uint32_t odd[8][4];            // its nodes with a non-finite V row
   float factor[kManyRows];
-  float top[2][2][kManyRows];      // [tile parity][warpgroup]: maxima of a row's halves
-  float ml[2][kManyRows];
+  float top[2][kManyRows][kManyGroups];  // [tile parity]: maxima of a row's quarters
+  float ml[kManyGroups][kManyRows];
   uint32_t upto[kMaxSeqs + 1];
   Ring ring;
   uint64_t kfull[2], kempty[2], vfull[2], vclean[2], vempty[2], sfull[2], pfull[2], ofull[2], qfull, drain;
@@ -40,26 +45,26 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   using Smem = ManySmem<HD>;
   extern __shared__ __align__(16) uint8_t raw[];
   Smem &sm = *reinterpret_cast<Smem *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-  constexpr uint32_t BL = Smem::kBlock;
+  constexpr uint32_t BL = Smem::kBlock, MMA = kManySoft / 32;  // first warp behind the softmax
   const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
   pdl_trigger();
   if (t == 0) {
     for (int i = 0; i < 2; i++) {
       mbar_init(&sm.kfull[i], 1);
       mbar_init(&sm.vfull[i], 1);
-      mbar_init(&sm.vclean[i], 2);
+      mbar_init(&sm.vclean[i], 1);
       mbar_init(&sm.kempty[i], 1);
       mbar_init(&sm.vempty[i], 1);
       mbar_init(&sm.sfull[i], 1);
-      mbar_init(&sm.pfull[i], 8);
+      mbar_init(&sm.pfull[i], MMA);
       mbar_init(&sm.ofull[i], 1);
     }
-    mbar_init(&sm.qfull, 8);
+    mbar_init(&sm.qfull, MMA);
     mbar_init(&sm.drain, 1);
     for (uint32_t i = 0; i < kRing; i++) mbar_init(&sm.ring.full[i], 1);
     fence_mbar_init();
   }
-  if (warp == 8) {
+  if (warp == MMA) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -72,18 +77,16 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   Segment g;
   Waiter wait{p.wait_ns, p.err};
 
-  if (warp >= 12) {
+  if (warp >= MMA) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 12)
+    if (warp == MMA + 1) {
       copy_tiles<HD, kManyRows, 2, true>(p, &kmap, sm.upto, sm.ring, sm.kt[0], sm.kfull, sm.kempty, sm.valid);
-    else if (warp == 13)
+    } else if (warp == MMA + 2) {
       copy_tiles<HD, kManyRows, 2, false>(p, &vmap, sm.upto, sm.ring, sm.vt[0], sm.vfull, sm.vempty, nullptr);
-    else
-      clean_tiles<HD, 2, 2>(p, sm.ring, warp - 14, sm.vt[0], sm.vfull, sm.vclean, sm.odd);
-  } else if (warp >= 8) {
-    // ---- MMA issue ----
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 8) {
+    } else if (warp == MMA + 3) {
+      clean_tiles<HD, 2, 1>(p, sm.ring, 0, sm.vt[0], sm.vfull, sm.vclean, sm.odd);
+    } else {
+      // ---- MMA issue ----
       const uint32_t leader = elect_one();
       const uint64_t qd = desc_k(smem_u32(sm.q[0])), kd = desc_k(smem_u32(sm.kt[0])), vd = desc_mn(smem_u32(sm.vt[0]), BL);
       constexpr uint64_t kPart = Smem::kTileBytes >> 4;  // from one part of Q, or one tile, to the next, in 16 bytes
@@ -135,39 +138,37 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       __syncwarp();
     }
   } else {
-    // ---- softmax: a thread a row, warpgroup wg half of the positions and half of the dims ----
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    // ---- softmax: a thread a row, warpgroup wg a quarter of the positions and 32 dims ----
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     const uint32_t wg = warp >> 2, r = t & 127;
     const uint32_t lanes = (warp & 3) * 32 << 16;
     uint32_t i = 0;
-    for (uint32_t seg = 0; next_segment<1, 256>(sm.ring, seg, wait, g); seg++) {
+    for (uint32_t seg = 0; next_segment<1, kManySoft>(sm.ring, seg, wait, g); seg++) {
       const uint32_t rows = min(kManyRows, g.nodes * p.g - g.block * kManyRows);
       // the last segment's products are done: Q may be written
-      put_queries<HD, kManyRows, 8>(p, g, rows, warp, sm.q[0], BL, Smem::kTileBytes, sm.factor);
+      put_queries<HD, kManyRows, MMA>(p, g, rows, warp, sm.q[0], BL, Smem::kTileBytes, sm.factor);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.qfull);
-      named_sync<1, 256>();
+      named_sync<1, kManySoft>();
       const float factor = sm.factor[r];
       const bool work = (warp & 3) * 32 < rows;  // a warp whose rows are all past the last one keeps step only
       const uint32_t rr = g.block * kManyRows + r, nd = rr / p.g;
       const bool live = r < rows;
-      float o[HD / 2], m = -INFINITY, l = 0.0f, corr = 1.0f;
+      float o[32], m = -INFINITY, l = 0.0f, corr = 1.0f;
 #pragma unroll
-      for (int d = 0; d < HD / 2; d++) o[d] = 0.0f;
-      // add the P V of tile n (the n-th of the run) to this thread's half of the dims; `tile` its number in the unit
+      for (int d = 0; d < 32; d++) o[d] = 0.0f;
+      // add the P V of tile n (the n-th of the run) to this thread's 32 dims; `tile` its number in the unit
       auto fold = [&](uint32_t n, uint32_t tile, uint64_t sees0, uint64_t sees1) {
+        if (wg >= HD / 32) return;  // no dims
         wait(&sm.ofull[n & 1], n >> 1);
         __syncwarp();
         tc_after();
         if (work) {
-          const uint32_t oa = tmem + lanes + 256 + 128 * (n & 1) + wg * (HD / 2);
-          uint32_t v[HD / 2];
+          uint32_t v[32];
+          tc_ld32(tmem + lanes + 256 + 128 * (n & 1) + wg * 32, v);
+          tc_ld_wait(v);
 #pragma unroll
-          for (int c = 0; c < HD / 64; c++) tc_ld32(oa + 32 * c, v + 32 * c);
-#pragma unroll
-          for (int c = 0; c < HD / 64; c++) tc_ld_wait(v + 32 * c);
-#pragma unroll
-          for (int d = 0; d < HD / 2; d++) o[d] = fmaf(o[d], corr, __uint_as_float(v[d]));
+          for (int d = 0; d < 32; d++) o[d] = fmaf(o[d], corr, __uint_as_float(v[d]));
           if ((tile + 1) * kTcTile > g.len) {
             // non-finite V elements of nodes that this row sees
 #pragma unroll 1
@@ -177,9 +178,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                    left &= left - 1) {
                 const int64_t at_row = kv_row(p.c, g.s, tile * kTcTile + 32 * x + __ffs(left) - 1);
                 const __half2 *vr =
-                    reinterpret_cast<const __half2 *>(p.c.v + (size_t)g.kvh * p.c.head_stride + at_row + wg * (HD / 2));
+                    reinterpret_cast<const __half2 *>(p.c.v + (size_t)g.kvh * p.c.head_stride + at_row + wg * 32);
 #pragma unroll
-                for (int d = 0; d < HD / 4; d++) {
+                for (int d = 0; d < 16; d++) {
                   const float2 f = __half22float2(vr[d]);
                   if (!isfinite(f.x)) o[2 * d] += f.x;
                   if (!isfinite(f.y)) o[2 * d + 1] += f.y;
@@ -192,16 +193,15 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       };
       uint64_t sees0 = 0, sees1 = 0;  // of the tile that is folded next
       for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
-        const uint32_t sa = tmem + lanes + 128 * (i & 1) + 64 * wg;
+        const uint32_t sa = tmem + lanes + 128 * (i & 1) + 32 * wg;
         wait(&sm.sfull[i & 1], i >> 1);
         __syncwarp();
         tc_after();
         float corr1 = 1.0f;
         uint64_t now0 = 0, now1 = 0;
         if (work) {
-          uint32_t v[64];
+          uint32_t v[32];
           tc_ld32(sa, v);
-          tc_ld32(sa + 32, v + 32);
           const bool drafted = (tile + 1) * kTcTile > g.len;
           const uint64_t ok0 = (uint64_t)sm.valid[i & 7][0] | (uint64_t)sm.valid[i & 7][1] << 32;
           const uint64_t ok1 = (uint64_t)sm.valid[i & 7][2] | (uint64_t)sm.valid[i & 7][3] << 32;
@@ -212,49 +212,36 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             now1 &= seen(p, tile * kTcTile + 64 - g.len, live, nd, g.first);
           }
           tc_ld_wait(v);
-          tc_ld_wait(v + 32);
           if (masked) {
-            const uint64_t bits = wg ? now1 : now0;
-            const uint32_t b0 = (uint32_t)bits, b1 = (uint32_t)(bits >> 32);
+            const uint32_t bits = (uint32_t)((wg < 2 ? now0 : now1) >> (32 * (wg & 1)));
 #pragma unroll
-            for (int e = 0; e < 64; e++)
-              if (!(((e < 32 ? b0 : b1) >> (e & 31)) & 1)) v[e] = 0xFF800000u;  // -inf, for the second pass too
-            tc_st32(sa, v);
-            tc_st32(sa + 32, v + 32);
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            for (int e = 0; e < 32; e++)
+              if (!((bits >> e) & 1)) v[e] = 0xFF800000u;  // -inf
           }
           float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int e = 0; e < 64; e += 8)
+          for (int e = 0; e < 32; e += 8)
 #pragma unroll
             for (int u = 0; u < 4; u++)
               t4[u] = fmaxf(t4[u], fmaxf(__uint_as_float(v[e + 2 * u]), __uint_as_float(v[e + 2 * u + 1])));
-          float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
-          // the row's other 64 positions are the other warpgroup's
-          sm.top[i & 1][wg][r] = top;
-          __syncwarp();
-          asm volatile("bar.sync %0, 64;" ::"r"(4 + (warp & 3)) : "memory");
-          top = fmaxf(top, sm.top[i & 1][1 - wg][r]);
-          const float mn = fmaxf(m, top * factor);
+          // the row's other positions are the other warpgroups'
+          sm.top[i & 1][r][wg] = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+          group_sync(4 + (warp & 3));
+          const float4 tops = *reinterpret_cast<const float4 *>(sm.top[i & 1][r]);
+          const float mn = fmaxf(m, fmaxf(fmaxf(tops.x, tops.y), fmaxf(tops.z, tops.w)) * factor);
           corr1 = m == mn ? 1.0f : ex2(m - mn);
           m = mn;
           const float sub = mn == -INFINITY ? 0.0f : mn - kPShift;
           float part[4] = {0.f, 0.f, 0.f, 0.f};
-          __syncwarp();
-#pragma unroll 1
-          for (int c = 0; c < 2; c++) {
-            uint32_t x[32], w[32];  // 16 words of parts, 16 of remainders
-            tc_ld32(sa + 32 * c, x);
-            tc_ld_wait(x);
+          uint32_t w[32];  // 16 words of parts, 16 of remainders
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float p0 = ex2(fmaf(__uint_as_float(x[e]), factor, -sub));
-              const float p1 = ex2(fmaf(__uint_as_float(x[e + 1]), factor, -sub));
-              part[(e / 2) & 3] += p0 + p1;
-              split_f16(p0, p1, w[e / 2], w[16 + e / 2]);
-            }
-            tc_st32(sa + 32 * c, w);
+          for (int e = 0; e < 32; e += 2) {
+            const float p0 = ex2(fmaf(__uint_as_float(v[e]), factor, -sub));
+            const float p1 = ex2(fmaf(__uint_as_float(v[e + 1]), factor, -sub));
+            part[(e / 2) & 3] += p0 + p1;
+            split_f16(p0, p1, w[e / 2], w[16 + e / 2]);
           }
+          tc_st32(sa, w);
           l = l * corr1 + ((part[0] + part[1]) + (part[2] + part[3]));
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         }
@@ -266,20 +253,20 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         corr = corr1, sees0 = now0, sees1 = now1;
       }
       fold(i - 1, g.tile1 - 1, sees0, sees1);
-      // the two halves' sums of weights
+      // the four quarters' sums of weights
       sm.ml[wg][r] = l;
-      named_sync<1, 256>();
-      const float L = sm.ml[0][r] + sm.ml[1][r];
+      named_sync<1, kManySoft>();
+      const float L = (sm.ml[0][r] + sm.ml[1][r]) + (sm.ml[2][r] + sm.ml[3][r]);
       const bool whole = g.whole();
       const size_t slot = g.slot;
       const float scale = whole ? (L != 0.0f ? 1.0f / L : 0.0f) : 1.0f;
       // whole units go to their rows of out; parts lie [hd / 4][row] float4
-      float *dst = whole ? p.out + ((size_t)(g.first + (live ? nd : 0)) * p.h + g.kvh * p.g + rr % p.g) * HD + wg * (HD / 2)
-                         : p.part_o + ((slot * (HD / 4) + wg * (HD / 8)) * kManyRows + r) * 4;
+      float *dst = whole ? p.out + ((size_t)(g.first + (live ? nd : 0)) * p.h + g.kvh * p.g + rr % p.g) * HD + wg * 32
+                         : p.part_o + ((slot * (HD / 4) + wg * 8) * kManyRows + r) * 4;
       const uint32_t step = whole ? 4 : 4 * kManyRows;
-      if (live) {
+      if (live && wg < HD / 32) {
 #pragma unroll
-        for (int d = 0; d < HD / 2; d += 4)
+        for (int d = 0; d < 32; d += 4)
           *reinterpret_cast<float4 *>(dst + (size_t)(d / 4) * step) =
               make_float4(o[d] * scale, o[d + 1] * scale, o[d + 2] * scale, o[d + 3] * scale);
         if (!whole && wg == 0) {
@@ -288,12 +275,12 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         }
       }
       if (g.tile0 == 0 && t == 0) note_unit(p, g);
-      named_sync<1, 256>();  // Q and the sums may be written again
+      named_sync<1, kManySoft>();  // Q and the sums may be written again
     }
   }
   tc_before();
   __syncthreads();
-  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  if (warp == MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
 }  // namespace
