@@ -10,7 +10,7 @@
 // Registers: 640 threads at 96; setmaxnreg gives the softmax warps 104 and leaves 56 to the others (512 * 104 + 128 * 56
 // = 60416 of 61440, what the block was launched with).
 //
-// 8 sequences of 64 nodes x 4 heads a kv head at 32768 positions: 461-468 us on a box where it had 487-470 with 64
+// 8 sequences of 64 nodes x 4 heads a kv head at 32768 positions: 461-468 us on a GPU where it had 487-470 with 64
 // positions a thread (a second pass over the scores then, for want of registers); one tree of 16 at 4096 22.9 us, 24.7
 // then. With both parts that is 1.18 PFLOP/s, 0.72 of the dense rate in short bursts, and what the power limit leaves: the
 // same instructions on weights of random bits take 1.2 times as long, half of the products save 10 %.
