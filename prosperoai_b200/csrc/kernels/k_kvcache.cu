@@ -15,7 +15,9 @@ namespace {
 // ---- rotary append ---------------------------------------------------------------------------
 // CTA (node, sequence, group of heads): hd/8 threads a head, 4 pairs (i, i +
 // hd/2) each, so that every access is 16 bytes (8 of fp16). The products and
-// sums are rounded one by one (rope_pair), as in the decode step.
+// sums are rounded one by one (rope_pair), as in the decode step. Bound by the
+// launch and three loads that need one another: 4.7 us for 8 rows of 32 + 16
+// heads of 128, 8.3 for 512 rows (21 MB, 3.2 us).
 constexpr uint32_t kAppendThreads = 128;
 
 struct AppendParams {
@@ -83,7 +85,9 @@ __global__ void __launch_bounds__(kAppendThreads) k_rope_append(AppendParams p) 
 // CTA (layer x plane, sequence): its columns are (kv head, 16 bytes of a
 // row), one thread each. A path ascends, so a row's target never lies behind
 // the sources of later rows: a thread reads kAcceptBatch rows of its column
-// and then writes them, in path order, and needs no other thread.
+// and then writes them, in path order, and needs no other thread. 6 rows of 8
+// sequences in 32 layers of 8 heads of 128 (10 MB, 1.6 us): 6.2 us; a launch
+// that moves nothing 5.0.
 constexpr uint32_t kAcceptThreads = 128;
 constexpr int kAcceptBatch = 8;
 
@@ -143,7 +147,10 @@ __global__ void __launch_bounds__(kAcceptThreads) k_kv_accept(KvDev c, uint32_t 
 // One CTA plans: it reads the tables and lengths, writes the new table and
 // lists the copies; a second kernel makes the copies. What a page is used
 // for is a maximum (its rows in use) and a minimum (the first sequence that
-// extends it), so the order of the atomics changes nothing.
+// extends it), so the order of the atomics changes nothing. The copying kernel
+// is launched beside the plan and waits for it. 8 beams, 4 of them copying a
+// partly filled page in 32 layers (63 MB, 9.6 us): 18.5 us, 23.3 with one
+// kernel behind the other; 8 runs of 700 positions (734 MB, 112 us): 119 us.
 struct ForkCopy {
   int32_t src, dst;    // pages; without a table: the parent sequence, this sequence
   uint32_t from, rows; // rows [from, rows) of the page
