@@ -529,6 +529,8 @@ pai_status_t launch_tree_hd(pai_b200_ctx_t *ctx, TreeParams &p) {
   CUtensorMap kmap, vmap;
   if ((!p.c.table || p.c.page_tokens % p.chunk == 0) && plane_map(p, p.c.k, &kmap) && plane_map(p, p.c.v, &vmap))
   {
+    // 8 sequences at 16384 positions, with the exchanged operands and without: 8 rows 93 and 121 us, 32 rows 109 and 127.
+    // 8 rows with 16 at compile time 97, 16 rows with 32 106 instead of 99.
     if (rows > kFewRows)
       return launch_tc<HD, kManyRows, 0>(ctx, p, k_attn_tree_many<HD>, kManyThreads, sizeof(ManySmem<HD>) + 1024, kmap, vmap);
     constexpr size_t smem = sizeof(FewSmem<HD>) + 1024;
@@ -536,7 +538,9 @@ pai_status_t launch_tree_hd(pai_b200_ctx_t *ctx, TreeParams &p) {
     if (rows <= 16) return launch_tc<HD, kFewRows, 2>(ctx, p, k_attn_tree_few<HD, 2, 1>, few_threads(1), smem, kmap, vmap);
     return launch_tc<HD, kFewRows, 4>(ctx, p, k_attn_tree_few<HD, 2, 2>, few_threads(2), smem, kmap, vmap);
   }
-  if (rows <= 16) return launch_tree<HD, 1>(ctx, p);
+  // 8 sequences at 16384 positions in pages of 100: 16 rows 126 us in tiles of 16, 253 in one of 64; 20 rows (two tiles)
+  // 217 and 255; 64 rows 432 and 279
+  if (rows <= 32) return launch_tree<HD, 1>(ctx, p);
   return launch_tree<HD, 4>(ctx, p);
 }
 

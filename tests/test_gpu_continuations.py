@@ -600,7 +600,8 @@ def check_beams(dev, logits, scores, done, pad, n_out, stride=None):
 
 @pytest.mark.parametrize("prompts,beams,vocab,n_out,stride", [
     (1, 1, 1, 1, None), (1, 1, 5, 8, None), (1, 4, 300, 4, None), (2, 3, 2048, 6, 2050), (3, 5, 8192, 10, None),
-    (1, 8, 8193, 16, 8196), (1, 2, 128256, 4, None), (5, 1, 4097, 1, 4099), (1, 64, 777, 64, None), (2, 7, 30000, 64, 30004)])
+    (1, 8, 8193, 16, 8196), (1, 2, 128256, 4, None), (5, 1, 4097, 1, 4099), (1, 64, 777, 64, None), (2, 7, 30000, 64, 30004),
+    (1, 13, 128256, 26, None), (1, 64, 40000, 64, None), (1, 1, 128256, 64, None)])
 @pytest.mark.parametrize("ended", [False, True])
 def test_beams(dev, prompts, beams, vocab, n_out, stride, ended):
     rng = np.random.default_rng(vocab + beams)
