@@ -1,4 +1,4 @@
-// Tree attention of at most 32 rows a kv head (decoding, small trees): bound by the cache's bytes.
+// Tree attention of at most 32 rows a kv head, 16 with head_dim 64 (decoding, small trees): bound by the cache's bytes.
 //
 // The operands change places, so that the tensor cores and the softmax do the rows' work and not that of 128 rows:
 //   S^T = K Q^T      M = 128 positions, N = 64: the 32 rows' fp16 parts, then their remainders
@@ -6,8 +6,7 @@
 // A softmax thread has a position and all rows: the weights of a tile need no exchange as long as no row's maximum
 // grows by more than 2^3 (they are relative to a maximum that may be that much too small: fp16 holds 2^15.99, and the
 // weights carry 2^12). Only when some row's does, in a sequence's first tiles, are the rows' maxima taken over the
-// tile. The sums of weights stay in the threads, one a row and
-// position, until a unit ends.
+// tile. The sums of weights stay in the threads, one a row and position, until a unit ends.
 //   first 4 or 8 warps  softmax; the weights go to shared memory, 128 bytes a position, as an MN-major B
 //   next 4              add the tiles' O^T to the running output, a thread a dim, the rows in registers
 //   last 4              issue the MMAs (8 + 8 of 48 cycles of shared memory a tile), copy K and V, clean V
@@ -20,29 +19,32 @@
 
 namespace {
 
-constexpr uint32_t kFewRows = 32, kFewK = 3, kFewV = 2;
+constexpr uint32_t kFewRows = 32;
 
 template <int HD>
 struct FewSmem {
   static constexpr uint32_t kBlock = kTcTile * 128;         // a tile's 64 dims: 16 KB
   static constexpr uint32_t kTileBytes = HD / 64 * kBlock;  // a K or V tile
   static constexpr uint32_t kQBlock = 64 * 128;             // 64 dims of the rows' parts and remainders
+  // tiles of K and V in flight, 96 and 64 KB (head_dim 64 with half of that: 8 x one token at 16384 62 us instead of 60)
+  static constexpr uint32_t kK = 3 * 128 / HD, kV = 2 * 128 / HD;
+  static constexpr uint32_t kWords = HD == 64 ? 16 : 8;
   uint8_t q[HD / 64 * kQBlock];
-  uint8_t kt[kFewK][kTileBytes];
-  uint8_t vt[kFewV][kTileBytes];
+  uint8_t kt[kK][kTileBytes];
+  uint8_t vt[kV][kTileBytes];
   uint8_t pt[2][kTcTile * 128];  // weights: [position][32 rows' parts, 32 rows' remainders]
   // Words of a tile are read long before the tile that takes their place: P V of a tile waits for the tile before the
-  // last to be folded, so no warp is more than a few tiles ahead of another.
-  uint32_t valid[8][4];  // positions of a tile that hold a row
-  uint32_t odd[8][4];    // its nodes with a non-finite V row
-  uint32_t grew[8][2];   // [tile][softmax warpgroup]: whether the weights are relative to new maxima
-  float corr[8][kFewRows];  // then: 2^(old - new)
+  // last to be folded, and K of a tile for the scores kK tiles before, so no warp is kK + 3 tiles ahead of another.
+  uint32_t valid[kWords][4];  // positions of a tile that hold a row
+  uint32_t odd[kWords][4];    // its nodes with a non-finite V row
+  uint32_t grew[kWords][2];   // [tile][softmax warpgroup]: whether the weights are relative to new maxima
+  float corr[kWords][kFewRows];  // then: 2^(old - new)
   float factor[kFewRows], sub[kFewRows];
   float wmax[2][4][kFewRows];
   float lsum[4][4][kFewRows], msum[4][kFewRows];  // [segment][warp]: sums of weights; maxima
   uint32_t upto[kMaxSeqs + 1];
   Ring ring;
-  uint64_t kfull[kFewK], kempty[kFewK], vfull[kFewV], vclean[kFewV], vempty[kFewV], sfull[2], pfull[2], ofull[2], ofree[2],
+  uint64_t kfull[kK], kempty[kK], vfull[kV], vclean[kV], vempty[kV], sfull[2], pfull[2], ofull[2], ofree[2],
       lfull[4], qfull, drain;
   uint32_t tmem;
 };
@@ -63,6 +65,7 @@ __global__ void __launch_bounds__(few_threads(SW), 1)
   using Smem = FewSmem<HD>;
   extern __shared__ __align__(16) uint8_t raw[];
   Smem &sm = *reinterpret_cast<Smem *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  constexpr uint32_t kFewK = Smem::kK, kFewV = Smem::kV, WM = Smem::kWords - 1;
   constexpr uint32_t BL = Smem::kBlock, FOLD = 4 * SW, MMA = FOLD + 4;  // first warps of those roles
   const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
   pdl_trigger();
@@ -103,11 +106,11 @@ __global__ void __launch_bounds__(few_threads(SW), 1)
   uint32_t i = 0, seg = 0;  // tiles and segments of the run so far
 
   if (warp == MMA + 1) {
-    copy_tiles<HD, kFewRows, kFewK, true>(p, &kmap, sm.upto, sm.ring, sm.kt[0], sm.kfull, sm.kempty, sm.valid);
+    copy_tiles<HD, kFewRows, kFewK, true, WM>(p, &kmap, sm.upto, sm.ring, sm.kt[0], sm.kfull, sm.kempty, sm.valid);
   } else if (warp == MMA + 2) {
-    copy_tiles<HD, kFewRows, kFewV, false>(p, &vmap, sm.upto, sm.ring, sm.vt[0], sm.vfull, sm.vempty, nullptr);
+    copy_tiles<HD, kFewRows, kFewV, false, WM>(p, &vmap, sm.upto, sm.ring, sm.vt[0], sm.vfull, sm.vempty, nullptr);
   } else if (warp == MMA + 3) {
-    clean_tiles<HD, kFewV, 1>(p, sm.ring, 0, sm.vt[0], sm.vfull, sm.vclean, sm.odd);
+    clean_tiles<HD, kFewV, 1, WM>(p, sm.ring, 0, sm.vt[0], sm.vfull, sm.vclean, sm.odd);
   } else if (warp == MMA) {
     // ---- MMA issue ----
     const uint32_t leader = elect_one();
@@ -177,9 +180,9 @@ __global__ void __launch_bounds__(few_threads(SW), 1)
 #pragma unroll
         for (uint32_t gr = 0; gr < FR / 8; gr++) {
           uint32_t *v = w + 16 * gr;
-          if (sm.grew[i & 7][gr / RG]) {
+          if (sm.grew[i & WM][gr / RG]) {
 #pragma unroll
-            for (uint32_t e = 0; e < 8; e++) o[8 * gr + e] *= sm.corr[i & 7][8 * gr + e];
+            for (uint32_t e = 0; e < 8; e++) o[8 * gr + e] *= sm.corr[i & WM][8 * gr + e];
           }
           tc_ld_wait8(v);
           tc_ld_wait8(v + 8);
@@ -194,7 +197,7 @@ __global__ void __launch_bounds__(few_threads(SW), 1)
 #pragma unroll 1
           for (int x = 0; x < 4; x++)
 #pragma unroll 1
-            for (uint32_t left = sm.odd[i & 7][x] & sm.valid[i & 7][x]; left; left &= left - 1) {
+            for (uint32_t left = sm.odd[i & WM][x] & sm.valid[i & WM][x]; left; left &= left - 1) {
               const uint32_t pos = tile * kTcTile + 32 * x + __ffs(left) - 1;
               const float f = __half2float(p.c.v[(size_t)g.kvh * p.c.head_stride + kv_row(p.c, g.s, pos) + d]);
               if (isfinite(f)) continue;
@@ -250,7 +253,7 @@ __global__ void __launch_bounds__(few_threads(SW), 1)
         wait(&sm.sfull[i & 1], i >> 1);
         __syncwarp();
         tc_after();
-        const bool there = (sm.valid[i & 7][w4] >> lane) & 1;
+        const bool there = (sm.valid[i & WM][w4] >> lane) & 1;
         const uint32_t pos = tile * kTcTile + (t & 127);
         const bool is_node = (tile + 1) * kTcTile > g.len && pos >= g.len;
         // scores in powers of two, unseen ones -inf, and the largest exponent relative to the rows' maxima so far
@@ -308,7 +311,7 @@ __global__ void __launch_bounds__(few_threads(SW), 1)
           m = mn;
           if (w4 == 0 && lane < 8 * RG) {
             sm.sub[row0 + lane] = mn == -INFINITY ? kNone : mn - kPShift;
-            sm.corr[i & 7][row0 + lane] = corr;
+            sm.corr[i & WM][row0 + lane] = corr;
           }
 #pragma unroll
           for (uint32_t gr = 0; gr < RG; gr++) {
@@ -317,7 +320,7 @@ __global__ void __launch_bounds__(few_threads(SW), 1)
           }
           group_sync(2 + wg);
         }
-        if (w4 == 0 && lane == 0) sm.grew[i & 7][wg] = any;
+        if (w4 == 0 && lane == 0) sm.grew[i & WM][wg] = any;
         // weights, in groups of 8 rows, to the position's 128 bytes (16 of parts and 16 of remainders a group)
         uint8_t *dst = sm.pt[i & 1] + (t & 127) * 128;
 #pragma unroll

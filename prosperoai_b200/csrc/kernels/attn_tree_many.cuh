@@ -26,8 +26,9 @@ struct ManySmem {
   static constexpr uint32_t kBlock = 128 * 128;             // 128 rows of 64 dims: 16 KB
   static constexpr uint32_t kTileBytes = HD / 64 * kBlock;  // a K or V tile, or one part of Q
   uint8_t q[2][kTileBytes];
-  uint8_t kt[2][kTileBytes];
-  uint8_t vt[2][kTileBytes];
+  static constexpr uint32_t kSlots = 2 * 128 / HD;          // tiles of K and of V in flight, 64 KB each
+  uint8_t kt[kSlots][kTileBytes];
+  uint8_t vt[kSlots][kTileBytes];
   uint32_t valid[8][4];          // positions of a tile that hold a row; a tile's words are read long before 8 tiles on
   uint32_t odd[8][4];            // its nodes with a non-finite V row
   float factor[kManyRows];
@@ -35,7 +36,7 @@ struct ManySmem {
   float ml[kManyGroups][kManyRows];
   uint32_t upto[kMaxSeqs + 1];
   Ring ring;
-  uint64_t kfull[2], kempty[2], vfull[2], vclean[2], vempty[2], sfull[2], pfull[2], ofull[2], qfull, drain;
+  uint64_t kfull[kSlots], kempty[kSlots], vfull[kSlots], vclean[kSlots], vempty[kSlots], sfull[2], pfull[2], ofull[2], qfull, drain;
   uint32_t tmem;
 };
 
@@ -45,16 +46,18 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   using Smem = ManySmem<HD>;
   extern __shared__ __align__(16) uint8_t raw[];
   Smem &sm = *reinterpret_cast<Smem *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-  constexpr uint32_t BL = Smem::kBlock, MMA = kManySoft / 32;  // first warp behind the softmax
+  constexpr uint32_t kSlots = Smem::kSlots, BL = Smem::kBlock, MMA = kManySoft / 32;  // first warp behind the softmax
   const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
   pdl_trigger();
   if (t == 0) {
-    for (int i = 0; i < 2; i++) {
+    for (uint32_t i = 0; i < kSlots; i++) {
       mbar_init(&sm.kfull[i], 1);
       mbar_init(&sm.vfull[i], 1);
       mbar_init(&sm.vclean[i], 1);
       mbar_init(&sm.kempty[i], 1);
       mbar_init(&sm.vempty[i], 1);
+    }
+    for (int i = 0; i < 2; i++) {
       mbar_init(&sm.sfull[i], 1);
       mbar_init(&sm.pfull[i], MMA);
       mbar_init(&sm.ofull[i], 1);
@@ -80,11 +83,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   if (warp >= MMA) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == MMA + 1) {
-      copy_tiles<HD, kManyRows, 2, true>(p, &kmap, sm.upto, sm.ring, sm.kt[0], sm.kfull, sm.kempty, sm.valid);
+      copy_tiles<HD, kManyRows, kSlots, true, 7>(p, &kmap, sm.upto, sm.ring, sm.kt[0], sm.kfull, sm.kempty, sm.valid);
     } else if (warp == MMA + 2) {
-      copy_tiles<HD, kManyRows, 2, false>(p, &vmap, sm.upto, sm.ring, sm.vt[0], sm.vfull, sm.vempty, nullptr);
+      copy_tiles<HD, kManyRows, kSlots, false, 7>(p, &vmap, sm.upto, sm.ring, sm.vt[0], sm.vfull, sm.vempty, nullptr);
     } else if (warp == MMA + 3) {
-      clean_tiles<HD, 2, 1>(p, sm.ring, 0, sm.vt[0], sm.vfull, sm.vclean, sm.odd);
+      clean_tiles<HD, kSlots, 1, 7>(p, sm.ring, 0, sm.vt[0], sm.vfull, sm.vclean, sm.odd);
     } else {
       // ---- MMA issue ----
       const uint32_t leader = elect_one();
@@ -92,9 +95,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       constexpr uint64_t kPart = Smem::kTileBytes >> 4;  // from one part of Q, or one tile, to the next, in 16 bytes
       uint32_t i = 0, seg = 0;
       auto scores = [&](uint32_t n) {  // S = Q K^T of tile n: both parts of Q
-        wait(&sm.kfull[n & 1], n >> 1);
+        wait(&sm.kfull[n % kSlots], n / kSlots);
         tc_after();
-        const uint64_t kb = kd + (n & 1) * kPart;
+        const uint64_t kb = kd + (n % kSlots) * kPart;
         const uint32_t d = tmem + 128 * (n & 1);
         if (wait.ok) {
 #pragma unroll
@@ -104,7 +107,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             tc_mma_ss(leader, d, qd + kPart + off, kb + off, idesc_f16(kTcTile, false), true);
           }
           tc_commit(leader, &sm.sfull[n & 1]);
-          tc_commit(leader, &sm.kempty[n & 1]);
+          tc_commit(leader, &sm.kempty[n % kSlots]);
         }
         __syncwarp();
       };
@@ -114,9 +117,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         for (uint32_t tile = g.tile0; tile < g.tile1; tile++, i++) {
           if (tile + 1 < g.tile1) scores(i + 1);
           wait(&sm.pfull[i & 1], i >> 1);
-          wait(&sm.vclean[i & 1], i >> 1);
+          wait(&sm.vclean[i % kSlots], i / kSlots);
           tc_after();
-          const uint64_t vb = vd + (i & 1) * kPart;
+          const uint64_t vb = vd + (i % kSlots) * kPart;
           const uint32_t a = tmem + 128 * (i & 1), d = tmem + 256 + 128 * (i & 1);
           if (wait.ok) {  // this tile's P V, from zero: the sum over tiles is made in registers, where it is rounded
 #pragma unroll
@@ -126,7 +129,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
               tc_mma_ts(leader, d, at + 16, vb + k * (2048 >> 4), idesc_f16(HD, true), true);
             }
             tc_commit(leader, &sm.ofull[i & 1]);
-            tc_commit(leader, &sm.vempty[i & 1]);
+            tc_commit(leader, &sm.vempty[i % kSlots]);
           }
           __syncwarp();
         }

@@ -262,7 +262,7 @@ struct Lead {
 // Copies, one warp for all K tiles or all V tiles: a lane a chunk of p.chunk positions, which lie in one page. The warp
 // of K (LEADS) also hands out the segments, and notes in `valid` which positions of a tile hold a row. SLOTS tiles are
 // in flight.
-template <int HD, uint32_t MR, uint32_t SLOTS, bool LEADS>
+template <int HD, uint32_t MR, uint32_t SLOTS, bool LEADS, uint32_t WM>
 __device__ __forceinline__ void copy_tiles(const TreeParams &p, const CUtensorMap *map, const uint32_t *upto, Ring &ring,
                                            uint8_t *slot0, uint64_t *full, uint64_t *empty,
                                            uint32_t (*valid)[4]) {
@@ -308,7 +308,7 @@ __device__ __forceinline__ void copy_tiles(const TreeParams &p, const CUtensorMa
             for (uint32_t c = 0; c < 32 / chunk; c++)
               if ((there >> (32 / chunk * lane + c)) & 1) bits |= ((1u << chunk) - 1) << (c * chunk);
           }
-          valid[i & 7][lane] = bits & (uint32_t)low_bits((int64_t)cap - pos);
+          valid[i & WM][lane] = bits & (uint32_t)low_bits((int64_t)cap - pos);
         }
         __syncwarp();
       }
@@ -334,7 +334,7 @@ __device__ __forceinline__ void copy_tiles(const TreeParams &p, const CUtensorMa
 // product. Such elements (those of stale rows behind the last node too) become 0 here, and `odd` tells where; they are
 // added later to the rows that see them. (Every tile is handed on: a barrier that was watched for some phases only could
 // be two phases on.)
-template <int HD, uint32_t SLOTS, uint32_t WARPS>
+template <int HD, uint32_t SLOTS, uint32_t WARPS, uint32_t WM>
 __device__ __forceinline__ void clean_tiles(const TreeParams &p, Ring &ring, uint32_t w, uint8_t *slot0, uint64_t *full,
                                             uint64_t *clean, uint32_t (*odd)[4]) {
   constexpr uint32_t BL = kTcTile * 128, BYTES = HD / 64 * BL, CH = HD / 8;
@@ -374,7 +374,7 @@ __device__ __forceinline__ void clean_tiles(const TreeParams &p, Ring &ring, uin
             }
           }
           const uint32_t word = __ballot_sync(0xffffffffu, bad);
-          if (lane == 0) odd[i & 7][x] = word;
+          if (lane == 0) odd[i & WM][x] = word;
         }
         fence_proxy_async();
       }

@@ -1,7 +1,8 @@
 // Attention of drafted nodes over a cache view (pai_b200_attn_tree_f16kv): the choice of kernel, and the form that
 // takes any page size.
 //
-//   attn_tree_few.cuh    at most 32 rows (nodes x query heads of a kv head) of a sequence: decoding, small trees
+//   attn_tree_few.cuh    at most 32 rows (nodes x query heads of a kv head; 16 with head_dim 64) of a sequence: decoding,
+//                        small trees
 //   attn_tree_many.cuh   more rows
 //   k_attn_tree (here)   where tensor copies cannot fetch the cache: page sizes that no power of two from 8 divides
 //                        (a page of 8 n positions is fetched in shares), strides beyond a tensor map's
@@ -529,14 +530,18 @@ pai_status_t launch_tree_hd(pai_b200_ctx_t *ctx, TreeParams &p) {
   CUtensorMap kmap, vmap;
   if ((!p.c.table || p.c.page_tokens % p.chunk == 0) && plane_map(p, p.c.k, &kmap) && plane_map(p, p.c.v, &vmap))
   {
-    // 8 sequences at 16384 positions, with the exchanged operands and without: 8 rows 93 and 121 us, 32 rows 109 and 127.
-    // 8 rows with 16 at compile time 97, 16 rows with 32 106 instead of 99.
-    if (rows > kFewRows)
+    // 8 sequences at 16384 positions, with the exchanged operands and without: 8 rows 93 and 121 us, 32 rows 109 and 127
+    // (at 4096 positions 55 and 51, the lengths are not known here); 8 rows with 16 at compile time 97, 16 rows with 32
+    // 106 instead of 99. With head_dim 64 a tile is half the bytes and the same softmax: 16 rows 84 and 108, 32 rows 119
+    // and 108 (one sequence at 4096: 24.8 and 20.6).
+    constexpr uint32_t kMost = HD == 64 ? 16 : kFewRows;
+    if (rows > kMost)
       return launch_tc<HD, kManyRows, 0>(ctx, p, k_attn_tree_many<HD>, kManyThreads, sizeof(ManySmem<HD>) + 1024, kmap, vmap);
     constexpr size_t smem = sizeof(FewSmem<HD>) + 1024;
     if (rows <= 8) return launch_tc<HD, kFewRows, 1>(ctx, p, k_attn_tree_few<HD, 1, 1>, few_threads(1), smem, kmap, vmap);
     if (rows <= 16) return launch_tc<HD, kFewRows, 2>(ctx, p, k_attn_tree_few<HD, 2, 1>, few_threads(1), smem, kmap, vmap);
-    return launch_tc<HD, kFewRows, 4>(ctx, p, k_attn_tree_few<HD, 2, 2>, few_threads(2), smem, kmap, vmap);
+    if constexpr (kMost > 16)
+      return launch_tc<HD, kFewRows, 4>(ctx, p, k_attn_tree_few<HD, 2, 2>, few_threads(2), smem, kmap, vmap);
   }
   // 8 sequences at 16384 positions in pages of 100: 16 rows 126 us in tiles of 16, 253 in one of 64; 20 rows (two tiles)
   // 217 and 255; 64 rows 432 and 279
