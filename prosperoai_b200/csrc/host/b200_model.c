@@ -426,6 +426,7 @@ struct pai_b200_session {
   uint32_t dr_nodes;   /* ... and their number; 0: none that can be accepted */
   pai_b200_graph_t *dr_graph; /* a verification's kernels for dr_shape nodes, once that many came twice in a row */
   uint32_t dr_shape;
+  uint64_t dr_wait; /* the wait limit that its kernels carry */
   int beam_ready;      /* the logits belong to the position, and no selection has used them */
 };
 
@@ -1149,12 +1150,12 @@ pai_status_t pai_b200_session_verify(pai_b200_session_t *s, const int32_t *token
   if (!st) st = pai_b200_memcpy_h2d(ctx, s->pf_tok, s->pf_htok, rows * 4ull);
   /* the launches of 8 layers cost 220 to 300 us more than a replay of them: 1
    * row 1108 against 890 us, 4 rows 1278 and 1046, 16 rows 1925 and 1622 */
-  if (!st && s->dr_shape != n) {
+  if (!st && (s->dr_shape != n || s->dr_wait != b200_ctx_wait_ns(ctx))) {
     pai_b200_graph_destroy(s->dr_graph);
     s->dr_graph = NULL;
     s->dr_shape = 0;
     st = draft_kernels(s, n); /* sizes the scratch too */
-    if (!st) s->dr_shape = n;
+    if (!st) s->dr_shape = n, s->dr_wait = b200_ctx_wait_ns(ctx);
   } else if (!st) {
     if (!s->dr_graph) {
       st = pai_b200_graph_begin(ctx);

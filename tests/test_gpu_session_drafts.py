@@ -162,6 +162,10 @@ def test_verifications_of_one_size_follow_their_inputs(model, batch, n):
         np.testing.assert_array_equal(got, want)
         if turn == 2:
             s.verify(draft[:, :1])  # another size in between
+        if turn == 3:  # the kernels carry the limit on their waits
+            _native.check(_native.load().pai_b200_set_wait_limit(model.dev.ctx, 3_000_000_000), "set_wait_limit")
+            np.testing.assert_array_equal(s.verify(draft, parents), want)
+            _native.check(_native.load().pai_b200_set_wait_limit(model.dev.ctx, 0), "set_wait_limit")
         s.step(draft[:, 0])
         history = np.concatenate([history, draft[:, :1]], 1)
     s.close()
