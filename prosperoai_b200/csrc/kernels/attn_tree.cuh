@@ -44,6 +44,7 @@ struct TreeParams {
   float *part_ml;  // scratch [2 gridDim.x][MR][2]
   uint32_t *cnt;   // counters [n_seq][kv head][row tile], left at zero
   uint32_t *units; // scratch [n_seq][kv head][row tile][2]: parts of a unit, slot of the first
+  uint32_t slots;  // parts that the scratch holds, two a CTA
   uint32_t *err;
   uint64_t wait_ns;
   uint32_t chunk;  // tcgen05 form: positions of one tensor copy
@@ -76,6 +77,17 @@ __device__ __forceinline__ uint64_t window(const uint64_t *m, uint32_t words, in
 // The lowest n bits (n below 0: none; above 63: all).
 __device__ __forceinline__ uint64_t low_bits(int64_t n) {
   return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1;
+}
+
+// Where part q of a unit lies whose first part lies in slot `first`: the other parts are the first ones of their CTAs.
+__host__ __device__ __forceinline__ uint32_t part_slot(uint32_t first, uint32_t q) {
+  return q == 0 ? first : (first & ~1u) + 2 * q;
+}
+// How many parts a unit's entry names, 0 where they would lie outside the scratch. After a wait has run out in some CTA
+// its other units have no entry, and what lies there instead is whatever the scratch held before.
+__host__ __device__ __forceinline__ uint32_t unit_parts(uint32_t parts, uint32_t first, uint32_t slots) {
+  if (parts == 0 || parts > slots || first >= slots) return 0;
+  return part_slot(first, parts - 1) < slots ? parts : 0;
 }
 
 // One sequence's share of the work.

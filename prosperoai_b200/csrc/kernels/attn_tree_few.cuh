@@ -199,7 +199,9 @@ __global__ void __launch_bounds__(few_threads(SW), 1)
 #pragma unroll 1
             for (uint32_t left = sm.odd[i & WM][x] & sm.valid[i & WM][x]; left; left &= left - 1) {
               const uint32_t pos = tile * kTcTile + 32 * x + __ffs(left) - 1;
-              const float f = __half2float(p.c.v[(size_t)g.kvh * p.c.head_stride + kv_row(p.c, g.s, pos) + d]);
+              const int64_t at_row = kv_row(p.c, g.s, pos);
+              if (at_row < 0) continue;  // the words are old ones: a wait has run out
+              const float f = __half2float(p.c.v[(size_t)g.kvh * p.c.head_stride + at_row + d]);
               if (isfinite(f)) continue;
 #pragma unroll
               for (uint32_t r = 0; r < FR; r++)

@@ -180,6 +180,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
               for (uint32_t left = sm.odd[n & 7][x] & (uint32_t)((x < 2 ? sees0 : sees1) >> (32 * (x & 1))); left;
                    left &= left - 1) {
                 const int64_t at_row = kv_row(p.c, g.s, tile * kTcTile + 32 * x + __ffs(left) - 1);
+                if (at_row < 0) continue;  // the words are old ones: a wait has run out
                 const __half2 *vr =
                     reinterpret_cast<const __half2 *>(p.c.v + (size_t)g.kvh * p.c.head_stride + at_row + wg * 32);
 #pragma unroll

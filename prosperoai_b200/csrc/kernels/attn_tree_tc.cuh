@@ -273,7 +273,10 @@ __device__ __forceinline__ void copy_tiles(const TreeParams &p, const CUtensorMa
   if (LEADS) lead.begin(p, upto);
   Segment g;
   uint32_t i = 0;  // tiles so far
-  for (uint32_t n = 0; LEADS ? lead.next<MR>(p, upto, ring, g) : next_segment(ring, n, wait, g); n++) {
+  // After a wait has run out the leading warp hands out nothing more: the entries that it would write may still be read.
+  for (uint32_t n = 0; LEADS ? __all_sync(0xffffffffu, wait.ok) && lead.next<MR>(p, upto, ring, g)
+                             : next_segment(ring, n, wait, g);
+       n++) {
     const uint32_t total = g.len + g.nodes;
     // where the lane's chunk of a tile lies: page (n_pages for a hole, which reads zeros), first row; -1: behind the
     // last position, not copied
@@ -446,9 +449,9 @@ __global__ void __launch_bounds__(kJoinRows * HD / 4) k_attn_tree_join(TreeParam
   const SeqWork w = seq_work<MR, kTcTile>(p, s);
   if (block >= w.blocks) return;
   const uint32_t rows = min(MR, w.nodes * p.g - block * MR);
-  const uint32_t parts = min(made.x, kTcGrid), first = made.y;
+  const uint32_t parts = unit_parts(made.x, made.y, p.slots), first = made.y;
   if (parts == 0 || row0 >= rows) return;
-  auto slot = [&](uint32_t q) -> size_t { return q == 0 ? first : (first & ~1u) + 2 * q; };
+  auto slot = [&](uint32_t q) -> size_t { return part_slot(first, q); };
   const uint32_t n = min(kJoinRows, rows - row0), warps = kJoinRows * HD / 128, lane = t & 31;
   const uint32_t r = BY_ROW ? t / (HD / 4) : t % kJoinRows, d4 = BY_ROW ? t % (HD / 4) : t / kJoinRows;
   float4 f[kJoinParts];

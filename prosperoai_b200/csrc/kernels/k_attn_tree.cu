@@ -477,6 +477,7 @@ pai_status_t launch_tc(pai_b200_ctx_t *ctx, TreeParams &p, void (*kern)(TreePara
   const uint32_t grid = (uint32_t)std::min<uint64_t>(kTcGrid, pairs);
   float *scratch;
   const uint64_t slots = 2ull * grid;
+  p.slots = (uint32_t)slots;
   st = b200_ctx_scratch(ctx, slots * MR * (HD + 2) + 2 * units, 1, &scratch, &p.cnt);
   if (st) return st;
   p.part_o = scratch;
