@@ -883,17 +883,18 @@ static pai_status_t prefill_alloc(pai_b200_session_t *s) {
   const uint64_t R = PF_MAX_ROWS, E = m->cfg.n_embd;
   const uint64_t kmax = E > m->k_o ? (E > m->ffl ? E : m->ffl) : (m->k_o > m->ffl ? m->k_o : m->ffl);
   pai_status_t st = PAI_OK;
-  if (s->pf_x) return PAI_OK;
-  SALLOC(s->pf_x, R * E * 4);
-  SALLOC(s->pf_xn, R * E * 4);
-  SALLOC(s->pf_qkv, R * m->n_qkv * 4);
-  SALLOC(s->pf_att, R * m->k_o * 4);
-  SALLOC(s->pf_gu, R * 2 * m->ffl * 4);
-  SALLOC(s->pf_h, R * m->ffl * 4);
-  SALLOC(s->pf_tmp, R * E * 4);
-  SALLOC(s->pf_tok, R * 4);
-  SALLOC(s->pf_xq_buf, b200_xq_bytes(8, kmax));
-  if (!st) st = pai_b200_host_alloc(ctx, R * 4, (void **)&s->pf_htok);
+  if (s->pf_rows) return PAI_OK;
+  /* after an allocation that failed, the next call makes what is missing */
+  if (!s->pf_x) SALLOC(s->pf_x, R * E * 4);
+  if (!s->pf_xn) SALLOC(s->pf_xn, R * E * 4);
+  if (!s->pf_qkv) SALLOC(s->pf_qkv, R * m->n_qkv * 4);
+  if (!s->pf_att) SALLOC(s->pf_att, R * m->k_o * 4);
+  if (!s->pf_gu) SALLOC(s->pf_gu, R * 2 * m->ffl * 4);
+  if (!s->pf_h) SALLOC(s->pf_h, R * m->ffl * 4);
+  if (!s->pf_tmp) SALLOC(s->pf_tmp, R * E * 4);
+  if (!s->pf_tok) SALLOC(s->pf_tok, R * 4);
+  if (!s->pf_xq_buf) SALLOC(s->pf_xq_buf, b200_xq_bytes(8, kmax));
+  if (!st && !s->pf_htok) st = pai_b200_host_alloc(ctx, R * 4, (void **)&s->pf_htok);
   if (!st) s->pf_rows = PF_MAX_ROWS;
   return st;
 }
