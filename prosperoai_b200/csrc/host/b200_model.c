@@ -418,8 +418,9 @@ struct pai_b200_session {
   int32_t *pf_tok, *pf_htok;
   void *pf_xq_buf;
   b200_xq_t pf_xq;
-  /* drafted trees and beams (allocated by the first use): rotated q rows, 8
-   * rows of logits, small arrays on the device and their pinned staging */
+  /* drafted trees and beams (allocated by the first use): rotated q rows and 8
+   * rows of logits of a verification; small arrays on the device and their
+   * pinned staging */
   float *dr_q, *dr_logits;
   uint8_t *dr_dev, *dr_host;
   int32_t *dr_parents; /* host: the nodes of the last verification */
@@ -1012,15 +1013,23 @@ enum {
   DR_MASK = DR_NEXT + 4 * PF_MAX_ROWS, DR_BYTES = DR_MASK + 8 * PF_MAX_ROWS * (DR_MAX_NODES / 64)
 };
 
+/* The small arrays that verifications, acceptance and beams exchange with the host. */
+static pai_status_t stage_alloc(pai_b200_session_t *s) {
+  pai_b200_ctx_t *ctx = s->m->ctx;
+  pai_status_t st = PAI_OK;
+  if (!s->dr_dev) SALLOC(s->dr_dev, DR_BYTES);
+  if (!st && !s->dr_host) st = pai_b200_host_alloc(ctx, DR_BYTES, (void **)&s->dr_host);
+  return st;
+}
+
 static pai_status_t draft_alloc(pai_b200_session_t *s) {
   pai_b200_model_t *m = s->m;
   pai_b200_ctx_t *ctx = m->ctx;
   pai_status_t st = prefill_alloc(s);
+  if (!st) st = stage_alloc(s);
   if (st || s->dr_parents) return st;
   if (!s->dr_q) SALLOC(s->dr_q, (uint64_t)PF_MAX_ROWS * m->k_o * 4);
   if (!s->dr_logits) SALLOC(s->dr_logits, 8ull * m->vl * 4);
-  if (!s->dr_dev) SALLOC(s->dr_dev, DR_BYTES);
-  if (!st && !s->dr_host) st = pai_b200_host_alloc(ctx, DR_BYTES, (void **)&s->dr_host);
   if (!st) {
     s->dr_parents = (int32_t *)malloc(DR_MAX_NODES * sizeof(int32_t));
     if (!s->dr_parents) st = b200_fail(PAI_ERR_NOMEM, "session: host allocation");
@@ -1221,7 +1230,7 @@ pai_status_t pai_b200_session_beam(pai_b200_session_t *s, const float *scores, c
   if (first > s->pos) return b200_fail(PAI_ERR_INVALID_ARG, "session_beam: %u common positions of %u", first, s->pos);
   if (pad < 0 || (uint32_t)pad >= s->m->cfg.vocab)
     return b200_fail(PAI_ERR_INVALID_ARG, "session_beam: pad token %d outside vocab %u", pad, s->m->cfg.vocab);
-  st = draft_alloc(s);
+  st = stage_alloc(s);
   if (!st) st = seen(s, pai_b200_sync(ctx));
   if (!st) st = pai_b200_session_kv_view(s, &kv);
   if (st) return st;

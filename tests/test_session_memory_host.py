@@ -116,3 +116,9 @@ def test_a_call_after_a_failed_allocation(run, what):
         first, second, made, _ = run(what, n)
         assert (first, second) == (NOMEM, OK)
         assert made == allocations + 1  # the failed one again, nothing twice
+
+
+def test_beams_hold_their_staging_only(run):
+    """A selection works on arrays of batch entries: none of the row arrays of a prefill or a verification."""
+    assert run("beam", 0)[2] == 2
+    assert run("beam", 0)[3] < 2 << 20 < run("verify", 0)[3]
