@@ -773,7 +773,8 @@ pai_status_t pai_b200_session_kv_view(const pai_b200_session_t *s, pai_b200_kv_v
  * position (parents NULL: node i follows node i - 1). next[batch][n] receives
  * the greedy token after every node. Nothing is committed: the position
  * stays, and the nodes are forgotten with the next call that moves it
- * (pai_b200_session_accept keeps some), verifies or selects.
+ * (pai_b200_session_accept keeps some), verifies, selects or runs the
+ * layers alone (pai_b200_session_run_layers).
  * Up to 8 rows (batch x n) the layers are the decode step's GEMVs, above
  * that the prefill's GEMM (see pai_b200_session_prefill for its precision).
  * PAI_ERR_NOMEM when the nodes do not fit behind the position,

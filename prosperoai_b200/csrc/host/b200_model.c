@@ -867,6 +867,7 @@ pai_status_t pai_b200_session_run_layers(pai_b200_session_t *s, uint32_t reps) {
   if (!s) return b200_fail(PAI_ERR_INVALID_ARG, "session_run_layers: NULL");
   if (!s->plan) return b200_fail(PAI_ERR_UNSUPPORTED, "session_run_layers: the session runs one launch per op");
   st = usable(s);
+  if (!st && reps) s->dr_nodes = 0; /* the first node's row is written over */
   for (uint32_t i = 0; i < reps && !st; i++) st = b200_decode_launch(s->m->ctx, s->plan);
   return st;
 }

@@ -10,7 +10,7 @@ import subprocess
 import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-OK, NOMEM = 0, -2
+OK, INVALID, NOMEM = 0, -1, -2
 
 # The entry points that the session's host code calls. Allocation number `fail_at` fails (0: none).
 STUBS = r"""
@@ -38,7 +38,7 @@ int pai_b200_memcpy_d2d(void *c, void *d, const void *s, uint64_t n) { (void)c; 
 int pai_b200_memset(void *c, void *d, int v, uint64_t n) { (void)c; memset(d, v, n); return 0; }
 uint64_t b200_ctx_wait_ns(void *c) { (void)c; return 1; }
 #define NOTHING(name) int name(void) { return 0; }
-NOTHING(pai_b200_sync) NOTHING(b200_launch_embed) NOTHING(b200_launch_rmsnorm_xq) NOTHING(b200_launch_gemv)
+NOTHING(pai_b200_sync) NOTHING(b200_decode_launch) NOTHING(b200_launch_embed) NOTHING(b200_launch_rmsnorm_xq) NOTHING(b200_launch_gemv)
 NOTHING(b200_launch_gemv_norm) NOTHING(b200_launch_argmax) NOTHING(b200_launch_xprep) NOTHING(pai_b200_gemm_f32)
 NOTHING(pai_b200_kv_accept_f16) NOTHING(pai_b200_kv_fork_f16) NOTHING(pai_b200_beam_select_f32)
 NOTHING(pai_b200_graph_begin) NOTHING(pai_b200_graph_launch) NOTHING(pai_b200_graph_destroy)
@@ -78,6 +78,15 @@ int main(int argc, char **argv) {
   (void)argc;
   pai_b200_model_t m;
   pai_b200_session_t *s = session(&m);
+  if (argv[1][0] == 'l') { /* the layers run between a verification and its acceptance */
+    int32_t path[B] = {0, 0}, next[B] = {1, 1};
+    s->plan = (void *)s;
+    const int a = call(s, "verify"), b = pai_b200_session_accept(s, path, 1, next);
+    const int c = call(s, "verify"), d = pai_b200_session_run_layers(s, atoi(argv[2]));
+    const int e = pai_b200_session_accept(s, path, 1, next);
+    printf("%d %d %d %d %d\n", a, b, c, d, e);
+    return 0;
+  }
   fail_at = strtoull(argv[2], NULL, 10);
   const int first = call(s, argv[1]);
   const int second = call(s, argv[1]);
@@ -122,3 +131,9 @@ def test_beams_hold_their_staging_only(run):
     """A selection works on arrays of batch entries: none of the row arrays of a prefill or a verification."""
     assert run("beam", 0)[2] == 2
     assert run("beam", 0)[3] < 2 << 20 < run("verify", 0)[3]
+
+
+def test_layers_that_run_alone_overwrite_verified_nodes(run):
+    """pai_b200_session_run_layers appends the step's K/V where the first node's lie: the nodes cannot be accepted any more."""
+    assert run("layers", 0) == [OK] * 5
+    assert run("layers", 1) == [OK] * 4 + [INVALID]
