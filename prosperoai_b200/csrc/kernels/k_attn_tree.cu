@@ -402,8 +402,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tree(TreeParams p) {
       float L = 0.0f;
 #pragma unroll
       for (uint32_t y = 0; y < WN; y++) {
+        // a share without a maximum has seen nothing (zeros) or only scores that are not numbers (NaN, which stays)
         const float my = sm[(y * MR + r) * 2], wy = my == -INFINITY ? 0.0f : ex2(my - M);
-        if (my == -INFINITY) continue;
         const float4 f = *reinterpret_cast<const float4 *>(so + (y * MR + r) * OS + d);
         acc.x = fmaf(f.x, wy, acc.x), acc.y = fmaf(f.y, wy, acc.y);
         acc.z = fmaf(f.z, wy, acc.z), acc.w = fmaf(f.w, wy, acc.w);

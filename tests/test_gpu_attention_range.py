@@ -1,0 +1,89 @@
+"""Tree attention over the whole range of its inputs, in every form of its kernels.
+
+The bounds are those of test_gpu_continuations.attend unless a test says otherwise.
+"""
+import numpy as np
+import pytest
+
+from test_gpu_continuations import Cache, attend, close, pack, random_tree, run_tree
+
+pytestmark = pytest.mark.gpu
+
+# page, nodes, h, hk, hd: the rows of a kv head (nodes x h / hk), the page size and head_dim choose the kernel
+FORMS = {
+    "few 8": (16, 2, 8, 2, 128), "few 16": (0, 4, 4, 1, 128), "few 32": (64, 8, 8, 2, 128), "few 8 of 64": (16, 2, 8, 2, 64),
+    "few 16 of 64": (0, 4, 8, 2, 64), "many": (16, 12, 8, 2, 128), "many of 64": (0, 40, 4, 2, 64),
+    "any page": (20, 5, 8, 2, 128), "any page of 64": (7, 3, 4, 2, 64), "any page, rows": (100, 12, 8, 2, 128),
+    "any page, rows of 64": (20, 40, 4, 2, 64),
+}
+forms = pytest.mark.parametrize("page,n,h,hk,hd", list(FORMS.values()), ids=list(FORMS))
+
+
+def one_sequence(dev, rng, form, past, spare=16):
+    page, n, h, hk, hd = form
+    cache = Cache(dev, rng, [past + n + spare], page, hk, hd, cap=past + n + spare)
+    return cache, rng.standard_normal((n, h, hd)).astype(np.float32)
+
+
+# ---- what is not a number reaches the rows that attend it, and no others ------------------------------------
+
+
+@forms
+def test_nan_queries(dev, page, n, h, hk, hd):
+    """As rotary append leaves them for a position behind its tables."""
+    rng = np.random.default_rng(hd + n)
+    cache, q = one_sequence(dev, rng, (page, n, h, hk, hd), 70)
+    sees = [random_tree(rng, n)]
+    want, bound = attend(cache, 0, [70], sees, q, h)
+    q[1, h - 1, 3] = np.nan
+    got = run_tree(dev, cache, 0, [70], [n], h, pack(sees, n), q)
+    others = np.ones((n, h), bool)
+    others[1, h - 1] = False
+    assert np.isnan(got[1, h - 1]).all()
+    close(got[others], want[others], bound[others])
+
+
+@forms
+@pytest.mark.parametrize("past", [0, 16, 48, 64, 130])
+def test_one_nan_key(dev, page, n, h, hk, hd, past):
+    """The first key behind 16 positions may be the only one that a warp's share of a tile shows a row."""
+    rng = np.random.default_rng(past + n)
+    cache, q = one_sequence(dev, rng, (page, n, h, hk, hd), past)
+    sees = [random_tree(rng, n)]
+    sees[0][:, 0] = False
+    sees[0][0] = np.arange(n) == 0
+    want, bound = attend(cache, 0, [past], sees, q, h)
+    p, e = cache.where(0, past)
+    cache.k[0, p, :, e + 1] = np.nan
+    cache.put()
+    got = run_tree(dev, cache, 0, [past], [n], h, pack(sees, n), q)
+    assert np.isnan(got[0]).all()
+    close(got[1:], want[1:], bound[1:])
+
+
+@forms
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_nonfinite_nodes(dev, page, n, h, hk, hd, bad):
+    rng = np.random.default_rng(n * hd)
+    cache, q = one_sequence(dev, rng, (page, n, h, hk, hd), 70)
+    sees = [random_tree(rng, n)]
+    sees[0][:, 1] = np.arange(n) == 1
+    want, bound = attend(cache, 0, [70], sees, q, h)
+    others = np.arange(n) != 1
+    for pos in [71] + list(range(70 + n, 70 + n + 16)):  # node 1, and the stale rows behind the last node
+        p, e = cache.where(0, pos)
+        cache.k[0, p, :, e:e + hd] = bad
+        cache.v[0, p, :, e:e + hd] = bad
+    cache.put()
+    got = run_tree(dev, cache, 0, [70], [n], h, pack(sees, n), q)
+    assert not np.isfinite(got[1]).any()
+    close(got[others], want[others], bound[others])
+    # one element of the node's V row: that element of the row that sees it
+    p, e = cache.where(0, 71)
+    cache.k[0, p, :, e:e + hd] = 0
+    cache.v[0, p, :, e:e + hd] = 0
+    cache.v[0, p, :, e + 5] = bad
+    cache.put()
+    got = run_tree(dev, cache, 0, [70], [n], h, pack(sees, n), q)
+    assert np.array_equal(np.isfinite(got[1]), np.tile(np.arange(hd) != 5, (h, 1)))
+    close(got[others], want[others], bound[others])
