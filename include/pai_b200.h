@@ -422,7 +422,9 @@ pai_status_t pai_b200_rope_append_f16kv(pai_b200_ctx_t *ctx, const pai_b200_kv_v
  * nothing gets zeros. Non-finite K or V rows make the rows that attend them
  * non-finite and no others. Results match fp32 arithmetic to about 1e-6
  * relative: K and V enter the tensor cores as stored, q and the softmax
- * weights as two fp16 parts each. The same call gives the same bits.
+ * weights as two fp16 parts each (an element of q is held to 2^-22 of itself
+ * or 2^-39 of its row's largest, a weight to 2^-22 or 2^-37 of the largest).
+ * The same call gives the same bits.
  * PAI_ERR_UNSUPPORTED when the sequences' rows and the positions that the
  * tables allow make more than 2^31 tiles. A device wait that runs out is
  * reported by pai_b200_sync, as everywhere. */

@@ -87,3 +87,26 @@ def test_nonfinite_nodes(dev, page, n, h, hk, hd, bad):
     got = run_tree(dev, cache, 0, [70], [n], h, pack(sees, n), q)
     assert np.array_equal(np.isfinite(got[1]), np.tile(np.arange(hd) != 5, (h, 1)))
     close(got[others], want[others], bound[others])
+
+
+# ---- queries of unequal elements ------------------------------------------------------------------------------
+
+
+@forms
+@pytest.mark.parametrize("outlier", [64, 1024, 8192])
+def test_outlier_query_dimensions(dev, page, n, h, hk, hd, outlier):
+    """One large dimension of q against a K channel that is small by as much, as the channels of trained models are: the
+    other dimensions count as much as that one. Half of fp16's smallest step is 2^-25, and a row's largest element lies
+    at 2^14 or above: what is too small for both of its parts is off by 2^-39 of it, a score by 2^-39 max |q| sum |k| /
+    sqrt(hd) more than with equal elements."""
+    rng = np.random.default_rng(outlier + n)
+    cache, q = one_sequence(dev, rng, (page, n, h, hk, hd), 300)
+    row = cache.page * hd
+    cache.k[..., 0:row:hd] = (cache.k[..., 0:row:hd].astype(np.float32) / outlier).astype(np.float16)
+    cache.put()
+    q[..., 0] = 3 * outlier * np.where(rng.random((n, h)) < 0.5, -1, 1)
+    sees = [random_tree(rng, n)]
+    want, bound = attend(cache, 0, [300], sees, q, h)
+    most = np.abs(cache.k.astype(np.float64)[..., :row].reshape(-1, hd)).sum(-1).max()
+    bound = bound + 2 * 2.0 ** -39 * np.abs(q).max() * most / np.sqrt(hd) * np.abs(cache.v.astype(np.float64)).max()
+    close(run_tree(dev, cache, 0, [300], [n], h, pack(sees, n), q), want, bound)
