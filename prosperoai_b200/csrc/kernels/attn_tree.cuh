@@ -50,7 +50,7 @@ struct TreeParams {
   uint32_t *err;
   uint64_t wait_ns;
   uint32_t chunk;  // tcgen05 form: positions of one tensor copy
-  float scale;     // log2(e) / sqrt(hd)
+  float scale;     // log2(e) / sqrt(hd): multiplies q, so that scores are exponents of two but for a power of two
 };
 
 // (x, y) -> packed fp16 parts and packed fp16 remainders
@@ -68,6 +68,10 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// What a row's scores are taken relative to, from their maximum: 2^12 times the weights. Rounded up, so that no weight is
+// above 2^12 where a score's steps are larger than 12 (rounded to nearest, 2^26 - 12 is 2^26 - 16, and 2^16 is no fp16).
+__device__ __forceinline__ float shifted(float top) { return __fsub_ru(top, kPShift); }
 
 // Bits [at, at + 64) of a row of `words` 64-bit words; at may be negative.
 __device__ __forceinline__ uint64_t window(const uint64_t *m, uint32_t words, int32_t at) {

@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(few_threads(SW), 1)
           const float corr = m == mn ? 1.0f : ex2(m - mn);
           m = mn;
           if (w4 == 0 && lane < 8 * RG) {
-            sm.sub[row0 + lane] = mn == -INFINITY ? kNone : mn - kPShift;
+            sm.sub[row0 + lane] = mn == -INFINITY ? kNone : shifted(mn);
             sm.corr[i & WM][row0 + lane] = corr;
           }
 #pragma unroll

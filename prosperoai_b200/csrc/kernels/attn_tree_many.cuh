@@ -232,10 +232,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           sm.top[i & 1][r][wg] = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
           group_sync(4 + (warp & 3));
           const float4 tops = *reinterpret_cast<const float4 *>(sm.top[i & 1][r]);
+          // the factor is a power of two: the products are exact, so that no exponent below is above that of the maximum
           const float mn = fmaxf(m, fmaxf(fmaxf(tops.x, tops.y), fmaxf(tops.z, tops.w)) * factor);
           corr1 = m == mn ? 1.0f : ex2(m - mn);
           m = mn;
-          const float sub = mn == -INFINITY ? 0.0f : mn - kPShift;
+          const float sub = mn == -INFINITY ? 0.0f : shifted(mn);
           float part[4] = {0.f, 0.f, 0.f, 0.f};
           uint32_t w[32];  // 16 words of parts, 16 of remainders
 #pragma unroll

@@ -386,8 +386,8 @@ __device__ __forceinline__ void clean_tiles(const TreeParams &p, Ring &ring, uin
     }
 }
 
-// Query rows into shared memory as a K-major operand [64 dims][rows][128 bytes], a power of two and two fp16 parts a
-// row: warp `w` of WARPS has MR / WARPS rows; the remainders lie `rem` bytes behind the parts.
+// Query rows, with the scores' scale, into shared memory as a K-major operand [64 dims][rows][128 bytes], a power of two
+// and two fp16 parts a row: warp `w` of WARPS has MR / WARPS rows; the remainders lie `rem` bytes behind the parts.
 template <int HD, uint32_t MR, uint32_t WARPS>
 __device__ __forceinline__ void put_queries(const TreeParams &p, const Segment &g, uint32_t rows, uint32_t w, uint8_t *q,
                                             uint32_t block, uint32_t rem, float *factor) {
@@ -407,6 +407,7 @@ __device__ __forceinline__ void put_queries(const TreeParams &p, const Segment &
 #pragma unroll
     for (uint32_t u = 0; u < UN; u++) {
       const uint32_t rl = w * WR + b0 + u * RW + lane / LR;
+      f[u].x *= p.scale, f[u].y *= p.scale, f[u].z *= p.scale, f[u].w *= p.scale;
       float top = fmaxf(fmaxf(fabsf(f[u].x), fabsf(f[u].y)), fmaxf(fabsf(f[u].z), fabsf(f[u].w)));
 #pragma unroll
       for (uint32_t o = LR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -418,7 +419,7 @@ __device__ __forceinline__ void put_queries(const TreeParams &p, const Segment &
       const uint32_t at = (d4 / 16) * block + rl * 128 + (((d4 % 16) / 2 ^ (rl & 7)) << 4) + (d4 & 1) * 8;
       *reinterpret_cast<uint2 *>(q + at) = hi;
       *reinterpret_cast<uint2 *>(q + rem + at) = lo;
-      if (d4 == 0) factor[rl] = p.scale * up;
+      if (d4 == 0) factor[rl] = up;
     }
   }
   fence_proxy_async();

@@ -171,15 +171,15 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tree(TreeParams p) {
 #pragma unroll
         for (int e = 0; e < 2; e++) {
           const float2 f = live[x] ? *reinterpret_cast<const float2 *>(qr + 16 * k + 8 * e + 2 * tq) : make_float2(0.f, 0.f);
-          qh[k][x + 2 * e] = __float_as_uint(f.x);
-          ql[k][x + 2 * e] = __float_as_uint(f.y);
-          top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+          const float a = f.x * p.scale, b = f.y * p.scale;
+          qh[k][x + 2 * e] = __float_as_uint(a);
+          ql[k][x + 2 * e] = __float_as_uint(b);
+          top = fmaxf(top, fmaxf(fabsf(a), fabsf(b)));
         }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      float down, up;
-      row_scale(top, down, up);
-      factor[x] = p.scale * up;
+      float down;
+      row_scale(top, down, factor[x]);
 #pragma unroll
       for (int k = 0; k < HD / 16; k++)
 #pragma unroll
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tree(TreeParams p) {
         const float mn = fmaxf(m[x], mt[x]);
         corr[x] = m[x] == mn ? 1.0f : ex2(m[x] - mn);
         m[x] = mn;
-        sub[x] = mn == -INFINITY ? 0.0f : mn - kPShift;
+        sub[x] = mn == -INFINITY ? 0.0f : shifted(mn);
         l[x] *= corr[x];
       }
       // weights as A fragments

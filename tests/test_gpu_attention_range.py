@@ -110,3 +110,37 @@ def test_outlier_query_dimensions(dev, page, n, h, hk, hd, outlier):
     most = np.abs(cache.k.astype(np.float64)[..., :row].reshape(-1, hd)).sum(-1).max()
     bound = bound + 2 * 2.0 ** -39 * np.abs(q).max() * most / np.sqrt(hd) * np.abs(cache.v.astype(np.float64)).max()
     close(run_tree(dev, cache, 0, [300], [n], h, pack(sees, n), q), want, bound)
+
+
+# ---- scores of any size ---------------------------------------------------------------------------------------
+
+
+@forms
+@pytest.mark.parametrize("scale", [1e6, 1e7, 2e7, 4e7, 1e8, 1e9, 1e12, 1e20])
+def test_large_scores(dev, page, n, h, hk, hd, scale):
+    """Scores whose steps are larger than the exponents of the weights. The outputs are means of the V rows; where the best
+    score is further from the next than both may be off (2^-20 + hd / 8 2^-23 of sum |q_d k_d| / sqrt(hd) each) and e^-40
+    more, the output is the best key's V row."""
+    rng = np.random.default_rng(n + hd)
+    past = 500
+    cache, q = one_sequence(dev, rng, (page, n, h, hk, hd), past)
+    q = (q * np.float32(scale)).astype(np.float32)
+    sees = [random_tree(rng, n)]
+    got = run_tree(dev, cache, 0, [past], [n], h, pack(sees, n), q)
+    assert np.isfinite(got).all()
+    k, _ = cache.rows(cache.k, 0, 0, past + n)
+    v, _ = cache.rows(cache.v, 0, 0, past + n)
+    top, decided = np.abs(v).max(), 0
+    assert np.abs(got).max() <= top * (1 + 2.0 ** -19)
+    for i in range(n):
+        ok = np.concatenate([np.ones(past, bool), sees[0][i]])
+        for j in range(h):
+            kk, qq = k[j // (h // hk)][ok], q[i, j].astype(np.float64)
+            sc = kk @ qq / np.sqrt(hd)
+            ds = (2.0 ** -20 + hd / 8 * 2.0 ** -23) * (np.abs(kk) @ np.abs(qq)).max() / np.sqrt(hd)
+            best = sc.argmax()
+            if np.partition(sc, -2)[-2] < sc[best] - 2 * ds - 40:
+                decided += 1
+                tol = (2.0 ** -21 + (len(kk) / 8 + 4) * 2.0 ** -23) * top
+                assert np.abs(got[i, j] - v[j // (h // hk)][ok][best]).max() <= tol
+    assert decided > n * h // 2
