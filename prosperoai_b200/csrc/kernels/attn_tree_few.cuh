@@ -15,6 +15,8 @@
 // a compile-time value: with 1 for 8 rows that took 101 us, with 4 and three of them idle 125 (these warps wait for
 // instructions more than for anything else).
 #pragma once
+#include <cfloat>
+
 #include "attn_tree_tc.cuh"
 
 namespace {
@@ -237,7 +239,8 @@ __global__ void __launch_bounds__(few_threads(SW), 1)
   } else {
     // ---- softmax: a thread a position and 8 RG rows, from row0 ----
     const uint32_t wg = warp / 4, w4 = warp & 3, row0 = 8 * RG * wg;
-    constexpr float kNone = -1e30f, kFull = 15.5f;  // no maximum yet; the largest exponent that weights may have
+    // no maximum yet: below every score; the largest exponent that weights may have
+    constexpr float kNone = -FLT_MAX, kFull = 15.5f;
     for (; next_segment<1, 128 * SW>(sm.ring, seg, wait, g); seg++) {
       const uint32_t rows = min(kFewRows, g.nodes * p.g - g.block * kFewRows);
       // every score of the last segment has been read, so its products are done: Q may be written

@@ -144,3 +144,26 @@ def test_large_scores(dev, page, n, h, hk, hd, scale):
                 tol = (2.0 ** -21 + (len(kk) / 8 + 4) * 2.0 ** -23) * top
                 assert np.abs(got[i, j] - v[j // (h // hk)][ok][best]).max() <= tol
     assert decided > n * h // 2
+
+
+@forms
+@pytest.mark.parametrize("query,key", [(1e33, 1.0), (1e29, 1.0), (1.7e38, 2.0 ** -10), (3e38, 2.0 ** -14), (1e-40, 60000.0), (0.0, 1.0)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_equal_scores_of_any_size(dev, page, n, h, hk, hd, query, key, sign):
+    """All keys have the same score, whatever it is: the output is the mean of the V rows. The weights are equal, so
+    only the sum's roundings are left: 2^-23 for each of n / 8 + 4 steps, 2^-21 for the weights' parts."""
+    rng = np.random.default_rng(n)
+    past = 300
+    cache, q = one_sequence(dev, rng, (page, n, h, hk, hd), past)
+    row = cache.page * hd
+    cache.k[..., 0:row:hd] = key
+    cache.put()
+    q[:] = 0
+    q[..., 0] = sign * query
+    sees = [random_tree(rng, n)]
+    got = run_tree(dev, cache, 0, [past], [n], h, pack(sees, n), q)
+    v, _ = cache.rows(cache.v, 0, 0, past + n)
+    for i in range(n):
+        ok = np.concatenate([np.ones(past, bool), sees[0][i]])
+        want = np.repeat(v[:, ok].mean(1), h // hk, 0)
+        assert np.abs(got[i] - want).max() <= (2.0 ** -21 + (ok.sum() / 8 + 4) * 2.0 ** -23) * np.abs(v).max()
