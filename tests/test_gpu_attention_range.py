@@ -5,7 +5,9 @@ The bounds are those of test_gpu_continuations.attend unless a test says otherwi
 import numpy as np
 import pytest
 
-from test_gpu_continuations import Cache, attend, close, pack, random_tree, run_tree
+from prosperoai_b200 import _native
+from prosperoai_b200.api import KvView
+from test_gpu_continuations import Cache, attend, close, i32, pack, random_tree, run_tree
 
 pytestmark = pytest.mark.gpu
 
@@ -167,3 +169,93 @@ def test_equal_scores_of_any_size(dev, page, n, h, hk, hd, query, key, sign):
         ok = np.concatenate([np.ones(past, bool), sees[0][i]])
         want = np.repeat(v[:, ok].mean(1), h // hk, 0)
         assert np.abs(got[i] - want).max() <= (2.0 ** -21 + (ok.sum() / 8 + 4) * 2.0 ** -23) * np.abs(v).max()
+
+
+# ---- holes, empty rows, long trees ----------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("page,n,h,hk,hd", [f for f in FORMS.values() if f[0]], ids=[k for k, f in FORMS.items() if f[0]])
+def test_holes_and_rows_that_see_nothing(dev, page, n, h, hk, hd):
+    rng = np.random.default_rng(page + n)
+    lens, nodes = [230, 0, 90], [n, n, max(n - 1, 1)]
+    width = -(-(230 + n) // page) + 1
+    table = rng.permutation(3 * width).reshape(3, width)
+    table[rng.random((3, width)) < 0.3] = -1
+    table[0, 0], table[2, -1] = 3 * width, -(1 << 31)
+    table[1, :-(-n // page)] = -1  # every node of a sequence without a past
+    cache = Cache(dev, rng, [1] * 3, page, hk, hd, table=table, n_pages=3 * width, max_pages=width)
+    sees = [random_tree(rng, k) for k in nodes]
+    sees[0][0] = False
+    sees[2][:] = False
+    q = rng.standard_normal((sum(nodes), h, hd)).astype(np.float32)
+    got = run_tree(dev, cache, 0, lens, nodes, h, pack(sees, n), q)
+    close(got, *attend(cache, 0, lens, sees, q, h))
+    assert not got[n:2 * n].any()
+    # nothing committed, nothing seen
+    alone = Cache(dev, rng, [n], page, hk, hd)
+    assert not run_tree(dev, alone, 0, [0], [n], h, pack([np.zeros((n, n), bool)], n), q[:n]).any()
+
+
+@pytest.mark.parametrize("lens,nodes,page,h,hk,hd", [
+    ([50], [1024], 16, 2, 1, 64), ([10, 300], [200, 513], 20, 2, 2, 128), ([700], [257], 0, 2, 1, 128), ([0], [131], 100, 1, 1, 64),
+    ([33, 1, 0], [1, 1024, 129], 64, 1, 1, 128)])
+@pytest.mark.parametrize("kind", ["tree", "chain"])
+def test_long_trees(dev, lens, nodes, page, h, hk, hd, kind):
+    """Masks of up to 16 words, row tiles behind the first."""
+    rng = np.random.default_rng(sum(nodes))
+    total = [a + b for a, b in zip(lens, nodes)]
+    cache = Cache(dev, rng, total, page, hk, hd, cap=max(total))
+    sees = [random_tree(rng, n) if kind == "tree" else np.tril(np.ones((n, n), bool)) for n in nodes]
+    q = rng.standard_normal((sum(nodes), h, hd)).astype(np.float32)
+    got = run_tree(dev, cache, 0, lens, nodes, h, pack(sees, max(nodes)) if kind == "tree" else None, q)
+    close(got, *attend(cache, 0, lens, sees, q, h))
+
+
+# ---- dependent launches ---------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("page,n,h,hk,hd", [FORMS[k] for k in ("few 16", "many", "any page")], ids=["few", "many", "any page"])
+def test_dependent_launches(dev, page, n, h, hk, hd):
+    """Selection, fork, append, attention and acceptance, each launched while the one before runs (pai_b200_set_pdl), give
+    the bits that they give one behind the other."""
+    L, rng = _native.load(), np.random.default_rng(n)
+    beams, vocab, past = 4, 3001, 61
+    width = -(-(past + 3 * n) // page) if page else 1
+    table = rng.permutation(2 * beams * width).reshape(2, beams, width)[0] if page else None
+    cache = Cache(dev, rng, [past] * beams, page, hk, hd, layers=2, table=table, n_pages=2 * beams * width if page else None,
+                  max_pages=width if page else None, cap=past + 3 * n)
+    rows, lens = beams * n, i32([past - b for b in range(beams)])
+    off, path = i32(np.arange(beams + 1) * n), i32([[0, n - 1]] * beams)
+    sees = [random_tree(rng, n) for _ in range(beams)]
+    ang = rng.standard_normal((past + 4 * n, hd // 2)).astype(np.float32)
+    given = dict(logits=rng.standard_normal((beams, vocab)).astype(np.float32), scores=np.zeros(beams, np.float32),
+                 qkv=rng.standard_normal((rows, h + 2 * hk, hd)).astype(np.float32), cos=np.cos(ang), sin=np.sin(ang), lens=lens,
+                 off=off, path=path, n_path=i32([2] * beams), mask=pack(sees, n), grow=i32([n] * beams))
+    d = {k: dev.put(v) for k, v in given.items()}
+    out = {k: dev.alloc(4 * size) for k, size in dict(score=beams, parent=beams, token=beams, table=beams * width, lens=beams,
+                                                      granted=beams, q=rows * h * hd, att=rows * h * hd, after=beams).items()}
+    forked = KvView.from_buffer_copy(cache.view)
+    if page:
+        forked.table = out["table"].ptr
+
+    def step():
+        cache.put()
+        for o in out.values():
+            o.upload(np.zeros(o.nbytes // 4, np.int32))
+        dev.beam_select(1, beams, vocab, d["logits"], vocab, d["scores"], None, 0, beams, out["score"], out["parent"], out["token"])
+        dev.kv_fork(cache.view, 0, d["lens"], out["parent"], d["grow"], out["table"] if page else None, out["lens"], out["granted"])
+        for layer in range(2):
+            dev.rope_append(forked, layer, h, rows, n, out["lens"], d["off"], None, d["qkv"], d["cos"], d["sin"], len(ang), out["q"])
+            dev.attn_tree(forked, layer, h, rows, n, out["lens"], d["off"], d["mask"], out["q"], out["att"])
+        dev.kv_accept(forked, 2, out["lens"], d["path"], d["n_path"], out["after"])
+        return [o.download(np.uint32) for o in out.values()] + [cache.dk.download(np.uint16), cache.dv.download(np.uint16)]
+
+    want = step()
+    assert (want[5] == n).all() and np.isfinite(want[7].view(np.float32)).all()  # room for all, attended
+    _native.check(L.pai_b200_set_pdl(dev.ctx, 1), "set_pdl")
+    try:
+        for _ in range(20):
+            for a, b in zip(step(), want):
+                np.testing.assert_array_equal(a, b)
+    finally:
+        L.pai_b200_set_pdl(dev.ctx, 0)
