@@ -13,7 +13,10 @@
  * failure (the message is kept for pai_b200_last_error).
  *
  * Operations are asynchronous on the context's stream, like kernel
- * launches; pai_b200_sync() waits. The reference executor is synchronous
+ * launches; pai_b200_sync() waits. Memory that another stream writes before
+ * or reads after an operation needs an order between the two: a context on
+ * that stream (pai_b200_init_on_stream), events on pai_b200_stream(), or a
+ * wait on the host. The reference executor is synchronous
  * (scheduler/scheduler.c:346-632 returns when every step is done), so
  * the integration shim syncs at the same boundaries.
  */
@@ -116,6 +119,16 @@ typedef struct pai_b200_ctx pai_b200_ctx_t;
  * scratch memory. Replaces the PS5 HAL's device bring-up
  * (runtime/runtime.c:18-80, gpu/hal/hal.h:45-61). */
 pai_status_t pai_b200_init(int device, pai_b200_ctx_t **out);
+/* The same on a stream of the caller's: `stream` is a cudaStream_t of that
+ * device, NULL CUDA's default stream, and outlives the context. What the
+ * context does is then in order with the stream's other work, without a wait
+ * or an event. The stream's owner may capture it, once the scratch is sized
+ * (run each operation once before); pai_b200_graph_begin, and
+ * pai_b200_session_create, which captures its step, need a stream that can
+ * be captured: not the default one. */
+pai_status_t pai_b200_init_on_stream(int device, void *stream, pai_b200_ctx_t **out);
+/* The context's stream, a cudaStream_t. */
+void *pai_b200_stream(pai_b200_ctx_t *ctx);
 pai_status_t pai_b200_shutdown(pai_b200_ctx_t *ctx);
 pai_status_t pai_b200_device_count(int *out);
 /* Text of the last failure on this thread ("" when none). */

@@ -81,6 +81,8 @@ PP = C.POINTER(C.c_void_p)
 # name -> (restype, argtypes)
 SIGNATURES = {
     "pai_b200_init": (I32, [C.c_int, PP]),
+    "pai_b200_init_on_stream": (I32, [C.c_int, P, PP]),
+    "pai_b200_stream": (P, [P]),
     "pai_b200_shutdown": (I32, [P]),
     "pai_b200_device_count": (I32, [C.POINTER(C.c_int)]),
     "pai_b200_last_error": (C.c_char_p, []),

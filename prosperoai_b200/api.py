@@ -98,12 +98,17 @@ class PackedMatrix:
 
 
 class Device:
-    """One CUDA device context (pai_b200_init)."""
+    """One CUDA device context. It has a stream of its own (pai_b200_init), or runs on a caller's: stream is a
+    cudaStream_t's address, 0 the default stream (pai_b200_init_on_stream; torch.cuda.current_stream().cuda_stream
+    puts it in order with torch's work). Arrays that another stream writes or reads need an order with Device.stream."""
 
-    def __init__(self, device: int = 0):
+    def __init__(self, device: int = 0, stream: int | None = None):
         L = load()
         ctx = C.c_void_p()
-        check(L.pai_b200_init(device, C.byref(ctx)), "init")
+        if stream is None:
+            check(L.pai_b200_init(device, C.byref(ctx)), "init")
+        else:
+            check(L.pai_b200_init_on_stream(device, stream or None, C.byref(ctx)), "init_on_stream")
         self.ctx = ctx.value
         self.device = device
 
@@ -111,6 +116,11 @@ class Device:
         if self.ctx:
             load().pai_b200_shutdown(self.ctx)
             self.ctx = None
+
+    @property
+    def stream(self) -> int:
+        """The context's stream, a cudaStream_t's address (0: the default stream)."""
+        return load().pai_b200_stream(self.ctx) or 0
 
     def sync(self):
         check(load().pai_b200_sync(self.ctx), "sync")

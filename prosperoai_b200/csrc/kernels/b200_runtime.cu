@@ -1,8 +1,8 @@
 // Runtime shim: device context, memory, copies, events, CUDA graphs and
 // error reporting behind the C ABI of include/pai_b200.h. The PS5 backend
 // this replaces kept the same duties in gpu/hal (hal.h:45-61: device
-// open, allocation, submit/wait); here a context owns one CUDA stream and
-// the split-K scratch the kernels share.
+// open, allocation, submit/wait); here a context has one CUDA stream, its
+// own or a caller's, and the split-K scratch the kernels share.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -24,6 +24,7 @@ constexpr uint64_t kMaxWaitNs = 60000000000ull;
 struct pai_b200_ctx {
   int device;
   cudaStream_t stream;
+  int owns_stream;        // 0: the caller's
   float *partial;         // split-K partial sums
   uint64_t partial_floats;
   uint32_t *counters;     // split-K arrival counters, left at zero
@@ -107,7 +108,7 @@ extern "C" pai_status_t pai_b200_device_count(int *out) {
   return PAI_OK;
 }
 
-extern "C" pai_status_t pai_b200_init(int device, pai_b200_ctx_t **out) {
+static pai_status_t open_ctx(int device, bool own, cudaStream_t stream, pai_b200_ctx_t **out) {
   if (!out) return b200_fail(PAI_ERR_INVALID_ARG, "init: NULL out");
   *out = nullptr;
   int n = 0;
@@ -126,6 +127,12 @@ extern "C" pai_status_t pai_b200_init(int device, pai_b200_ctx_t **out) {
     return b200_fail(PAI_ERR_UNSUPPORTED, "init: device %d is sm_%d%d; this library is built for sm_100a only",
                      device, prop.major, prop.minor);
   }
+  if (stream) {
+    int at = -1;
+    st = b200_cuda(cudaStreamGetDevice(stream, &at), "cudaStreamGetDevice");
+    if (st) return st;
+    if (at != device) return b200_fail(PAI_ERR_INVALID_ARG, "init: a stream of device %d for device %d", at, device);
+  }
   pai_b200_ctx *c = new (std::nothrow) pai_b200_ctx();
   if (!c) return b200_fail(PAI_ERR_NOMEM, "init: host allocation");
   c->device = device;
@@ -134,7 +141,9 @@ extern "C" pai_status_t pai_b200_init(int device, pai_b200_ctx_t **out) {
     const char *e = getenv("PAI_B200_PDL");
     c->pdl_allowed = !(e && e[0] == '0');
   }
-  st = b200_cuda(cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking), "cudaStreamCreate");
+  c->stream = stream;
+  c->owns_stream = own;
+  if (own) st = b200_cuda(cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking), "cudaStreamCreate");
   if (st) {
     delete c;
     return st;
@@ -143,7 +152,7 @@ extern "C" pai_status_t pai_b200_init(int device, pai_b200_ctx_t **out) {
   if (!st) st = b200_cuda(cudaHostGetDevicePointer((void **)&c->err_dev, c->err_host, 0), "error word mapping");
   if (st) {
     if (c->err_host) cudaFreeHost(c->err_host);
-    cudaStreamDestroy(c->stream);
+    if (own) cudaStreamDestroy(c->stream);
     delete c;
     return st;
   }
@@ -151,6 +160,12 @@ extern "C" pai_status_t pai_b200_init(int device, pai_b200_ctx_t **out) {
   *out = c;
   return PAI_OK;
 }
+
+extern "C" pai_status_t pai_b200_init(int device, pai_b200_ctx_t **out) { return open_ctx(device, true, nullptr, out); }
+extern "C" pai_status_t pai_b200_init_on_stream(int device, void *stream, pai_b200_ctx_t **out) {
+  return open_ctx(device, false, (cudaStream_t)stream, out);
+}
+extern "C" void *pai_b200_stream(pai_b200_ctx_t *c) { return c ? c->stream : nullptr; }
 
 extern "C" pai_status_t pai_b200_shutdown(pai_b200_ctx_t *c) {
   if (!c) return PAI_OK;
@@ -161,9 +176,15 @@ extern "C" pai_status_t pai_b200_shutdown(pai_b200_ctx_t *c) {
   if (c->xq) cudaFree(c->xq);
   for (uint32_t i = 0; i < c->nretired; i++) cudaFree(c->retired[i]);
   if (c->err_host) cudaFreeHost(c->err_host);
-  cudaStreamDestroy(c->stream);
+  if (c->owns_stream) cudaStreamDestroy(c->stream);
   delete c;
   return PAI_OK;
+}
+
+// Whether launches are recorded and not run: by this context's own capture, or by one that the owner of the stream began.
+static bool recording(pai_b200_ctx_t *c) {
+  cudaStreamCaptureStatus is = cudaStreamCaptureStatusNone;
+  return c->capturing || (!c->owns_stream && cudaStreamIsCapturing(c->stream, &is) == cudaSuccess && is != cudaStreamCaptureStatusNone);
 }
 
 extern "C" void *b200_ctx_stream(pai_b200_ctx_t *c) { return c->stream; }
@@ -192,7 +213,7 @@ extern "C" pai_status_t pai_b200_set_wait_limit(pai_b200_ctx_t *c, uint64_t ns) 
 
 extern "C" pai_status_t b200_ctx_xq(pai_b200_ctx_t *c, uint64_t bytes, void **buf) {
   if (bytes > c->xq_bytes) {
-    if (c->capturing) return b200_fail(PAI_ERR_INTERNAL, "activation scratch growth during graph capture");
+    if (recording(c)) return b200_fail(PAI_ERR_INTERNAL, "activation scratch growth during graph capture");
     const uint64_t want = std::max<uint64_t>(std::max<uint64_t>(bytes, 1u << 20), 2 * c->xq_bytes);
     pai_status_t rs = retire(c, c->xq);
     if (rs) return rs;
@@ -225,7 +246,7 @@ static int sync_check_enabled() {
 extern "C" pai_status_t b200_launched(pai_b200_ctx_t *c, uint32_t k, const char *name) {
   b200_ctx_count_launch(c, k);
   pai_status_t st = b200_cuda(cudaGetLastError(), name);
-  if (st || c->capturing || !sync_check_enabled()) return st;
+  if (st || !sync_check_enabled() || recording(c)) return st;
   st = b200_cuda(cudaStreamSynchronize(c->stream), name);
   if (st) return st;
   return b200_cuda(cudaGetLastError(), name);
@@ -235,7 +256,7 @@ extern "C" pai_status_t b200_ctx_scratch(pai_b200_ctx_t *c, uint64_t partial_flo
                                          uint32_t counters, float **partial,
                                          uint32_t **counter) {
   if (partial_floats > c->partial_floats) {
-    if (c->capturing) return b200_fail(PAI_ERR_INTERNAL, "scratch growth during graph capture");
+    if (recording(c)) return b200_fail(PAI_ERR_INTERNAL, "scratch growth during graph capture");
     const uint64_t want =
         std::max<uint64_t>(std::max<uint64_t>(partial_floats, 1u << 20), 2 * c->partial_floats);
     pai_status_t rs = retire(c, c->partial);
@@ -249,7 +270,7 @@ extern "C" pai_status_t b200_ctx_scratch(pai_b200_ctx_t *c, uint64_t partial_flo
     c->partial_floats = want;
   }
   if (counters > c->ncounters) {
-    if (c->capturing) return b200_fail(PAI_ERR_INTERNAL, "scratch growth during graph capture");
+    if (recording(c)) return b200_fail(PAI_ERR_INTERNAL, "scratch growth during graph capture");
     const uint32_t want = std::max<uint32_t>(std::max<uint32_t>(counters, 16384u), 2 * c->ncounters);
     pai_status_t rs = retire(c, c->counters);
     if (rs) return rs;
