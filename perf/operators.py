@@ -20,16 +20,19 @@ import torch
 
 own = False
 
-_DEV = None
+_DEVS = {}
 
 
-def _dev():
-    """The framework's device context, kept for the process."""
-    global _DEV
-    if _DEV is None:
-        from prosperoai_b200.api import Device
-        _DEV = Device(torch.cuda.current_device())
-    return _DEV
+def _dev(s):
+    """The framework's device context on the stream of the state's first pass, torch's current one, which fills the inputs and
+    reads the outputs; one a stream, kept for the process."""
+    if "dev" not in s:
+        at = torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream
+        if at not in _DEVS:
+            from prosperoai_b200.api import Device
+            _DEVS[at] = Device(at[0], stream=at[1])
+        s["dev"] = _DEVS[at]
+    return s["dev"]
 
 
 # ---- the cases --------------------------------------------------------------------------------------
@@ -274,7 +277,7 @@ def _view(s):
 
 
 def _own_tree(s):
-    dev, kv, h = _dev(), _view(s), s["case"]["h"]
+    dev, kv, h = _dev(s), _view(s), s["case"]["h"]
     lens, off, q = s["lens"].data_ptr(), s["off"].data_ptr(), s["q"].data_ptr()
     dev.rope_append(kv, 0, h, s["rows"], s["most"], lens, off, s["depth"].data_ptr(), s["qkv"].data_ptr(),
                     s["cos"].data_ptr(), s["sin"].data_ptr(), s["cos"].shape[0], q)
@@ -284,16 +287,16 @@ def _own_tree(s):
 
 def _own_beam(s):
     c = s["case"]
-    _dev().beam_select(c["prompts"], c["beams"], c["vocab"], s["logits"].data_ptr(), c["vocab"], s["scores"].data_ptr(),
-                       s["done"].data_ptr(), s["pad"], c["pick"], s["out_scores"].data_ptr(),
-                       s["out_parents"].data_ptr(), s["out_tokens"].data_ptr())
+    _dev(s).beam_select(c["prompts"], c["beams"], c["vocab"], s["logits"].data_ptr(), c["vocab"], s["scores"].data_ptr(),
+                        s["done"].data_ptr(), s["pad"], c["pick"], s["out_scores"].data_ptr(),
+                        s["out_parents"].data_ptr(), s["out_tokens"].data_ptr())
     return {"scores": s["out_scores"], "parents": s["out_parents"], "tokens": s["out_tokens"]}
 
 
 def _own_fork(s):
     paged = s["table"] is not None
-    _dev().kv_fork(_view(s), 0, s["lens"].data_ptr(), s["parents"].data_ptr(), s["grow"].data_ptr(),
-                   s["table_out"].data_ptr() if paged else None, s["lens_out"].data_ptr(), s["granted"].data_ptr())
+    _dev(s).kv_fork(_view(s), 0, s["lens"].data_ptr(), s["parents"].data_ptr(), s["grow"].data_ptr(),
+                    s["table_out"].data_ptr() if paged else None, s["lens_out"].data_ptr(), s["granted"].data_ptr())
     return _forked(s)
 
 
@@ -303,8 +306,8 @@ def _forked(s):
 
 
 def _own_accept(s):
-    _dev().kv_accept(_view(s), s["path"].shape[1], s["lens"].data_ptr(), s["path"].data_ptr(), s["n_path"].data_ptr(),
-                     s["lens_out"].data_ptr())
+    _dev(s).kv_accept(_view(s), s["path"].shape[1], s["lens"].data_ptr(), s["path"].data_ptr(), s["n_path"].data_ptr(),
+                      s["lens_out"].data_ptr())
     return {"k": s["k"], "v": s["v"], "lens": s["lens_out"]}
 
 
