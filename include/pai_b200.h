@@ -412,7 +412,8 @@ typedef struct pai_b200_kv_view {
  * lens[s] + i, behind the lens[s] committed positions. lens, node_off
  * [n_seq + 1], depth, mask are device arrays. At most max_nodes (1 to 1024)
  * nodes of a sequence and rows below `rows` are computed; other rows of the
- * outputs are left as they were. A chain of one node is plain decoding, a
+ * outputs are left as they were, and a length outside [0, max_pages *
+ * page_tokens] counts as the nearer end. A chain of one node is plain decoding, a
  * chain of n with mask and depth NULL a causal chunk of n tokens. */
 
 /* Rotate q and k of every row at position lens[s] + depth[row] (depth NULL:
@@ -421,7 +422,8 @@ typedef struct pai_b200_kv_view {
  * to fp16, in layer `layer` of the cache. qkv is [rows][h + 2 kv_heads]
  * [head_dim] (the fused projection row), cos_t and sin_t [table_len]
  * [head_dim / 2]. A node whose position is not below table_len gets NaN in
- * q_out and is not stored. qkv, q_out, cos_t, sin_t 16-byte aligned. */
+ * q_out and is not stored. qkv, q_out, cos_t, sin_t 16-byte aligned; q_out
+ * overlaps no input. */
 pai_status_t pai_b200_rope_append_f16kv(pai_b200_ctx_t *ctx, const pai_b200_kv_view_t *kv, uint32_t layer, uint64_t h,
                                         uint64_t rows, uint32_t max_nodes, const int32_t *lens,
                                         const int32_t *node_off, const int32_t *depth, const float *qkv,
@@ -432,8 +434,10 @@ pai_status_t pai_b200_rope_append_f16kv(pai_b200_ctx_t *ctx, const pai_b200_kv_v
  * set); NULL lets node i attend nodes 0..i. Scores are scaled by
  * 1/sqrtf(head_dim); q and out are [rows][h][head_dim] fp32, 16-byte
  * aligned; head_dim 64 or 128, h a multiple of kv_heads. A node that attends
- * nothing gets zeros. Non-finite K or V rows make the rows that attend them
- * non-finite and no others. Results match fp32 arithmetic to about 1e-6
+ * nothing gets zeros. A NaN in q, or in a K or V row that a node attends,
+ * makes that node's output NaN, an infinity in V that element of it not
+ * finite; an infinity in K makes it NaN, or is not attended where its score
+ * is -inf. No other rows change. Results match fp32 arithmetic to about 1e-6
  * relative: K and V enter the tensor cores as stored, q and the softmax
  * weights as two fp16 parts each (an element of q is held to 2^-22 of itself
  * or 2^-39 of its row's largest, a weight to 2^-22 or 2^-37 of the largest).
@@ -462,8 +466,8 @@ pai_status_t pai_b200_kv_accept_f16(pai_b200_ctx_t *ctx, const pai_b200_kv_view_
  * each sequence's last page; kv->table stays as it is). Sequences share the
  * pages of their common past. A partly filled last page that a sequence is
  * about to extend stays its own if no other sequence uses as many rows of it
- * (of several, the first that extends it keeps it); else its rows are copied
- * to a new page, in all layers. New pages are those that no sequence's
+ * (of several, the first with a grow above 0 keeps it, whether or not it gets
+ * its room); else its rows are copied to a new page, in all layers. New pages are those that no sequence's
  * committed positions use after the fork, lowest first, given to the
  * sequences in order; from the first that finds too few on, no sequence
  * gets any. Pages are in use by being in a table: ending a sequence frees
@@ -483,8 +487,12 @@ pai_status_t pai_b200_kv_fork_f16(pai_b200_ctx_t *ctx, const pai_b200_kv_view_t 
  * logits is [prompts * beams] rows of `vocab` with `stride` elements between
  * rows, scores and done [prompts][beams]. Best first; equal scores go to
  * the lowest beam, then the lowest token. out_parents holds rows (prompt *
- * beams + b), so that it serves pai_b200_kv_fork_f16. Scores are computed in
- * double and rounded once. A logit of NaN counts as -inf; where logits are
+ * beams + b), so that it serves pai_b200_kv_fork_f16. Within a beam the order
+ * is that of its logits. The exponentials of log sum exp are of 32 bits, their
+ * sums of 64 (each slice's rounded to 32), the rest is computed in double: a
+ * score is off by less than 2^-18 before it is rounded, a beam's all by the
+ * same, so candidates of different beams that are closer than twice that may
+ * come in either order. The same call gives the same bits. A logit of NaN counts as -inf; where logits are
  * +inf, they share the beam's probability; candidates of score -inf or NaN
  * are never chosen: with fewer than n_out others the rest are score -inf,
  * parent -1, token `pad`. beams and n_out at most 64. */

@@ -10,10 +10,11 @@
 // Registers: 640 threads at 96; setmaxnreg gives the softmax warps 104 and leaves 56 to the others (512 * 104 + 128 * 56
 // = 60416 of 61440, what the block was launched with).
 //
-// 8 sequences of 64 nodes x 4 heads a kv head at 32768 positions: 461-468 us on a GPU where it had 487-470 with 64
-// positions a thread (a second pass over the scores then, for want of registers); one tree of 16 at 4096 22.9 us, 24.7
-// then. With both parts that is 1.18 PFLOP/s, 0.72 of the dense rate in short bursts, and what the power limit leaves: the
-// same instructions on weights of random bits take 1.2 times as long, half of the products save 10 %.
+// 8 sequences of 64 nodes x 4 heads a kv head at 32768 positions: 533 us (1.03 PFLOP/s with both parts) after a second's
+// rest, 642 us in a run of seconds, which the power limit holds at 1335 MHz; the same instructions on a cache of zeros take
+// 425 us at 1965 MHz. That is 858 and 835 thousand cycles: the clock is what differs. One tree of 16 at 4096: 22.8 us.
+// (64 positions a thread instead of 32, with a second pass over the scores for want of registers: 24.7 there, and 1.04
+// times as long for the large case on one GPU.) At 96 registers the compiler spills: 48 bytes of stores, 112 of loads.
 #pragma once
 #include "attn_tree_tc.cuh"
 
