@@ -201,8 +201,8 @@ __global__ void __launch_bounds__(few_threads(SW), 1)
 #pragma unroll 1
             for (uint32_t left = sm.odd[i & WM][x] & sm.valid[i & WM][x]; left; left &= left - 1) {
               const uint32_t pos = tile * kTcTile + 32 * x + __ffs(left) - 1;
-              const int64_t at_row = kv_row(p.c, g.s, pos);
-              if (at_row < 0) continue;  // the words are old ones: a wait has run out
+              // (no row, where a wait has run out and the words are old ones: then the plane's first)
+              const int64_t at_row = max(kv_row(p.c, g.s, pos), (int64_t)0);
               const float f = __half2float(p.c.v[(size_t)g.kvh * p.c.head_stride + at_row + d]);
               if (isfinite(f)) continue;
 #pragma unroll

@@ -532,7 +532,7 @@ pai_status_t launch_tree_hd(pai_b200_ctx_t *ctx, TreeParams &p) {
   CUtensorMap kmap, vmap;
   if ((!p.c.table || p.c.page_tokens % p.chunk == 0) && plane_map(p, p.c.k, &kmap) && plane_map(p, p.c.v, &vmap))
   {
-    // 8 sequences at 16384 positions, with the exchanged operands and without: 8 rows 93 and 121 us, 32 rows 111 and 127
+    // 8 sequences at 16384 positions, with the exchanged operands and without: 8 rows 93 and 121 us, 32 rows 109 and 127
     // (at 4096 positions 55 and 51, the lengths are not known here); 8 rows with 16 at compile time 97, 16 rows with 32
     // 106 instead of 99. With head_dim 64 a tile is half the bytes and the same softmax: 16 rows 84 and 108, 32 rows 119
     // and 108 (one sequence at 4096: 24.8 and 20.6).
