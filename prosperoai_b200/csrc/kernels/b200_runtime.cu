@@ -183,8 +183,11 @@ extern "C" pai_status_t pai_b200_shutdown(pai_b200_ctx_t *c) {
 
 // Whether launches are recorded and not run: by this context's own capture, or by one that the owner of the stream began.
 static bool recording(pai_b200_ctx_t *c) {
+  if (c->capturing || c->owns_stream) return c->capturing;
   cudaStreamCaptureStatus is = cudaStreamCaptureStatusNone;
-  return c->capturing || (!c->owns_stream && cudaStreamIsCapturing(c->stream, &is) == cudaSuccess && is != cudaStreamCaptureStatusNone);
+  if (cudaStreamIsCapturing(c->stream, &is) == cudaSuccess) return is != cudaStreamCaptureStatusNone;
+  cudaGetLastError();  // the default stream, while another thread captures in a mode that forbids its use
+  return true;
 }
 
 extern "C" void *b200_ctx_stream(pai_b200_ctx_t *c) { return c->stream; }
