@@ -490,9 +490,9 @@ pai_status_t pai_b200_kv_fork_f16(pai_b200_ctx_t *ctx, const pai_b200_kv_view_t 
  * beams + b), so that it serves pai_b200_kv_fork_f16. Within a beam the order
  * is that of its logits. The exponentials of log sum exp are of 32 bits, their
  * sums of 64 (each slice's rounded to 32), the rest is computed in double: a
- * score is off by less than 2^-18 before it is rounded, a beam's all by the
- * same, so candidates of different beams that are closer than twice that may
- * come in either order. The same call gives the same bits. A logit of NaN counts as -inf; where logits are
+ * score is off by less than 2^-18 (2^-17 above 128256 tokens) before it is
+ * rounded, a beam's all by the same, so candidates of different beams that
+ * are closer than twice that may come in either order. The same call gives the same bits. A logit of NaN counts as -inf; where logits are
  * +inf, they share the beam's probability; candidates of score -inf or NaN
  * are never chosen: with fewer than n_out others the rest are score -inf,
  * parent -1, token `pad`. beams and n_out at most 64. */
